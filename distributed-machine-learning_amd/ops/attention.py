@@ -1,4 +1,10 @@
-"""Short-sequence attention: one fused HIP kernel per direction on a GPU, plain PyTorch elsewhere.
+"""Attention: fused HIP kernels on a GPU, plain PyTorch elsewhere.
+
+**Packed sequences of any length** (``packed_attention``): rows of sequences of different lengths one after the other, causal
+or not, query heads in groups that share a key / value head, forward and backward (``ops/csrc/packed_attention.hip``).
+``self_attention`` and ``self_attention_qkv`` use it past the short kernels' 128 tokens.
+
+**Short sequences**: one fused kernel per direction.
 
 The reference's sequences are 50 or 96 tokens long
 (/root/reference/ray-tune-hpo-regression-sample.py:28, /root/reference/ray-tune-hpo-regression.py:446), so a
@@ -17,9 +23,12 @@ accumulation); anything else -- and every CPU call -- runs ``attention_reference
 from __future__ import annotations
 
 import math
-from typing import Optional
+from typing import Optional, Sequence, Union
 
+import numpy as np
 import torch
+
+from .lib import PACKED_TILE_ROWS as _TILE
 
 RELU_EPS = 1e-6
 MAX_SEQ = 128
@@ -122,3 +131,139 @@ def self_attention(qk: torch.Tensor, v: torch.Tensor, num_heads: int, kind: str 
     split = lambda t, d: t.reshape(B, S, h, d).transpose(1, 2)          # noqa: E731
     o = attention_reference(split(q, dk), split(k, dk), split(v, dv), kind, keep, dropout_p)
     return o.transpose(1, 2).reshape(B, S, h * dv)
+
+
+# ---- packed sequences -----------------------------------------------------------------------------------------------------
+PACKED_MAX_HEAD_DIM = 128
+
+
+class SequencePack:
+    """Where the sequences of a packed batch lie: sequence ``i`` takes the ``lengths[i]`` rows after those before it, and
+    ``rows`` (default: their sum) is the number of rows of the tensors; rows behind the last sequence belong to none.
+
+    Made once per batch and used by every layer and both passes: the lengths are checked on the host, and the list of
+    128-row tiles the kernels work through, longest first, is laid out on ``device`` (default: the current GPU if there is
+    one).  ``SequencePack.uniform(count, length)`` is ``count`` sequences of one length; it needs no list."""
+
+    def __init__(self, lengths: Union[Sequence[int], np.ndarray, torch.Tensor], rows: Optional[int] = None, device=None):
+        if isinstance(lengths, torch.Tensor):
+            if lengths.is_cuda:
+                raise TypeError("SequencePack takes the lengths on the host (a list, an array or a CPU tensor)")
+            lengths = lengths.numpy()
+        n = np.asarray(lengths)
+        if n.size == 0:
+            n = n.reshape(-1).astype(np.int64)
+        if n.ndim != 1 or n.dtype.kind not in "iu":
+            raise TypeError("lengths must be a flat list of whole numbers")
+        if (n < 0).any():
+            raise ValueError("a sequence's length cannot be negative")
+        # summed as Python integers: an int64 sum of absurd lengths could wrap around the check below
+        total = sum(int(v) for v in n)
+        self._fix(total, total if rows is None else rows, device)
+        self.lengths = n.astype(np.int64)
+        self.longest = int(self.lengths.max(initial=0))
+        self.uniform_length = 0
+        self._lay_out()
+
+    @classmethod
+    def uniform(cls, count: int, length: int, device=None) -> "SequencePack":
+        if count < 0 or length < 0:
+            raise ValueError("a pack has no negative counts or lengths")
+        self = cls.__new__(cls)
+        self._fix(int(count) * int(length), int(count) * int(length), device)
+        self.lengths = np.full(int(count), int(length), dtype=np.int64)
+        self.longest = int(length) if count else 0
+        self.uniform_length = int(length) if count else 0
+        tiles = -(-int(length) // _TILE) * int(count)
+        self._counts, self._lists = (tiles, tiles, tiles), None
+        return self
+
+    def _fix(self, total: int, rows: int, device) -> None:
+        rows = int(rows)
+        if rows < total:
+            raise ValueError(f"sequences of {total} rows do not fit {rows} rows")
+        if rows > 0x7FFFFFFF - _TILE:
+            raise ValueError(f"a pack holds at most {0x7FFFFFFF - _TILE} rows, got {rows}")
+        device = torch.device(device if device is not None else ("cuda" if torch.cuda.is_available() else "cpu"))
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.total, self.rows, self.device = total, rows, device
+
+    def _lay_out(self) -> None:
+        """Three orders of the same tiles (``{first row of the sequence, its length, tile's first row in it}``), most work
+        first: by keys up to the tile's end (causal queries), by queries from its start (causal keys), by length (all see
+        all).  Rows of no sequence follow as entries of negative length, which the kernels fill with zeros."""
+        n = self.lengths
+        starts = np.concatenate([[0], np.cumsum(n)])[:-1]
+        tiles = -(-n // _TILE)
+        seq = np.repeat(np.arange(len(n)), tiles)
+        first = (np.arange(len(seq)) - np.repeat(np.cumsum(tiles) - tiles, tiles)) * _TILE
+        items = np.zeros((len(seq), 4), dtype=np.int32)
+        items[:, 0], items[:, 1], items[:, 2] = starts[seq], n[seq], first
+        at = np.arange(self.total, self.rows, _TILE)
+        tail = np.zeros((len(at), 4), dtype=np.int32)
+        tail[:, 0], tail[:, 1] = at, -np.minimum(_TILE, self.rows - at)
+        orders = [np.argsort(-work, kind="stable") for work in (np.minimum(first + _TILE, n[seq]), n[seq] - first, n[seq])]
+        lists = np.concatenate([np.concatenate([items[o], tail]) for o in orders]) if len(items) + len(tail) else items
+        count = len(items) + len(tail)
+        self._counts = (count, count, count)
+        # a blocking copy: the list is there for whichever stream uses it first
+        self._lists = torch.from_numpy(lists).to(self.device) if self.device.type == "cuda" else None
+
+
+
+def packed_attention_reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pack: SequencePack, causal: bool = False,
+                               scale: Optional[float] = None) -> torch.Tensor:
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+    group = q.shape[1] // k.shape[1]
+    out, at = [], 0
+    for n in pack.lengths.tolist():
+        qs, ks, vs = (t[at:at + n].transpose(0, 1) for t in (q, k, v))
+        ks, vs = ks.repeat_interleave(group, 0), vs.repeat_interleave(group, 0)
+        s = (qs @ ks.transpose(1, 2)) * scale
+        if causal:
+            s = s.masked_fill(torch.ones(n, n, dtype=torch.bool, device=q.device).triu(1), float("-inf"))
+        out.append((torch.softmax(s, dim=-1) @ vs).transpose(0, 1))
+        at += n
+    out.append(q.new_zeros(pack.rows - at, q.shape[1], v.shape[-1]))
+    return torch.cat(out)
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pack: SequencePack, causal: bool = False,
+                     scale: Optional[float] = None) -> torch.Tensor:
+    """Softmax attention within every sequence of ``pack``: ``q`` [rows, heads, dk], ``k`` [rows, kv_heads, dk], ``v``
+    [rows, kv_heads, dv] -> [rows, heads, dv], all f32 or all bf16, differentiable.  Query head ``i`` reads key / value head
+    ``i // (heads // kv_heads)``; with ``causal`` a row sees its sequence's rows up to itself.  ``scale`` defaults to
+    ``1 / sqrt(dk)``.  Rows behind the last sequence give zeros, and nothing of what they hold is used.
+
+    On a GPU: heads of at most 128 elements.  Operands may be strided (a slice of a fused projection is read in place when its
+    rows lie on 16-byte boundaries and is copied otherwise).  f32 operands are multiplied exactly; for bf16 the probabilities
+    are rounded to bf16 for the second product.  A value that is not finite reaches every row of its own sequence that lies
+    within 128 rows of one that may see it, and no other sequence."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 3:
+            raise ValueError(f"{name} must be [rows, heads, width], got {tuple(t.shape)}")
+        if t.shape[0] != pack.rows:
+            raise ValueError(f"{name} has {t.shape[0]} rows, the pack {pack.rows}")
+        if t.dtype != q.dtype or t.device != q.device:
+            raise TypeError(f"q, k and v must share one type and device, got {q.dtype} on {q.device} and {t.dtype} on {t.device}")
+    heads, kv_heads, dk, dv = q.shape[1], k.shape[1], q.shape[2], v.shape[2]
+    if k.shape[2] != dk or v.shape[1] != kv_heads:
+        raise ValueError(f"k {tuple(k.shape)} does not fit q {tuple(q.shape)} and v {tuple(v.shape)}")
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise ValueError(f"{heads} query heads cannot share {kv_heads} key / value heads")
+    if dk < 1 or dv < 1:
+        raise ValueError("heads must have at least one element")
+    scale = 1.0 / math.sqrt(dk) if scale is None else float(scale)
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if not q.is_cuda:
+        return packed_attention_reference(q, k, v, pack, causal, scale)
+    if q.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"packed_attention on a GPU takes f32 or bf16 operands, got {q.dtype}")
+    if max(dk, dv) > PACKED_MAX_HEAD_DIM:
+        raise ValueError(f"packed_attention on a GPU takes heads of at most {PACKED_MAX_HEAD_DIM} elements, got {max(dk, dv)}")
+    if pack.device != q.device:
+        raise ValueError(f"the pack lies on {pack.device}, the operands on {q.device}")
+    from .attention_hip import PackedAttention
+    return PackedAttention.apply(q, k, v, pack, bool(causal), scale)

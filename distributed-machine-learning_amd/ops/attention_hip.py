@@ -1,10 +1,13 @@
-"""Autograd binding of the fused short-sequence attention kernels (``csrc/attention.hip``)."""
+"""Autograd bindings of the attention kernels: short sequences (``csrc/attention.hip``) and packed sequences of any length
+(``csrc/packed_attention.hip``)."""
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import Optional
 
 import torch
+import torch.nn.functional as F
 
 from . import lib as L
 
@@ -160,3 +163,74 @@ class FusedSelfAttention(torch.autograd.Function):
                                               ctx.seed.data_ptr() if ctx.seed is not None else None, ctx.p,
                                               L.raw_stream(qk.device)), "mt_attn_bwd_strided_launch")
         return dqk, dv_, None, None, None, None, None
+
+
+def _in_place(t: torch.Tensor) -> torch.Tensor:
+    """``t`` [rows, heads, width] as the packed kernels can read it: 16-byte rows and heads, or else a copy padded with zero
+    columns to that (zeros add nothing to a score; zero value columns give output columns that are cut off again)."""
+    es = t.element_size()
+    per = 16 // es
+    if (t.stride(2) == 1 and t.shape[2] % per == 0 and t.stride(0) % per == 0 and t.stride(1) % per == 0
+            and max(t.stride(0), t.stride(1)) * es <= 1 << 24 and t.data_ptr() % 16 == 0):
+        return t
+    pad = -t.shape[2] % per
+    return F.pad(t, (0, pad)).contiguous() if pad else t.clone(memory_format=torch.contiguous_format)
+
+
+def _packed_args(pack, which: int, q, k, v, causal: bool, scale: float) -> "L.PackedAttn":
+    a = L.PackedAttn(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_row=q.stride(0), q_head=q.stride(1),
+                     k_row=k.stride(0), k_head=k.stride(1), v_row=v.stride(0), v_head=v.stride(1), rows=pack.rows,
+                     heads=q.shape[1], kv_heads=k.shape[1], head_k=q.shape[2], head_v=v.shape[2], causal=int(causal),
+                     scale=scale, uniform_len=pack.uniform_length, count=len(pack.lengths))
+    _tile_list(a, pack, which)
+    return a
+
+
+def _tile_list(a, pack, which: int) -> None:
+    """Which order of the pack's tiles a launch takes: 0 causal queries, 1 causal keys, 2 no mask."""
+    a.n_items = pack._counts[which]
+    if pack._lists is not None:
+        a.items = pack._lists.data_ptr() + which * a.n_items * L.PACKED_ITEM_BYTES
+        pack._lists.record_stream(torch.cuda.current_stream(pack.device))
+
+
+class PackedAttention(torch.autograd.Function):
+    """``ops.attention.packed_attention`` on a GPU; operands checked there."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, pack, causal: bool, scale: float):
+        so = L.load()
+        dk, dv = q.shape[2], v.shape[2]
+        qc, kc, vc = _in_place(q), _in_place(k), _in_place(v)
+        out = torch.empty(pack.rows, q.shape[1], vc.shape[2], device=q.device, dtype=q.dtype)
+        keeps = any(ctx.needs_input_grad[:3])
+        lse = torch.empty(q.shape[1], pack.rows, device=q.device, dtype=torch.float32) if keeps else None
+        a = _packed_args(pack, 0 if causal else 2, qc, kc, vc, causal, scale)
+        a.o, a.lse = out.data_ptr(), lse.data_ptr() if keeps else None
+        with torch.cuda.device(q.device):
+            L.check(so.mt_packed_attn_launch(ctypes.byref(a), 0, int(q.dtype == torch.bfloat16), L.raw_stream(q.device)),
+                    "mt_packed_attn_launch")
+        if keeps:
+            ctx.save_for_backward(qc, kc, vc, out, lse)
+        ctx.pack, ctx.meta = pack, (causal, scale, dk, dv)
+        return out if vc.shape[2] == dv else out[..., :dv].contiguous()
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        so = L.load()
+        q, k, v, out, lse = ctx.saved_tensors
+        pack, (causal, scale, dk, dv) = ctx.pack, ctx.meta
+        do = _in_place(grad_out.to(q.dtype))
+        delta = torch.empty_like(lse)
+        grads = [torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v)]
+        a = _packed_args(pack, 0 if causal else 2, q, k, v, causal, scale)
+        a.out, a.dout, a.do_row, a.do_head = out.data_ptr(), do.data_ptr(), do.stride(0), do.stride(1)
+        a.lse, a.delta = lse.data_ptr(), delta.data_ptr()
+        a.dq, a.dk, a.dv = (g.data_ptr() for g in grads)
+        bf16, stream = int(q.dtype == torch.bfloat16), L.raw_stream(q.device)
+        with torch.cuda.device(q.device):
+            L.check(so.mt_packed_attn_launch(ctypes.byref(a), 1, bf16, stream), "mt_packed_attn_launch(dq)")
+            _tile_list(a, pack, 1 if causal else 2)
+            L.check(so.mt_packed_attn_launch(ctypes.byref(a), 2, bf16, stream), "mt_packed_attn_launch(dk, dv)")
+        gq, gk, gv = (g if g.shape[2] == w else g[..., :w].contiguous() for g, w in zip(grads, (dk, dk, dv)))
+        return gq, gk, gv, None, None, None

@@ -1,0 +1,565 @@
+// Attention over packed sequences, forward and backward (gfx950): rows of q [T][heads][dk], k [T][kv_heads][dk] and
+// v [T][kv_heads][dv] hold sequences of different lengths one after the other; a query sees the keys of its own sequence,
+// all of them or (causal) those up to its own position; query head i reads key / value head i / (heads / kv_heads).
+//
+//   forward : s_ij = c q_i.k_j (c = scale log2 e),  p_ij = 2^(s_ij - L_i),  o_i = sum_j p_ij v_j,  L_i = log2 sum_j 2^s_ij
+//             one pass over the keys with the running maximum m_i and sum of a softmax; L_i is kept for the backward pass
+//   backward: D_i = do_i.o_i,  ds_ij = p_ij (do_i.v_j - D_i),
+//             dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij do_i
+//
+// A workgroup is four waves.  In the forward and the dq kernel a wave owns 32 queries and walks over the keys; in the dk / dv
+// kernel it owns 32 keys and walks over the queries of every head of the group, so each gradient element is summed by one
+// wave in a fixed order: no atomics, no workspace, and the gradients of shared heads need no second pass.  The price is that
+// the scores are computed again in both backward kernels (7 products where 5 are the least).
+//
+// Every product is v_mfma_*_32x32: the walked-over rows come from LDS as the first operand, the owned rows stay in registers
+// as the second, so an accumulator lane belongs to ONE owned row: row statistics are one register, a row maximum is a chain in
+// the lane and one exchange with lane ^ 32.  The accumulator of the scores then IS the second operand of the next product
+// (sum over the walked-over rows): lane half h holds rows 8 g + 4 h + 0..3 of each 32, and the transposed LDS read fetches the
+// other operand in that same order, so probabilities never move between lanes or through LDS.
+//
+// f32 operands use v_mfma_f32_32x32x2_f32 (exact f32 products) in the same layout: eight instructions where bf16 takes one.
+// Scores, statistics, gradients and all sums are f32 for both types; for bf16 p and ds are rounded to bf16 (at most
+// 2^-8 of the value) as operands of the second product, which is what the matrix instruction takes.
+#include "mt_common.h"
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(8))) float f32x8;
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+
+#define PA_THREADS 256
+#define PA_OWN 128          // rows a workgroup owns (32 per wave)
+
+// One tile of PA_OWN owned rows: rows [row0, row0 + len) are its sequence, `first` is the tile's first row in it.
+// len < 0: -len rows from row0 belong to no sequence and are filled with zeros.
+struct MtSeqItem {
+  int32_t row0, len, first, pad;
+};
+
+struct MtPackedAttn {
+  const void *q, *k, *v;        // inputs, element strides below; the last dimension is contiguous
+  const void *out, *dout;       // backward only: forward output (contiguous) and its gradient
+  void *o, *dq, *dk, *dv;       // outputs, contiguous [T][heads or kv_heads][dk or dv]
+  float *lse, *delta;           // [heads][rows]
+  const MtSeqItem* items;       // null: count sequences of uniform_len rows each
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, do_row, do_head;
+  int64_t rows;
+  int32_t n_items, uniform_len, count;
+  int32_t heads, kv_heads, head_k, head_v, causal;
+  float scale;
+  int32_t pad;
+};
+
+// ---- per-type pieces ----------------------------------------------------------------------------------------------------
+// A fragment is 8 elements per lane = 16 of the contraction (lane half h holds 8 of them) of row (lane & 31).
+template <typename T> struct PaFrag;
+template <> struct PaFrag<__bf16> { typedef bf16x8 type; };
+template <> struct PaFrag<float> { typedef f32x8 type; };
+
+__device__ __forceinline__ f32x16 pa_mma(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 pa_mma(f32x8 a, f32x8 b, f32x16 c) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+  return c;
+}
+
+// Accumulator rows 16 s .. 16 s + 15 (eight registers per lane) as a fragment of the next product.
+template <typename T> __device__ __forceinline__ typename PaFrag<T>::type pa_pack(const f32x16& a, int s);
+template <> __device__ __forceinline__ bf16x8 pa_pack<__bf16>(const f32x16& a, int s) {
+  const u32x4 w = {pack_bf16x2(a[8 * s], a[8 * s + 1]), pack_bf16x2(a[8 * s + 2], a[8 * s + 3]),
+                   pack_bf16x2(a[8 * s + 4], a[8 * s + 5]), pack_bf16x2(a[8 * s + 6], a[8 * s + 7])};
+  return __builtin_bit_cast(bf16x8, w);
+}
+template <> __device__ __forceinline__ f32x8 pa_pack<float>(const f32x16& a, int s) {
+  return f32x8{a[8 * s], a[8 * s + 1], a[8 * s + 2], a[8 * s + 3], a[8 * s + 4], a[8 * s + 5], a[8 * s + 6], a[8 * s + 7]};
+}
+
+// LDS image of rows of D elements: 16-byte chunk c of row r sits at chunk c ^ swz(r), so that eight rows read at one column
+// (row fragments) and four rows x 32 bytes (transposed reads) both cover all banks.
+template <typename T, int D> struct PaImg {
+  static constexpr int ROWB = D * (int)sizeof(T);
+  static constexpr int CHUNKS = ROWB / 16;
+  static constexpr int EPC = 16 / (int)sizeof(T);
+  static __device__ __forceinline__ int swz(int r) {
+    if (sizeof(T) == 4) return r & 7;
+    if (D == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
+    if (D == 64) return ((r & 3) << 1) | ((r >> 2) & 1);
+    return (((r >> 1) & 1) << 1) | ((r >> 2) & 1);
+  }
+  static __device__ __forceinline__ int at(int r, int chunk) { return r * ROWB + ((chunk ^ swz(r)) << 4); }
+
+  // 16 columns 16 s + 8 h + j of row row0 + (lane & 31)
+  static __device__ __forceinline__ typename PaFrag<T>::type rows(const uint8_t* img, int row0, int s, int lane) {
+    const int r = row0 + (lane & 31), h = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      return __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(img + at(r, 2 * s + h)));
+    } else {
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(img + at(r, 4 * s + 2 * h));
+      const f32x4 hi = *reinterpret_cast<const f32x4*>(img + at(r, 4 * s + 2 * h + 1));
+      return f32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    }
+  }
+  // column col0 + (lane & 31) of the 16 rows row0 + 8 (j / 4) + 4 h + j % 4: the order of an accumulator's rows
+  static __device__ __forceinline__ typename PaFrag<T>::type cols(const uint8_t* img, int row0, int col0, int lane) {
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      const int i = lane & 15, q = i >> 2, p = i & 3;
+      const int c = (col0 + (lane & 16)) / 8 + (p >> 1);
+      const int r = row0 + 4 * h + q;
+      const lds_u8* a0 = (const lds_u8*)(img + at(r, c) + 8 * (p & 1));
+      const lds_u8* a1 = (const lds_u8*)(img + at(r + 8, c) + 8 * (p & 1));
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a0);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a1);
+      typedef __attribute__((ext_vector_type(8))) short s16x8;
+      const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      return __builtin_bit_cast(bf16x8, v);
+    } else {
+      const int col = col0 + (lane & 31);
+      f32x8 v;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int r = row0 + 8 * (j >> 2) + 4 * h + (j & 3);
+        v[j] = *reinterpret_cast<const float*>(img + at(r, col >> 2) + 4 * (col & 3));
+      }
+      return v;
+    }
+  }
+  // LDS-DMA of NROWS rows of `d` valid columns into an image, four waves sharing the 1-KiB pieces.  `base` is the first row's
+  // first element; rows at and past `valid` and columns past `d` arrive as zeros through the buffer's range check.
+  template <int NROWS>
+  static __device__ __forceinline__ void stage(uint8_t* img, const T* base, int64_t row_stride, int valid, int d, int wave, int lane) {
+    constexpr int PIECES = NROWS * ROWB / 1024;
+    const int64_t stride = row_stride * (int64_t)sizeof(T);
+    const int rows = valid < NROWS ? valid : NROWS;
+    const uint32_t bytes = rows > 0 ? (uint32_t)((rows - 1) * stride + d * (int)sizeof(T)) : 0u;
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, bytes, 0x00027000);
+#pragma unroll
+    for (int t = 0; t < PIECES / 4; ++t) {
+      const int j = wave * (PIECES / 4) + t;
+      const int at_byte = j * 1024 + lane * 16;
+      const int r = at_byte / ROWB, c = ((at_byte % ROWB) >> 4) ^ swz(r);
+      const uint32_t off = c * EPC < d ? (uint32_t)(r * (uint32_t)stride + c * 16) : 0xFFFFFF00u;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(img + j * 1024), 16, off, 0, 0, 0);
+    }
+  }
+};
+
+__device__ __forceinline__ float pa_other_half(float v) { return __shfl_xor(v, 32, 64); }
+
+template <typename T> __device__ __forceinline__ typename PaFrag<T>::type pa_zero_frag() {
+  typename PaFrag<T>::type f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = (T)0.f;
+  return f;
+}
+// An owned row as fragments: columns 16 s + 8 h + j, zeros past d or when the row is outside its sequence.
+template <typename T, int D>
+__device__ __forceinline__ void pa_own_row(typename PaFrag<T>::type (&f)[D / 16], const T* row, bool ok, int d, int lane) {
+  const int h = lane >> 5;
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) {
+    f[s] = pa_zero_frag<T>();
+    const int c = 16 * s + 8 * h;
+    if constexpr (sizeof(T) == 2) {
+      if (ok && c < d) f[s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(row + c));
+    } else {
+      f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+      if (ok && c < d) lo = *reinterpret_cast<const f32x4*>(row + c);
+      if (ok && c + 4 < d) hi = *reinterpret_cast<const f32x4*>(row + c + 4);
+      f[s] = f32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    }
+  }
+}
+// Store a transposed accumulator (rows = columns of the output, lane & 31 = owned row): four consecutive columns at a time.
+template <typename T, int D>
+__device__ __forceinline__ void pa_store_row(T* row, const f32x16 (&acc)[D / 32], float factor, int d, int lane) {
+  const int h = lane >> 5;
+#pragma unroll
+  for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 32 * b + 8 * g + 4 * h;
+      if (c < d) {
+        const float v0 = acc[b][4 * g] * factor, v1 = acc[b][4 * g + 1] * factor, v2 = acc[b][4 * g + 2] * factor,
+                    v3 = acc[b][4 * g + 3] * factor;
+        if constexpr (sizeof(T) == 2) {
+          const u32x2 w = {pack_bf16x2(v0, v1), pack_bf16x2(v2, v3)};
+          *reinterpret_cast<u32x2*>(row + c) = w;
+        } else {
+          *reinterpret_cast<f32x4*>(row + c) = f32x4{v0, v1, v2, v3};
+        }
+      }
+    }
+}
+template <int N> __device__ __forceinline__ void pa_clear(f32x16 (&a)[N]) {
+#pragma unroll
+  for (int b = 0; b < N; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) a[b][i] = 0.f;
+}
+
+// Which tile this workgroup takes.  Tiles come longest first (causal: the last queries, or the first keys).
+__device__ __forceinline__ MtSeqItem pa_item(const MtPackedAttn& p, int i, bool last_first) {
+  if (p.items != nullptr) return p.items[i];
+  const int tiles = (p.uniform_len + PA_OWN - 1) / PA_OWN;
+  const int t = i / p.count, seq = i - t * p.count;
+  return MtSeqItem{seq * p.uniform_len, p.uniform_len, (last_first ? tiles - 1 - t : t) * PA_OWN, 0};
+}
+// Zeros for `n` rows of `d` columns of one head, which belong to no sequence.
+template <typename T>
+__device__ __forceinline__ void pa_zero_rows(T* base, int64_t row_stride, int n, int d) {
+  for (int i = threadIdx.x; i < n * d; i += PA_THREADS) {
+    const int r = i / d;
+    base[r * row_stride + (i - r * d)] = (T)0.f;
+  }
+}
+// This wave's LDS-DMA has landed and its reads of the other stage are back; past the barrier that holds for everybody.
+__device__ __forceinline__ void pa_tile_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// ---- forward ------------------------------------------------------------------------------------------------------------
+template <typename T, int D, int BN>
+__global__ __launch_bounds__(PA_THREADS, 2) void mt_pattn_fwd_kernel(const MtPackedAttn p) {
+  typedef PaImg<T, D> Img;
+  typedef typename PaFrag<T>::type Frag;
+  constexpr int IMG = BN * Img::ROWB;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * IMG];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int it = blockIdx.x / p.heads, r = blockIdx.x - it * p.heads;
+  // heads of one group are kv_heads workgroups apart: the XCDs (workgroup number mod 8) then share few key / value heads each
+  const int kvh = r % p.kv_heads, head = kvh * (p.heads / p.kv_heads) + r / p.kv_heads;
+  const MtSeqItem item = pa_item(p, it, p.causal);
+  const int64_t o_row = (int64_t)p.heads * p.head_v;
+  T* o = reinterpret_cast<T*>(p.o) + item.row0 * o_row + (int64_t)head * p.head_v;
+  if (item.len <= 0) {
+    pa_zero_rows<T>(o, o_row, -item.len, p.head_v);
+    return;
+  }
+  const int first = item.first + wave * 32, mine = first + (lane & 31);
+  Frag qf[D / 16];
+  pa_own_row<T, D>(qf, reinterpret_cast<const T*>(p.q) + (item.row0 + (int64_t)mine) * p.q_row + (int64_t)head * p.q_head,
+                   mine < item.len, p.head_k, lane);
+  const T* kb = reinterpret_cast<const T*>(p.k) + item.row0 * p.k_row + (int64_t)kvh * p.k_head;
+  const T* vb = reinterpret_cast<const T*>(p.v) + item.row0 * p.v_row + (int64_t)kvh * p.v_head;
+  const int keys = p.causal && item.first + PA_OWN < item.len ? item.first + PA_OWN : item.len;
+  const int tiles = (keys + BN - 1) / BN;
+  const float c = p.scale * 1.4426950408889634f;
+
+  auto issue = [&](int t) {
+    uint8_t* st = lds + (t & 1) * 2 * IMG;
+    const int64_t k0 = (int64_t)t * BN;
+    Img::template stage<BN>(st, kb + k0 * p.k_row, p.k_row, item.len - t * BN, p.head_k, wave, lane);
+    Img::template stage<BN>(st + IMG, vb + k0 * p.v_row, p.v_row, item.len - t * BN, p.head_v, wave, lane);
+  };
+
+  f32x16 acc[D / 32];
+  pa_clear(acc);
+  float m = -INFINITY, sum = 0.f;
+  issue(0);
+  for (int t = 0; t < tiles; ++t) {
+    pa_tile_barrier();
+    if (t + 1 < tiles) issue(t + 1);
+    const int k0 = t * BN;
+    if (p.causal && k0 > first + 31) continue;          // none of this wave's queries sees the tile (uniform; still at the barriers)
+    const uint8_t* kimg = lds + (t & 1) * 2 * IMG;
+    const uint8_t* vimg = kimg + IMG;
+    f32x16 s[BN / 32];
+    pa_clear(s);
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+      for (int u = 0; u < BN / 32; ++u) s[u] = pa_mma(Img::rows(kimg, 32 * u, ks, lane), qf[ks], s[u]);
+    if (k0 + BN > item.len || (p.causal && k0 + BN - 1 > first)) {
+      const int last = p.causal && mine < item.len ? mine : item.len - 1;
+#pragma unroll
+      for (int u = 0; u < BN / 32; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          s[u][i] = k0 + 32 * u + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3) <= last ? s[u][i] : -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int u = 0; u < BN / 32; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
+    mx = fmaxf(mx, pa_other_half(mx)) * c;
+    // The subtracted maximum is only moved when some row grew by more than 2^8 over it: probabilities stay within f32 (and
+    // bf16 keeps its relative precision), and most tiles skip the pass over the accumulator.
+    if (__any(mx > m + 8.f)) {
+      const float mn = fmaxf(m, mx);
+      const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      sum *= f;
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[b][i] *= f;
+    }
+    const float sub = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int u = 0; u < BN / 32; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], c, -sub));
+        sum += s[u][i];
+      }
+#pragma unroll
+    for (int u = 0; u < BN / 32; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const Frag pf = pa_pack<T>(s[u], h);
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) acc[b] = pa_mma(Img::cols(vimg, 32 * u + 16 * h, 32 * b, lane), pf, acc[b]);
+      }
+  }
+  sum += pa_other_half(sum);
+  if (mine < item.len) {
+    pa_store_row<T, D>(o + (int64_t)mine * o_row, acc, sum > 0.f || sum != sum ? 1.f / sum : 0.f, p.head_v, lane);
+    if (p.lse != nullptr && lane < 32)      // a row whose scores are all -inf weighs nothing in the backward pass
+      p.lse[(int64_t)head * p.rows + item.row0 + mine] = sum > 0.f || sum != sum ? m + __builtin_amdgcn_logf(sum) : INFINITY;
+  }
+}
+
+// ---- backward: dq (and D = do . o, which the dk / dv kernel reads) --------------------------------------------------------
+template <typename T, int D, int BN>
+__global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) void mt_pattn_dq_kernel(const MtPackedAttn p) {
+  typedef PaImg<T, D> Img;
+  typedef typename PaFrag<T>::type Frag;
+  constexpr int IMG = BN * Img::ROWB;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * IMG];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int it = blockIdx.x / p.heads, r = blockIdx.x - it * p.heads;
+  const int kvh = r % p.kv_heads, head = kvh * (p.heads / p.kv_heads) + r / p.kv_heads;
+  const MtSeqItem item = pa_item(p, it, p.causal);
+  const int64_t dq_row = (int64_t)p.heads * p.head_k;
+  T* dq = reinterpret_cast<T*>(p.dq) + item.row0 * dq_row + (int64_t)head * p.head_k;
+  if (item.len <= 0) {
+    pa_zero_rows<T>(dq, dq_row, -item.len, p.head_k);
+    return;
+  }
+  const int first = item.first + wave * 32, mine = first + (lane & 31);
+  const bool ok = mine < item.len;
+  const int64_t row = item.row0 + (int64_t)mine;
+  Frag qf[D / 16], df[D / 16];
+  float delta = 0.f, lse = INFINITY;                    // rows outside the sequence: p = 2^(s - inf) = 0
+  {
+    pa_own_row<T, D>(df, reinterpret_cast<const T*>(p.dout) + row * p.do_row + (int64_t)head * p.do_head, ok, p.head_v, lane);
+    pa_own_row<T, D>(qf, reinterpret_cast<const T*>(p.out) + row * ((int64_t)p.heads * p.head_v) + (int64_t)head * p.head_v, ok,
+                     p.head_v, lane);
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta = __builtin_fmaf((float)df[s][j], (float)qf[s][j], delta);
+    delta += pa_other_half(delta);
+    if (ok) {
+      lse = p.lse[(int64_t)head * p.rows + row];
+      if (lane < 32) p.delta[(int64_t)head * p.rows + row] = delta;
+    }
+    pa_own_row<T, D>(qf, reinterpret_cast<const T*>(p.q) + row * p.q_row + (int64_t)head * p.q_head, ok, p.head_k, lane);
+  }
+  const T* kb = reinterpret_cast<const T*>(p.k) + item.row0 * p.k_row + (int64_t)kvh * p.k_head;
+  const T* vb = reinterpret_cast<const T*>(p.v) + item.row0 * p.v_row + (int64_t)kvh * p.v_head;
+  const int keys = p.causal && item.first + PA_OWN < item.len ? item.first + PA_OWN : item.len;
+  const int tiles = (keys + BN - 1) / BN;
+  const float c = p.scale * 1.4426950408889634f;
+  auto issue = [&](int t) {
+    uint8_t* st = lds + (t & 1) * 2 * IMG;
+    const int64_t k0 = (int64_t)t * BN;
+    Img::template stage<BN>(st, kb + k0 * p.k_row, p.k_row, item.len - t * BN, p.head_k, wave, lane);
+    Img::template stage<BN>(st + IMG, vb + k0 * p.v_row, p.v_row, item.len - t * BN, p.head_v, wave, lane);
+  };
+  f32x16 acc[D / 32];
+  pa_clear(acc);
+  issue(0);
+  for (int t = 0; t < tiles; ++t) {
+    pa_tile_barrier();
+    if (t + 1 < tiles) issue(t + 1);
+    const int k0 = t * BN;
+    if (p.causal && k0 > first + 31) continue;
+    const uint8_t* kimg = lds + (t & 1) * 2 * IMG;
+    const uint8_t* vimg = kimg + IMG;
+    const bool masked = k0 + BN > item.len || (p.causal && k0 + BN - 1 > first);
+    const int last = p.causal && ok ? mine : item.len - 1;
+#pragma unroll
+    for (int u = 0; u < BN / 32; ++u) {
+      f32x16 s[1], d[1];
+      pa_clear(s);
+      pa_clear(d);
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) s[0] = pa_mma(Img::rows(kimg, 32 * u, ks, lane), qf[ks], s[0]);
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) d[0] = pa_mma(Img::rows(vimg, 32 * u, ks, lane), df[ks], d[0]);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        s[0][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][i], c, -lse)) * (d[0][i] - delta);
+      if (masked) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[0][i] = k0 + 32 * u + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3) <= last ? s[0][i] : 0.f;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const Frag sf = pa_pack<T>(s[0], h);
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) acc[b] = pa_mma(Img::cols(kimg, 32 * u + 16 * h, 32 * b, lane), sf, acc[b]);
+      }
+    }
+  }
+  if (ok) pa_store_row<T, D>(dq + (int64_t)mine * dq_row, acc, p.scale, p.head_k, lane);
+}
+
+// ---- backward: dk and dv ------------------------------------------------------------------------------------------------
+template <typename T, int D, int BQ>
+__global__ __launch_bounds__(PA_THREADS, 1) void mt_pattn_dkv_kernel(const MtPackedAttn p) {
+  typedef PaImg<T, D> Img;
+  typedef typename PaFrag<T>::type Frag;
+  constexpr int IMG = BQ * Img::ROWB;
+  constexpr int STAGE = 2 * IMG + 2 * 256;                          // q rows, do rows, L and D of up to 64 rows
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int it = blockIdx.x / p.kv_heads, kvh = blockIdx.x - it * p.kv_heads;
+  const int group = p.heads / p.kv_heads;
+  const MtSeqItem item = pa_item(p, it, false);
+  const int64_t dk_row = (int64_t)p.kv_heads * p.head_k, dv_row = (int64_t)p.kv_heads * p.head_v;
+  T* dk = reinterpret_cast<T*>(p.dk) + item.row0 * dk_row + (int64_t)kvh * p.head_k;
+  T* dv = reinterpret_cast<T*>(p.dv) + item.row0 * dv_row + (int64_t)kvh * p.head_v;
+  if (item.len <= 0) {
+    pa_zero_rows<T>(dk, dk_row, -item.len, p.head_k);
+    pa_zero_rows<T>(dv, dv_row, -item.len, p.head_v);
+    return;
+  }
+  const int first = item.first + wave * 32, mine = first + (lane & 31);
+  const bool ok = mine < item.len;
+  const int64_t row = item.row0 + (int64_t)mine;
+  Frag kf[D / 16], vf[D / 16];
+  pa_own_row<T, D>(kf, reinterpret_cast<const T*>(p.k) + row * p.k_row + (int64_t)kvh * p.k_head, ok, p.head_k, lane);
+  pa_own_row<T, D>(vf, reinterpret_cast<const T*>(p.v) + row * p.v_row + (int64_t)kvh * p.v_head, ok, p.head_v, lane);
+  const int q_lo = p.causal ? item.first / BQ : 0;                  // first query tile that sees a key of this workgroup
+  const int per_head = (item.len + BQ - 1) / BQ - q_lo;
+  const int tiles = per_head * group;
+  const float c = p.scale * 1.4426950408889634f;
+  auto issue = [&](int n, int hg, int qt) {
+    uint8_t* st = lds + (n & 1) * STAGE;
+    const int head = kvh * group + hg, q0 = qt * BQ, left = item.len - q0;
+    const int64_t r0 = item.row0 + (int64_t)q0;
+    Img::template stage<BQ>(st, reinterpret_cast<const T*>(p.q) + r0 * p.q_row + (int64_t)head * p.q_head, p.q_row, left, p.head_k,
+                            wave, lane);
+    Img::template stage<BQ>(st + IMG, reinterpret_cast<const T*>(p.dout) + r0 * p.do_row + (int64_t)head * p.do_head, p.do_row,
+                            left, p.head_v, wave, lane);
+    if (wave < 2) {
+      const float* src = (wave == 0 ? p.lse : p.delta) + (int64_t)head * p.rows + r0;
+      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<float*>(src), 0, (uint32_t)(left < BQ ? left : BQ) * 4u, 0x00027000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(st + 2 * IMG + wave * 256), 4,
+                                               lane * 4, 0, 0, 0);
+    }
+  };
+  f32x16 ak[D / 32], av[D / 32];
+  pa_clear(ak);
+  pa_clear(av);
+  issue(0, 0, q_lo);
+  int hg = 0, qt = q_lo;
+  for (int n = 0; n < tiles; ++n) {
+    const int q0 = qt * BQ;
+    if (++qt == q_lo + per_head) { qt = q_lo; ++hg; }
+    pa_tile_barrier();
+    if (n + 1 < tiles) issue(n + 1, hg, qt);
+    const uint8_t* qimg = lds + (n & 1) * STAGE;
+    const uint8_t* dimg = qimg + IMG;
+    const float* stat = reinterpret_cast<const float*>(qimg + 2 * IMG);
+#pragma unroll
+    for (int u = 0; u < BQ / 32; ++u) {
+      const int qu = q0 + 32 * u;
+      if (qu >= item.len || (p.causal && qu + 31 < first)) continue;
+      f32x16 s[1], d[1];
+      pa_clear(s);
+      pa_clear(d);
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) s[0] = pa_mma(Img::rows(qimg, 32 * u, ks, lane), kf[ks], s[0]);
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) d[0] = pa_mma(Img::rows(dimg, 32 * u, ks, lane), vf[ks], d[0]);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int at = 32 * u + 8 * g + 4 * (lane >> 5);
+        const f32x4 lse = *reinterpret_cast<const f32x4*>(stat + at), delta = *reinterpret_cast<const f32x4*>(stat + 64 + at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][4 * g + e], c, -lse[e]));
+          s[0][4 * g + e] = pr;
+          d[0][4 * g + e] = pr * (d[0][4 * g + e] - delta[e]);
+        }
+      }
+      if (qu + 32 > item.len || (p.causal && qu < first + 31)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int qi = qu + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
+          const bool see = qi < item.len && (!p.causal || mine <= qi);
+          s[0][i] = see ? s[0][i] : 0.f;
+          d[0][i] = see ? d[0][i] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const Frag pf = pa_pack<T>(s[0], h), sf = pa_pack<T>(d[0], h);
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) av[b] = pa_mma(Img::cols(dimg, 32 * u + 16 * h, 32 * b, lane), pf, av[b]);
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) ak[b] = pa_mma(Img::cols(qimg, 32 * u + 16 * h, 32 * b, lane), sf, ak[b]);
+      }
+    }
+  }
+  if (ok) {
+    pa_store_row<T, D>(dk + (int64_t)mine * dk_row, ak, p.scale, p.head_k, lane);
+    pa_store_row<T, D>(dv + (int64_t)mine * dv_row, av, 1.f, p.head_v, lane);
+  }
+}
+
+// ---- launchers ----------------------------------------------------------------------------------------------------------
+template <typename T, int D>
+static int pa_launch(const MtPackedAttn& p, int pass, hipStream_t stream) {
+  constexpr int BN = sizeof(T) == 2 ? 64 : 32;
+  if (pass == 0)
+    hipLaunchKernelGGL((mt_pattn_fwd_kernel<T, D, BN>), dim3(p.n_items * p.heads), dim3(PA_THREADS), 0, stream, p);
+  else if (pass == 1)
+    hipLaunchKernelGGL((mt_pattn_dq_kernel<T, D, BN>), dim3(p.n_items * p.heads), dim3(PA_THREADS), 0, stream, p);
+  else
+    hipLaunchKernelGGL((mt_pattn_dkv_kernel<T, D, BN>), dim3(p.n_items * p.kv_heads), dim3(PA_THREADS), 0, stream, p);
+  return (int)hipGetLastError();
+}
+
+extern "C" int mt_packed_attn_sizes(int* item_bytes, int* tile_rows) {
+  *item_bytes = (int)sizeof(MtSeqItem);
+  *tile_rows = PA_OWN;
+  return (int)sizeof(MtPackedAttn);
+}
+
+// pass: 0 forward, 1 dq + D, 2 dk + dv.  bf16: 0 = f32 operands, 1 = bf16.  Rows are read in 16-byte pieces.
+extern "C" int mt_packed_attn_launch(const MtPackedAttn* a, int pass, int bf16, hipStream_t stream) {
+  if (a == nullptr || pass < 0 || pass > 2) return -2;
+  const MtPackedAttn p = *a;
+  if (p.n_items <= 0) return 0;
+  const int es = bf16 ? 2 : 4, per = 16 / es;
+  const int widest = p.head_k > p.head_v ? p.head_k : p.head_v;
+  if (p.head_k < 1 || p.head_v < 1 || widest > 128 || p.head_k % per || p.head_v % per) return -2;
+  if (p.heads < 1 || p.kv_heads < 1 || p.heads % p.kv_heads) return -2;
+  if ((p.items == nullptr) && (p.uniform_len < 1 || p.count < 1)) return -2;
+  if ((int64_t)p.n_items * p.heads > 0x7FFFFFFF || !(p.scale > 0.f)) return -2;
+  const int64_t strides[8] = {p.q_row, p.q_head, p.k_row, p.k_head, p.v_row, p.v_head, p.do_row, p.do_head};
+  for (int i = 0; i < 8; ++i)      // 32-bit byte offsets inside a staged tile of at most 64 rows
+    if (strides[i] < 0 || strides[i] % per || strides[i] * es > (1 << 24)) return -2;
+  const void* ptrs[9] = {p.q, p.k, p.v, p.out, p.dout, p.o, p.dq, p.dk, p.dv};
+  for (int i = 0; i < 9; ++i)
+    if (reinterpret_cast<uintptr_t>(ptrs[i]) & 15) return -2;
+  if (bf16) {
+    if (widest <= 32) return pa_launch<__bf16, 32>(p, pass, stream);
+    if (widest <= 64) return pa_launch<__bf16, 64>(p, pass, stream);
+    return pa_launch<__bf16, 128>(p, pass, stream);
+  }
+  if (widest <= 32) return pa_launch<float, 32>(p, pass, stream);
+  if (widest <= 64) return pa_launch<float, 64>(p, pass, stream);
+  return pa_launch<float, 128>(p, pass, stream);
+}

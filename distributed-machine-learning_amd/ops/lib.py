@@ -16,6 +16,7 @@ import numpy as np
 from . import build as _build
 
 MT_MAX_LAYERS = 8
+PACKED_TILE_ROWS, PACKED_ITEM_BYTES = 128, 16      # csrc/packed_attention.hip: rows of a tile, bytes of a tile list entry
 
 c_void_p, c_int32, c_uint32, c_float, c_size_t = C.c_void_p, C.c_int32, C.c_uint32, C.c_float, C.c_size_t
 
@@ -50,6 +51,17 @@ class OptSlot(C.Structure):
                 ("opt_type", c_int32), ("warmup", c_int32), ("total", c_int32), ("n_params", c_int32),
                 ("active_steps", c_int32), ("step_base", c_int32), ("first_end", c_int32),
                 ("first_splits", c_int32), ("pad", c_int32)]
+
+
+class PackedAttn(C.Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p), ("dout", c_void_p),
+                ("o", c_void_p), ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p),
+                ("lse", c_void_p), ("delta", c_void_p), ("items", c_void_p),
+                ("q_row", C.c_int64), ("q_head", C.c_int64), ("k_row", C.c_int64), ("k_head", C.c_int64),
+                ("v_row", C.c_int64), ("v_head", C.c_int64), ("do_row", C.c_int64), ("do_head", C.c_int64),
+                ("rows", C.c_int64), ("n_items", c_int32), ("uniform_len", c_int32), ("count", c_int32),
+                ("heads", c_int32), ("kv_heads", c_int32), ("head_k", c_int32), ("head_v", c_int32),
+                ("causal", c_int32), ("scale", c_float), ("pad", c_int32)]
 
 
 class MlpPlan(C.Structure):
@@ -211,6 +223,13 @@ def load(build_if_missing: bool = True) -> C.CDLL:
     lib.mt_attn_fwd_strided_launch.restype = lib.mt_attn_bwd_strided_launch.restype = C.c_int
     lib.mt_attn_exact_level.argtypes = [C.c_int]
     lib.mt_attn_exact_level.restype = C.c_int
+    item_bytes, tile_rows = C.c_int(), C.c_int()
+    if lib.mt_packed_attn_sizes(C.byref(item_bytes), C.byref(tile_rows)) != C.sizeof(PackedAttn):
+        raise KernelLibraryError("MtPackedAttn layout mismatch between lib.py and the library")
+    if (item_bytes.value, tile_rows.value) != (PACKED_ITEM_BYTES, PACKED_TILE_ROWS):
+        raise KernelLibraryError("packed attention: tile list layout mismatch between lib.py and the library")
+    lib.mt_packed_attn_launch.argtypes = [C.POINTER(PackedAttn), C.c_int, C.c_int, c_void_p]
+    lib.mt_packed_attn_launch.restype = C.c_int
     lib.mt_ln_fwd_launch.argtypes = [c_void_p] * 8 + [C.c_int, C.c_int, c_float, c_float, c_void_p, c_float, c_void_p]
     lib.mt_ln_bwd_launch.argtypes = [c_void_p] * 8 + [C.c_int, C.c_int, c_float, c_void_p, c_float, c_void_p]
     lib.mt_ln_bwd_blocks.argtypes = [C.c_int]
