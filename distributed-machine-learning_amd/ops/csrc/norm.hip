@@ -1,0 +1,476 @@
+// Layer norm over rows of any width, forward and backward (gfx950, f32 or bf16 rows, f32 statistics).
+//
+//   forward : y = (x - mean) rstd w + b,  rstd = 1 / sqrt(var + eps); {mean, rstd} kept per row for the backward pass
+//   backward: with u = (x - mean) rstd and g = dy w:  dx = rstd (g - mean(g) - u mean(g u)),
+//             dw = sum over rows of dy u,  db = sum over rows of dy
+//
+// Both directions move each element once (forward 2, backward 3 tensors) and are bound by memory.  TPR threads share a row and
+// keep it in registers (NV 16-byte vectors each): the variance is the mean of the centred squares, not a difference of sums, at
+// no further read.  A row group walks over rows a grid apart with w and b in registers and the next row's loads issued before
+// the current row's reductions, so the loads of two rows are always in flight.  The column sums of the backward pass stay in
+// the same threads' registers over all their rows; a workgroup writes one partial row of each, and a second launch adds the
+// partial rows in order: no atomics, the same bits every time.
+//
+// TPR is 16 or 64 (a part of a wave, or a wave: rows reduce by lane exchanges alone), 256 or 1024 (through LDS, one barrier per
+// reduction, alternating buffers).  Rows wider than the registers of 1024 threads are read again for each pass.
+// Vectors are loaded at whatever alignment the row has (global memory takes dwordx4 at any address); the last, partial vector
+// of an odd row is read and written by elements.
+#include "mt_common.h"
+
+template <typename T> struct NormVec;
+template <> struct NormVec<float> {
+  static constexpr int N = 4;
+  typedef float type __attribute__((ext_vector_type(4), aligned(4)));
+};
+template <> struct NormVec<__bf16> {
+  static constexpr int N = 8;
+  typedef __bf16 type __attribute__((ext_vector_type(8), aligned(2)));
+};
+// N = columns per vector of the ROW type; parameters of another type load as many columns.
+template <typename T, int N> struct NormPack { T v[N]; };
+
+template <typename T, int N>
+__device__ __forceinline__ void norm_load(NormPack<T, N>& o, const T* __restrict__ p, int col, int d) {
+  if (col + N <= d) {
+    __builtin_memcpy(&o, p + col, sizeof(o));
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) o.v[e] = col + e < d ? p[col + e] : (T)0.f;
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void norm_store(T* __restrict__ p, const NormPack<T, N>& o, int col, int d) {
+  if (col + N <= d) {
+    __builtin_memcpy(p + col, &o, sizeof(o));
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (col + e < d) p[col + e] = o.v[e];
+  }
+}
+
+// Sum of K values over the TPR threads of a row.  TPR > 64: `red` holds 2 x K x 16 floats, `turn` alternates the halves so that
+// one barrier per call is enough.
+template <int TPR, int K>
+__device__ __forceinline__ void norm_sum(float (&v)[K], float* red, int& turn) {
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) v[k] += __shfl_xor(v[k], o, 64);
+  if constexpr (TPR > 64) {
+    float* buf = red + (turn & 1) * 32;
+    ++turn;
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) buf[k * 16 + wave] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < TPR / 64; ++w) s += buf[k * 16 + w];
+      v[k] = s;
+    }
+  }
+}
+
+template <typename T, typename P, int TPR, int NV>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void mt_norm_fwd_kernel(const T* __restrict__ x, const P* __restrict__ w,
+                                                                            const P* __restrict__ b, T* __restrict__ y,
+                                                                            float* __restrict__ stats, int64_t rows,
+                                                                            int64_t stride, int d, float eps) {
+  constexpr int N = NormVec<T>::N;
+  __shared__ float red[64];
+  const int groups = blockDim.x / TPR, lane = threadIdx.x & (TPR - 1);
+  const int64_t step = (int64_t)gridDim.x * groups;
+  int64_t row = (int64_t)blockIdx.x * groups + threadIdx.x / TPR;
+  if (row >= rows) return;                       // whole groups only; a workgroup of one group always has its row
+  int turn = 0;
+  NormPack<P, N> wv[NV], bv[NV];
+  NormPack<T, N> cur[NV], nxt[NV];
+#pragma unroll
+  for (int t = 0; t < NV; ++t) {
+    const int col = (t * TPR + lane) * N;
+    if (col >= d) continue;
+    norm_load(cur[t], x + row * stride, col, d);
+    if (w != nullptr) norm_load(wv[t], w, col, d);
+    if (b != nullptr) norm_load(bv[t], b, col, d);
+  }
+  const float inv = 1.f / (float)d;
+  for (; row < rows; row += step) {
+    if (row + step < rows) {
+#pragma unroll
+      for (int t = 0; t < NV; ++t) {
+        const int col = (t * TPR + lane) * N;
+        if (col < d) norm_load(nxt[t], x + (row + step) * stride, col, d);
+      }
+    }
+    float s[1] = {0.f};
+#pragma unroll
+    for (int t = 0; t < NV; ++t) {
+      if ((t * TPR + lane) * N >= d) continue;
+#pragma unroll
+      for (int e = 0; e < N; ++e) s[0] += (float)cur[t].v[e];          // columns past d were loaded as zeros
+    }
+    norm_sum<TPR>(s, red, turn);
+    const float mean = s[0] * inv;
+    s[0] = 0.f;
+#pragma unroll
+    for (int t = 0; t < NV; ++t) {
+      const int col = (t * TPR + lane) * N;
+      if (col >= d) continue;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float c = col + e < d ? (float)cur[t].v[e] - mean : 0.f;
+        s[0] = __builtin_fmaf(c, c, s[0]);
+      }
+    }
+    norm_sum<TPR>(s, red, turn);
+    const float rstd = 1.f / sqrtf(s[0] * inv + eps);
+#pragma unroll
+    for (int t = 0; t < NV; ++t) {
+      const int col = (t * TPR + lane) * N;
+      if (col >= d) continue;
+      NormPack<T, N> o;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        float v = ((float)cur[t].v[e] - mean) * rstd;
+        if (w != nullptr) v *= (float)wv[t].v[e];
+        if (b != nullptr) v += (float)bv[t].v[e];
+        o.v[e] = (T)v;
+      }
+      norm_store(y + row * d, o, col, d);
+      cur[t] = nxt[t];
+    }
+    if (stats != nullptr && lane == 0) {
+      stats[2 * row] = mean;
+      stats[2 * row + 1] = rstd;
+    }
+  }
+}
+
+// part: [workgroups][2][d] partial sums of dw and db (null: not wanted)
+template <typename T, typename P, int TPR, int NV>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void mt_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
+                                                                            const P* __restrict__ w,
+                                                                            const float* __restrict__ stats, T* __restrict__ dx,
+                                                                            float* __restrict__ part, int64_t rows,
+                                                                            int64_t stride, int64_t dy_stride, int d) {
+  constexpr int N = NormVec<T>::N;
+  __shared__ float red[64];
+  __shared__ float cols[TPR <= 64 ? 2 * TPR * NV * N : 1];
+  const int groups = blockDim.x / TPR, lane = threadIdx.x & (TPR - 1), mine = threadIdx.x / TPR;
+  const int64_t step = (int64_t)gridDim.x * groups;
+  int64_t row = (int64_t)blockIdx.x * groups + mine;
+  int turn = 0;
+  NormPack<P, N> wv[NV];
+  NormPack<T, N> cx[NV], cd[NV], nx[NV], nd[NV];
+  float aw[NV][N], ab[NV][N];
+#pragma unroll
+  for (int t = 0; t < NV; ++t) {
+    const int col = (t * TPR + lane) * N;
+#pragma unroll
+    for (int e = 0; e < N; ++e) aw[t][e] = ab[t][e] = 0.f;
+    if (col >= d) continue;
+    if (w != nullptr) norm_load(wv[t], w, col, d);
+    if (row < rows) {
+      norm_load(cx[t], x + row * stride, col, d);
+      norm_load(cd[t], dy + row * dy_stride, col, d);
+    }
+  }
+  const float inv = 1.f / (float)d;
+  for (; row < rows; row += step) {
+    const float mean = stats[2 * row], rstd = stats[2 * row + 1];
+    if (row + step < rows) {
+#pragma unroll
+      for (int t = 0; t < NV; ++t) {
+        const int col = (t * TPR + lane) * N;
+        if (col >= d) continue;
+        norm_load(nx[t], x + (row + step) * stride, col, d);
+        norm_load(nd[t], dy + (row + step) * dy_stride, col, d);
+      }
+    }
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < NV; ++t) {
+      const int col = (t * TPR + lane) * N;
+      if (col >= d) continue;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float g0 = (float)cd[t].v[e], u = ((float)cx[t].v[e] - mean) * rstd;
+        const float g = w != nullptr ? g0 * (float)wv[t].v[e] : g0;    // columns past d: dy was loaded as zero
+        s[0] += g;
+        s[1] = __builtin_fmaf(g, u, s[1]);
+        ab[t][e] += g0;
+        aw[t][e] = __builtin_fmaf(g0, u, aw[t][e]);
+      }
+    }
+    norm_sum<TPR>(s, red, turn);
+    const float mg = s[0] * inv, mu = s[1] * inv;
+#pragma unroll
+    for (int t = 0; t < NV; ++t) {
+      const int col = (t * TPR + lane) * N;
+      if (col >= d) continue;
+      NormPack<T, N> o;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float g0 = (float)cd[t].v[e], u = ((float)cx[t].v[e] - mean) * rstd;
+        const float g = w != nullptr ? g0 * (float)wv[t].v[e] : g0;
+        o.v[e] = (T)(rstd * (g - mg - u * mu));
+      }
+      norm_store(dx + row * d, o, col, d);
+      cx[t] = nx[t];
+      cd[t] = nd[t];
+    }
+  }
+  if (part == nullptr) return;
+  float* pw = part + (int64_t)blockIdx.x * 2 * d;
+  if constexpr (TPR <= 64) {      // the groups of a workgroup own the same columns: added in group order
+    for (int g = 0; g < groups; ++g) {
+      if (mine == g) {
+#pragma unroll
+        for (int t = 0; t < NV; ++t)
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const int at = (t * TPR + lane) * N + e;
+            cols[at] = g == 0 ? aw[t][e] : cols[at] + aw[t][e];
+            cols[TPR * NV * N + at] = g == 0 ? ab[t][e] : cols[TPR * NV * N + at] + ab[t][e];
+          }
+      }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < d; c += blockDim.x) {
+      pw[c] = cols[c];
+      pw[d + c] = cols[TPR * NV * N + c];
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < NV; ++t) {
+      const int col = (t * TPR + lane) * N;
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (col + e < d) {
+          pw[col + e] = aw[t][e];
+          pw[d + col + e] = ab[t][e];
+        }
+    }
+  }
+}
+
+// Rows wider than the registers of one workgroup: every pass reads the row again (from the caches).
+template <typename T, typename P>
+__global__ __launch_bounds__(1024) void mt_norm_wide_fwd_kernel(const T* __restrict__ x, const P* __restrict__ w,
+                                                                const P* __restrict__ b, T* __restrict__ y,
+                                                                float* __restrict__ stats, int64_t rows, int64_t stride, int d,
+                                                                float eps) {
+  __shared__ float red[64];
+  int turn = 0;
+  const float inv = 1.f / (float)d;
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const T* xr = x + row * stride;
+    float s[1] = {0.f};
+    for (int c = threadIdx.x; c < d; c += 1024) s[0] += (float)xr[c];
+    norm_sum<1024>(s, red, turn);
+    const float mean = s[0] * inv;
+    s[0] = 0.f;
+    for (int c = threadIdx.x; c < d; c += 1024) {
+      const float v = (float)xr[c] - mean;
+      s[0] = __builtin_fmaf(v, v, s[0]);
+    }
+    norm_sum<1024>(s, red, turn);
+    const float rstd = 1.f / sqrtf(s[0] * inv + eps);
+    for (int c = threadIdx.x; c < d; c += 1024) {
+      float v = ((float)xr[c] - mean) * rstd;
+      if (w != nullptr) v *= (float)w[c];
+      if (b != nullptr) v += (float)b[c];
+      y[row * d + c] = (T)v;
+    }
+    if (stats != nullptr && threadIdx.x == 0) {
+      stats[2 * row] = mean;
+      stats[2 * row + 1] = rstd;
+    }
+  }
+}
+
+template <typename T, typename P>
+__global__ __launch_bounds__(1024) void mt_norm_wide_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
+                                                                const P* __restrict__ w, const float* __restrict__ stats,
+                                                                T* __restrict__ dx, int64_t rows, int64_t stride,
+                                                                int64_t dy_stride, int d) {
+  __shared__ float red[64];
+  int turn = 0;
+  const float inv = 1.f / (float)d;
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const T *xr = x + row * stride, *gr = dy + row * dy_stride;
+    const float mean = stats[2 * row], rstd = stats[2 * row + 1];
+    float s[2] = {0.f, 0.f};
+    for (int c = threadIdx.x; c < d; c += 1024) {
+      const float g = (float)gr[c] * (w != nullptr ? (float)w[c] : 1.f);
+      s[0] += g;
+      s[1] = __builtin_fmaf(g, ((float)xr[c] - mean) * rstd, s[1]);
+    }
+    norm_sum<1024>(s, red, turn);
+    const float mg = s[0] * inv, mu = s[1] * inv;
+    for (int c = threadIdx.x; c < d; c += 1024) {
+      const float g = (float)gr[c] * (w != nullptr ? (float)w[c] : 1.f);
+      dx[row * d + c] = (T)(rstd * (g - mg - ((float)xr[c] - mean) * rstd * mu));
+    }
+  }
+}
+// Column sums for the wide form: workgroup (column block, row chunk), a thread per column.
+template <typename T>
+__global__ __launch_bounds__(256) void mt_norm_wide_cols_kernel(const T* __restrict__ dy, const T* __restrict__ x,
+                                                                const float* __restrict__ stats, float* __restrict__ part,
+                                                                int64_t rows, int64_t stride, int64_t dy_stride, int d) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= d) return;
+  const int64_t per = (rows + gridDim.y - 1) / gridDim.y, lo = per * blockIdx.y, hi = lo + per < rows ? lo + per : rows;
+  float sw = 0.f, sb = 0.f;
+  for (int64_t row = lo; row < hi; ++row) {
+    const float g = (float)dy[row * dy_stride + c];
+    sw = __builtin_fmaf(g, ((float)x[row * stride + c] - stats[2 * row]) * stats[2 * row + 1], sw);
+    sb += g;
+  }
+  part[(int64_t)blockIdx.y * 2 * d + c] = sw;
+  part[((int64_t)blockIdx.y * 2 + 1) * d + c] = sb;
+}
+
+// dw, db [d] = sums of the partial rows, in order: 16 x 16 threads, sixteen columns per workgroup, each thread every 16th
+// partial row, the sixteen strands added in order through LDS.
+template <typename P>
+__global__ __launch_bounds__(256) void mt_norm_cols_kernel(const float* __restrict__ part, P* __restrict__ dw, P* __restrict__ db,
+                                                           int n, int d) {
+  __shared__ float strands[16][17];
+  const int cl = threadIdx.x & 15, st = threadIdx.x >> 4;
+  const int c = blockIdx.x * 16 + cl;                  // 0 .. 2 d - 1: dw, then db
+  float s = 0.f;
+  if (c < 2 * d)
+    for (int i = st; i < n; i += 16) s += part[(int64_t)i * 2 * d + c];
+  strands[st][cl] = s;
+  __syncthreads();
+  if (st == 0 && c < 2 * d) {
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += strands[i][cl];
+    if (c < d) {
+      if (dw != nullptr) dw[c] = (P)s;
+    } else if (db != nullptr) {
+      db[c - d] = (P)s;
+    }
+  }
+}
+
+// ---- launchers ----------------------------------------------------------------------------------------------------------
+struct NormShape {
+  int tpr, nv;      // tpr 0: the wide form
+};
+// The fewest threads that keep a row in at most four vectors each.
+static NormShape norm_shape(int d, int per) {
+  const int vecs = (d + per - 1) / per;
+  if (vecs <= 16) return {16, 1};
+  if (vecs <= 64) return {64, 1};
+  if (vecs <= 128) return {64, 2};
+  if (vecs <= 256) return {64, 4};
+  if (vecs <= 512) return {256, 2};
+  if (vecs <= 1024) return {256, 4};
+  if (vecs <= 2048) return {1024, 2};
+  if (vecs <= 4096) return {1024, 4};
+  return {0, 0};
+}
+static int norm_threads(const NormShape& s, int64_t rows) {
+  if (s.tpr == 0 || s.tpr > 256) return 1024;
+  if (s.tpr == 256) return 256;
+  return rows >= 4096 ? 256 : 64;                 // few rows: one wave per workgroup, spread over the chip
+}
+static int norm_blocks(const NormShape& s, int64_t rows, int threads, int most) {
+  const int groups = s.tpr == 0 ? 1 : threads / s.tpr;
+  const int64_t want = (rows + groups - 1) / groups;
+  return (int)(want < most ? want : most);
+}
+#define NORM_FWD_BLOCKS 2048
+#define NORM_BWD_BLOCKS 1024
+
+#define NORM_SHAPES(GO) \
+  if (s.tpr == 16) GO(16, 1) else if (s.tpr == 64 && s.nv == 1) GO(64, 1) else if (s.tpr == 64 && s.nv == 2) GO(64, 2) \
+  else if (s.tpr == 64) GO(64, 4) else if (s.tpr == 256 && s.nv == 2) GO(256, 2) else if (s.tpr == 256) GO(256, 4) \
+  else if (s.nv == 2) GO(1024, 2) else GO(1024, 4)
+
+template <typename T, typename P>
+static int norm_fwd(const void* x, const void* w, const void* b, void* y, float* stats, int64_t rows, int64_t stride, int d,
+                    float eps, hipStream_t stream) {
+  const NormShape s = norm_shape(d, NormVec<T>::N);
+  const int threads = norm_threads(s, rows), blocks = norm_blocks(s, rows, threads, NORM_FWD_BLOCKS);
+  const T* xt = (const T*)x;
+  const P *wt = (const P*)w, *bt = (const P*)b;
+  if (s.tpr == 0) {
+    hipLaunchKernelGGL((mt_norm_wide_fwd_kernel<T, P>), dim3(blocks), dim3(1024), 0, stream, xt, wt, bt, (T*)y, stats, rows,
+                       stride, d, eps);
+    return (int)hipGetLastError();
+  }
+#define GO(TPR, NV)                                                                                                       \
+  hipLaunchKernelGGL((mt_norm_fwd_kernel<T, P, TPR, NV>), dim3(blocks), dim3(threads), 0, stream, xt, wt, bt, (T*)y, stats, rows, \
+                     stride, d, eps);
+  NORM_SHAPES(GO)
+#undef GO
+  return (int)hipGetLastError();
+}
+
+template <typename T, typename P>
+static int norm_bwd(const void* dy, const void* x, const void* w, const float* stats, void* dx, float* part, void* dw, void* db,
+                    int64_t rows, int64_t stride, int64_t dy_stride, int d, hipStream_t stream) {
+  const NormShape s = norm_shape(d, NormVec<T>::N);
+  const int threads = norm_threads(s, rows), blocks = norm_blocks(s, rows, threads, NORM_BWD_BLOCKS);
+  const T *xt = (const T*)x, *gt = (const T*)dy;
+  const P* wt = (const P*)w;
+  if (s.tpr == 0) {
+    hipLaunchKernelGGL((mt_norm_wide_bwd_kernel<T, P>), dim3(blocks), dim3(1024), 0, stream, gt, xt, wt, stats, (T*)dx, rows,
+                       stride, dy_stride, d);
+    if (part != nullptr)
+      hipLaunchKernelGGL((mt_norm_wide_cols_kernel<T>), dim3((d + 255) / 256, blocks < 64 ? blocks : 64), dim3(256), 0, stream, gt,
+                         xt, stats, part, rows, stride, dy_stride, d);
+  } else {
+#define GO(TPR, NV)                                                                                                          \
+  hipLaunchKernelGGL((mt_norm_bwd_kernel<T, P, TPR, NV>), dim3(blocks), dim3(threads), 0, stream, gt, xt, wt, stats, (T*)dx, part, \
+                     rows, stride, dy_stride, d);
+    NORM_SHAPES(GO)
+#undef GO
+  }
+  if (part != nullptr) {
+    const int n = s.tpr == 0 && blocks > 64 ? 64 : blocks;
+    hipLaunchKernelGGL((mt_norm_cols_kernel<P>), dim3((2 * d + 15) / 16), dim3(256), 0, stream, part, (P*)dw, (P*)db, n, d);
+  }
+  return (int)hipGetLastError();
+}
+
+static bool norm_args(int64_t rows, int64_t stride, int d, int x_bf16, int w_bf16) {
+  return rows >= 0 && stride >= 0 && d >= 1 && d <= (1 << 29) && (x_bf16 || !w_bf16);
+}
+
+// Rows of the partial-sum workspace [n][2][d] f32 of a backward pass.
+extern "C" int mt_norm_bwd_parts(int64_t rows, int d, int x_bf16) {
+  if (!norm_args(rows, 0, d, x_bf16, 0)) return -2;
+  const NormShape s = norm_shape(d, x_bf16 ? 8 : 4);
+  const int blocks = norm_blocks(s, rows, norm_threads(s, rows), NORM_BWD_BLOCKS);
+  return s.tpr == 0 && blocks > 64 ? 64 : blocks;
+}
+// y [rows][d] contiguous; x rows `stride` elements apart; w, b [d] (each may be null); stats [rows][2] (may be null).
+extern "C" int mt_norm_fwd_launch(const void* x, const void* w, const void* b, void* y, float* stats, int64_t rows, int64_t stride,
+                                  int d, float eps, int x_bf16, int w_bf16, hipStream_t stream) {
+  if (!norm_args(rows, stride, d, x_bf16, w_bf16)) return -2;
+  if (rows == 0) return 0;
+  if (!x_bf16) return norm_fwd<float, float>(x, w, b, y, stats, rows, stride, d, eps, stream);
+  if (!w_bf16) return norm_fwd<__bf16, float>(x, w, b, y, stats, rows, stride, d, eps, stream);
+  return norm_fwd<__bf16, __bf16>(x, w, b, y, stats, rows, stride, d, eps, stream);
+}
+// dx [rows][d] contiguous; part as mt_norm_bwd_parts says, or null when neither dw nor db is wanted.
+extern "C" int mt_norm_bwd_launch(const void* dy, const void* x, const void* w, const float* stats, void* dx, float* part, void* dw,
+                                  void* db, int64_t rows, int64_t stride, int64_t dy_stride, int d, int x_bf16, int w_bf16,
+                                  hipStream_t stream) {
+  if (!norm_args(rows, stride, d, x_bf16, w_bf16) || dy_stride < 0) return -2;
+  if (rows == 0) return 0;
+  if (!x_bf16) return norm_bwd<float, float>(dy, x, w, stats, dx, part, dw, db, rows, stride, dy_stride, d, stream);
+  if (!w_bf16) return norm_bwd<__bf16, float>(dy, x, w, stats, dx, part, dw, db, rows, stride, dy_stride, d, stream);
+  return norm_bwd<__bf16, __bf16>(dy, x, w, stats, dx, part, dw, db, rows, stride, dy_stride, d, stream);
+}

@@ -5,6 +5,8 @@ This is the step that closes both halves of a post-norm encoder block
 memory-bound passes over [tokens, d]; fused it is one read of each input and one write.  On a GPU
 ``ops/csrc/layernorm.hip`` runs it with one wave per row (forward and backward); elsewhere the
 reference below is used.
+
+``layer_norm`` is the norm alone, over rows of any width in f32 or bf16 (``ops/csrc/norm.hip``).
 """
 from __future__ import annotations
 
@@ -12,6 +14,39 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension, differentiable, in ``x``'s type; statistics and
+    column sums in f32.  ``weight`` and ``bias`` ([d], either may be missing) have ``x``'s type, or f32 beside a bf16 ``x``.  On a
+    GPU ``x`` is f32 or bf16, rows of any width; rows may lie apart (a column slice of a wider tensor is read in place)."""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"layer_norm needs rows of at least one column, got {tuple(x.shape)}")
+    d = x.shape[-1]
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if t.shape != (d,):
+            raise ValueError(f"{name} must be [{d}], got {tuple(t.shape)}")
+        if t.device != x.device:
+            raise TypeError(f"{name} is on {t.device}, x on {x.device}")
+        if t.dtype != x.dtype and not (x.dtype == torch.bfloat16 and t.dtype == torch.float32):
+            raise TypeError(f"{name} must be {x.dtype} (or f32 beside a bf16 x), got {t.dtype}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError(f"weight and bias must share a type, got {weight.dtype} and {bias.dtype}")
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    if not x.is_cuda:
+        wide = torch.promote_types(x.dtype, weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype)
+        cast = lambda t: None if t is None else t.to(wide)          # noqa: E731
+        return F.layer_norm(x.to(wide), (d,), cast(weight), cast(bias), eps).to(x.dtype)
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"layer_norm on a GPU takes f32 or bf16 rows, got {x.dtype}")
+    if d > 1 << 29:
+        raise ValueError(f"layer_norm on a GPU takes rows of at most {1 << 29} columns, got {d}")
+    from .layernorm_hip import LayerNorm
+    return LayerNorm.apply(x, weight, bias, float(eps))
 
 
 def residual_layer_norm_reference(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,

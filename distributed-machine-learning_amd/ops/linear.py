@@ -16,6 +16,11 @@ GPU no call reaches a BLAS-library GEMM:
   ``dW = dY^T X`` -- a long skinny contraction over the token rows -- is split over enough workgroups to fill the chip
   and the partial slabs are added in a fixed order by one small launch.
 
+``linear(x, weight, bias, activation=..., residual=...)`` is the layer with its activation (``"relu"`` or ``"gelu"``, the erf
+form) and the addition of a residual in the GEMM's epilogue, ``act(x W^T + b) + residual`` rounded once (``FusedLinear``,
+``csrc/linear_ep.hip``); it also takes bf16 parameters with bf16 activations, outside autocast, and gives their gradients in
+bf16.
+
 The tile kernels read rows in 16-byte pieces, so a dimension that is not a multiple of 4 (f32) or 8 (bf16) -- 81 input
 features, a scalar output -- is padded with zero columns / zero rows up to the next multiple before the launch and the
 result is sliced back; autograd carries the slice through, so gradients of the padding are dropped.  Operands these
@@ -64,10 +69,62 @@ def _pad_operands(x, weight, bias, mult: int):
     return x, weight, bias
 
 
-def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``x @ weight.T + bias``; on a GPU always on this package's own MFMA kernels (see the module text)."""
-    if not x.is_cuda or x.numel() == 0:
-        return F.linear(x, weight, bias)
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2}
+
+
+def _check_fused(x, weight, bias, activation, residual) -> None:
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {tuple(ACTIVATIONS)}, got {activation!r}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x {tuple(x.shape)} does not fit weight {tuple(weight.shape)}")
+    if bias is not None and bias.shape != weight.shape[:1]:
+        raise ValueError(f"bias must be [{weight.shape[0]}], got {tuple(bias.shape)}")
+    if residual is not None and residual.shape != x.shape[:-1] + weight.shape[:1]:
+        raise ValueError(f"residual must have the output's shape {tuple(x.shape[:-1] + weight.shape[:1])}, got "
+                         f"{tuple(residual.shape)}")
+    for name, t in (("weight", weight), ("bias", bias), ("residual", residual)):
+        if t is not None and t.device != x.device:
+            raise TypeError(f"{name} is on {t.device}, x on {x.device}")
+
+
+def _plain_fused(x, weight, bias, activation, residual) -> torch.Tensor:
+    y = F.linear(x, weight, bias)
+    y = F.relu(y) if activation == "relu" else F.gelu(y) if activation == "gelu" else y
+    return y if residual is None else y + residual
+
+
+def _fused_linear(x, weight, bias, activation, residual) -> torch.Tensor:
+    """The layer through ``FusedLinear``, operands brought to the types it takes."""
+    w16 = None
+    if torch.is_autocast_enabled():
+        if not _bf16_autocast() or weight.dtype != torch.float32:
+            raise TypeError("mitune.ops.linear under autocast takes f32 master weights and bf16 compute only, got "
+                            f"autocast {torch.get_autocast_dtype('cuda')} / weight {weight.dtype}")
+        x, w16 = x.to(torch.bfloat16), _shadow(weight)
+        residual = residual.to(torch.bfloat16) if residual is not None else None
+    elif x.dtype not in (torch.float32, torch.bfloat16) or weight.dtype != x.dtype:
+        raise TypeError(f"mitune.ops.linear on a GPU takes f32 or bf16 operands of one type (or bf16 autocast), got x {x.dtype} "
+                        f"/ weight {weight.dtype}")
+    if bias is not None and bias.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"bias must be {x.dtype} or f32, got {bias.dtype}")
+    if residual is not None and residual.dtype != x.dtype:
+        raise TypeError(f"residual must be {x.dtype}, got {residual.dtype}")
+    return FusedLinear.apply(x, weight, bias, residual, ACTIVATIONS[activation], w16)
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
+           residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``act(x @ weight.T + bias) + residual``; on a GPU always on this package's own MFMA kernels (see the module text)."""
+    fused = activation is not None or residual is not None
+    if fused:
+        _check_fused(x, weight, bias, activation, residual)
+    if not x.is_cuda or x.numel() == 0 or weight.numel() == 0:
+        return _plain_fused(x, weight, bias, activation, residual)
+    if not fused and x.dtype == weight.dtype == torch.bfloat16 and not torch.is_autocast_enabled():
+        _check_fused(x, weight, bias, activation, residual)
+        fused = True
+    if fused:
+        return _fused_linear(x, weight, bias, activation, residual)
     out_f, in_f = weight.shape
     if torch.is_autocast_enabled():
         if not _bf16_autocast() or weight.dtype != torch.float32:
@@ -279,3 +336,152 @@ class SmallLinear(torch.autograd.Function):
                                                     OPTIONS.small_linear_tile, L.raw_stream(dev)),
                 "mt_small_linear_bwd_tiled_launch")
         return (dx.view(ctx.x_shape) if dx is not None else None), dw, db
+
+
+def _pieces(t: torch.Tensor) -> torch.Tensor:
+    """``t`` [rows, columns] with rows of whole 16-byte pieces: itself when its rows start on such a boundary and its width is a
+    multiple of one, else a copy padded with zero columns."""
+    per = 16 // t.element_size()
+    pad = -t.shape[1] % per
+    if pad == 0 and t.stride(1) == 1 and t.stride(0) % per == 0 and t.data_ptr() % 16 == 0 and t.stride(0) >= t.shape[1]:
+        return t
+    return F.pad(t, (0, pad)).contiguous() if pad else t.clone(memory_format=torch.contiguous_format)
+
+
+def _rows_of(t: torch.Tensor, width: int) -> torch.Tensor:
+    return t.reshape(-1, width)
+
+
+class FusedLinear(torch.autograd.Function):
+    """``act(x W^T + b) + residual`` with x, W, residual and the output of one type, f32 or bf16 (under bf16 autocast W is the
+    f32 master and its gradient f32); operands checked in ``linear``."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act: int, w16):
+        from . import lib as L
+        so = L.load()
+        out_f, in_f = weight.shape
+        with torch.autocast("cuda", enabled=False):
+            xc = _pieces(_rows_of(x, in_f))
+            wc = _pieces(w16 if w16 is not None else weight.detach().to(x.dtype))
+            bc = bias.detach().contiguous() if bias is not None else None
+            rc = _rows_of(residual, out_f).contiguous() if residual is not None else None
+            M, bf16 = xc.shape[0], int(x.dtype == torch.bfloat16)
+            y = torch.empty(M, out_f, device=x.device, dtype=x.dtype)
+            backward = any(ctx.needs_input_grad[:3])
+            # what act' is read from: y itself has z's sign under ReLU, unless a residual was added to it
+            keep_z = backward and act != 0 and not (act == 1 and rc is None)
+            z = torch.empty_like(y) if keep_z else None
+            with torch.cuda.device(x.device):
+                L.check(so.mt_linear_fwd_launch(xc.data_ptr(), wc.data_ptr(), bc.data_ptr() if bc is not None else None,
+                                                rc.data_ptr() if rc is not None else None, y.data_ptr(),
+                                                z.data_ptr() if z is not None else None, M, out_f, xc.shape[1], xc.stride(0),
+                                                wc.stride(0), act, int(bc is not None and bc.dtype == torch.bfloat16), bf16,
+                                                L.raw_stream(x.device)), "mt_linear_fwd_launch")
+        if backward:
+            ctx.save_for_backward(xc, wc, z if keep_z else y if act else None)
+        ctx.meta = (act, x.shape, in_f, weight.dtype, bias.dtype if bias is not None else None,
+                    residual.shape if residual is not None else None)
+        return y.view(x.shape[:-1] + (out_f,))
+
+    @staticmethod
+    def backward(ctx, dy):
+        from . import lib as L
+        so = L.load()
+        act, x_shape, in_f, w_dtype, b_dtype, r_shape = ctx.meta
+        dx = dw = db = None
+        if any(ctx.needs_input_grad[:3]):
+            xc, wc, s = ctx.saved_tensors
+            out_f = wc.shape[0]
+            bf16, dev, M = xc.dtype == torch.bfloat16, xc.device, xc.shape[0]
+            per = 8 if bf16 else 4
+            stream = L.raw_stream(dev)
+            with torch.autocast("cuda", enabled=False), torch.cuda.device(dev):
+                g = _rows_of(dy.to(xc.dtype), out_f)
+                if act:
+                    g = g if g.stride(1) == 1 else g.contiguous()
+                    dz = torch.empty(M, out_f + -out_f % per, device=dev, dtype=xc.dtype)
+                    L.check(so.mt_linear_act_bwd_launch(g.data_ptr(), s.data_ptr(), dz.data_ptr(), M, out_f, g.stride(0),
+                                                        dz.shape[1], act, int(bf16), stream), "mt_linear_act_bwd_launch")
+                else:
+                    dz = _pieces(g)
+                    dz = dz if dz.stride(0) == dz.shape[1] else dz.contiguous()
+                if not bf16 and _small(M, xc.shape[1], dz.shape[1], True):
+                    dx, dw, db = _small_grads(so, dz, xc, wc, ctx.needs_input_grad[0], b_dtype is not None, stream)
+                    dx = dx[:, :in_f].reshape(x_shape) if dx is not None else None
+                    return (dx, dw[:out_f, :in_f], db[:out_f] if db is not None else None,
+                            dy if r_shape is not None else None, None, None)
+                if ctx.needs_input_grad[0]:
+                    dx = _input_grad(so, dz, wc, out_f, stream)[:, :in_f].reshape(x_shape)
+                if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+                    dw, db = _weight_grad(so, dz, xc, out_f, in_f, w_dtype, b_dtype, stream)
+        return dx, dw, db, (dy if r_shape is not None else None), None, None
+
+
+def _small_grads(so, dz, xc, wc, want_dx: bool, want_db: bool, stream):
+    """The gradients of a small f32 layer in one launch, as ``SmallLinear`` computes them; widths stay padded."""
+    from . import lib as L
+    (R, out), in_f, dev = dz.shape, xc.shape[1], dz.device
+    xc = xc if xc.stride(0) == in_f else xc.contiguous()
+    if wc.shape[0] != out:
+        wc = F.pad(wc, (0, 0, 0, out - wc.shape[0]))
+    wc = wc if wc.stride(0) == in_f else wc.contiguous()
+    dx = torch.empty(R, in_f, device=dev, dtype=torch.float32) if want_dx else None
+    dw = torch.empty(out, in_f, device=dev, dtype=torch.float32)
+    db = torch.empty(out, device=dev, dtype=torch.float32) if want_db else None
+    L.check(so.mt_small_linear_bwd_tiled_launch(xc.data_ptr(), wc.data_ptr(), dz.data_ptr(),
+                                                dx.data_ptr() if want_dx else None, dw.data_ptr(),
+                                                db.data_ptr() if want_db else None, R, in_f, out, OPTIONS.small_linear_tile,
+                                                stream), "mt_small_linear_bwd_tiled_launch")
+    return dx, dw, db
+
+
+def _input_grad(so, dz, wc, out_f: int, stream) -> torch.Tensor:
+    """dz W [rows, W's padded width]; the contraction runs over W's ``out_f`` rows."""
+    from . import lib as L
+    M, width = dz.shape[0], wc.shape[1]
+    dx = torch.empty(M, width, device=dz.device, dtype=dz.dtype)
+    es, most = dz.element_size(), 1 << 20          # a launch's tile coordinates are 16 bits
+    for m0 in range(0, M, most):
+        m = min(most, M - m0)
+        a, c = dz.data_ptr() + m0 * dz.shape[1] * es, dx.data_ptr() + m0 * width * es
+        if es == 2:
+            L.check(so.mt_gemm_single_launch(1, a, wc.data_ptr(), c, None, m, width, out_f, dz.shape[1], wc.stride(0), width, 0,
+                                             0, stream), "mt_gemm_single_launch")
+        else:
+            L.check(so.mt_gemm_f32_single_launch(1, a, wc.data_ptr(), c, None, None, m, width, out_f, dz.shape[1], wc.stride(0),
+                                                 width, 0, stream), "mt_gemm_f32_single_launch")
+    return dx
+
+
+def _weight_grad(so, dz, xc, out_f: int, in_f: int, w_dtype, b_dtype, stream):
+    """(dW [out_f, in_f], db [out_f] or None): split over the rows, the slabs added in order and rounded once."""
+    from . import lib as L
+    M, width, rows = dz.shape[0], xc.shape[1], dz.shape[1]
+    xc = xc if xc.stride(0) == width else xc.contiguous()
+    bf16 = dz.dtype == torch.bfloat16
+    tile = 128 if bf16 else 64
+    most = 255 * tile                               # output rows of a launch: its tile rows are 8 bits
+    dw = torch.empty(out_f, in_f, device=dz.device, dtype=w_dtype)
+    db = torch.empty(out_f, device=dz.device, dtype=b_dtype) if b_dtype is not None else None
+    if rows > most:
+        parts = [dz[:, r:r + most].contiguous() for r in range(0, rows, most)]
+    else:
+        parts = [dz]
+    for i, part in enumerate(parts):
+        n = part.shape[1]
+        real = min(n, out_f - i * most)
+        splits = _wgrad_splits(M, -(-n // tile) * -(-width // tile), 64 if bf16 else 128)
+        slab = (n * width + n + 63) // 64 * 64
+        arena = torch.empty(splits, slab, device=dz.device, dtype=torch.float32)
+        if bf16:
+            L.check(so.mt_wgrad_single_launch(part.data_ptr(), xc.data_ptr(), arena.data_ptr(),
+                                              arena.data_ptr() + n * width * 4 if db is not None else None, M, n, width, splits,
+                                              slab, stream), "mt_wgrad_single_launch")
+        else:
+            L.check(so.mt_wgrad_f32_single_launch(part.data_ptr(), xc.data_ptr(), arena.data_ptr(), M, n, width, splits, slab,
+                                                  int(db is not None), stream), "mt_wgrad_f32_single_launch")
+        L.check(so.mt_linear_wsum_launch(arena.data_ptr(), dw[i * most:].data_ptr(), db[i * most:].data_ptr() if db is not None else None,
+                                         real, in_f, width, n * width, splits, slab, int(w_dtype == torch.bfloat16),
+                                         int(b_dtype == torch.bfloat16), stream), "mt_linear_wsum_launch")
+    return dw, db
