@@ -194,6 +194,16 @@ def _tile_list(a, pack, which: int) -> None:
         pack._lists.record_stream(torch.cuda.current_stream(pack.device))
 
 
+# bf16 launches of fewer workgroups than this (two per CU) take the split form, whose four waves share one walk over the keys.
+SPLIT_BELOW = 512
+
+
+def _launch(so, a, which: int, bf16: bool, device, what: str) -> None:
+    lanes = a.kv_heads if which == 2 else a.heads
+    L.check(so.mt_packed_attn_launch(ctypes.byref(a), which, int(bf16), int(not bf16 or a.n_items * lanes < SPLIT_BELOW),
+                                     L.raw_stream(device)), what)
+
+
 class PackedAttention(torch.autograd.Function):
     """``ops.attention.packed_attention`` on a GPU; operands checked there."""
 
@@ -208,8 +218,7 @@ class PackedAttention(torch.autograd.Function):
         a = _packed_args(pack, 0 if causal else 2, qc, kc, vc, causal, scale)
         a.o, a.lse = out.data_ptr(), lse.data_ptr() if keeps else None
         with torch.cuda.device(q.device):
-            L.check(so.mt_packed_attn_launch(ctypes.byref(a), 0, int(q.dtype == torch.bfloat16), L.raw_stream(q.device)),
-                    "mt_packed_attn_launch")
+            _launch(so, a, 0, q.dtype == torch.bfloat16, q.device, "mt_packed_attn_launch")
         if keeps:
             ctx.save_for_backward(qc, kc, vc, out, lse)
         ctx.pack, ctx.meta = pack, (causal, scale, dk, dv)
@@ -227,10 +236,10 @@ class PackedAttention(torch.autograd.Function):
         a.out, a.dout, a.do_row, a.do_head = out.data_ptr(), do.data_ptr(), do.stride(0), do.stride(1)
         a.lse, a.delta = lse.data_ptr(), delta.data_ptr()
         a.dq, a.dk, a.dv = (g.data_ptr() for g in grads)
-        bf16, stream = int(q.dtype == torch.bfloat16), L.raw_stream(q.device)
+        bf16 = q.dtype == torch.bfloat16
         with torch.cuda.device(q.device):
-            L.check(so.mt_packed_attn_launch(ctypes.byref(a), 1, bf16, stream), "mt_packed_attn_launch(dq)")
+            _launch(so, a, 1, bf16, q.device, "mt_packed_attn_launch(dq)")
             _tile_list(a, pack, 1 if causal else 2)
-            L.check(so.mt_packed_attn_launch(ctypes.byref(a), 2, bf16, stream), "mt_packed_attn_launch(dk, dv)")
+            _launch(so, a, 2, bf16, q.device, "mt_packed_attn_launch(dk, dv)")
         gq, gk, gv = (g if g.shape[2] == w else g[..., :w].contiguous() for g, w in zip(grads, (dk, dk, dv)))
         return gq, gk, gv, None, None, None

@@ -126,18 +126,18 @@ template <typename T, int D> struct PaImg {
       return v;
     }
   }
-  // LDS-DMA of NROWS rows of `d` valid columns into an image, four waves sharing the 1-KiB pieces.  `base` is the first row's
+  // LDS-DMA of NROWS rows of `d` valid columns into an image, WAVES waves sharing the 1-KiB pieces.  `base` is the first row's
   // first element; rows at and past `valid` and columns past `d` arrive as zeros through the buffer's range check.
-  template <int NROWS>
+  template <int NROWS, int WAVES = 4>
   static __device__ __forceinline__ void stage(uint8_t* img, const T* base, int64_t row_stride, int valid, int d, int wave, int lane) {
-    constexpr int PIECES = NROWS * ROWB / 1024;
+    constexpr int PIECES = NROWS * ROWB / 1024 / WAVES;
     const int64_t stride = row_stride * (int64_t)sizeof(T);
     const int rows = valid < NROWS ? valid : NROWS;
     const uint32_t bytes = rows > 0 ? (uint32_t)((rows - 1) * stride + d * (int)sizeof(T)) : 0u;
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, bytes, 0x00027000);
 #pragma unroll
-    for (int t = 0; t < PIECES / 4; ++t) {
-      const int j = wave * (PIECES / 4) + t;
+    for (int t = 0; t < PIECES; ++t) {
+      const int j = wave * PIECES + t;
       const int at_byte = j * 1024 + lane * 16;
       const int r = at_byte / ROWB, c = ((at_byte % ROWB) >> 4) ^ swz(r);
       const uint32_t off = c * EPC < d ? (uint32_t)(r * (uint32_t)stride + c * 16) : 0xFFFFFF00u;
@@ -220,6 +220,54 @@ __device__ __forceinline__ void pa_tile_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
+}
+
+// The four waves' partial results of 32 rows: [wave][column][row] f32, added in wave order and stored.
+template <int D>
+__device__ __forceinline__ void pa_join(float* join, const f32x16 (&acc)[D / 32], float factor, int wave, int lane) {
+#pragma unroll
+  for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      join[(wave * D + 32 * b + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3)) * 32 + (lane & 31)] = acc[b][i] * factor;
+}
+template <typename T, int D>
+__device__ __forceinline__ void pa_join_store(T* base, int64_t row_stride, const float* join, int rows, int d) {
+  const int r = threadIdx.x & 31;
+  if (r >= rows) return;
+#pragma unroll
+  for (int c0 = 0; c0 < D / 8; c0 += 4) {
+    const int c = (threadIdx.x >> 5) * (D / 8) + c0;
+    if (c >= d) return;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += join[(w * D + c + e) * 32 + r];
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2*>(base + r * row_stride + c) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    else *reinterpret_cast<f32x4*>(base + r * row_stride + c) = v;
+  }
+}
+// What the dq kernels hold of an owned row: q, do, L and D = do . o (stored for the dk / dv kernel by the waves with `store`).
+template <typename T, int D>
+__device__ __forceinline__ void pa_dq_rows(const MtPackedAttn& p, typename PaFrag<T>::type (&qf)[D / 16],
+                                           typename PaFrag<T>::type (&df)[D / 16], float& delta, float& lse, int64_t row, int head, bool ok,
+                                           bool store, int lane) {
+  pa_own_row<T, D>(df, reinterpret_cast<const T*>(p.dout) + row * p.do_row + (int64_t)head * p.do_head, ok, p.head_v, lane);
+  pa_own_row<T, D>(qf, reinterpret_cast<const T*>(p.out) + row * ((int64_t)p.heads * p.head_v) + (int64_t)head * p.head_v, ok, p.head_v,
+                   lane);
+  delta = 0.f;
+  lse = INFINITY;                                       // rows outside the sequence: p = 2^(s - inf) = 0
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) delta = __builtin_fmaf((float)df[s][j], (float)qf[s][j], delta);
+  delta += pa_other_half(delta);
+  if (ok) {
+    lse = p.lse[(int64_t)head * p.rows + row];
+    if (store && lane < 32) p.delta[(int64_t)head * p.rows + row] = delta;
+  }
+  pa_own_row<T, D>(qf, reinterpret_cast<const T*>(p.q) + row * p.q_row + (int64_t)head * p.q_head, ok, p.head_k, lane);
 }
 
 // ---- forward ------------------------------------------------------------------------------------------------------------
@@ -344,24 +392,9 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
   }
   const int first = item.first + wave * 32, mine = first + (lane & 31);
   const bool ok = mine < item.len;
-  const int64_t row = item.row0 + (int64_t)mine;
   Frag qf[D / 16], df[D / 16];
-  float delta = 0.f, lse = INFINITY;                    // rows outside the sequence: p = 2^(s - inf) = 0
-  {
-    pa_own_row<T, D>(df, reinterpret_cast<const T*>(p.dout) + row * p.do_row + (int64_t)head * p.do_head, ok, p.head_v, lane);
-    pa_own_row<T, D>(qf, reinterpret_cast<const T*>(p.out) + row * ((int64_t)p.heads * p.head_v) + (int64_t)head * p.head_v, ok,
-                     p.head_v, lane);
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) delta = __builtin_fmaf((float)df[s][j], (float)qf[s][j], delta);
-    delta += pa_other_half(delta);
-    if (ok) {
-      lse = p.lse[(int64_t)head * p.rows + row];
-      if (lane < 32) p.delta[(int64_t)head * p.rows + row] = delta;
-    }
-    pa_own_row<T, D>(qf, reinterpret_cast<const T*>(p.q) + row * p.q_row + (int64_t)head * p.q_head, ok, p.head_k, lane);
-  }
+  float delta, lse;
+  pa_dq_rows<T, D>(p, qf, df, delta, lse, item.row0 + (int64_t)mine, head, ok, true, lane);
   const T* kb = reinterpret_cast<const T*>(p.k) + item.row0 * p.k_row + (int64_t)kvh * p.k_head;
   const T* vb = reinterpret_cast<const T*>(p.v) + item.row0 * p.v_row + (int64_t)kvh * p.v_head;
   const int keys = p.causal && item.first + PA_OWN < item.len ? item.first + PA_OWN : item.len;
@@ -518,16 +551,364 @@ __global__ __launch_bounds__(PA_THREADS, 1) void mt_pattn_dkv_kernel(const MtPac
   }
 }
 
+// ---- the split form -----------------------------------------------------------------------------------------------------
+// A workgroup owns 32 rows and its four waves share the walk: wave w takes tiles w, w + 4, ... of 32 rows, in its own part of
+// LDS and without barriers, and the four partial results are joined through LDS in wave order.  Against the form above a tile
+// fetched feeds 32 owned rows instead of 128, and a quarter of the longest sequence's walk is the longest any wave has to go.
+// An image is single-buffered: it is refilled as soon as the last product that reads it has its fragments, and the other
+// image's products run meanwhile.
+#define PA_TILE 32
+template <int N> __device__ __forceinline__ void pa_wait_vm() {          // at most N of this wave's loads are still in flight
+  static_assert(N >= 0 && N < 64, "vmcnt is a six-bit counter");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void pa_reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// Which 32 owned rows: `lanes` heads or key / value heads side by side, then the quarters of a 128-row tile.
+struct PaSlot {
+  int it, lane_head, sub;
+};
+__device__ __forceinline__ PaSlot pa_slot(int block, int lanes) {
+  const int it = block / (4 * lanes), r = block - it * 4 * lanes;
+  return PaSlot{it, r % lanes, r / lanes};
+}
+// f32 steps are eight slow instructions: those behind the head's width are skipped.  bf16 steps are one, and stay in line.
+template <typename T> __device__ __forceinline__ bool pa_step(int column, int width) { return sizeof(T) == 2 || column < width; }
+
+template <typename T, int D>
+__global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) void mt_pattn_split_fwd_kernel(const MtPackedAttn p) {
+  typedef PaImg<T, D> Img;
+  typedef typename PaFrag<T>::type Frag;
+  constexpr int IMG = PA_TILE * Img::ROWB, PIECES = IMG / 1024;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[8 * IMG < 512 * D ? 512 * D : 8 * IMG];
+  __shared__ float stat[2][4][32];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const PaSlot slot = pa_slot(blockIdx.x, p.heads);
+  const int kvh = slot.lane_head % p.kv_heads, head = kvh * (p.heads / p.kv_heads) + slot.lane_head / p.kv_heads;
+  const MtSeqItem item = pa_item(p, slot.it, p.causal);
+  const int64_t o_row = (int64_t)p.heads * p.head_v;
+  T* o = reinterpret_cast<T*>(p.o) + item.row0 * o_row + (int64_t)head * p.head_v;
+  if (item.len <= 0) {
+    if (slot.sub == 0) pa_zero_rows<T>(o, o_row, -item.len, p.head_v);
+    return;
+  }
+  const int first = item.first + slot.sub * 32, mine = first + (lane & 31);
+  if (first >= item.len) return;
+  Frag qf[D / 16];
+  pa_own_row<T, D>(qf, reinterpret_cast<const T*>(p.q) + (item.row0 + (int64_t)mine) * p.q_row + (int64_t)head * p.q_head,
+                   mine < item.len, p.head_k, lane);
+  const T* kb = reinterpret_cast<const T*>(p.k) + item.row0 * p.k_row + (int64_t)kvh * p.k_head;
+  const T* vb = reinterpret_cast<const T*>(p.v) + item.row0 * p.v_row + (int64_t)kvh * p.v_head;
+  const int keys = p.causal && first + 32 < item.len ? first + 32 : item.len;
+  const int tiles = (keys + PA_TILE - 1) / PA_TILE;
+  const float c = p.scale * 1.4426950408889634f;
+  uint8_t* kimg = lds + wave * 2 * IMG;
+  uint8_t* vimg = kimg + IMG;
+  auto load_k = [&](int t) {
+    Img::template stage<PA_TILE, 1>(kimg, kb + (int64_t)t * PA_TILE * p.k_row, p.k_row, item.len - t * PA_TILE, p.head_k, 0, lane);
+  };
+  auto load_v = [&](int t) {
+    Img::template stage<PA_TILE, 1>(vimg, vb + (int64_t)t * PA_TILE * p.v_row, p.v_row, item.len - t * PA_TILE, p.head_v, 0, lane);
+  };
+  f32x16 acc[D / 32];
+  pa_clear(acc);
+  float m = -INFINITY, sum = 0.f;
+  if (wave < tiles) {
+    load_k(wave);
+    load_v(wave);
+  }
+  for (int t = wave; t < tiles; t += 4) {
+    const bool more = t + 4 < tiles;
+    pa_wait_vm<PIECES>();                      // K of this tile; its V may still be on the way
+    f32x16 s[1];
+    pa_clear(s);
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks)
+      if (pa_step<T>(16 * ks, p.head_k)) s[0] = pa_mma(Img::rows(kimg, 0, ks, lane), qf[ks], s[0]);
+    pa_reads_done();
+    if (more) load_k(t + 4);
+    const int k0 = t * PA_TILE;
+    if (k0 + PA_TILE > item.len || (p.causal && k0 + PA_TILE - 1 > first)) {
+      const int last = p.causal && mine < item.len ? mine : item.len - 1;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[0][i] = k0 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3) <= last ? s[0][i] : -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[0][i]);
+    mx = fmaxf(mx, pa_other_half(mx)) * c;
+    if (__any(mx > m + 8.f)) {
+      const float mn = fmaxf(m, mx);
+      const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      sum *= f;
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[b][i] *= f;
+    }
+    const float sub = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[0][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][i], c, -sub));
+      sum += s[0][i];
+    }
+    if (more) pa_wait_vm<PIECES>();            // V of this tile; the next K may still be on the way
+    else pa_wait_vm<0>();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const Frag pf = pa_pack<T>(s[0], h);
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b)
+        if (pa_step<T>(32 * b, p.head_v)) acc[b] = pa_mma(Img::cols(vimg, 16 * h, 32 * b, lane), pf, acc[b]);
+    }
+    pa_reads_done();
+    if (more) load_v(t + 4);
+  }
+  sum += pa_other_half(sum);
+  if (lane < 32) {
+    stat[0][wave][lane] = m;
+    stat[1][wave][lane] = sum;
+  }
+  __syncthreads();                             // and every wave is done with its images
+  const int q = lane & 31;
+  float top = -INFINITY, total = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[0][w][q]);
+  const float sub = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) total += stat[1][w][q] * __builtin_amdgcn_exp2f(stat[0][w][q] - sub);
+  const bool real = total > 0.f || total != total;
+  const float f = __builtin_amdgcn_exp2f(m - sub) * (real ? 1.f / total : 0.f);
+  pa_join<D>(reinterpret_cast<float*>(lds), acc, f, wave, lane);
+  __syncthreads();
+  pa_join_store<T, D>(o + (int64_t)first * o_row, o_row, reinterpret_cast<const float*>(lds), item.len - first, p.head_v);
+  if (p.lse != nullptr && threadIdx.x < 32 && mine < item.len)
+    p.lse[(int64_t)head * p.rows + item.row0 + mine] = real ? sub + __builtin_amdgcn_logf(total) : INFINITY;
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) void mt_pattn_split_dq_kernel(const MtPackedAttn p) {
+  typedef PaImg<T, D> Img;
+  typedef typename PaFrag<T>::type Frag;
+  constexpr int IMG = PA_TILE * Img::ROWB, PIECES = IMG / 1024;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[8 * IMG < 512 * D ? 512 * D : 8 * IMG];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const PaSlot slot = pa_slot(blockIdx.x, p.heads);
+  const int kvh = slot.lane_head % p.kv_heads, head = kvh * (p.heads / p.kv_heads) + slot.lane_head / p.kv_heads;
+  const MtSeqItem item = pa_item(p, slot.it, p.causal);
+  const int64_t dq_row = (int64_t)p.heads * p.head_k;
+  T* dq = reinterpret_cast<T*>(p.dq) + item.row0 * dq_row + (int64_t)head * p.head_k;
+  if (item.len <= 0) {
+    if (slot.sub == 0) pa_zero_rows<T>(dq, dq_row, -item.len, p.head_k);
+    return;
+  }
+  const int first = item.first + slot.sub * 32, mine = first + (lane & 31);
+  if (first >= item.len) return;
+  Frag qf[D / 16], df[D / 16];
+  float delta, lse;
+  pa_dq_rows<T, D>(p, qf, df, delta, lse, item.row0 + (int64_t)mine, head, mine < item.len, wave == 0, lane);
+  const T* kb = reinterpret_cast<const T*>(p.k) + item.row0 * p.k_row + (int64_t)kvh * p.k_head;
+  const T* vb = reinterpret_cast<const T*>(p.v) + item.row0 * p.v_row + (int64_t)kvh * p.v_head;
+  const int keys = p.causal && first + 32 < item.len ? first + 32 : item.len;
+  const int tiles = (keys + PA_TILE - 1) / PA_TILE;
+  const float c = p.scale * 1.4426950408889634f;
+  uint8_t* kimg = lds + wave * 2 * IMG;
+  uint8_t* vimg = kimg + IMG;
+  auto load_k = [&](int t) {
+    Img::template stage<PA_TILE, 1>(kimg, kb + (int64_t)t * PA_TILE * p.k_row, p.k_row, item.len - t * PA_TILE, p.head_k, 0, lane);
+  };
+  auto load_v = [&](int t) {
+    Img::template stage<PA_TILE, 1>(vimg, vb + (int64_t)t * PA_TILE * p.v_row, p.v_row, item.len - t * PA_TILE, p.head_v, 0, lane);
+  };
+  f32x16 acc[D / 32];
+  pa_clear(acc);
+  if (wave < tiles) {
+    load_v(wave);
+    load_k(wave);
+  }
+  for (int t = wave; t < tiles; t += 4) {
+    const bool more = t + 4 < tiles;
+    pa_wait_vm<PIECES>();                      // V; K may still be on the way
+    f32x16 s[1], d[1];
+    pa_clear(s);
+    pa_clear(d);
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks)
+      if (pa_step<T>(16 * ks, p.head_v)) d[0] = pa_mma(Img::rows(vimg, 0, ks, lane), df[ks], d[0]);
+    pa_reads_done();
+    if (more) {
+      load_v(t + 4);
+      pa_wait_vm<PIECES>();
+    } else {
+      pa_wait_vm<0>();
+    }
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks)
+      if (pa_step<T>(16 * ks, p.head_k)) s[0] = pa_mma(Img::rows(kimg, 0, ks, lane), qf[ks], s[0]);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[0][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][i], c, -lse)) * (d[0][i] - delta);
+    const int k0 = t * PA_TILE;
+    if (k0 + PA_TILE > item.len || (p.causal && k0 + PA_TILE - 1 > first)) {
+      const int last = p.causal && mine < item.len ? mine : item.len - 1;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[0][i] = k0 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3) <= last ? s[0][i] : 0.f;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const Frag sf = pa_pack<T>(s[0], h);
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b)
+        if (pa_step<T>(32 * b, p.head_k)) acc[b] = pa_mma(Img::cols(kimg, 16 * h, 32 * b, lane), sf, acc[b]);
+    }
+    pa_reads_done();
+    if (more) load_k(t + 4);
+  }
+  __syncthreads();
+  pa_join<D>(reinterpret_cast<float*>(lds), acc, p.scale, wave, lane);
+  __syncthreads();
+  pa_join_store<T, D>(dq + (int64_t)first * dq_row, dq_row, reinterpret_cast<const float*>(lds), item.len - first, p.head_k);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(PA_THREADS, 1) void mt_pattn_split_dkv_kernel(const MtPackedAttn p) {
+  typedef PaImg<T, D> Img;
+  typedef typename PaFrag<T>::type Frag;
+  constexpr int IMG = PA_TILE * Img::ROWB, PIECES = IMG / 1024;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[8 * IMG < 512 * D ? 512 * D : 8 * IMG];
+  __shared__ __attribute__((aligned(16))) float stat[4][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const PaSlot slot = pa_slot(blockIdx.x, p.kv_heads);
+  const int kvh = slot.lane_head, group = p.heads / p.kv_heads;
+  const MtSeqItem item = pa_item(p, slot.it, false);
+  const int64_t dk_row = (int64_t)p.kv_heads * p.head_k, dv_row = (int64_t)p.kv_heads * p.head_v;
+  T* dk = reinterpret_cast<T*>(p.dk) + item.row0 * dk_row + (int64_t)kvh * p.head_k;
+  T* dv = reinterpret_cast<T*>(p.dv) + item.row0 * dv_row + (int64_t)kvh * p.head_v;
+  if (item.len <= 0) {
+    if (slot.sub == 0) {
+      pa_zero_rows<T>(dk, dk_row, -item.len, p.head_k);
+      pa_zero_rows<T>(dv, dv_row, -item.len, p.head_v);
+    }
+    return;
+  }
+  const int first = item.first + slot.sub * 32, mine = first + (lane & 31);
+  if (first >= item.len) return;
+  const bool ok = mine < item.len;
+  const int64_t row = item.row0 + (int64_t)mine;
+  Frag kf[D / 16], vf[D / 16];
+  pa_own_row<T, D>(kf, reinterpret_cast<const T*>(p.k) + row * p.k_row + (int64_t)kvh * p.k_head, ok, p.head_k, lane);
+  pa_own_row<T, D>(vf, reinterpret_cast<const T*>(p.v) + row * p.v_row + (int64_t)kvh * p.v_head, ok, p.head_v, lane);
+  const int q_lo = p.causal ? first / PA_TILE : 0;
+  const int per_head = (item.len + PA_TILE - 1) / PA_TILE - q_lo, tiles = per_head * group;
+  const float c = p.scale * 1.4426950408889634f;
+  uint8_t* qimg = lds + wave * 2 * IMG;
+  uint8_t* dimg = qimg + IMG;
+  auto at = [&](int n, int& head, int& q0) {
+    const int hg = n / per_head;
+    head = kvh * group + hg;
+    q0 = (q_lo + n - hg * per_head) * PA_TILE;
+  };
+  auto load_q = [&](int n) {
+    int head, q0;
+    at(n, head, q0);
+    Img::template stage<PA_TILE, 1>(qimg, reinterpret_cast<const T*>(p.q) + (item.row0 + (int64_t)q0) * p.q_row + (int64_t)head * p.q_head,
+                                    p.q_row, item.len - q0, p.head_k, 0, lane);
+  };
+  auto load_d = [&](int n) {
+    int head, q0;
+    at(n, head, q0);
+    Img::template stage<PA_TILE, 1>(dimg, reinterpret_cast<const T*>(p.dout) + (item.row0 + (int64_t)q0) * p.do_row + (int64_t)head * p.do_head,
+                                    p.do_row, item.len - q0, p.head_v, 0, lane);
+  };
+  f32x16 ak[D / 32], av[D / 32];
+  pa_clear(ak);
+  pa_clear(av);
+  if (wave < tiles) {
+    load_d(wave);
+    load_q(wave);
+  }
+  for (int n = wave; n < tiles; n += 4) {
+    const bool more = n + 4 < tiles;
+    int head, q0;
+    at(n, head, q0);
+    // L and D of the tile's rows: lanes 0-31 fetch one, 32-63 the other, read back from LDS four at a time
+    const int qi = q0 + (lane & 31);
+    const float* src = lane < 32 ? p.lse : p.delta;
+    stat[wave][lane] = qi < item.len ? src[(int64_t)head * p.rows + item.row0 + qi] : 0.f;
+    pa_wait_vm<0>();
+    f32x16 s[1], d[1];
+    pa_clear(s);
+    pa_clear(d);
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks)
+      if (pa_step<T>(16 * ks, p.head_v)) d[0] = pa_mma(Img::rows(dimg, 0, ks, lane), vf[ks], d[0]);
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks)
+      if (pa_step<T>(16 * ks, p.head_k)) s[0] = pa_mma(Img::rows(qimg, 0, ks, lane), kf[ks], s[0]);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int r = 8 * g + 4 * (lane >> 5);
+      const f32x4 lse = *reinterpret_cast<const f32x4*>(&stat[wave][r]), delta = *reinterpret_cast<const f32x4*>(&stat[wave][32 + r]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][4 * g + e], c, -lse[e]));
+        s[0][4 * g + e] = pr;
+        d[0][4 * g + e] = pr * (d[0][4 * g + e] - delta[e]);
+      }
+    }
+    if (q0 + PA_TILE > item.len || (p.causal && q0 < first + 31)) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int qr = q0 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
+        const bool see = qr < item.len && (!p.causal || mine <= qr);
+        s[0][i] = see ? s[0][i] : 0.f;
+        d[0][i] = see ? d[0][i] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const Frag pf = pa_pack<T>(s[0], h);
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b)
+        if (pa_step<T>(32 * b, p.head_v)) av[b] = pa_mma(Img::cols(dimg, 16 * h, 32 * b, lane), pf, av[b]);
+    }
+    pa_reads_done();
+    if (more) load_d(n + 4);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const Frag sf = pa_pack<T>(d[0], h);
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b)
+        if (pa_step<T>(32 * b, p.head_k)) ak[b] = pa_mma(Img::cols(qimg, 16 * h, 32 * b, lane), sf, ak[b]);
+    }
+    pa_reads_done();
+    if (more) load_q(n + 4);
+  }
+  float* join = reinterpret_cast<float*>(lds);
+  __syncthreads();
+  pa_join<D>(join, ak, p.scale, wave, lane);
+  __syncthreads();
+  pa_join_store<T, D>(dk + (int64_t)first * dk_row, dk_row, join, item.len - first, p.head_k);
+  __syncthreads();
+  pa_join<D>(join, av, 1.f, wave, lane);
+  __syncthreads();
+  pa_join_store<T, D>(dv + (int64_t)first * dv_row, dv_row, join, item.len - first, p.head_v);
+}
+
 // ---- launchers ----------------------------------------------------------------------------------------------------------
 template <typename T, int D>
-static int pa_launch(const MtPackedAttn& p, int pass, hipStream_t stream) {
-  constexpr int BN = sizeof(T) == 2 ? 64 : 32;
-  if (pass == 0)
-    hipLaunchKernelGGL((mt_pattn_fwd_kernel<T, D, BN>), dim3(p.n_items * p.heads), dim3(PA_THREADS), 0, stream, p);
-  else if (pass == 1)
-    hipLaunchKernelGGL((mt_pattn_dq_kernel<T, D, BN>), dim3(p.n_items * p.heads), dim3(PA_THREADS), 0, stream, p);
-  else
-    hipLaunchKernelGGL((mt_pattn_dkv_kernel<T, D, BN>), dim3(p.n_items * p.kv_heads), dim3(PA_THREADS), 0, stream, p);
+static int pa_launch(const MtPackedAttn& p, int pass, bool split, hipStream_t stream) {
+  const int lanes = pass == 2 ? p.kv_heads : p.heads;
+  const dim3 grid((unsigned)(p.n_items * lanes * (split ? 4 : 1))), block(PA_THREADS);
+  if (split) {
+    if (pass == 0) hipLaunchKernelGGL((mt_pattn_split_fwd_kernel<T, D>), grid, block, 0, stream, p);
+    else if (pass == 1) hipLaunchKernelGGL((mt_pattn_split_dq_kernel<T, D>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((mt_pattn_split_dkv_kernel<T, D>), grid, block, 0, stream, p);
+  } else if constexpr (sizeof(T) == 2) {
+    if (pass == 0) hipLaunchKernelGGL((mt_pattn_fwd_kernel<T, D, 64>), grid, block, 0, stream, p);
+    else if (pass == 1) hipLaunchKernelGGL((mt_pattn_dq_kernel<T, D, 64>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((mt_pattn_dkv_kernel<T, D, 64>), grid, block, 0, stream, p);
+  }
   return (int)hipGetLastError();
 }
 
@@ -537,8 +918,9 @@ extern "C" int mt_packed_attn_sizes(int* item_bytes, int* tile_rows) {
   return (int)sizeof(MtPackedAttn);
 }
 
-// pass: 0 forward, 1 dq + D, 2 dk + dv.  bf16: 0 = f32 operands, 1 = bf16.  Rows are read in 16-byte pieces.
-extern "C" int mt_packed_attn_launch(const MtPackedAttn* a, int pass, int bf16, hipStream_t stream) {
+// pass: 0 forward, 1 dq + D, 2 dk + dv.  bf16: 0 = f32 operands (always the split form), 1 = bf16.  Rows are read in 16-byte
+// pieces.
+extern "C" int mt_packed_attn_launch(const MtPackedAttn* a, int pass, int bf16, int split, hipStream_t stream) {
   if (a == nullptr || pass < 0 || pass > 2) return -2;
   const MtPackedAttn p = *a;
   if (p.n_items <= 0) return 0;
@@ -547,7 +929,7 @@ extern "C" int mt_packed_attn_launch(const MtPackedAttn* a, int pass, int bf16, 
   if (p.head_k < 1 || p.head_v < 1 || widest > 128 || p.head_k % per || p.head_v % per) return -2;
   if (p.heads < 1 || p.kv_heads < 1 || p.heads % p.kv_heads) return -2;
   if ((p.items == nullptr) && (p.uniform_len < 1 || p.count < 1)) return -2;
-  if ((int64_t)p.n_items * p.heads > 0x7FFFFFFF || !(p.scale > 0.f)) return -2;
+  if ((int64_t)p.n_items * p.heads * 4 > 0x7FFFFFFF || !(p.scale > 0.f)) return -2;
   const int64_t strides[8] = {p.q_row, p.q_head, p.k_row, p.k_head, p.v_row, p.v_head, p.do_row, p.do_head};
   for (int i = 0; i < 8; ++i)      // 32-bit byte offsets inside a staged tile of at most 64 rows
     if (strides[i] < 0 || strides[i] % per || strides[i] * es > (1 << 24)) return -2;
@@ -555,11 +937,11 @@ extern "C" int mt_packed_attn_launch(const MtPackedAttn* a, int pass, int bf16, 
   for (int i = 0; i < 9; ++i)
     if (reinterpret_cast<uintptr_t>(ptrs[i]) & 15) return -2;
   if (bf16) {
-    if (widest <= 32) return pa_launch<__bf16, 32>(p, pass, stream);
-    if (widest <= 64) return pa_launch<__bf16, 64>(p, pass, stream);
-    return pa_launch<__bf16, 128>(p, pass, stream);
+    if (widest <= 32) return pa_launch<__bf16, 32>(p, pass, split != 0, stream);
+    if (widest <= 64) return pa_launch<__bf16, 64>(p, pass, split != 0, stream);
+    return pa_launch<__bf16, 128>(p, pass, split != 0, stream);
   }
-  if (widest <= 32) return pa_launch<float, 32>(p, pass, stream);
-  if (widest <= 64) return pa_launch<float, 64>(p, pass, stream);
-  return pa_launch<float, 128>(p, pass, stream);
+  if (widest <= 32) return pa_launch<float, 32>(p, pass, true, stream);
+  if (widest <= 64) return pa_launch<float, 64>(p, pass, true, stream);
+  return pa_launch<float, 128>(p, pass, true, stream);
 }

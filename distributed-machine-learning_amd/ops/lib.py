@@ -239,7 +239,7 @@ def load(build_if_missing: bool = True) -> C.CDLL:
     lib.mt_norm_fwd_launch.argtypes = [c_void_p] * 5 + [C.c_int64, C.c_int64, C.c_int, c_float, C.c_int, C.c_int, c_void_p]
     lib.mt_norm_bwd_launch.argtypes = [c_void_p] * 8 + [C.c_int64] * 3 + [C.c_int] * 3 + [c_void_p]
     lib.mt_norm_bwd_parts.restype = lib.mt_norm_fwd_launch.restype = lib.mt_norm_bwd_launch.restype = C.c_int
-    lib.mt_packed_attn_launch.argtypes = [C.POINTER(PackedAttn), C.c_int, C.c_int, c_void_p]
+    lib.mt_packed_attn_launch.argtypes = [C.POINTER(PackedAttn), C.c_int, C.c_int, C.c_int, c_void_p]
     lib.mt_packed_attn_launch.restype = C.c_int
     lib.mt_ln_fwd_launch.argtypes = [c_void_p] * 8 + [C.c_int, C.c_int, c_float, c_float, c_void_p, c_float, c_void_p]
     lib.mt_ln_bwd_launch.argtypes = [c_void_p] * 8 + [C.c_int, C.c_int, c_float, c_void_p, c_float, c_void_p]

@@ -106,6 +106,24 @@ def test_forward_and_gradients(dtype, causal, lengths, heads, kv_heads, dk, dv):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("below", [0, 1 << 30])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,dk,dv", [(2, 2, 64, 64), (4, 2, 32, 32), (3, 1, 128, 128), (2, 1, 20, 36)])
+def test_both_bf16_forms(monkeypatch, below, causal, heads, kv_heads, dk, dv):
+    """The form whose waves share a tile and the one whose waves share a walk, whatever the launch's size would pick."""
+    from mitune.ops import attention_hip
+    from mitune.ops.attention import SequencePack
+    monkeypatch.setattr(attention_hip, "SPLIT_BELOW", below)
+    lengths = [129, 5, 0, 300, 64, 33]
+    rows = sum(lengths) + 150
+    q, k, v, do = _inputs(lengths, rows, heads, kv_heads, dk, dv, torch.bfloat16)
+    got = _grads(q, k, v, SequencePack(lengths, rows=rows), do, causal)
+    _check(got, *_plain(q, k, v, lengths, causal, dk ** -0.5, do, True))
+    for t in got:
+        assert not t[sum(lengths):].any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_a_longer_sequence_with_a_scale_and_many_tiles(dtype):
     from mitune.ops.attention import SequencePack
