@@ -76,6 +76,14 @@ template <> __device__ __forceinline__ f32x8 pa_pack<float>(const f32x16& a, int
   return f32x8{a[8 * s], a[8 * s + 1], a[8 * s + 2], a[8 * s + 3], a[8 * s + 4], a[8 * s + 5], a[8 * s + 6], a[8 * s + 7]};
 }
 
+template <typename V> __device__ __forceinline__ const __attribute__((address_space(3))) V* pa_lds(uint32_t at) {
+  return (const __attribute__((address_space(3))) V*)at;
+}
+template <typename V> __device__ __forceinline__ __attribute__((address_space(3))) V* pa_lds_mut(uint32_t at) {
+  return (__attribute__((address_space(3))) V*)at;
+}
+__device__ __forceinline__ uint32_t pa_lds_at(const uint8_t* p) { return (uint32_t)(uintptr_t)(const lds_u8*)p; }
+
 // LDS image of rows of D elements: 16-byte chunk c of row r sits at chunk c ^ swz(r), so that eight rows read at one column
 // (row fragments) and four rows x 32 bytes (transposed reads) both cover all banks.
 template <typename T, int D> struct PaImg {
@@ -90,39 +98,45 @@ template <typename T, int D> struct PaImg {
   }
   static __device__ __forceinline__ int at(int r, int chunk) { return r * ROWB + ((chunk ^ swz(r)) << 4); }
 
+  // Fragment reads take an LDS byte address: the image's (a multiple of 1 KiB) plus row_base or col_base of the lane, worked out
+  // once.  What is left per fragment is one exclusive-or with a constant (the swizzle leaves bits above a row alone) and an
+  // immediate offset.
+  static __device__ __forceinline__ uint32_t row_base(int lane) {
+    const int r = lane & 31, h = lane >> 5;
+    return (uint32_t)at(r, sizeof(T) == 2 ? h : 2 * h);
+  }
   // 16 columns 16 s + 8 h + j of row row0 + (lane & 31)
-  static __device__ __forceinline__ typename PaFrag<T>::type rows(const uint8_t* img, int row0, int s, int lane) {
-    const int r = row0 + (lane & 31), h = lane >> 5;
+  static __device__ __forceinline__ typename PaFrag<T>::type rows(uint32_t base, int row0, int s) {
     if constexpr (sizeof(T) == 2) {
-      return __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(img + at(r, 2 * s + h)));
+      return __builtin_bit_cast(bf16x8, *pa_lds<u32x4>((base ^ (s << 5)) + row0 * ROWB));
     } else {
-      const f32x4 lo = *reinterpret_cast<const f32x4*>(img + at(r, 4 * s + 2 * h));
-      const f32x4 hi = *reinterpret_cast<const f32x4*>(img + at(r, 4 * s + 2 * h + 1));
+      const f32x4 lo = *pa_lds<f32x4>((base ^ (s << 6)) + row0 * ROWB), hi = *pa_lds<f32x4>((base ^ (s << 6) ^ 16) + row0 * ROWB);
       return f32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     }
   }
-  // column col0 + (lane & 31) of the 16 rows row0 + 8 (j / 4) + 4 h + j % 4: the order of an accumulator's rows
-  static __device__ __forceinline__ typename PaFrag<T>::type cols(const uint8_t* img, int row0, int col0, int lane) {
+  static __device__ __forceinline__ uint32_t col_base(int lane) {
     const int h = lane >> 5;
     if constexpr (sizeof(T) == 2) {
       const int i = lane & 15, q = i >> 2, p = i & 3;
-      const int c = (col0 + (lane & 16)) / 8 + (p >> 1);
-      const int r = row0 + 4 * h + q;
-      const lds_u8* a0 = (const lds_u8*)(img + at(r, c) + 8 * (p & 1));
-      const lds_u8* a1 = (const lds_u8*)(img + at(r + 8, c) + 8 * (p & 1));
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a0);
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a1);
+      return (uint32_t)(at(4 * h + q, (lane & 16) / 8 + (p >> 1)) + 8 * (p & 1));
+    } else {
+      return (uint32_t)(at(4 * h, (lane & 31) >> 2) + 4 * (lane & 3));
+    }
+  }
+  // column 32 b + (lane & 31) of the 16 rows row0 + 8 (j / 4) + 4 h + j % 4 (row0 a multiple of 16): the order of an
+  // accumulator's rows
+  static __device__ __forceinline__ typename PaFrag<T>::type cols(uint32_t base, int row0, int b) {
+    if constexpr (sizeof(T) == 2) {
+      constexpr int FAR = D == 128 ? 32 : 0;           // how the swizzle of row r + 8 differs from that of r
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(pa_lds_mut<s16x4>((base ^ (b << 6)) + row0 * ROWB));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(pa_lds_mut<s16x4>((base ^ (b << 6) ^ FAR) + (row0 + 8) * ROWB));
       typedef __attribute__((ext_vector_type(8))) short s16x8;
       const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
       return __builtin_bit_cast(bf16x8, v);
     } else {
-      const int col = col0 + (lane & 31);
       f32x8 v;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int r = row0 + 8 * (j >> 2) + 4 * h + (j & 3);
-        v[j] = *reinterpret_cast<const float*>(img + at(r, col >> 2) + 4 * (col & 3));
-      }
+      for (int j = 0; j < 8; ++j) v[j] = *pa_lds<float>((base ^ (b << 7) ^ ((j & 3) << 4)) + (row0 + 8 * (j >> 2) + (j & 3)) * ROWB);
       return v;
     }
   }
@@ -146,7 +160,15 @@ template <typename T, int D> struct PaImg {
   }
 };
 
-__device__ __forceinline__ float pa_other_half(float v) { return __shfl_xor(v, 32, 64); }
+// max / sum with the lane 32 further on: one exchange of the wave's halves, no LDS
+__device__ __forceinline__ float pa_half_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float pa_half_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 
 template <typename T> __device__ __forceinline__ typename PaFrag<T>::type pa_zero_frag() {
   typename PaFrag<T>::type f;
@@ -262,7 +284,7 @@ __device__ __forceinline__ void pa_dq_rows(const MtPackedAttn& p, typename PaFra
   for (int s = 0; s < D / 16; ++s)
 #pragma unroll
     for (int j = 0; j < 8; ++j) delta = __builtin_fmaf((float)df[s][j], (float)qf[s][j], delta);
-  delta += pa_other_half(delta);
+  delta = pa_half_sum(delta);
   if (ok) {
     lse = p.lse[(int64_t)head * p.rows + row];
     if (store && lane < 32) p.delta[(int64_t)head * p.rows + row] = delta;
@@ -308,34 +330,52 @@ __global__ __launch_bounds__(PA_THREADS, 2) void mt_pattn_fwd_kernel(const MtPac
   f32x16 acc[D / 32];
   pa_clear(acc);
   float m = -INFINITY, sum = 0.f;
-  issue(0);
-  for (int t = 0; t < tiles; ++t) {
-    pa_tile_barrier();
-    if (t + 1 < tiles) issue(t + 1);
+  const uint32_t lds_at = pa_lds_at(lds);
+  // One tile.  Fragments are read in groups, the next group on its way while the products of one run: the scheduling barriers
+  // keep that order (left alone the compiler reads each fragment right before its product and waits for it: 1.4x the time).
+  auto step = [&](int t, bool masked) {
     const int k0 = t * BN;
-    if (p.causal && k0 > first + 31) continue;          // none of this wave's queries sees the tile (uniform; still at the barriers)
-    const uint8_t* kimg = lds + (t & 1) * 2 * IMG;
-    const uint8_t* vimg = kimg + IMG;
-    f32x16 s[BN / 32];
+    const uint32_t krow = lds_at + (t & 1) * 2 * IMG + Img::row_base(lane), vcol = lds_at + ((t & 1) * 2 + 1) * IMG + Img::col_base(lane);
+    constexpr int U = BN / 32, KG = D / 32, PG = BN / 16;      // groups: two steps of the scores; 16 keys of the output
+    Frag kf[2][2][U], vf[2][D / 32];
+    auto read_k = [&](int g) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int u = 0; u < U; ++u) kf[g & 1][e][u] = Img::rows(krow, 32 * u, 2 * g + e);
+    };
+    auto read_v = [&](int g) {
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b) vf[g & 1][b] = Img::cols(vcol, 16 * g, b);
+    };
+    f32x16 s[U];
     pa_clear(s);
+    read_k(0);
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks)
+    for (int g = 0; g < KG; ++g) {
+      if (g + 1 < KG) read_k(g + 1);
+      else read_v(0);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int u = 0; u < BN / 32; ++u) s[u] = pa_mma(Img::rows(kimg, 32 * u, ks, lane), qf[ks], s[u]);
-    if (k0 + BN > item.len || (p.causal && k0 + BN - 1 > first)) {
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int u = 0; u < U; ++u) s[u] = pa_mma(kf[g & 1][e][u], qf[2 * g + e], s[u]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (masked) {
       const int last = p.causal && mine < item.len ? mine : item.len - 1;
 #pragma unroll
-      for (int u = 0; u < BN / 32; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           s[u][i] = k0 + 32 * u + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3) <= last ? s[u][i] : -INFINITY;
     }
     float mx = s[0][0];
 #pragma unroll
-    for (int u = 0; u < BN / 32; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
-    mx = fmaxf(mx, pa_other_half(mx)) * c;
+    mx = pa_half_max(mx) * c;
     // The subtracted maximum is only moved when some row grew by more than 2^8 over it: probabilities stay within f32 (and
     // bf16 keeps its relative precision), and most tiles skip the pass over the accumulator.
     if (__any(mx > m + 8.f)) {
@@ -350,22 +390,42 @@ __global__ __launch_bounds__(PA_THREADS, 2) void mt_pattn_fwd_kernel(const MtPac
     }
     const float sub = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int u = 0; u < BN / 32; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         s[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], c, -sub));
         sum += s[u][i];
       }
 #pragma unroll
-    for (int u = 0; u < BN / 32; ++u)
+    for (int g = 0; g < PG; ++g) {
+      if (g + 1 < PG) read_v(g + 1);
+      const Frag pf = pa_pack<T>(s[g >> 1], g & 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const Frag pf = pa_pack<T>(s[u], h);
-#pragma unroll
-        for (int b = 0; b < D / 32; ++b) acc[b] = pa_mma(Img::cols(vimg, 32 * u + 16 * h, 32 * b, lane), pf, acc[b]);
-      }
+      for (int b = 0; b < D / 32; ++b) acc[b] = pa_mma(vf[g & 1][b], pf, acc[b]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // Tiles that all of this wave's queries see whole, tiles that need the mask, and tiles it only helps to fetch.
+  const int mine_end = p.causal && first + 32 < keys ? first + 32 : keys;          // keys this wave looks at
+  const int own = first < item.len ? (mine_end + BN - 1) / BN : 0;
+  const int whole = p.causal && first + 1 < mine_end ? (first + 1) / BN : mine_end / BN;
+  issue(0);
+  auto enter = [&](int t) {
+    pa_tile_barrier();
+    if (t + 1 < tiles) issue(t + 1);
+  };
+  int t = 0;
+  for (; t < whole && t < own; ++t) {
+    enter(t);
+    step(t, false);
   }
-  sum += pa_other_half(sum);
+  for (; t < own; ++t) {
+    enter(t);
+    step(t, true);
+  }
+  for (; t < tiles; ++t) enter(t);
+  sum = pa_half_sum(sum);
   if (mine < item.len) {
     pa_store_row<T, D>(o + (int64_t)mine * o_row, acc, sum > 0.f || sum != sum ? 1.f / sum : 0.f, p.head_v, lane);
     if (p.lse != nullptr && lane < 32)      // a row whose scores are all -inf weighs nothing in the backward pass
@@ -408,40 +468,73 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
   };
   f32x16 acc[D / 32];
   pa_clear(acc);
+  const uint32_t lds_at = pa_lds_at(lds);
+  const int last = p.causal && ok ? mine : item.len - 1;
+  // 32 keys at a time; fragments in groups read one group ahead, as in the forward kernel: V, K, then K's columns
+  auto step = [&](int t, int u, bool masked) {
+    const uint32_t kimg = lds_at + (t & 1) * 2 * IMG, krow = kimg + Img::row_base(lane), kcol = kimg + Img::col_base(lane), vrow = krow + IMG;
+    constexpr int G = D / 16 < 4 ? D / 16 : 4, NG = D / 16 / G;
+    Frag fr[2][G], cf[2][D / 32];
+    auto read_rows = [&](int g) {          // groups 0 .. NG - 1 of V, then of K
+#pragma unroll
+      for (int e = 0; e < G; ++e) fr[g & 1][e] = Img::rows(g < NG ? vrow : krow, 32 * u, (g % NG) * G + e);
+    };
+    auto read_cols = [&](int h) {
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b) cf[h][b] = Img::cols(kcol, 32 * u + 16 * h, b);
+    };
+    f32x16 s[1], d[1];
+    pa_clear(s);
+    pa_clear(d);
+    read_rows(0);
+#pragma unroll
+    for (int g = 0; g < 2 * NG; ++g) {
+      if (g + 1 < 2 * NG) read_rows(g + 1);
+      else read_cols(0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int e = 0; e < G; ++e) {
+        if (g < NG) d[0] = pa_mma(fr[g & 1][e], df[(g % NG) * G + e], d[0]);
+        else s[0] = pa_mma(fr[g & 1][e], qf[(g % NG) * G + e], s[0]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[0][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][i], c, -lse)) * (d[0][i] - delta);
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[0][i] = t * BN + 32 * u + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3) <= last ? s[0][i] : 0.f;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (h == 0) read_cols(1);
+      const Frag sf = pa_pack<T>(s[0], h);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b) acc[b] = pa_mma(cf[h][b], sf, acc[b]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  const int mine_end = p.causal && first + 32 < keys ? first + 32 : keys;
+  const int own = first < item.len ? (mine_end + BN - 1) / BN : 0;
+  const int whole = p.causal && first + 1 < mine_end ? (first + 1) / BN : mine_end / BN;
   issue(0);
-  for (int t = 0; t < tiles; ++t) {
+  auto enter = [&](int t) {
     pa_tile_barrier();
     if (t + 1 < tiles) issue(t + 1);
-    const int k0 = t * BN;
-    if (p.causal && k0 > first + 31) continue;
-    const uint8_t* kimg = lds + (t & 1) * 2 * IMG;
-    const uint8_t* vimg = kimg + IMG;
-    const bool masked = k0 + BN > item.len || (p.causal && k0 + BN - 1 > first);
-    const int last = p.causal && ok ? mine : item.len - 1;
-#pragma unroll
-    for (int u = 0; u < BN / 32; ++u) {
-      f32x16 s[1], d[1];
-      pa_clear(s);
-      pa_clear(d);
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) s[0] = pa_mma(Img::rows(kimg, 32 * u, ks, lane), qf[ks], s[0]);
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) d[0] = pa_mma(Img::rows(vimg, 32 * u, ks, lane), df[ks], d[0]);
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        s[0][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][i], c, -lse)) * (d[0][i] - delta);
-      if (masked) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[0][i] = k0 + 32 * u + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3) <= last ? s[0][i] : 0.f;
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const Frag sf = pa_pack<T>(s[0], h);
-#pragma unroll
-        for (int b = 0; b < D / 32; ++b) acc[b] = pa_mma(Img::cols(kimg, 32 * u + 16 * h, 32 * b, lane), sf, acc[b]);
-      }
-    }
+  };
+  int t = 0;
+  for (; t < whole && t < own; ++t) {
+    enter(t);
+    step(t, 0, false);
+    if (BN > 32) step(t, 1, false);
   }
+  for (; t < own; ++t) {
+    enter(t);
+    step(t, 0, true);
+    if (BN > 32 && t * BN + 32 < mine_end) step(t, 1, true);
+  }
+  for (; t < tiles; ++t) enter(t);
   if (ok) pa_store_row<T, D>(dq + (int64_t)mine * dq_row, acc, p.scale, p.head_k, lane);
 }
 
@@ -494,6 +587,7 @@ __global__ __launch_bounds__(PA_THREADS, 1) void mt_pattn_dkv_kernel(const MtPac
   f32x16 ak[D / 32], av[D / 32];
   pa_clear(ak);
   pa_clear(av);
+  const uint32_t lds_at = pa_lds_at(lds);
   issue(0, 0, q_lo);
   int hg = 0, qt = q_lo;
   for (int n = 0; n < tiles; ++n) {
@@ -501,20 +595,38 @@ __global__ __launch_bounds__(PA_THREADS, 1) void mt_pattn_dkv_kernel(const MtPac
     if (++qt == q_lo + per_head) { qt = q_lo; ++hg; }
     pa_tile_barrier();
     if (n + 1 < tiles) issue(n + 1, hg, qt);
-    const uint8_t* qimg = lds + (n & 1) * STAGE;
-    const uint8_t* dimg = qimg + IMG;
-    const float* stat = reinterpret_cast<const float*>(qimg + 2 * IMG);
+    const float* stat = reinterpret_cast<const float*>(lds + (n & 1) * STAGE + 2 * IMG);
+    const uint32_t qimg = lds_at + (n & 1) * STAGE, qrow = qimg + Img::row_base(lane), qcol = qimg + Img::col_base(lane);
+    constexpr int G = D / 16 < 4 ? D / 16 : 4, NG = D / 16 / G;
 #pragma unroll
     for (int u = 0; u < BQ / 32; ++u) {
       const int qu = q0 + 32 * u;
       if (qu >= item.len || (p.causal && qu + 31 < first)) continue;
+      Frag fr[2][G], cf[2][D / 32];
+      auto read_rows = [&](int g) {          // groups 0 .. NG - 1 of q, then of do
+#pragma unroll
+        for (int e = 0; e < G; ++e) fr[g & 1][e] = Img::rows(g < NG ? qrow : qrow + IMG, 32 * u, (g % NG) * G + e);
+      };
+      auto read_cols = [&](int g) {          // do's columns of two times 16 rows, then q's
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) cf[g & 1][b] = Img::cols(g < 2 ? qcol + IMG : qcol, 32 * u + 16 * (g & 1), b);
+      };
       f32x16 s[1], d[1];
       pa_clear(s);
       pa_clear(d);
+      read_rows(0);
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) s[0] = pa_mma(Img::rows(qimg, 32 * u, ks, lane), kf[ks], s[0]);
+      for (int g = 0; g < 2 * NG; ++g) {
+        if (g + 1 < 2 * NG) read_rows(g + 1);
+        else read_cols(0);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) d[0] = pa_mma(Img::rows(dimg, 32 * u, ks, lane), vf[ks], d[0]);
+        for (int e = 0; e < G; ++e) {
+          if (g < NG) s[0] = pa_mma(fr[g & 1][e], kf[(g % NG) * G + e], s[0]);
+          else d[0] = pa_mma(fr[g & 1][e], vf[(g % NG) * G + e], d[0]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int at = 32 * u + 8 * g + 4 * (lane >> 5);
@@ -536,12 +648,16 @@ __global__ __launch_bounds__(PA_THREADS, 1) void mt_pattn_dkv_kernel(const MtPac
         }
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const Frag pf = pa_pack<T>(s[0], h), sf = pa_pack<T>(d[0], h);
+      for (int g = 0; g < 4; ++g) {
+        if (g < 3) read_cols(g + 1);
+        const Frag pf = pa_pack<T>(g < 2 ? s[0] : d[0], g & 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int b = 0; b < D / 32; ++b) av[b] = pa_mma(Img::cols(dimg, 32 * u + 16 * h, 32 * b, lane), pf, av[b]);
-#pragma unroll
-        for (int b = 0; b < D / 32; ++b) ak[b] = pa_mma(Img::cols(qimg, 32 * u + 16 * h, 32 * b, lane), sf, ak[b]);
+        for (int b = 0; b < D / 32; ++b) {
+          if (g < 2) av[b] = pa_mma(cf[g & 1][b], pf, av[b]);
+          else ak[b] = pa_mma(cf[g & 1][b], pf, ak[b]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
@@ -604,6 +720,7 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
   const float c = p.scale * 1.4426950408889634f;
   uint8_t* kimg = lds + wave * 2 * IMG;
   uint8_t* vimg = kimg + IMG;
+  const uint32_t krow = pa_lds_at(kimg) + Img::row_base(lane), kcol = pa_lds_at(kimg) + Img::col_base(lane);
   auto load_k = [&](int t) {
     Img::template stage<PA_TILE, 1>(kimg, kb + (int64_t)t * PA_TILE * p.k_row, p.k_row, item.len - t * PA_TILE, p.head_k, 0, lane);
   };
@@ -624,7 +741,7 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
     pa_clear(s);
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks)
-      if (pa_step<T>(16 * ks, p.head_k)) s[0] = pa_mma(Img::rows(kimg, 0, ks, lane), qf[ks], s[0]);
+      if (pa_step<T>(16 * ks, p.head_k)) s[0] = pa_mma(Img::rows(krow, 0, ks), qf[ks], s[0]);
     pa_reads_done();
     if (more) load_k(t + 4);
     const int k0 = t * PA_TILE;
@@ -636,7 +753,7 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
     float mx = s[0][0];
 #pragma unroll
     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[0][i]);
-    mx = fmaxf(mx, pa_other_half(mx)) * c;
+    mx = pa_half_max(mx) * c;
     if (__any(mx > m + 8.f)) {
       const float mn = fmaxf(m, mx);
       const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
@@ -660,12 +777,12 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
       const Frag pf = pa_pack<T>(s[0], h);
 #pragma unroll
       for (int b = 0; b < D / 32; ++b)
-        if (pa_step<T>(32 * b, p.head_v)) acc[b] = pa_mma(Img::cols(vimg, 16 * h, 32 * b, lane), pf, acc[b]);
+        if (pa_step<T>(32 * b, p.head_v)) acc[b] = pa_mma(Img::cols(kcol + IMG, 16 * h, b), pf, acc[b]);
     }
     pa_reads_done();
     if (more) load_v(t + 4);
   }
-  sum += pa_other_half(sum);
+  sum = pa_half_sum(sum);
   if (lane < 32) {
     stat[0][wave][lane] = m;
     stat[1][wave][lane] = sum;
@@ -715,6 +832,7 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
   const float c = p.scale * 1.4426950408889634f;
   uint8_t* kimg = lds + wave * 2 * IMG;
   uint8_t* vimg = kimg + IMG;
+  const uint32_t krow = pa_lds_at(kimg) + Img::row_base(lane), kcol = pa_lds_at(kimg) + Img::col_base(lane);
   auto load_k = [&](int t) {
     Img::template stage<PA_TILE, 1>(kimg, kb + (int64_t)t * PA_TILE * p.k_row, p.k_row, item.len - t * PA_TILE, p.head_k, 0, lane);
   };
@@ -735,7 +853,7 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
     pa_clear(d);
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks)
-      if (pa_step<T>(16 * ks, p.head_v)) d[0] = pa_mma(Img::rows(vimg, 0, ks, lane), df[ks], d[0]);
+      if (pa_step<T>(16 * ks, p.head_v)) d[0] = pa_mma(Img::rows(krow + IMG, 0, ks), df[ks], d[0]);
     pa_reads_done();
     if (more) {
       load_v(t + 4);
@@ -745,7 +863,7 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
     }
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks)
-      if (pa_step<T>(16 * ks, p.head_k)) s[0] = pa_mma(Img::rows(kimg, 0, ks, lane), qf[ks], s[0]);
+      if (pa_step<T>(16 * ks, p.head_k)) s[0] = pa_mma(Img::rows(krow, 0, ks), qf[ks], s[0]);
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[0][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][i], c, -lse)) * (d[0][i] - delta);
     const int k0 = t * PA_TILE;
@@ -759,7 +877,7 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
       const Frag sf = pa_pack<T>(s[0], h);
 #pragma unroll
       for (int b = 0; b < D / 32; ++b)
-        if (pa_step<T>(32 * b, p.head_k)) acc[b] = pa_mma(Img::cols(kimg, 16 * h, 32 * b, lane), sf, acc[b]);
+        if (pa_step<T>(32 * b, p.head_k)) acc[b] = pa_mma(Img::cols(kcol, 16 * h, b), sf, acc[b]);
     }
     pa_reads_done();
     if (more) load_k(t + 4);
@@ -803,6 +921,7 @@ __global__ __launch_bounds__(PA_THREADS, 1) void mt_pattn_split_dkv_kernel(const
   const float c = p.scale * 1.4426950408889634f;
   uint8_t* qimg = lds + wave * 2 * IMG;
   uint8_t* dimg = qimg + IMG;
+  const uint32_t qrow = pa_lds_at(qimg) + Img::row_base(lane), qcol = pa_lds_at(qimg) + Img::col_base(lane);
   auto at = [&](int n, int& head, int& q0) {
     const int hg = n / per_head;
     head = kvh * group + hg;
@@ -841,10 +960,10 @@ __global__ __launch_bounds__(PA_THREADS, 1) void mt_pattn_split_dkv_kernel(const
     pa_clear(d);
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks)
-      if (pa_step<T>(16 * ks, p.head_v)) d[0] = pa_mma(Img::rows(dimg, 0, ks, lane), vf[ks], d[0]);
+      if (pa_step<T>(16 * ks, p.head_v)) d[0] = pa_mma(Img::rows(qrow + IMG, 0, ks), vf[ks], d[0]);
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks)
-      if (pa_step<T>(16 * ks, p.head_k)) s[0] = pa_mma(Img::rows(qimg, 0, ks, lane), kf[ks], s[0]);
+      if (pa_step<T>(16 * ks, p.head_k)) s[0] = pa_mma(Img::rows(qrow, 0, ks), kf[ks], s[0]);
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int r = 8 * g + 4 * (lane >> 5);
@@ -870,7 +989,7 @@ __global__ __launch_bounds__(PA_THREADS, 1) void mt_pattn_split_dkv_kernel(const
       const Frag pf = pa_pack<T>(s[0], h);
 #pragma unroll
       for (int b = 0; b < D / 32; ++b)
-        if (pa_step<T>(32 * b, p.head_v)) av[b] = pa_mma(Img::cols(dimg, 16 * h, 32 * b, lane), pf, av[b]);
+        if (pa_step<T>(32 * b, p.head_v)) av[b] = pa_mma(Img::cols(qcol + IMG, 16 * h, b), pf, av[b]);
     }
     pa_reads_done();
     if (more) load_d(n + 4);
@@ -879,7 +998,7 @@ __global__ __launch_bounds__(PA_THREADS, 1) void mt_pattn_split_dkv_kernel(const
       const Frag sf = pa_pack<T>(d[0], h);
 #pragma unroll
       for (int b = 0; b < D / 32; ++b)
-        if (pa_step<T>(32 * b, p.head_k)) ak[b] = pa_mma(Img::cols(qimg, 16 * h, 32 * b, lane), sf, ak[b]);
+        if (pa_step<T>(32 * b, p.head_k)) ak[b] = pa_mma(Img::cols(qcol, 16 * h, b), sf, ak[b]);
     }
     pa_reads_done();
     if (more) load_q(n + 4);
