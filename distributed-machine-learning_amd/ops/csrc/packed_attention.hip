@@ -144,7 +144,8 @@ template <typename T, int D> struct PaImg {
   // first element; rows at and past `valid` and columns past `d` arrive as zeros through the buffer's range check.
   template <int NROWS, int WAVES = 4>
   static __device__ __forceinline__ void stage(uint8_t* img, const T* base, int64_t row_stride, int valid, int d, int wave, int lane) {
-    constexpr int PIECES = NROWS * ROWB / 1024 / WAVES;
+    constexpr int ALL = NROWS * ROWB / 1024, PIECES = (ALL + WAVES - 1) / WAVES;
+    static_assert(ALL * 1024 == NROWS * ROWB && (ALL % WAVES == 0 || PIECES == 1), "an image is whole pieces, shared evenly or one each");
     const int64_t stride = row_stride * (int64_t)sizeof(T);
     const int rows = valid < NROWS ? valid : NROWS;
     const uint32_t bytes = rows > 0 ? (uint32_t)((rows - 1) * stride + d * (int)sizeof(T)) : 0u;
@@ -152,6 +153,7 @@ template <typename T, int D> struct PaImg {
 #pragma unroll
     for (int t = 0; t < PIECES; ++t) {
       const int j = wave * PIECES + t;
+      if (ALL % WAVES != 0 && j >= ALL) break;
       const int at_byte = j * 1024 + lane * 16;
       const int r = at_byte / ROWB, c = ((at_byte % ROWB) >> 4) ^ swz(r);
       const uint32_t off = c * EPC < d ? (uint32_t)(r * (uint32_t)stride + c * 16) : 0xFFFFFF00u;
@@ -232,7 +234,7 @@ __device__ __forceinline__ MtSeqItem pa_item(const MtPackedAttn& p, int i, bool 
 // Zeros for `n` rows of `d` columns of one head, which belong to no sequence.
 template <typename T>
 __device__ __forceinline__ void pa_zero_rows(T* base, int64_t row_stride, int n, int d) {
-  for (int i = threadIdx.x; i < n * d; i += PA_THREADS) {
+  for (int i = threadIdx.x; i < n * d; i += blockDim.x) {
     const int r = i / d;
     base[r * row_stride + (i - r * d)] = (T)0.f;
   }
@@ -539,13 +541,18 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
 }
 
 // ---- backward: dk and dv ------------------------------------------------------------------------------------------------
-template <typename T, int D, int BQ>
-__global__ __launch_bounds__(PA_THREADS, 1) void mt_pattn_dkv_kernel(const MtPackedAttn p) {
+// Eight waves: waves w and w + 4 own the same 32 keys and take the two halves of every 64-query tile; their sums meet in LDS at
+// the end.  The workgroup's keys and values stay in LDS beside the query tiles and are read again for every tile, because the
+// two gradients' accumulators already take half the registers of a wave when two of them are to share a SIMD.
+#define PA_DKV_THREADS 512
+template <typename T, int D>
+__global__ __launch_bounds__(PA_DKV_THREADS, 2) void mt_pattn_dkv_kernel(const MtPackedAttn p) {
   typedef PaImg<T, D> Img;
   typedef typename PaFrag<T>::type Frag;
-  constexpr int IMG = BQ * Img::ROWB;
-  constexpr int STAGE = 2 * IMG + 2 * 256;                          // q rows, do rows, L and D of up to 64 rows
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];
+  constexpr int BQ = 64, IMG = BQ * Img::ROWB, KV = PA_OWN * Img::ROWB;
+  constexpr int STAGE = 2 * IMG + 1024;                              // q rows, do rows, L and D of the 64 rows
+  constexpr int BYTES = 2 * KV + 2 * STAGE, JOIN = 2 * 128 * D * 4;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[BYTES < JOIN ? JOIN : BYTES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int it = blockIdx.x / p.kv_heads, kvh = blockIdx.x - it * p.kv_heads;
   const int group = p.heads / p.kv_heads;
@@ -558,24 +565,28 @@ __global__ __launch_bounds__(PA_THREADS, 1) void mt_pattn_dkv_kernel(const MtPac
     pa_zero_rows<T>(dv, dv_row, -item.len, p.head_v);
     return;
   }
-  const int first = item.first + wave * 32, mine = first + (lane & 31);
-  const bool ok = mine < item.len;
-  const int64_t row = item.row0 + (int64_t)mine;
-  Frag kf[D / 16], vf[D / 16];
-  pa_own_row<T, D>(kf, reinterpret_cast<const T*>(p.k) + row * p.k_row + (int64_t)kvh * p.k_head, ok, p.head_k, lane);
-  pa_own_row<T, D>(vf, reinterpret_cast<const T*>(p.v) + row * p.v_row + (int64_t)kvh * p.v_head, ok, p.head_v, lane);
+  const int block = wave & 3, half = wave >> 2;
+  const int first = item.first + block * 32, mine = first + (lane & 31);
   const int q_lo = p.causal ? item.first / BQ : 0;                  // first query tile that sees a key of this workgroup
   const int per_head = (item.len + BQ - 1) / BQ - q_lo;
   const int tiles = per_head * group;
   const float c = p.scale * 1.4426950408889634f;
+  {
+    const int64_t r0 = item.row0 + (int64_t)item.first;
+    Img::template stage<PA_OWN, 8>(lds, reinterpret_cast<const T*>(p.k) + r0 * p.k_row + (int64_t)kvh * p.k_head, p.k_row,
+                                   item.len - item.first, p.head_k, wave, lane);
+    Img::template stage<PA_OWN, 8>(lds + KV, reinterpret_cast<const T*>(p.v) + r0 * p.v_row + (int64_t)kvh * p.v_head, p.v_row,
+                                   item.len - item.first, p.head_v, wave, lane);
+  }
+  uint8_t* stages = lds + 2 * KV;
   auto issue = [&](int n, int hg, int qt) {
-    uint8_t* st = lds + (n & 1) * STAGE;
+    uint8_t* st = stages + (n & 1) * STAGE;
     const int head = kvh * group + hg, q0 = qt * BQ, left = item.len - q0;
     const int64_t r0 = item.row0 + (int64_t)q0;
-    Img::template stage<BQ>(st, reinterpret_cast<const T*>(p.q) + r0 * p.q_row + (int64_t)head * p.q_head, p.q_row, left, p.head_k,
-                            wave, lane);
-    Img::template stage<BQ>(st + IMG, reinterpret_cast<const T*>(p.dout) + r0 * p.do_row + (int64_t)head * p.do_head, p.do_row,
-                            left, p.head_v, wave, lane);
+    Img::template stage<BQ, 8>(st, reinterpret_cast<const T*>(p.q) + r0 * p.q_row + (int64_t)head * p.q_head, p.q_row, left, p.head_k,
+                               wave, lane);
+    Img::template stage<BQ, 8>(st + IMG, reinterpret_cast<const T*>(p.dout) + r0 * p.do_row + (int64_t)head * p.do_head, p.do_row,
+                               left, p.head_v, wave, lane);
     if (wave < 2) {
       const float* src = (wave == 0 ? p.lse : p.delta) + (int64_t)head * p.rows + r0;
       const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
@@ -587,81 +598,94 @@ __global__ __launch_bounds__(PA_THREADS, 1) void mt_pattn_dkv_kernel(const MtPac
   f32x16 ak[D / 32], av[D / 32];
   pa_clear(ak);
   pa_clear(av);
-  const uint32_t lds_at = pa_lds_at(lds);
+  const uint32_t lds_at = pa_lds_at(lds), st_at = lds_at + 2 * KV;
   issue(0, 0, q_lo);
   int hg = 0, qt = q_lo;
   for (int n = 0; n < tiles; ++n) {
-    const int q0 = qt * BQ;
+    const int qu = qt * BQ + 32 * half;
     if (++qt == q_lo + per_head) { qt = q_lo; ++hg; }
     pa_tile_barrier();
     if (n + 1 < tiles) issue(n + 1, hg, qt);
-    const float* stat = reinterpret_cast<const float*>(lds + (n & 1) * STAGE + 2 * IMG);
-    const uint32_t qimg = lds_at + (n & 1) * STAGE, qrow = qimg + Img::row_base(lane), qcol = qimg + Img::col_base(lane);
-    constexpr int G = D / 16 < 4 ? D / 16 : 4, NG = D / 16 / G;
+    if (qu >= item.len || (p.causal && qu + 31 < first)) continue;
+    const uint32_t rb = Img::row_base(lane), qimg = st_at + (n & 1) * STAGE;
+    const uint32_t krow = lds_at + rb, qrow = qimg + rb, qcol = qimg + Img::col_base(lane);
+    constexpr int G = 2, NG = D / 16 / G;
+    Frag fr[2][G], kr[2][G], cf[2][D / 32];
+    auto read_rows = [&](int g) {          // groups 0 .. NG - 1 of q and k, then of do and v
 #pragma unroll
-    for (int u = 0; u < BQ / 32; ++u) {
-      const int qu = q0 + 32 * u;
-      if (qu >= item.len || (p.causal && qu + 31 < first)) continue;
-      Frag fr[2][G], cf[2][D / 32];
-      auto read_rows = [&](int g) {          // groups 0 .. NG - 1 of q, then of do
-#pragma unroll
-        for (int e = 0; e < G; ++e) fr[g & 1][e] = Img::rows(g < NG ? qrow : qrow + IMG, 32 * u, (g % NG) * G + e);
-      };
-      auto read_cols = [&](int g) {          // do's columns of two times 16 rows, then q's
-#pragma unroll
-        for (int b = 0; b < D / 32; ++b) cf[g & 1][b] = Img::cols(g < 2 ? qcol + IMG : qcol, 32 * u + 16 * (g & 1), b);
-      };
-      f32x16 s[1], d[1];
-      pa_clear(s);
-      pa_clear(d);
-      read_rows(0);
-#pragma unroll
-      for (int g = 0; g < 2 * NG; ++g) {
-        if (g + 1 < 2 * NG) read_rows(g + 1);
-        else read_cols(0);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int e = 0; e < G; ++e) {
-          if (g < NG) s[0] = pa_mma(fr[g & 1][e], kf[(g % NG) * G + e], s[0]);
-          else d[0] = pa_mma(fr[g & 1][e], vf[(g % NG) * G + e], d[0]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+      for (int e = 0; e < G; ++e) {
+        fr[g & 1][e] = Img::rows(g < NG ? qrow : qrow + IMG, 32 * half, (g % NG) * G + e);
+        kr[g & 1][e] = Img::rows(g < NG ? krow : krow + KV, 32 * block, (g % NG) * G + e);
       }
+    };
+    auto read_cols = [&](int g) {          // do's columns of two times 16 rows, then q's
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int at = 32 * u + 8 * g + 4 * (lane >> 5);
-        const f32x4 lse = *reinterpret_cast<const f32x4*>(stat + at), delta = *reinterpret_cast<const f32x4*>(stat + 64 + at);
+      for (int b = 0; b < D / 32; ++b) cf[g & 1][b] = Img::cols(g < 2 ? qcol + IMG : qcol, 32 * half + 16 * (g & 1), b);
+    };
+    f32x16 s[1], d[1];
+    pa_clear(s);
+    pa_clear(d);
+    read_rows(0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][4 * g + e], c, -lse[e]));
-          s[0][4 * g + e] = pr;
-          d[0][4 * g + e] = pr * (d[0][4 * g + e] - delta[e]);
-        }
+    for (int g = 0; g < 2 * NG; ++g) {
+      if (g + 1 < 2 * NG) read_rows(g + 1);
+      else read_cols(0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int e = 0; e < G; ++e) {
+        if (g < NG) s[0] = pa_mma(fr[g & 1][e], kr[g & 1][e], s[0]);
+        else d[0] = pa_mma(fr[g & 1][e], kr[g & 1][e], d[0]);
       }
-      if (qu + 32 > item.len || (p.causal && qu < first + 31)) {
+      __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int qi = qu + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
-          const bool see = qi < item.len && (!p.causal || mine <= qi);
-          s[0][i] = see ? s[0][i] : 0.f;
-          d[0][i] = see ? d[0][i] : 0.f;
-        }
-      }
+    for (int g = 0; g < 4; ++g) {
+      // (by address: through the array the compiler would first wait for the LDS-DMA of the next tile, which may alias)
+      const uint32_t at = qimg + 2 * IMG + 4 * (32 * half + 8 * g + 4 * (lane >> 5));
+      const f32x4 lse = *pa_lds<f32x4>(at), delta = *pa_lds<f32x4>(at + 256);
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        if (g < 3) read_cols(g + 1);
-        const Frag pf = pa_pack<T>(g < 2 ? s[0] : d[0], g & 1);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int b = 0; b < D / 32; ++b) {
-          if (g < 2) av[b] = pa_mma(cf[g & 1][b], pf, av[b]);
-          else ak[b] = pa_mma(cf[g & 1][b], pf, ak[b]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+      for (int e = 0; e < 4; ++e) {
+        const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][4 * g + e], c, -lse[e]));
+        s[0][4 * g + e] = pr;
+        d[0][4 * g + e] = pr * (d[0][4 * g + e] - delta[e]);
       }
     }
+    if (qu + 32 > item.len || (p.causal && qu < first + 31)) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int qi = qu + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
+        const bool see = qi < item.len && (!p.causal || mine <= qi);
+        s[0][i] = see ? s[0][i] : 0.f;
+        d[0][i] = see ? d[0][i] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      if (g < 3) read_cols(g + 1);
+      const Frag pf = pa_pack<T>(g < 2 ? s[0] : d[0], g & 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b) {
+        if (g < 2) av[b] = pa_mma(cf[g & 1][b], pf, av[b]);
+        else ak[b] = pa_mma(cf[g & 1][b], pf, ak[b]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
-  if (ok) {
+  // [dk, dv][key block][column][key] f32 of the second halves; no LDS-DMA is in flight past the last tile's barrier
+  float* join = reinterpret_cast<float*>(lds) + block * 32 * D;
+  __syncthreads();
+  auto each = [&](auto&& f) {
+#pragma unroll
+    for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) f(b, i, (32 * b + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3)) * 32 + (lane & 31));
+  };
+  if (half == 1) each([&](int b, int i, int at) { join[at] = ak[b][i]; join[128 * D + at] = av[b][i]; });
+  __syncthreads();
+  if (half == 1) return;
+  each([&](int b, int i, int at) { ak[b][i] += join[at]; av[b][i] += join[128 * D + at]; });
+  if (mine < item.len) {
     pa_store_row<T, D>(dk + (int64_t)mine * dk_row, ak, p.scale, p.head_k, lane);
     pa_store_row<T, D>(dv + (int64_t)mine * dv_row, av, 1.f, p.head_v, lane);
   }
@@ -1026,7 +1050,7 @@ static int pa_launch(const MtPackedAttn& p, int pass, bool split, hipStream_t st
   } else if constexpr (sizeof(T) == 2) {
     if (pass == 0) hipLaunchKernelGGL((mt_pattn_fwd_kernel<T, D, 64>), grid, block, 0, stream, p);
     else if (pass == 1) hipLaunchKernelGGL((mt_pattn_dq_kernel<T, D, 64>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((mt_pattn_dkv_kernel<T, D, 64>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((mt_pattn_dkv_kernel<T, D>), grid, dim3(PA_DKV_THREADS), 0, stream, p);
   }
   return (int)hipGetLastError();
 }
