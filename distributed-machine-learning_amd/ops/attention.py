@@ -28,7 +28,7 @@ from typing import Optional, Sequence, Union
 import numpy as np
 import torch
 
-from .lib import PACKED_TILE_ROWS as _TILE
+from .lib import PACKED_ITEM_BYTES as _ITEM, PACKED_TILE_ROWS as _TILE
 
 RELU_EPS = 1e-6
 MAX_SEQ = 128
@@ -175,7 +175,7 @@ class SequencePack:
         self.longest = int(length) if count else 0
         self.uniform_length = int(length) if count else 0
         tiles = -(-int(length) // _TILE) * int(count)
-        self._counts, self._lists = (tiles, tiles, tiles), None
+        self._count, self._lists, self._stream = tiles, None, 0
         return self
 
     def _fix(self, total: int, rows: int, device) -> None:
@@ -205,10 +205,21 @@ class SequencePack:
         tail[:, 0], tail[:, 1] = at, -np.minimum(_TILE, self.rows - at)
         orders = [np.argsort(-work, kind="stable") for work in (np.minimum(first + _TILE, n[seq]), n[seq] - first, n[seq])]
         lists = np.concatenate([np.concatenate([items[o], tail]) for o in orders]) if len(items) + len(tail) else items
-        count = len(items) + len(tail)
-        self._counts = (count, count, count)
-        # a blocking copy: the list is there for whichever stream uses it first
-        self._lists = torch.from_numpy(lists).to(self.device) if self.device.type == "cuda" else None
+        self._count = len(items) + len(tail)
+        self._lists, self._stream = None, 0
+        if self.device.type == "cuda":
+            from .lib import raw_stream
+            # a blocking copy: the list is there for whichever stream uses it first
+            self._lists, self._stream = torch.from_numpy(lists).to(self.device), raw_stream(self.device)
+
+    def _tiles(self, causal: bool, stream: int):
+        """Addresses of the query and the key tiles' lists (0: none needed) for a launch on ``stream``."""
+        if self._lists is None:
+            return 0, 0
+        if stream != self._stream:       # keeps the allocator from handing the list's memory on too early
+            self._lists.record_stream(torch.cuda.current_stream(self.device))
+        at, step = self._lists.data_ptr(), self._count * _ITEM
+        return (at, at + step) if causal else (at + 2 * step, at + 2 * step)
 
 
 
@@ -265,5 +276,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pack: Se
         raise ValueError(f"packed_attention on a GPU takes heads of at most {PACKED_MAX_HEAD_DIM} elements, got {max(dk, dv)}")
     if pack.device != q.device:
         raise ValueError(f"the pack lies on {pack.device}, the operands on {q.device}")
-    from .attention_hip import PackedAttention
-    return PackedAttention.apply(q, k, v, pack, bool(causal), scale)
+    from .attention_hip import PackedAttention, packed_forward
+    from .lib import wants_grad
+    if wants_grad(q, k, v):
+        return PackedAttention.apply(q, k, v, pack, bool(causal), scale)
+    return packed_forward(q, k, v, pack, bool(causal), scale, False)[0]

@@ -2,7 +2,6 @@
 (``csrc/packed_attention.hip``)."""
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import Optional
 
@@ -177,31 +176,34 @@ def _in_place(t: torch.Tensor) -> torch.Tensor:
     return F.pad(t, (0, pad)).contiguous() if pad else t.clone(memory_format=torch.contiguous_format)
 
 
-def _packed_args(pack, which: int, q, k, v, causal: bool, scale: float) -> "L.PackedAttn":
-    a = L.PackedAttn(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_row=q.stride(0), q_head=q.stride(1),
-                     k_row=k.stride(0), k_head=k.stride(1), v_row=v.stride(0), v_head=v.stride(1), rows=pack.rows,
-                     heads=q.shape[1], kv_heads=k.shape[1], head_k=q.shape[2], head_v=v.shape[2], causal=int(causal),
-                     scale=scale, uniform_len=pack.uniform_length, count=len(pack.lengths))
-    _tile_list(a, pack, which)
-    return a
+FORM = -1       # -1: the bf16 kernels by the launch's size; 0 / 1 force the ones whose waves share a tile / a walk (tests)
 
 
-def _tile_list(a, pack, which: int) -> None:
-    """Which order of the pack's tiles a launch takes: 0 causal queries, 1 causal keys, 2 no mask."""
-    a.n_items = pack._counts[which]
-    if pack._lists is not None:
-        a.items = pack._lists.data_ptr() + which * a.n_items * L.PACKED_ITEM_BYTES
-        pack._lists.record_stream(torch.cuda.current_stream(pack.device))
+def _packed_launch(so, pack, q, k, v, causal: bool, scale: float, backward: int, out=0, dout=None, o=0, dq=0, dk=0, dv=0, lse=0,
+                   delta=0) -> None:
+    stream = L.raw_stream(q.device)
+    items, kv_items = pack._tiles(causal, stream)
+    qr, qh, _ = q.stride()
+    kr, kh, _ = k.stride()
+    vr, vh, _ = v.stride()
+    dr, dh, _ = dout.stride() if dout is not None else (0, 0, 0)
+    args = L.PACKED_ATTN_FORMAT.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out, dout.data_ptr() if dout is not None else 0, o, dq,
+                                     dk, dv, lse, delta, items, kv_items, qr, qh, kr, kh, vr, vh, dr, dh, pack.rows, pack._count,
+                                     pack.uniform_length, len(pack.lengths), q.shape[1], k.shape[1], q.shape[2], v.shape[2],
+                                     int(causal), scale, 0)
+    with L.on(q.device):
+        L.check(so.mt_packed_attn_launch(args, backward, int(q.dtype == torch.bfloat16), FORM, stream), "mt_packed_attn_launch")
 
 
-# bf16 launches of fewer workgroups than this (two per CU) take the split form, whose four waves share one walk over the keys.
-SPLIT_BELOW = 512
-
-
-def _launch(so, a, which: int, bf16: bool, device, what: str) -> None:
-    lanes = a.kv_heads if which == 2 else a.heads
-    L.check(so.mt_packed_attn_launch(ctypes.byref(a), which, int(bf16), int(not bf16 or a.n_items * lanes < SPLIT_BELOW),
-                                     L.raw_stream(device)), what)
+def packed_forward(q, k, v, pack, causal: bool, scale: float, keeps: bool):
+    """(output, what a backward pass needs)."""
+    so = L.load()
+    dv = v.shape[2]
+    q, k, v = _in_place(q), _in_place(k), _in_place(v)
+    out = torch.empty(pack.rows, q.shape[1], v.shape[2], device=q.device, dtype=q.dtype)
+    lse = torch.empty(q.shape[1], pack.rows, device=q.device, dtype=torch.float32) if keeps else None
+    _packed_launch(so, pack, q, k, v, causal, scale, 0, o=out.data_ptr(), lse=lse.data_ptr() if keeps else 0)
+    return (out if v.shape[2] == dv else out[..., :dv].contiguous()), (q, k, v, out, lse)
 
 
 class PackedAttention(torch.autograd.Function):
@@ -209,37 +211,20 @@ class PackedAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, pack, causal: bool, scale: float):
-        so = L.load()
-        dk, dv = q.shape[2], v.shape[2]
-        qc, kc, vc = _in_place(q), _in_place(k), _in_place(v)
-        out = torch.empty(pack.rows, q.shape[1], vc.shape[2], device=q.device, dtype=q.dtype)
-        keeps = any(ctx.needs_input_grad[:3])
-        lse = torch.empty(q.shape[1], pack.rows, device=q.device, dtype=torch.float32) if keeps else None
-        a = _packed_args(pack, 0 if causal else 2, qc, kc, vc, causal, scale)
-        a.o, a.lse = out.data_ptr(), lse.data_ptr() if keeps else None
-        with torch.cuda.device(q.device):
-            _launch(so, a, 0, q.dtype == torch.bfloat16, q.device, "mt_packed_attn_launch")
-        if keeps:
-            ctx.save_for_backward(qc, kc, vc, out, lse)
-        ctx.pack, ctx.meta = pack, (causal, scale, dk, dv)
-        return out if vc.shape[2] == dv else out[..., :dv].contiguous()
+        ctx.pack, ctx.meta = pack, (causal, scale, q.shape[2], v.shape[2])
+        out, saved = packed_forward(q, k, v, pack, causal, scale, True)
+        ctx.save_for_backward(*saved)
+        return out
 
     @staticmethod
     def backward(ctx, grad_out):
         so = L.load()
         q, k, v, out, lse = ctx.saved_tensors
         pack, (causal, scale, dk, dv) = ctx.pack, ctx.meta
-        do = _in_place(grad_out.to(q.dtype))
+        do = _in_place(grad_out if grad_out.dtype == q.dtype else grad_out.to(q.dtype))
         delta = torch.empty_like(lse)
         grads = [torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v)]
-        a = _packed_args(pack, 0 if causal else 2, q, k, v, causal, scale)
-        a.out, a.dout, a.do_row, a.do_head = out.data_ptr(), do.data_ptr(), do.stride(0), do.stride(1)
-        a.lse, a.delta = lse.data_ptr(), delta.data_ptr()
-        a.dq, a.dk, a.dv = (g.data_ptr() for g in grads)
-        bf16 = q.dtype == torch.bfloat16
-        with torch.cuda.device(q.device):
-            _launch(so, a, 1, bf16, q.device, "mt_packed_attn_launch(dq)")
-            _tile_list(a, pack, 1 if causal else 2)
-            _launch(so, a, 2, bf16, q.device, "mt_packed_attn_launch(dk, dv)")
+        _packed_launch(so, pack, q, k, v, causal, scale, 1, out=out.data_ptr(), dout=do, dq=grads[0].data_ptr(),
+                       dk=grads[1].data_ptr(), dv=grads[2].data_ptr(), lse=lse.data_ptr(), delta=delta.data_ptr())
         gq, gk, gv = (g if g.shape[2] == w else g[..., :w].contiguous() for g, w in zip(grads, (dk, dk, dv)))
         return gq, gk, gv, None, None, None

@@ -41,7 +41,7 @@ struct MtPackedAttn {
   const void *out, *dout;       // backward only: forward output (contiguous) and its gradient
   void *o, *dq, *dk, *dv;       // outputs, contiguous [T][heads or kv_heads][dk or dv]
   float *lse, *delta;           // [heads][rows]
-  const MtSeqItem* items;       // null: count sequences of uniform_len rows each
+  const MtSeqItem *items, *kv_items;      // tiles of query rows and of key rows; null: count sequences of uniform_len rows each
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, do_row, do_head;
   int64_t rows;
   int32_t n_items, uniform_len, count;
@@ -77,10 +77,10 @@ template <> __device__ __forceinline__ f32x8 pa_pack<float>(const f32x16& a, int
 }
 
 template <typename V> __device__ __forceinline__ const __attribute__((address_space(3))) V* pa_lds(uint32_t at) {
-  return (const __attribute__((address_space(3))) V*)at;
+  return (const __attribute__((address_space(3))) V*)(uintptr_t)at;
 }
 template <typename V> __device__ __forceinline__ __attribute__((address_space(3))) V* pa_lds_mut(uint32_t at) {
-  return (__attribute__((address_space(3))) V*)at;
+  return (__attribute__((address_space(3))) V*)(uintptr_t)at;
 }
 __device__ __forceinline__ uint32_t pa_lds_at(const uint8_t* p) { return (uint32_t)(uintptr_t)(const lds_u8*)p; }
 
@@ -225,8 +225,8 @@ template <int N> __device__ __forceinline__ void pa_clear(f32x16 (&a)[N]) {
 }
 
 // Which tile this workgroup takes.  Tiles come longest first (causal: the last queries, or the first keys).
-__device__ __forceinline__ MtSeqItem pa_item(const MtPackedAttn& p, int i, bool last_first) {
-  if (p.items != nullptr) return p.items[i];
+__device__ __forceinline__ MtSeqItem pa_item(const MtPackedAttn& p, const MtSeqItem* items, int i, bool last_first) {
+  if (items != nullptr) return items[i];
   const int tiles = (p.uniform_len + PA_OWN - 1) / PA_OWN;
   const int t = i / p.count, seq = i - t * p.count;
   return MtSeqItem{seq * p.uniform_len, p.uniform_len, (last_first ? tiles - 1 - t : t) * PA_OWN, 0};
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void mt_pattn_fwd_kernel(const MtPac
   const int it = blockIdx.x / p.heads, r = blockIdx.x - it * p.heads;
   // heads of one group are kv_heads workgroups apart: the XCDs (workgroup number mod 8) then share few key / value heads each
   const int kvh = r % p.kv_heads, head = kvh * (p.heads / p.kv_heads) + r / p.kv_heads;
-  const MtSeqItem item = pa_item(p, it, p.causal);
+  const MtSeqItem item = pa_item(p, p.items, it, p.causal);
   const int64_t o_row = (int64_t)p.heads * p.head_v;
   T* o = reinterpret_cast<T*>(p.o) + item.row0 * o_row + (int64_t)head * p.head_v;
   if (item.len <= 0) {
@@ -445,7 +445,7 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int it = blockIdx.x / p.heads, r = blockIdx.x - it * p.heads;
   const int kvh = r % p.kv_heads, head = kvh * (p.heads / p.kv_heads) + r / p.kv_heads;
-  const MtSeqItem item = pa_item(p, it, p.causal);
+  const MtSeqItem item = pa_item(p, p.items, it, p.causal);
   const int64_t dq_row = (int64_t)p.heads * p.head_k;
   T* dq = reinterpret_cast<T*>(p.dq) + item.row0 * dq_row + (int64_t)head * p.head_k;
   if (item.len <= 0) {
@@ -556,7 +556,7 @@ __global__ __launch_bounds__(PA_DKV_THREADS, 2) void mt_pattn_dkv_kernel(const M
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int it = blockIdx.x / p.kv_heads, kvh = blockIdx.x - it * p.kv_heads;
   const int group = p.heads / p.kv_heads;
-  const MtSeqItem item = pa_item(p, it, false);
+  const MtSeqItem item = pa_item(p, p.kv_items, it, false);
   const int64_t dk_row = (int64_t)p.kv_heads * p.head_k, dv_row = (int64_t)p.kv_heads * p.head_v;
   T* dk = reinterpret_cast<T*>(p.dk) + item.row0 * dk_row + (int64_t)kvh * p.head_k;
   T* dv = reinterpret_cast<T*>(p.dv) + item.row0 * dv_row + (int64_t)kvh * p.head_v;
@@ -725,7 +725,7 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const PaSlot slot = pa_slot(blockIdx.x, p.heads);
   const int kvh = slot.lane_head % p.kv_heads, head = kvh * (p.heads / p.kv_heads) + slot.lane_head / p.kv_heads;
-  const MtSeqItem item = pa_item(p, slot.it, p.causal);
+  const MtSeqItem item = pa_item(p, p.items, slot.it, p.causal);
   const int64_t o_row = (int64_t)p.heads * p.head_v;
   T* o = reinterpret_cast<T*>(p.o) + item.row0 * o_row + (int64_t)head * p.head_v;
   if (item.len <= 0) {
@@ -837,7 +837,7 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const PaSlot slot = pa_slot(blockIdx.x, p.heads);
   const int kvh = slot.lane_head % p.kv_heads, head = kvh * (p.heads / p.kv_heads) + slot.lane_head / p.kv_heads;
-  const MtSeqItem item = pa_item(p, slot.it, p.causal);
+  const MtSeqItem item = pa_item(p, p.items, slot.it, p.causal);
   const int64_t dq_row = (int64_t)p.heads * p.head_k;
   T* dq = reinterpret_cast<T*>(p.dq) + item.row0 * dq_row + (int64_t)head * p.head_k;
   if (item.len <= 0) {
@@ -922,7 +922,7 @@ __global__ __launch_bounds__(PA_THREADS, 1) void mt_pattn_split_dkv_kernel(const
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const PaSlot slot = pa_slot(blockIdx.x, p.kv_heads);
   const int kvh = slot.lane_head, group = p.heads / p.kv_heads;
-  const MtSeqItem item = pa_item(p, slot.it, false);
+  const MtSeqItem item = pa_item(p, p.kv_items, slot.it, false);
   const int64_t dk_row = (int64_t)p.kv_heads * p.head_k, dv_row = (int64_t)p.kv_heads * p.head_v;
   T* dk = reinterpret_cast<T*>(p.dk) + item.row0 * dk_row + (int64_t)kvh * p.head_k;
   T* dv = reinterpret_cast<T*>(p.dv) + item.row0 * dv_row + (int64_t)kvh * p.head_v;
@@ -1039,10 +1039,15 @@ __global__ __launch_bounds__(PA_THREADS, 1) void mt_pattn_split_dkv_kernel(const
 }
 
 // ---- launchers ----------------------------------------------------------------------------------------------------------
+// bf16 launches of fewer workgroups than this (two per CU) take the split form, f32 ones always.  Measured, causal bf16, shared /
+// split: one sequence of 2048, 8 heads of 128 (128 workgroups) forward 54 / 28 us; 8192, 2 heads (128) 194 / 84, with its backward
+// pass 1085 / 337; 4 x 2048, 16 heads (1024) 120 / 134; documents of the benchmark, dk and dv (620) 265 / 480.
+#define PA_SPLIT_BELOW 512
 template <typename T, int D>
-static int pa_launch(const MtPackedAttn& p, int pass, bool split, hipStream_t stream) {
-  const int lanes = pass == 2 ? p.kv_heads : p.heads;
-  const dim3 grid((unsigned)(p.n_items * lanes * (split ? 4 : 1))), block(PA_THREADS);
+static void pa_launch(const MtPackedAttn& p, int pass, int form, hipStream_t stream) {
+  const int blocks = p.n_items * (pass == 2 ? p.kv_heads : p.heads);
+  const bool split = sizeof(T) == 4 || (form < 0 ? blocks < PA_SPLIT_BELOW : form == 1);
+  const dim3 grid((unsigned)(blocks * (split ? 4 : 1))), block(PA_THREADS);
   if (split) {
     if (pass == 0) hipLaunchKernelGGL((mt_pattn_split_fwd_kernel<T, D>), grid, block, 0, stream, p);
     else if (pass == 1) hipLaunchKernelGGL((mt_pattn_split_dq_kernel<T, D>), grid, block, 0, stream, p);
@@ -1052,7 +1057,13 @@ static int pa_launch(const MtPackedAttn& p, int pass, bool split, hipStream_t st
     else if (pass == 1) hipLaunchKernelGGL((mt_pattn_dq_kernel<T, D, 64>), grid, block, 0, stream, p);
     else hipLaunchKernelGGL((mt_pattn_dkv_kernel<T, D>), grid, dim3(PA_DKV_THREADS), 0, stream, p);
   }
-  return (int)hipGetLastError();
+}
+template <typename T>
+static void pa_launch_width(const MtPackedAttn& p, int pass, int form, hipStream_t stream) {
+  const int widest = p.head_k > p.head_v ? p.head_k : p.head_v;
+  if (widest <= 32) pa_launch<T, 32>(p, pass, form, stream);
+  else if (widest <= 64) pa_launch<T, 64>(p, pass, form, stream);
+  else pa_launch<T, 128>(p, pass, form, stream);
 }
 
 extern "C" int mt_packed_attn_sizes(int* item_bytes, int* tile_rows) {
@@ -1061,30 +1072,26 @@ extern "C" int mt_packed_attn_sizes(int* item_bytes, int* tile_rows) {
   return (int)sizeof(MtPackedAttn);
 }
 
-// pass: 0 forward, 1 dq + D, 2 dk + dv.  bf16: 0 = f32 operands (always the split form), 1 = bf16.  Rows are read in 16-byte
-// pieces.
-extern "C" int mt_packed_attn_launch(const MtPackedAttn* a, int pass, int bf16, int split, hipStream_t stream) {
-  if (a == nullptr || pass < 0 || pass > 2) return -2;
+// backward: 0 forward; 1 dq and D, then dk and dv.  bf16: 0 = f32 operands, 1 = bf16.  form: -1 by the launch's size; 0 / 1 the
+// bf16 kernels whose waves share a tile / a walk (tests).  Rows are read in 16-byte pieces.
+extern "C" int mt_packed_attn_launch(const MtPackedAttn* a, int backward, int bf16, int form, hipStream_t stream) {
+  if (a == nullptr) return -2;
   const MtPackedAttn p = *a;
   if (p.n_items <= 0) return 0;
   const int es = bf16 ? 2 : 4, per = 16 / es;
-  const int widest = p.head_k > p.head_v ? p.head_k : p.head_v;
-  if (p.head_k < 1 || p.head_v < 1 || widest > 128 || p.head_k % per || p.head_v % per) return -2;
+  if (p.head_k < 1 || p.head_v < 1 || p.head_k > 128 || p.head_v > 128 || p.head_k % per || p.head_v % per) return -2;
   if (p.heads < 1 || p.kv_heads < 1 || p.heads % p.kv_heads) return -2;
-  if ((p.items == nullptr) && (p.uniform_len < 1 || p.count < 1)) return -2;
+  if ((p.items == nullptr || p.kv_items == nullptr) && (p.uniform_len < 1 || p.count < 1)) return -2;
   if ((int64_t)p.n_items * p.heads * 4 > 0x7FFFFFFF || !(p.scale > 0.f)) return -2;
   const int64_t strides[8] = {p.q_row, p.q_head, p.k_row, p.k_head, p.v_row, p.v_head, p.do_row, p.do_head};
-  for (int i = 0; i < 8; ++i)      // 32-bit byte offsets inside a staged tile of at most 64 rows
+  for (int i = 0; i < 8; ++i)      // 32-bit byte offsets inside a staged tile of at most 128 rows
     if (strides[i] < 0 || strides[i] % per || strides[i] * es > (1 << 24)) return -2;
   const void* ptrs[9] = {p.q, p.k, p.v, p.out, p.dout, p.o, p.dq, p.dk, p.dv};
   for (int i = 0; i < 9; ++i)
     if (reinterpret_cast<uintptr_t>(ptrs[i]) & 15) return -2;
-  if (bf16) {
-    if (widest <= 32) return pa_launch<__bf16, 32>(p, pass, split != 0, stream);
-    if (widest <= 64) return pa_launch<__bf16, 64>(p, pass, split != 0, stream);
-    return pa_launch<__bf16, 128>(p, pass, split != 0, stream);
+  for (int pass = backward ? 1 : 0; pass <= (backward ? 2 : 0); ++pass) {
+    if (bf16) pa_launch_width<__bf16>(p, pass, form, stream);
+    else pa_launch_width<float>(p, pass, form, stream);
   }
-  if (widest <= 32) return pa_launch<float, 32>(p, pass, true, stream);
-  if (widest <= 64) return pa_launch<float, 64>(p, pass, true, stream);
-  return pa_launch<float, 128>(p, pass, true, stream);
+  return (int)hipGetLastError();
 }

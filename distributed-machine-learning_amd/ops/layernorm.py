@@ -45,8 +45,11 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         raise TypeError(f"layer_norm on a GPU takes f32 or bf16 rows, got {x.dtype}")
     if d > 1 << 29:
         raise ValueError(f"layer_norm on a GPU takes rows of at most {1 << 29} columns, got {d}")
-    from .layernorm_hip import LayerNorm
-    return LayerNorm.apply(x, weight, bias, float(eps))
+    from .layernorm_hip import LayerNorm, norm_forward
+    from .lib import wants_grad
+    if wants_grad(x, weight, bias):
+        return LayerNorm.apply(x, weight, bias, float(eps))
+    return norm_forward(x, weight, bias, float(eps), False)[0]
 
 
 def residual_layer_norm_reference(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,

@@ -127,8 +127,28 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     d = t.shape[-1]
     if t.stride(-1) != 1 and d > 1:
         t = t.contiguous()
+    if t.dim() == 2:
+        return t
     t = t.reshape(-1, d)
     return t if t.stride(1) == 1 or d == 1 else t.contiguous()
+
+
+def norm_forward(x, weight, bias, eps: float, keeps: bool):
+    """(output, x's rows, weight, statistics, type flags)."""
+    so = L.load()
+    xr = _rows(x)
+    M, d = xr.shape
+    w = weight.contiguous() if weight is not None else None
+    b = bias.contiguous() if bias is not None else None
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    stats = torch.empty(M, 2, device=x.device, dtype=torch.float32) if keeps else None
+    param = weight if weight is not None else bias
+    flags = (int(x.dtype == torch.bfloat16), int(param is not None and param.dtype == torch.bfloat16))
+    with L.on(x.device):
+        L.check(so.mt_norm_fwd_launch(xr.data_ptr(), w.data_ptr() if w is not None else None,
+                                      b.data_ptr() if b is not None else None, y.data_ptr(), stats.data_ptr() if keeps else None, M,
+                                      xr.stride(0), d, eps, *flags, L.raw_stream(x.device)), "mt_norm_fwd_launch")
+    return y, xr, w, stats, flags
 
 
 class LayerNorm(torch.autograd.Function):
@@ -136,23 +156,9 @@ class LayerNorm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps: float):
-        so = L.load()
-        xr = _rows(x)
-        M, d = xr.shape
-        w = weight.contiguous() if weight is not None else None
-        b = bias.contiguous() if bias is not None else None
-        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        keeps = any(ctx.needs_input_grad[:3])
-        stats = torch.empty(M, 2, device=x.device, dtype=torch.float32) if keeps else None
+        y, xr, w, stats, flags = norm_forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(xr, w, stats)
         param = weight if weight is not None else bias
-        flags = (int(x.dtype == torch.bfloat16), int(param is not None and param.dtype == torch.bfloat16))
-        with torch.cuda.device(x.device):
-            L.check(so.mt_norm_fwd_launch(xr.data_ptr(), w.data_ptr() if w is not None else None,
-                                          b.data_ptr() if b is not None else None, y.data_ptr(),
-                                          stats.data_ptr() if keeps else None, M, xr.stride(0), d, eps, *flags,
-                                          L.raw_stream(x.device)), "mt_norm_fwd_launch")
-        if keeps:
-            ctx.save_for_backward(xr, w, stats)
         ctx.meta = (x.shape, flags, weight is not None, bias is not None, param.dtype if param is not None else None)
         return y
 
@@ -162,18 +168,18 @@ class LayerNorm(torch.autograd.Function):
         xr, w, stats = ctx.saved_tensors
         shape, flags, has_w, has_b, pdtype = ctx.meta
         M, d = xr.shape
-        dy = _rows(grad_y.to(xr.dtype))
-        dx = torch.empty(M, d, device=xr.device, dtype=xr.dtype)
+        dy = _rows(grad_y if grad_y.dtype == xr.dtype else grad_y.to(xr.dtype))
+        dx = torch.empty(shape, device=xr.device, dtype=xr.dtype)
         want_w, want_b = has_w and ctx.needs_input_grad[1], has_b and ctx.needs_input_grad[2]
         fill = torch.empty if M else torch.zeros                       # no rows: the sums are zero
         dw = fill(d, device=xr.device, dtype=pdtype) if want_w else None
         db = fill(d, device=xr.device, dtype=pdtype) if want_b else None
         part = None
         if (want_w or want_b) and M:
-            part = torch.empty(int(so.mt_norm_bwd_parts(M, d, flags[0])), 2, d, device=xr.device, dtype=torch.float32)
-        with torch.cuda.device(xr.device):
+            part = torch.empty(so.mt_norm_bwd_parts(M, d, flags[0]), 2, d, device=xr.device, dtype=torch.float32)
+        with L.on(xr.device):
             L.check(so.mt_norm_bwd_launch(dy.data_ptr(), xr.data_ptr(), w.data_ptr() if has_w else None, stats.data_ptr(),
                                           dx.data_ptr(), part.data_ptr() if part is not None else None,
                                           dw.data_ptr() if want_w else None, db.data_ptr() if want_b else None, M, xr.stride(0),
                                           dy.stride(0), d, *flags, L.raw_stream(xr.device)), "mt_norm_bwd_launch")
-        return dx.view(shape), dw, db, None
+        return dx, dw, db, None

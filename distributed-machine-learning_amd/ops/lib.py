@@ -7,8 +7,10 @@ GPU a missing or stale library is an error, never a silent eager-PyTorch path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
+import struct
 from typing import Optional
 
 import numpy as np
@@ -56,12 +58,16 @@ class OptSlot(C.Structure):
 class PackedAttn(C.Structure):
     _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p), ("dout", c_void_p),
                 ("o", c_void_p), ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p),
-                ("lse", c_void_p), ("delta", c_void_p), ("items", c_void_p),
+                ("lse", c_void_p), ("delta", c_void_p), ("items", c_void_p), ("kv_items", c_void_p),
                 ("q_row", C.c_int64), ("q_head", C.c_int64), ("k_row", C.c_int64), ("k_head", C.c_int64),
                 ("v_row", C.c_int64), ("v_head", C.c_int64), ("do_row", C.c_int64), ("do_head", C.c_int64),
                 ("rows", C.c_int64), ("n_items", c_int32), ("uniform_len", c_int32), ("count", c_int32),
                 ("heads", c_int32), ("kv_heads", c_int32), ("head_k", c_int32), ("head_v", c_int32),
                 ("causal", c_int32), ("scale", c_float), ("pad", c_int32)]
+
+
+# The same layout for struct.pack: filling a ctypes structure field by field costs several microseconds of every call.
+PACKED_ATTN_FORMAT = struct.Struct("<13Q9q8ifi")
 
 
 class MlpPlan(C.Structure):
@@ -226,6 +232,8 @@ def load(build_if_missing: bool = True) -> C.CDLL:
     item_bytes, tile_rows = C.c_int(), C.c_int()
     if lib.mt_packed_attn_sizes(C.byref(item_bytes), C.byref(tile_rows)) != C.sizeof(PackedAttn):
         raise KernelLibraryError("MtPackedAttn layout mismatch between lib.py and the library")
+    if PACKED_ATTN_FORMAT.size != C.sizeof(PackedAttn):
+        raise KernelLibraryError("MtPackedAttn layout mismatch between the struct format and lib.py")
     if (item_bytes.value, tile_rows.value) != (PACKED_ITEM_BYTES, PACKED_TILE_ROWS):
         raise KernelLibraryError("packed attention: tile list layout mismatch between lib.py and the library")
     lib.mt_linear_fwd_launch.argtypes = [c_void_p] * 6 + [C.c_int64, C.c_int, C.c_int, C.c_int64, C.c_int64, C.c_int, C.c_int,
@@ -239,7 +247,7 @@ def load(build_if_missing: bool = True) -> C.CDLL:
     lib.mt_norm_fwd_launch.argtypes = [c_void_p] * 5 + [C.c_int64, C.c_int64, C.c_int, c_float, C.c_int, C.c_int, c_void_p]
     lib.mt_norm_bwd_launch.argtypes = [c_void_p] * 8 + [C.c_int64] * 3 + [C.c_int] * 3 + [c_void_p]
     lib.mt_norm_bwd_parts.restype = lib.mt_norm_fwd_launch.restype = lib.mt_norm_bwd_launch.restype = C.c_int
-    lib.mt_packed_attn_launch.argtypes = [C.POINTER(PackedAttn), C.c_int, C.c_int, C.c_int, c_void_p]
+    lib.mt_packed_attn_launch.argtypes = [C.c_char_p, C.c_int, C.c_int, C.c_int, c_void_p]
     lib.mt_packed_attn_launch.restype = C.c_int
     lib.mt_ln_fwd_launch.argtypes = [c_void_p] * 8 + [C.c_int, C.c_int, c_float, c_float, c_void_p, c_float, c_void_p]
     lib.mt_ln_bwd_launch.argtypes = [c_void_p] * 8 + [C.c_int, C.c_int, c_float, c_void_p, c_float, c_void_p]
@@ -356,3 +364,19 @@ def raw_stream(device) -> int:
     import torch
     idx = device.index
     return torch._C._cuda_getCurrentRawStream(idx if idx is not None else torch.cuda.current_device())
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on(device):
+    """Context in which ``device`` (a tensor's) is the current one; nothing to enter when it already is, the usual case."""
+    import torch
+    return _SAME_DEVICE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+
+
+def wants_grad(*tensors) -> bool:
+    """Whether autograd would record an operation on these (``None`` allowed): if not, a binding's forward is called directly,
+    which halves the host time of a small call."""
+    import torch
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)

@@ -109,7 +109,10 @@ def _fused_linear(x, weight, bias, activation, residual) -> torch.Tensor:
         raise TypeError(f"bias must be {x.dtype} or f32, got {bias.dtype}")
     if residual is not None and residual.dtype != x.dtype:
         raise TypeError(f"residual must be {x.dtype}, got {residual.dtype}")
-    return FusedLinear.apply(x, weight, bias, residual, ACTIVATIONS[activation], w16)
+    from .lib import wants_grad
+    if wants_grad(x, weight, bias, residual):
+        return FusedLinear.apply(x, weight, bias, residual, ACTIVATIONS[activation], w16)
+    return fused_forward(x, weight, bias, residual, ACTIVATIONS[activation], w16, False)[0]
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
@@ -349,7 +352,32 @@ def _pieces(t: torch.Tensor) -> torch.Tensor:
 
 
 def _rows_of(t: torch.Tensor, width: int) -> torch.Tensor:
-    return t.reshape(-1, width)
+    return t if t.dim() == 2 else t.reshape(-1, width)
+
+
+def fused_forward(x, weight, bias, residual, act: int, w16, keep_z: bool):
+    """(output, x's rows, the weight as multiplied, z or None)."""
+    from . import lib as L
+    so = L.load()
+    out_f, in_f = weight.shape
+    xc = _pieces(_rows_of(x, in_f))
+    if w16 is not None:
+        wc = w16
+    else:
+        wc = weight.detach() if weight.dtype == x.dtype else weight.detach().to(x.dtype)
+    wc = _pieces(wc)
+    bc = bias.detach().contiguous() if bias is not None else None
+    rc = _rows_of(residual, out_f).contiguous() if residual is not None else None
+    M = xc.shape[0]
+    y = torch.empty(M, out_f, device=x.device, dtype=x.dtype)
+    z = torch.empty_like(y) if keep_z else None
+    with L.on(x.device):
+        L.check(so.mt_linear_fwd_launch(xc.data_ptr(), wc.data_ptr(), bc.data_ptr() if bc is not None else None,
+                                        rc.data_ptr() if rc is not None else None, y.data_ptr(),
+                                        z.data_ptr() if z is not None else None, M, out_f, xc.shape[1], xc.stride(0), wc.stride(0),
+                                        act, int(bc is not None and bc.dtype == torch.bfloat16), int(x.dtype == torch.bfloat16),
+                                        L.raw_stream(x.device)), "mt_linear_fwd_launch")
+    return y.view(x.shape[:-1] + (out_f,)), xc, wc, z
 
 
 class FusedLinear(torch.autograd.Function):
@@ -358,31 +386,16 @@ class FusedLinear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act: int, w16):
-        from . import lib as L
-        so = L.load()
-        out_f, in_f = weight.shape
+        backward = any(ctx.needs_input_grad[:3])
+        # what act' is read from: y itself has z's sign under ReLU, unless a residual was added to it
+        keep_z = backward and act != 0 and not (act == 1 and residual is None)
         with torch.autocast("cuda", enabled=False):
-            xc = _pieces(_rows_of(x, in_f))
-            wc = _pieces(w16 if w16 is not None else weight.detach().to(x.dtype))
-            bc = bias.detach().contiguous() if bias is not None else None
-            rc = _rows_of(residual, out_f).contiguous() if residual is not None else None
-            M, bf16 = xc.shape[0], int(x.dtype == torch.bfloat16)
-            y = torch.empty(M, out_f, device=x.device, dtype=x.dtype)
-            backward = any(ctx.needs_input_grad[:3])
-            # what act' is read from: y itself has z's sign under ReLU, unless a residual was added to it
-            keep_z = backward and act != 0 and not (act == 1 and rc is None)
-            z = torch.empty_like(y) if keep_z else None
-            with torch.cuda.device(x.device):
-                L.check(so.mt_linear_fwd_launch(xc.data_ptr(), wc.data_ptr(), bc.data_ptr() if bc is not None else None,
-                                                rc.data_ptr() if rc is not None else None, y.data_ptr(),
-                                                z.data_ptr() if z is not None else None, M, out_f, xc.shape[1], xc.stride(0),
-                                                wc.stride(0), act, int(bc is not None and bc.dtype == torch.bfloat16), bf16,
-                                                L.raw_stream(x.device)), "mt_linear_fwd_launch")
+            y, xc, wc, z = fused_forward(x, weight, bias, residual, act, w16, keep_z)
         if backward:
             ctx.save_for_backward(xc, wc, z if keep_z else y if act else None)
-        ctx.meta = (act, x.shape, in_f, weight.dtype, bias.dtype if bias is not None else None,
+        ctx.meta = (act, x.shape, weight.shape[1], weight.dtype, bias.dtype if bias is not None else None,
                     residual.shape if residual is not None else None)
-        return y.view(x.shape[:-1] + (out_f,))
+        return y
 
     @staticmethod
     def backward(ctx, dy):
@@ -396,8 +409,8 @@ class FusedLinear(torch.autograd.Function):
             bf16, dev, M = xc.dtype == torch.bfloat16, xc.device, xc.shape[0]
             per = 8 if bf16 else 4
             stream = L.raw_stream(dev)
-            with torch.autocast("cuda", enabled=False), torch.cuda.device(dev):
-                g = _rows_of(dy.to(xc.dtype), out_f)
+            with torch.autocast("cuda", enabled=False), L.on(dev):
+                g = _rows_of(dy if dy.dtype == xc.dtype else dy.to(xc.dtype), out_f)
                 if act:
                     g = g if g.stride(1) == 1 else g.contiguous()
                     dz = torch.empty(M, out_f + -out_f % per, device=dev, dtype=xc.dtype)

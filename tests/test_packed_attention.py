@@ -106,14 +106,14 @@ def test_forward_and_gradients(dtype, causal, lengths, heads, kv_heads, dk, dv):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("below", [0, 1 << 30])
+@pytest.mark.parametrize("form", [0, 1])
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("heads,kv_heads,dk,dv", [(2, 2, 64, 64), (4, 2, 32, 32), (3, 1, 128, 128), (2, 1, 20, 36)])
-def test_both_bf16_forms(monkeypatch, below, causal, heads, kv_heads, dk, dv):
+def test_both_bf16_forms(monkeypatch, form, causal, heads, kv_heads, dk, dv):
     """The form whose waves share a tile and the one whose waves share a walk, whatever the launch's size would pick."""
     from mitune.ops import attention_hip
     from mitune.ops.attention import SequencePack
-    monkeypatch.setattr(attention_hip, "SPLIT_BELOW", below)
+    monkeypatch.setattr(attention_hip, "FORM", form)
     lengths = [129, 5, 0, 300, 64, 33]
     rows = sum(lengths) + 150
     q, k, v, do = _inputs(lengths, rows, heads, kv_heads, dk, dv, torch.bfloat16)
