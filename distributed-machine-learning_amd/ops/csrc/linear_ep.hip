@@ -44,6 +44,109 @@ __global__ __launch_bounds__(F32_THREADS) void mt_linear_fwd_f32_kernel(MtGemmGr
   f32_gemm_tile<0, 2, T, 1, 0, true>(&g, tile, 0, 0, 0, 0, 1, 0, lds, &ep);
 }
 
+// Weight gradient with the whole contraction in one workgroup: dW (and db) leave in their own types.
+template <int NSTAGE>
+__global__ __launch_bounds__(NTHREADS) void mt_linear_wgrad_kernel(MtGemmGroup g, MtLinearEp ep, int tiles_i, int tiles_j, int flags) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[NSTAGE * STAGE_BYTES];
+  const int n = tiles_i * tiles_j, per = (n + 7) / 8, t = (blockIdx.x % 8) * per + blockIdx.x / 8;
+  if (t >= n) return;
+  MtTile tile;
+  tile.group = 0;
+  tile.ti = (int16_t)(t % tiles_i);
+  tile.tj = (int16_t)(t / tiles_i);
+  gemm_tile<2, NSTAGE, true>(&g, tile, 0, flags, 0, 0, 1, 0, lds, &ep);
+}
+__global__ __launch_bounds__(P8_THREADS) void mt_linear_wgrad_p8_kernel(MtGemmGroup g, MtLinearEp ep, int tiles_i, int tiles_j, int flags) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BIG_STAGE_BYTES];
+  const int n = tiles_i * tiles_j, per = (n + 7) / 8, t = (blockIdx.x % 8) * per + blockIdx.x / 8;
+  if (t >= n) return;
+  const int in_band = LINEAR_BAND * tiles_j, first = (t / in_band) * LINEAR_BAND;
+  const int rows = tiles_i - first < LINEAR_BAND ? tiles_i - first : LINEAR_BAND;
+  const int r = t % in_band;
+  gemm_tile_p8<2, 0, true>(g, first + r % rows, r / rows, 0, flags, 1, 0, lds, &ep);
+}
+template <int T>
+__global__ __launch_bounds__(F32_THREADS) void mt_linear_wgrad_f32_kernel(MtGemmGroup g, MtLinearEp ep, int tiles_i, int tiles_j,
+                                                                          int flags) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * 2 * T * 128];
+  const int n = tiles_i * tiles_j, per = (n + 7) / 8, t = (blockIdx.x % 8) * per + blockIdx.x / 8;
+  if (t >= n) return;
+  MtTile tile;
+  tile.group = 0;
+  tile.ti = (int16_t)(t / tiles_j);
+  tile.tj = (int16_t)(t % tiles_j);
+  f32_gemm_tile<2, 2, T, 1, 0, true>(&g, tile, 0, flags, 0, 0, 1, 0, lds, &ep);
+}
+
+// A few rows (at most 16 MT): the weight is streamed once, straight from memory into the matrix instruction's operand.  A
+// workgroup owns 16 output features; its waves take equal parts of the contraction, and their sums meet in LDS in wave order.
+// Lane (n = lane & 15, h = lane >> 4) loads 16 bytes of weight row n at column 4 h (f32) or 8 h (bf16) of each step, and the same
+// columns of x row n; UNROLL steps are loaded before their products, which keeps 8 KB of weight per wave on its way.
+#define FEW_UNROLL 8
+template <typename T, int MT, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void mt_linear_few_kernel(const T* __restrict__ x, const T* __restrict__ w, MtLinearEp ep,
+                                                                   T* __restrict__ y, int M, int N, int K, int64_t ldx, int64_t ldw,
+                                                                   int steps_per_wave) {
+  constexpr int V = 16 / (int)sizeof(T), STEP = 4 * V;
+  __shared__ float part[WAVES][MT][16][17];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, h = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const T* wr = w + (int64_t)(n0 + r < N ? n0 + r : N - 1) * ldw + h * V;      // rows past the last repeat it: their sums are dropped
+  const T* xr[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) xr[t] = x + (int64_t)(16 * t + r < M ? 16 * t + r : M - 1) * ldx + h * V;
+  f32x4 acc[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto load = [&](const T* p, int k) {
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (k + h * V < K) v = *reinterpret_cast<const u32x4*>(p + k);
+    return v;
+  };
+  auto mma = [&](u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (sizeof(T) == 2) {
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
+      return c;
+    }
+  };
+  const int k_lo = wave * steps_per_wave * STEP, k_all = k_lo + steps_per_wave * STEP, k_hi = k_all < K ? k_all : K;
+  for (int k = k_lo; k < k_hi; k += FEW_UNROLL * STEP) {
+    u32x4 a[FEW_UNROLL], b[FEW_UNROLL][MT];
+#pragma unroll
+    for (int s = 0; s < FEW_UNROLL; ++s) {
+      const int ks = k + s * STEP < k_hi ? k + s * STEP : K;                   // K: zeros
+      a[s] = load(wr, ks);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) b[s][t] = load(xr[t], ks);
+    }
+#pragma unroll
+    for (int s = 0; s < FEW_UNROLL; ++s)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) acc[t] = mma(a[s], b[s][t], acc[t]);
+  }
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[wave][t][r][4 * h + i] = acc[t][i];       // [row][feature]
+  __syncthreads();
+  for (int o = threadIdx.x; o < MT * 256; o += WAVES * 64) {
+    const int t = o >> 8, row = 16 * t + ((o >> 4) & 15), col = n0 + (o & 15);
+    if (row >= M || col >= N) continue;
+    float v = 0.f;
+#pragma unroll
+    for (int q = 0; q < WAVES; ++q) v += part[q][t][(o >> 4) & 15][o & 15];
+    if (ep.bias != nullptr) v += mt_ep_bias(ep, col);
+    const int64_t at = (int64_t)row * N + col;
+    if (ep.z != nullptr) reinterpret_cast<T*>(ep.z)[at] = (T)v;
+    v = mt_ep_act<sizeof(T) == 2>(v, ep.act);
+    if (ep.residual != nullptr) v += (float)reinterpret_cast<const T*>(ep.residual)[at];
+    y[at] = (T)v;
+  }
+}
+
 // dz = dy act'(s): s is z, or (ReLU without a residual) y, whose sign is z's.  A thread takes one 16-byte piece of a dz row.
 template <typename T>
 __global__ __launch_bounds__(256) void mt_act_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ s, T* __restrict__ dz,
@@ -68,7 +171,7 @@ __global__ __launch_bounds__(256) void mt_act_bwd_kernel(const T* __restrict__ d
     }
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const float slope = mt_ep_slope((float)b[e], act);
+      const float slope = mt_ep_slope<sizeof(T) == 2>((float)b[e], act);
       o[e] = act == MT_ACT_RELU ? (slope != 0.f || (float)b[e] != (float)b[e] ? a[e] : (T)0.f) : (T)((float)a[e] * slope);
     }
     __builtin_memcpy(dz + row * ld_dz + col, o, 16);
@@ -105,6 +208,24 @@ static MtGemmGroup linear_group(const void* A, const void* B, void* C, int I, in
 }
 static int linear_grid(int tiles_i, int tiles_j) { return (tiles_i * tiles_j + 7) / 8 * 8; }
 
+// Few rows: as many waves per workgroup as leave each at least two unrolled groups of steps, up to about 16 waves per CU.
+template <typename T, int MT>
+static void linear_few(const void* x, const void* w, const MtLinearEp& ep, void* y, int M, int N, int K, int64_t ldx, int64_t ldw,
+                       hipStream_t stream) {
+  const int step = 64 / (int)sizeof(T), steps = (K + step - 1) / step, blocks = (N + 15) / 16;
+  int waves = 4;
+  while (waves < 16 && blocks * waves < 256 * 16 && steps >= 4 * FEW_UNROLL * waves) waves *= 2;
+  const int per = (steps + waves - 1) / waves;
+#define GO(W)                                                                                                                   \
+  hipLaunchKernelGGL((mt_linear_few_kernel<T, MT, W>), dim3(blocks), dim3(W * 64), 0, stream, (const T*)x, (const T*)w, ep, (T*)y, M, \
+                     N, K, ldx, ldw, per)
+  if (waves == 4) GO(4);
+  else if (waves == 8) GO(8);
+  else GO(16);
+#undef GO
+}
+#define LINEAR_FEW_ROWS 32
+
 // x [M][ldx], W [N][ldw]: rows of whole 16-byte pieces; K columns, a multiple of a piece.  residual, z, y: [M][N] contiguous.
 extern "C" int mt_linear_fwd_launch(const void* x, const void* w, const void* bias, const void* residual, void* y, void* z, int64_t M,
                                     int N, int K, int64_t ldx, int64_t ldw, int act, int bias_bf16, int bf16, hipStream_t stream) {
@@ -112,6 +233,14 @@ extern "C" int mt_linear_fwd_launch(const void* x, const void* w, const void* bi
   if (M < 0 || N < 1 || K < 1 || K % per || ldx % per || ldw % per || ldx < K || ldw < K) return -2;
   if (ldx > (1 << 28) || ldw > (1 << 28) || N > 4000000 || act < 0 || act > 2) return -2;
   if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15) return -2;
+  if (M > 0 && M <= LINEAR_FEW_ROWS) {
+    const MtLinearEp ep = {bias, residual, z, bias_bf16, act, N, N};
+    if (bf16 && M <= 16) linear_few<__bf16, 1>(x, w, ep, y, (int)M, N, K, ldx, ldw, stream);
+    else if (bf16) linear_few<__bf16, 2>(x, w, ep, y, (int)M, N, K, ldx, ldw, stream);
+    else if (M <= 16) linear_few<float, 1>(x, w, ep, y, (int)M, N, K, ldx, ldw, stream);
+    else linear_few<float, 2>(x, w, ep, y, (int)M, N, K, ldx, ldw, stream);
+    return (int)hipGetLastError();
+  }
   for (int64_t m0 = 0; m0 < M; m0 += LINEAR_ROWS) {
     const int m = (int)(M - m0 < LINEAR_ROWS ? M - m0 : LINEAR_ROWS);
     const size_t at = (size_t)m0 * N * es;
@@ -134,6 +263,37 @@ extern "C" int mt_linear_fwd_launch(const void* x, const void* w, const void* bi
         hipLaunchKernelGGL(mt_linear_fwd_f32_kernel<128>, dim3(linear_grid(ti, tj)), dim3(F32_THREADS), 0, stream, g, ep, ti, tj);
       else
         hipLaunchKernelGGL(mt_linear_fwd_f32_kernel<64>, dim3(linear_grid(ti, tj)), dim3(F32_THREADS), 0, stream, g, ep, ti, tj);
+    }
+  }
+  return (int)hipGetLastError();
+}
+
+// dW [N][K] and db [N] (may be null) of dz [M][ld_dz] and x [M][ldx], without a split of the contraction: the widths are multiples of
+// a 16-byte piece (what lies behind N and K is zeros or not stored), the gradients contiguous and of the given types.
+extern "C" int mt_linear_wgrad_launch(const void* dz, const void* x, void* dw, void* db, int64_t M, int N, int K, int ld_dz, int ldx,
+                                      int db_bf16, int bf16, hipStream_t stream) {
+  const int per = bf16 ? 8 : 4, es = bf16 ? 2 : 4;
+  if (M < 1 || M > 0x7FFFFFFF - 256 || N < 1 || K < 1 || ld_dz % per || ldx % per || ld_dz < N || ldx < K) return -2;
+  const int flags = db != nullptr ? MT_GEMM_FLAG_DBIAS : 0;
+  const int most = 255 * (bf16 ? 128 : 64);            // output rows of a launch: their tile numbers are 8 bits
+  for (int n0 = 0; n0 < N; n0 += most) {
+    const int n = N - n0 < most ? N - n0 : most;
+    MtGemmGroup g = linear_group((const uint8_t*)dz + (size_t)n0 * es, x, (uint8_t*)dw + (size_t)n0 * K * es, n, K, (int)M, ld_dz, ldx, K);
+    if (db != nullptr) g.aux_out = (uint8_t*)db + (size_t)n0 * (db_bf16 ? 2 : 4);
+    MtLinearEp ep = {};
+    ep.bias_bf16 = db_bf16;
+    if (bf16 && mt_p8_rule(n, K, (int)M, 1, 256)) {
+      const int ti = (n + BIGT - 1) / BIGT, tj = (K + BIGT - 1) / BIGT;
+      hipLaunchKernelGGL(mt_linear_wgrad_p8_kernel, dim3(linear_grid(ti, tj)), dim3(P8_THREADS), 0, stream, g, ep, ti, tj, flags);
+    } else if (bf16) {
+      const int ti = (n + BM - 1) / BM, tj = (K + BN - 1) / BN;
+      if (ti * tj <= 320)
+        hipLaunchKernelGGL(mt_linear_wgrad_kernel<4>, dim3(linear_grid(ti, tj)), dim3(NTHREADS), 0, stream, g, ep, ti, tj, flags);
+      else
+        hipLaunchKernelGGL(mt_linear_wgrad_kernel<2>, dim3(linear_grid(ti, tj)), dim3(NTHREADS), 0, stream, g, ep, ti, tj, flags);
+    } else {
+      const int ti = (n + 63) / 64, tj = (K + 63) / 64;
+      hipLaunchKernelGGL(mt_linear_wgrad_f32_kernel<64>, dim3(linear_grid(ti, tj)), dim3(F32_THREADS), 0, stream, g, ep, ti, tj, flags);
     }
   }
   return (int)hipGetLastError();

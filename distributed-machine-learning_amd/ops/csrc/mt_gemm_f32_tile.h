@@ -286,7 +286,7 @@ __device__ __forceinline__ void f32_gemm_tile(const MtGemmGroup* __restrict__ gr
 
   // ------------------------------------------------------------------------------ epilogues
   const int fq = lane >> 4, fr = lane & 15;
-  if (MODE == 2) {
+  if (MODE == 2 && !EP) {
     float* C = reinterpret_cast<float*>(g.C) + (size_t)split * split_stride;
 #pragma unroll
     for (int m = 0; m < R; ++m) {
@@ -340,7 +340,7 @@ __device__ __forceinline__ void f32_gemm_tile(const MtGemmGroup* __restrict__ gr
         };
         if (ep->z != nullptr) put(ep->z, ep->ldz);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = mt_ep_act(v[j], ep->act);
+        for (int j = 0; j < 4; ++j) v[j] = mt_ep_act<false>(v[j], ep->act);
         if (ep->residual != nullptr) {
           const float* p = reinterpret_cast<const float*>(ep->residual) + (size_t)row * ep->ldr + col;
           f32x4 r = {0.f, 0.f, 0.f, 0.f};
@@ -354,6 +354,12 @@ __device__ __forceinline__ void f32_gemm_tile(const MtGemmGroup* __restrict__ gr
         }
         put(g.C, g.ldc);
       }
+    }
+    if (want_db) {
+      float* red = reinterpret_cast<float*>(lds);    // all waves are past the last K-step barrier
+      red[tid] = db_acc;
+      __syncthreads();
+      if (tid < T && i0 + tid < g.I) mt_ep_put_db(g.aux_out, i0 + tid, red[tid] + red[tid + T], ep->bias_bf16);
     }
     return;
   }

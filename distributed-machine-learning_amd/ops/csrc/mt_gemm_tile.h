@@ -205,7 +205,7 @@ __device__ __forceinline__ void mt_linear_epilogue(const f32x4 (&acc)[R][4], uin
       u32x2* at = reinterpret_cast<u32x2*>(img + kmaj_off(lrow, lcol >> 3) + (lcol & 7) * 2);
       float v[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = mt_ep_act(acc[m][n][j] + b[j], ep.act);
+      for (int j = 0; j < 4; ++j) v[j] = mt_ep_act<true>(acc[m][n][j] + b[j], ep.act);
       if (ep.residual != nullptr) {
         const u32x2 r = *at;
 #pragma unroll
@@ -308,6 +308,13 @@ __device__ __forceinline__ void gemm_tile(const MtGemmGroup* __restrict__ groups
   // ------------------------------------------------------------------------------ epilogues
   if constexpr (EP) {
     mt_linear_epilogue<4>(acc, lds + wave * 8192, i0 + wr * 64, j0 + wc * 64, g, *ep, lane);
+    if (want_db) {
+      __syncthreads();                               // the staging images are read
+      float* red = reinterpret_cast<float*>(lds);
+      red[tid] = db_acc;
+      __syncthreads();
+      if (tid < 128 && i0 + tid < g.I) mt_ep_put_db(g.aux_out, i0 + tid, red[tid] + red[tid + 128], ep->bias_bf16);
+    }
     return;
   }
   const int fq = lane >> 4, fr = lane & 15;
@@ -582,6 +589,18 @@ __device__ __forceinline__ void gemm_tile_p8(const MtGemmGroup& g, int ti, int t
 
   }
   // ------------------------------------------------------------------------------ epilogues
+  if constexpr (EP && MODE == 2) {
+    if (live) mt_linear_epilogue<8>(acc, lds + wave * 16384, qi0, qj0, g, *ep, lane);
+    if (want_db) {
+      __syncthreads();
+      float* red = reinterpret_cast<float*>(lds);
+      red[tid] = db_acc;
+      __syncthreads();
+      const int t = tid & 255, row = i0 + (tid >> 8) * 128 + t;
+      if (t < 128 && row < g.I) mt_ep_put_db(g.aux_out, row, red[tid] + red[tid + 128], ep->bias_bf16);
+    }
+    return;
+  }
   const int fq = lane >> 4, fr = lane & 15;
   if (MODE == 2) {
     float* C = reinterpret_cast<float*>(g.C) + (size_t)split * split_stride;

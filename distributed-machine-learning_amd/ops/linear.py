@@ -468,7 +468,8 @@ def _input_grad(so, dz, wc, out_f: int, stream) -> torch.Tensor:
 
 
 def _weight_grad(so, dz, xc, out_f: int, in_f: int, w_dtype, b_dtype, stream):
-    """(dW [out_f, in_f], db [out_f] or None): split over the rows, the slabs added in order and rounded once."""
+    """(dW [out_f, in_f], db [out_f] or None).  A layer with enough tiles stores them as they leave the matrix instruction; a
+    smaller one is split over the rows, the slabs added in order and rounded once."""
     from . import lib as L
     M, width, rows = dz.shape[0], xc.shape[1], dz.shape[1]
     xc = xc if xc.stride(0) == width else xc.contiguous()
@@ -477,6 +478,11 @@ def _weight_grad(so, dz, xc, out_f: int, in_f: int, w_dtype, b_dtype, stream):
     most = 255 * tile                               # output rows of a launch: its tile rows are 8 bits
     dw = torch.empty(out_f, in_f, device=dz.device, dtype=w_dtype)
     db = torch.empty(out_f, device=dz.device, dtype=b_dtype) if b_dtype is not None else None
+    if w_dtype == dz.dtype and _wgrad_splits(M, -(-min(rows, most) // tile) * -(-width // tile), 64 if bf16 else 128) == 1:
+        L.check(so.mt_linear_wgrad_launch(dz.data_ptr(), xc.data_ptr(), dw.data_ptr(), db.data_ptr() if db is not None else None, M,
+                                          out_f, in_f, rows, width, int(b_dtype == torch.bfloat16), int(bf16), stream),
+                "mt_linear_wgrad_launch")
+        return dw, db
     if rows > most:
         parts = [dz[:, r:r + most].contiguous() for r in range(0, rows, most)]
     else:
