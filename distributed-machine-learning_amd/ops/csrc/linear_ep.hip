@@ -11,37 +11,82 @@
 #include "mt_gemm_tile.h"
 #include "mt_gemm_f32_tile.h"
 
-template <int NSTAGE>
-__global__ __launch_bounds__(NTHREADS) void mt_linear_fwd_kernel(MtGemmGroup g, MtLinearEp ep, int tiles_i, int tiles_j) {
+// MODE 0: A [I][KK] and B [J][KK] (forward); 1: B [KK][J] (input gradient).  A contraction may be split over workgroups: part `sp`
+// takes its share of the columns of A (and columns or rows of B) and leaves its accumulators in ep.part.
+template <int MODE, typename T>
+__device__ __forceinline__ void linear_split(MtGemmGroup& g, MtLinearEp& ep, int sp, int per) {
+  const int k0 = sp * per;
+  g.A = reinterpret_cast<const T*>(g.A) + k0;
+  g.B = reinterpret_cast<const T*>(g.B) + (MODE == 0 ? (size_t)k0 : (size_t)k0 * g.ldb);
+  g.KK = g.KK - k0 < per ? g.KK - k0 : per;
+  ep.part += (size_t)sp * g.I * g.J;
+}
+// block -> (tile, part): whole row panels per XCD, the parts of a tile side by side
+#define LINEAR_PICK()                                                                                                      \
+  const int all = tiles_i * tiles_j * splits, share = (all + 7) / 8, u = (blockIdx.x % 8) * share + blockIdx.x / 8; \
+  if (u >= all) return;                                                                                                    \
+  const int t = u / splits
+template <int MODE, int NSTAGE>
+__global__ __launch_bounds__(NTHREADS) void mt_linear_gemm_kernel(MtGemmGroup g, MtLinearEp ep, int tiles_i, int tiles_j, int splits,
+                                                                  int per) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[NSTAGE * STAGE_BYTES];
-  const int n = tiles_i * tiles_j, per = (n + 7) / 8, t = (blockIdx.x % 8) * per + blockIdx.x / 8;      // whole row panels per XCD
-  if (t >= n) return;
+  LINEAR_PICK();
+  if (splits > 1) linear_split<MODE, uint16_t>(g, ep, u % splits, per);
   MtTile tile;
   tile.group = 0;
   tile.ti = (int16_t)(t / tiles_j);
   tile.tj = (int16_t)(t % tiles_j);
-  gemm_tile<0, NSTAGE, true>(&g, tile, 0, 0, 0, 0, 1, 0, lds, &ep);
+  gemm_tile<MODE, NSTAGE, true>(&g, tile, 0, 0, 0, 0, 1, 0, lds, &ep);
 }
 #define LINEAR_BAND 4       // 256-tiles: row tiles of a band (mt_gemm_p8_kernel)
-__global__ __launch_bounds__(P8_THREADS) void mt_linear_fwd_p8_kernel(MtGemmGroup g, MtLinearEp ep, int tiles_i, int tiles_j) {
+template <int MODE>
+__global__ __launch_bounds__(P8_THREADS) void mt_linear_p8_kernel(MtGemmGroup g, MtLinearEp ep, int tiles_i, int tiles_j) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BIG_STAGE_BYTES];
-  const int n = tiles_i * tiles_j, per = (n + 7) / 8, t = (blockIdx.x % 8) * per + blockIdx.x / 8;
-  if (t >= n) return;
+  constexpr int splits = 1;
+  LINEAR_PICK();
   const int in_band = LINEAR_BAND * tiles_j, first = (t / in_band) * LINEAR_BAND;
   const int rows = tiles_i - first < LINEAR_BAND ? tiles_i - first : LINEAR_BAND;
   const int r = t % in_band;
-  gemm_tile_p8<0, 1, true>(g, first + r % rows, r / rows, 0, 0, 1, 0, lds, &ep);
+  gemm_tile_p8<MODE, MODE == 0 ? 1 : 0, true>(g, first + r % rows, r / rows, 0, 0, 1, 0, lds, &ep);
 }
-template <int T>
-__global__ __launch_bounds__(F32_THREADS) void mt_linear_fwd_f32_kernel(MtGemmGroup g, MtLinearEp ep, int tiles_i, int tiles_j) {
+template <int MODE, int T>
+__global__ __launch_bounds__(F32_THREADS) void mt_linear_gemm_f32_kernel(MtGemmGroup g, MtLinearEp ep, int tiles_i, int tiles_j,
+                                                                         int splits, int per) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * 2 * T * 128];
-  const int n = tiles_i * tiles_j, per = (n + 7) / 8, t = (blockIdx.x % 8) * per + blockIdx.x / 8;
-  if (t >= n) return;
+  LINEAR_PICK();
+  if (splits > 1) linear_split<MODE, float>(g, ep, u % splits, per);
   MtTile tile;
   tile.group = 0;
   tile.ti = (int16_t)(t / tiles_j);
   tile.tj = (int16_t)(t % tiles_j);
-  f32_gemm_tile<0, 2, T, 1, 0, true>(&g, tile, 0, 0, 0, 0, 1, 0, lds, &ep);
+  f32_gemm_tile<MODE, 2, T, 1, 0, true>(&g, tile, 0, 0, 0, 0, 1, 0, lds, &ep);
+}
+// The parts of a split contraction added in order, then the epilogue; four elements per thread.
+template <typename T>
+__global__ __launch_bounds__(256) void mt_linear_join_kernel(const float* __restrict__ part, MtLinearEp ep, T* __restrict__ y,
+                                                             int64_t total, int N, int splits) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= total) return;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  const bool whole = i + 4 <= total;
+  for (int s = 0; s < splits; ++s) {
+    f32x4 p = {0.f, 0.f, 0.f, 0.f};
+    const float* src = part + (int64_t)s * total + i;
+    if (whole) __builtin_memcpy(&p, src, 16);
+    else
+      for (int e = 0; e < 4; ++e) p[e] = i + e < total ? src[e] : 0.f;
+    v += p;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (i + e >= total) break;
+    const int col = (int)((i + e) % N);
+    float o = v[e] + (ep.bias != nullptr ? mt_ep_bias(ep, col) : 0.f);
+    if (ep.z != nullptr) reinterpret_cast<T*>(ep.z)[i + e] = (T)o;
+    o = mt_ep_act<sizeof(T) == 2>(o, ep.act);
+    if (ep.residual != nullptr) o += (float)reinterpret_cast<const T*>(ep.residual)[i + e];
+    y[i + e] = (T)o;
+  }
 }
 
 // Weight gradient with the whole contraction in one workgroup: dW (and db) leave in their own types.
@@ -206,7 +251,7 @@ static MtGemmGroup linear_group(const void* A, const void* B, void* C, int I, in
   g.active_steps = 1;
   return g;
 }
-static int linear_grid(int tiles_i, int tiles_j) { return (tiles_i * tiles_j + 7) / 8 * 8; }
+static int linear_grid(int tiles_i, int tiles_j, int splits) { return (tiles_i * tiles_j * splits + 7) / 8 * 8; }
 
 // Few rows: as many waves per workgroup as leave each at least two unrolled groups of steps, up to about 16 waves per CU.
 template <typename T, int MT>
@@ -226,43 +271,84 @@ static void linear_few(const void* x, const void* w, const MtLinearEp& ep, void*
 }
 #define LINEAR_FEW_ROWS 32
 
-// x [M][ldx], W [N][ldw]: rows of whole 16-byte pieces; K columns, a multiple of a piece.  residual, z, y: [M][N] contiguous.
-extern "C" int mt_linear_fwd_launch(const void* x, const void* w, const void* bias, const void* residual, void* y, void* z, int64_t M,
-                                    int N, int K, int64_t ldx, int64_t ldw, int act, int bias_bf16, int bf16, hipStream_t stream) {
-  const int per = bf16 ? 8 : 4, es = bf16 ? 2 : 4;
-  if (M < 0 || N < 1 || K < 1 || K % per || ldx % per || ldw % per || ldx < K || ldw < K) return -2;
-  if (ldx > (1 << 28) || ldw > (1 << 28) || N > 4000000 || act < 0 || act > 2) return -2;
-  if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15) return -2;
-  if (M > 0 && M <= LINEAR_FEW_ROWS) {
-    const MtLinearEp ep = {bias, residual, z, bias_bf16, act, N, N};
-    if (bf16 && M <= 16) linear_few<__bf16, 1>(x, w, ep, y, (int)M, N, K, ldx, ldw, stream);
-    else if (bf16) linear_few<__bf16, 2>(x, w, ep, y, (int)M, N, K, ldx, ldw, stream);
-    else if (M <= 16) linear_few<float, 1>(x, w, ep, y, (int)M, N, K, ldx, ldw, stream);
-    else linear_few<float, 2>(x, w, ep, y, (int)M, N, K, ldx, ldw, stream);
+// Tile edge of an f32 launch, and how many parts the contraction of a launch is split into: launches of at most half as many tiles
+// as the chip has CUs, whose contraction is long enough to leave every part 512 deep.
+static int linear_edge(int64_t M, int N, int bf16) {
+  if (bf16) return 128;
+  return ((M + 127) / 128) * ((N + 127) / 128) >= 512 ? 128 : 64;
+}
+static int linear_splits(int mode, int64_t M, int N, int KK, int bf16, int* per) {
+  const int edge = linear_edge(M, N, bf16), step = bf16 ? BK : F32_BK;
+  const int64_t tiles = ((M + edge - 1) / edge) * ((N + edge - 1) / edge);
+  *per = KK;
+  if ((mode == 0 && M <= LINEAR_FEW_ROWS) || M > LINEAR_ROWS || tiles > 128) return 1;
+  int64_t want = 256 / tiles, deep = KK / 512;
+  if (deep < want) want = deep;
+  if (want < 2) return 1;
+  *per = ((KK + (int)want - 1) / (int)want + step - 1) / step * step;
+  return (KK + *per - 1) / *per;
+}
+// Parts [n][M][N] f32 of workspace that mt_linear_gemm_launch wants; 1: none.
+extern "C" int mt_linear_parts(int mode, int64_t M, int N, int KK, int bf16) {
+  if (M < 0 || N < 1 || KK < 1 || mode < 0 || mode > 1) return -2;
+  int per;
+  return linear_splits(mode, M, N, KK, bf16, &per);
+}
+
+// C [M][N] = act(A B + bias) + residual, contiguous, as residual and z.  A [M][lda], KK columns.  mode 0: B [N][ldb]; mode 1: B
+// [KK][ldb].  Rows of A and B start on 16-byte boundaries and are whole 16-byte pieces: what an operand holds between KK (N) and the
+// end of its last piece is multiplied (zeros, or rows of the other operand that are).
+extern "C" int mt_linear_gemm_launch(int mode, const void* A, const void* B, const void* bias, const void* residual, void* C, void* z,
+                                     float* part, int64_t M, int N, int KK, int64_t lda, int64_t ldb, int act, int bias_bf16, int bf16,
+                                     hipStream_t stream) {
+  const int per16 = bf16 ? 8 : 4, es = bf16 ? 2 : 4;
+  if (mode < 0 || mode > 1 || M < 0 || N < 1 || KK < 1 || lda % per16 || ldb % per16 || lda < KK || ldb < (mode == 0 ? KK : N)) return -2;
+  if (mode == 0 && KK % per16) return -2;
+  if (lda > (1 << 28) || ldb > (1 << 28) || N > 2000000 || act < 0 || act > 2) return -2;
+  if ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B)) & 15) return -2;
+  if (M == 0) return 0;
+  if (mode == 0 && M <= LINEAR_FEW_ROWS) {
+    const MtLinearEp ep = {bias, residual, z, nullptr, bias_bf16, act, N, N};
+    if (bf16 && M <= 16) linear_few<__bf16, 1>(A, B, ep, C, (int)M, N, KK, lda, ldb, stream);
+    else if (bf16) linear_few<__bf16, 2>(A, B, ep, C, (int)M, N, KK, lda, ldb, stream);
+    else if (M <= 16) linear_few<float, 1>(A, B, ep, C, (int)M, N, KK, lda, ldb, stream);
+    else linear_few<float, 2>(A, B, ep, C, (int)M, N, KK, lda, ldb, stream);
     return (int)hipGetLastError();
   }
+  int per;
+  const int splits = linear_splits(mode, M, N, KK, bf16, &per);
+  if (splits > 1 && part == nullptr) return -2;
   for (int64_t m0 = 0; m0 < M; m0 += LINEAR_ROWS) {
     const int m = (int)(M - m0 < LINEAR_ROWS ? M - m0 : LINEAR_ROWS);
     const size_t at = (size_t)m0 * N * es;
-    MtGemmGroup g = linear_group((const uint8_t*)x + (size_t)m0 * ldx * es, w, (uint8_t*)y + at, m, N, K, (int)ldx, (int)ldw, N);
-    MtLinearEp ep = {bias, residual ? (const uint8_t*)residual + at : nullptr, z ? (uint8_t*)z + at : nullptr, bias_bf16, act, N, N};
-    if (bf16 && mt_p8_rule(m, N, K, 1, 256)) {
+    MtGemmGroup g = linear_group((const uint8_t*)A + (size_t)m0 * lda * es, B, (uint8_t*)C + at, m, N, KK, (int)lda, (int)ldb, N);
+    MtLinearEp ep = {bias, residual ? (const uint8_t*)residual + at : nullptr, z ? (uint8_t*)z + at : nullptr,
+                     splits > 1 ? part : nullptr, bias_bf16, act, N, N};
+    if (bf16 && splits == 1 && mt_p8_rule(m, N, KK, 1, 256)) {
       const int ti = (m + BIGT - 1) / BIGT, tj = (N + BIGT - 1) / BIGT;
-      hipLaunchKernelGGL(mt_linear_fwd_p8_kernel, dim3(linear_grid(ti, tj)), dim3(P8_THREADS), 0, stream, g, ep, ti, tj);
-    } else if (bf16) {
-      const int ti = (m + BM - 1) / BM, tj = (N + BN - 1) / BN;
-      if (ti * tj <= 320)
-        hipLaunchKernelGGL(mt_linear_fwd_kernel<4>, dim3(linear_grid(ti, tj)), dim3(NTHREADS), 0, stream, g, ep, ti, tj);
-      else
-        hipLaunchKernelGGL(mt_linear_fwd_kernel<2>, dim3(linear_grid(ti, tj)), dim3(NTHREADS), 0, stream, g, ep, ti, tj);
+      const dim3 grid(linear_grid(ti, tj, 1)), block(P8_THREADS);
+      if (mode == 0) hipLaunchKernelGGL(mt_linear_p8_kernel<0>, grid, block, 0, stream, g, ep, ti, tj);
+      else hipLaunchKernelGGL(mt_linear_p8_kernel<1>, grid, block, 0, stream, g, ep, ti, tj);
+      continue;
+    }
+    const int edge = linear_edge(m, N, bf16), ti = (m + edge - 1) / edge, tj = (N + edge - 1) / edge;
+    const dim3 grid(linear_grid(ti, tj, splits)), block(256);
+#define GO(K, ...) hipLaunchKernelGGL((K<__VA_ARGS__>), grid, block, 0, stream, g, ep, ti, tj, splits, per)
+    if (bf16) {
+      const bool deep = ti * tj * splits <= 320;      // a workgroup or less per CU: four stages, else two workgroups of two
+      if (mode == 0) { if (deep) GO(mt_linear_gemm_kernel, 0, 4); else GO(mt_linear_gemm_kernel, 0, 2); }
+      else { if (deep) GO(mt_linear_gemm_kernel, 1, 4); else GO(mt_linear_gemm_kernel, 1, 2); }
+    } else if (edge == 128) {
+      if (mode == 0) GO(mt_linear_gemm_f32_kernel, 0, 128); else GO(mt_linear_gemm_f32_kernel, 1, 128);
     } else {
-      const int64_t n128 = (int64_t)((m + 127) / 128) * ((N + 127) / 128);
-      const int T = n128 >= 512 ? 128 : 64;
-      const int ti = (m + T - 1) / T, tj = (N + T - 1) / T;
-      if (T == 128)
-        hipLaunchKernelGGL(mt_linear_fwd_f32_kernel<128>, dim3(linear_grid(ti, tj)), dim3(F32_THREADS), 0, stream, g, ep, ti, tj);
-      else
-        hipLaunchKernelGGL(mt_linear_fwd_f32_kernel<64>, dim3(linear_grid(ti, tj)), dim3(F32_THREADS), 0, stream, g, ep, ti, tj);
+      if (mode == 0) GO(mt_linear_gemm_f32_kernel, 0, 64); else GO(mt_linear_gemm_f32_kernel, 1, 64);
+    }
+#undef GO
+    if (splits > 1) {
+      const int64_t total = (int64_t)m * N;
+      const dim3 jgrid((unsigned)((total + 1023) / 1024));
+      if (bf16) hipLaunchKernelGGL(mt_linear_join_kernel<__bf16>, jgrid, dim3(256), 0, stream, part, ep, (__bf16*)g.C, total, N, splits);
+      else hipLaunchKernelGGL(mt_linear_join_kernel<float>, jgrid, dim3(256), 0, stream, part, ep, (float*)g.C, total, N, splits);
     }
   }
   return (int)hipGetLastError();
@@ -284,16 +370,16 @@ extern "C" int mt_linear_wgrad_launch(const void* dz, const void* x, void* dw, v
     ep.bias_bf16 = db_bf16;
     if (bf16 && mt_p8_rule(n, K, (int)M, 1, 256)) {
       const int ti = (n + BIGT - 1) / BIGT, tj = (K + BIGT - 1) / BIGT;
-      hipLaunchKernelGGL(mt_linear_wgrad_p8_kernel, dim3(linear_grid(ti, tj)), dim3(P8_THREADS), 0, stream, g, ep, ti, tj, flags);
+      hipLaunchKernelGGL(mt_linear_wgrad_p8_kernel, dim3(linear_grid(ti, tj, 1)), dim3(P8_THREADS), 0, stream, g, ep, ti, tj, flags);
     } else if (bf16) {
       const int ti = (n + BM - 1) / BM, tj = (K + BN - 1) / BN;
       if (ti * tj <= 320)
-        hipLaunchKernelGGL(mt_linear_wgrad_kernel<4>, dim3(linear_grid(ti, tj)), dim3(NTHREADS), 0, stream, g, ep, ti, tj, flags);
+        hipLaunchKernelGGL(mt_linear_wgrad_kernel<4>, dim3(linear_grid(ti, tj, 1)), dim3(NTHREADS), 0, stream, g, ep, ti, tj, flags);
       else
-        hipLaunchKernelGGL(mt_linear_wgrad_kernel<2>, dim3(linear_grid(ti, tj)), dim3(NTHREADS), 0, stream, g, ep, ti, tj, flags);
+        hipLaunchKernelGGL(mt_linear_wgrad_kernel<2>, dim3(linear_grid(ti, tj, 1)), dim3(NTHREADS), 0, stream, g, ep, ti, tj, flags);
     } else {
       const int ti = (n + 63) / 64, tj = (K + 63) / 64;
-      hipLaunchKernelGGL(mt_linear_wgrad_f32_kernel<64>, dim3(linear_grid(ti, tj)), dim3(F32_THREADS), 0, stream, g, ep, ti, tj, flags);
+      hipLaunchKernelGGL(mt_linear_wgrad_f32_kernel<64>, dim3(linear_grid(ti, tj, 1)), dim3(F32_THREADS), 0, stream, g, ep, ti, tj, flags);
     }
   }
   return (int)hipGetLastError();

@@ -327,6 +327,10 @@ __device__ __forceinline__ void f32_gemm_tile(const MtGemmGroup* __restrict__ gr
       for (int m = 0; m < R; ++m) {
         const int row = i0 + wr * W + m * 16 + fr;
         if (row >= g.I || col >= g.J) continue;
+        if (ep->part != nullptr) {
+          mt_ep_put_part(ep->part, row, col, g.J, acc[m][n]);
+          continue;
+        }
         const bool whole = col + 4 <= g.J;
         f32x4 v = acc[m][n] + bb;
         auto put = [&](void* base, int ld) {

@@ -127,6 +127,16 @@ template <int R>
 __device__ __forceinline__ void mt_linear_epilogue(const f32x4 (&acc)[R][4], uint8_t* img, int qi0, int qj0, const MtGemmGroup& g,
                                                    const MtLinearEp& ep, int lane) {
   const int fq = lane >> 4, fr = lane & 15;
+  if (ep.part != nullptr) {
+#pragma unroll
+    for (int m = 0; m < R; ++m)
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int row = qi0 + m * 16 + fr, col = qj0 + n * 16 + fq * 4;
+        if (row < g.I && col < g.J) mt_ep_put_part(ep.part, row, col, g.J, acc[m][n]);
+      }
+    return;
+  }
   auto fence = [] {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_wave_barrier();

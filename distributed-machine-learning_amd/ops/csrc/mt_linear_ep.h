@@ -10,11 +10,23 @@ struct MtLinearEp {
   const void* bias;        // [J] f32, or bf16 with bias_bf16; may be null
   const void* residual;    // [I][ldr], the output's type; may be null
   void* z;                 // [I][ldz], the output's type; may be null
+  float* part;             // [I][J] f32: the bare accumulators go here instead (one part of a split contraction); may be null
   int32_t bias_bf16, act, ldr, ldz;
 };
 __device__ __forceinline__ float mt_ep_bias(const MtLinearEp& ep, int col) {
   return ep.bias_bf16 ? bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(ep.bias)[col])
                       : reinterpret_cast<const float*>(ep.bias)[col];
+}
+// Four accumulator columns of a row, at whatever alignment the row has; columns past J are left alone.
+__device__ __forceinline__ void mt_ep_put_part(float* part, int64_t row, int col, int J, f32x4 v) {
+  float* p = part + row * J + col;
+  if (col + 4 <= J) {
+    __builtin_memcpy(p, &v, 16);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col + j < J) p[j] = v[j];
+  }
 }
 __device__ __forceinline__ void mt_ep_put_db(void* db, int row, float v, int bf16) {
   if (bf16) reinterpret_cast<uint16_t*>(db)[row] = (uint16_t)f32_to_bf16_bits(v);

@@ -355,6 +355,21 @@ def _rows_of(t: torch.Tensor, width: int) -> torch.Tensor:
     return t if t.dim() == 2 else t.reshape(-1, width)
 
 
+def _fused_gemm(so, mode: int, a, b, c, depth: int, bias=None, residual=None, z=None, act: int = 0) -> None:
+    """c = act(a b + bias) + residual: b is [columns, depth] in mode 0, [depth, columns] in mode 1."""
+    from . import lib as L
+    M, N = c.shape
+    bf16 = int(c.dtype == torch.bfloat16)
+    n = so.mt_linear_parts(mode, M, N, depth, bf16)
+    part = torch.empty(n, M, N, device=c.device, dtype=torch.float32) if n > 1 else None
+    ptr = lambda t: t.data_ptr() if t is not None else None          # noqa: E731
+    with L.on(c.device):
+        L.check(so.mt_linear_gemm_launch(mode, a.data_ptr(), b.data_ptr(), ptr(bias), ptr(residual), c.data_ptr(), ptr(z), ptr(part),
+                                         M, N, depth, a.stride(0), b.stride(0), act,
+                                         int(bias is not None and bias.dtype == torch.bfloat16), bf16, L.raw_stream(c.device)),
+                "mt_linear_gemm_launch")
+
+
 def fused_forward(x, weight, bias, residual, act: int, w16, keep_z: bool):
     """(output, x's rows, the weight as multiplied, z or None)."""
     from . import lib as L
@@ -368,15 +383,9 @@ def fused_forward(x, weight, bias, residual, act: int, w16, keep_z: bool):
     wc = _pieces(wc)
     bc = bias.detach().contiguous() if bias is not None else None
     rc = _rows_of(residual, out_f).contiguous() if residual is not None else None
-    M = xc.shape[0]
-    y = torch.empty(M, out_f, device=x.device, dtype=x.dtype)
+    y = torch.empty(xc.shape[0], out_f, device=x.device, dtype=x.dtype)
     z = torch.empty_like(y) if keep_z else None
-    with L.on(x.device):
-        L.check(so.mt_linear_fwd_launch(xc.data_ptr(), wc.data_ptr(), bc.data_ptr() if bc is not None else None,
-                                        rc.data_ptr() if rc is not None else None, y.data_ptr(),
-                                        z.data_ptr() if z is not None else None, M, out_f, xc.shape[1], xc.stride(0), wc.stride(0),
-                                        act, int(bc is not None and bc.dtype == torch.bfloat16), int(x.dtype == torch.bfloat16),
-                                        L.raw_stream(x.device)), "mt_linear_fwd_launch")
+    _fused_gemm(so, 0, xc, wc, y, xc.shape[1], bc, rc, z, act)
     return y.view(x.shape[:-1] + (out_f,)), xc, wc, z
 
 
@@ -425,7 +434,9 @@ class FusedLinear(torch.autograd.Function):
                     return (dx, dw[:out_f, :in_f], db[:out_f] if db is not None else None,
                             dy if r_shape is not None else None, None, None)
                 if ctx.needs_input_grad[0]:
-                    dx = _input_grad(so, dz, wc, out_f, stream)[:, :in_f].reshape(x_shape)
+                    dx = torch.empty(M, in_f, device=dev, dtype=xc.dtype)
+                    _fused_gemm(so, 1, dz, wc, dx, out_f)
+                    dx = dx.view(x_shape)
                 if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
                     dw, db = _weight_grad(so, dz, xc, out_f, in_f, w_dtype, b_dtype, stream)
         return dx, dw, db, (dy if r_shape is not None else None), None, None
@@ -447,24 +458,6 @@ def _small_grads(so, dz, xc, wc, want_dx: bool, want_db: bool, stream):
                                                 db.data_ptr() if want_db else None, R, in_f, out, OPTIONS.small_linear_tile,
                                                 stream), "mt_small_linear_bwd_tiled_launch")
     return dx, dw, db
-
-
-def _input_grad(so, dz, wc, out_f: int, stream) -> torch.Tensor:
-    """dz W [rows, W's padded width]; the contraction runs over W's ``out_f`` rows."""
-    from . import lib as L
-    M, width = dz.shape[0], wc.shape[1]
-    dx = torch.empty(M, width, device=dz.device, dtype=dz.dtype)
-    es, most = dz.element_size(), 1 << 20          # a launch's tile coordinates are 16 bits
-    for m0 in range(0, M, most):
-        m = min(most, M - m0)
-        a, c = dz.data_ptr() + m0 * dz.shape[1] * es, dx.data_ptr() + m0 * width * es
-        if es == 2:
-            L.check(so.mt_gemm_single_launch(1, a, wc.data_ptr(), c, None, m, width, out_f, dz.shape[1], wc.stride(0), width, 0,
-                                             0, stream), "mt_gemm_single_launch")
-        else:
-            L.check(so.mt_gemm_f32_single_launch(1, a, wc.data_ptr(), c, None, None, m, width, out_f, dz.shape[1], wc.stride(0),
-                                                 width, 0, stream), "mt_gemm_f32_single_launch")
-    return dx
 
 
 def _weight_grad(so, dz, xc, out_f: int, in_f: int, w_dtype, b_dtype, stream):

@@ -100,6 +100,17 @@ def test_the_large_tiles(act, residual):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("act,residual", [("gelu", True), ("relu", True), (None, False)])
+@pytest.mark.parametrize("M,K,N", [(40, 2200, 70), (130, 1025, 1100), (5, 1500, 2600)])
+def test_long_contractions_over_few_tiles_are_split(dtype, act, residual, M, K, N):
+    """Forward over K, input gradient over N: parts added in order, odd widths and last parts of another depth."""
+    x, w, b, r, dy = _make(M, K, N, dtype, act == "relu", residual)
+    bf16 = dtype == torch.bfloat16
+    _check(_run(x, w, b, r, dy, act), _formula(x, w, b, r, dy, act, bf16, bf16))
+
+
+@pytest.mark.gpu
 def test_more_output_features_than_one_weight_gradient_launch_takes():
     M, K, N = 40, 16, 16400
     x, w, b, r, dy = _make(M, K, N, torch.float32, False, False)
