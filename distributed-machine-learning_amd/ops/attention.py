@@ -28,7 +28,7 @@ from typing import Optional, Sequence, Union
 import numpy as np
 import torch
 
-from .lib import PACKED_ITEM_BYTES as _ITEM, PACKED_TILE_ROWS as _TILE
+from .lib import PACKED_ITEM_BYTES, PACKED_OWN_ROWS, PACKED_SPLIT_ROWS
 
 RELU_EPS = 1e-6
 MAX_SEQ = 128
@@ -135,6 +135,7 @@ def self_attention(qk: torch.Tensor, v: torch.Tensor, num_heads: int, kind: str 
 
 # ---- packed sequences -----------------------------------------------------------------------------------------------------
 PACKED_MAX_HEAD_DIM = 128
+SOLO_ROWS = 256          # packs' short sequences: see attention_hip.packed_form
 
 
 class SequencePack:
@@ -142,7 +143,7 @@ class SequencePack:
     ``rows`` (default: their sum) is the number of rows of the tensors; rows behind the last sequence belong to none.
 
     Made once per batch and used by every layer and both passes: the lengths are checked on the host, and the list of
-    128-row tiles the kernels work through, longest first, is laid out on ``device`` (default: the current GPU if there is
+    pieces the kernels work through, longest first, is laid out on ``device`` (default: the current GPU if there is
     one).  ``SequencePack.uniform(count, length)`` is ``count`` sequences of one length; it needs no list."""
 
     def __init__(self, lengths: Union[Sequence[int], np.ndarray, torch.Tensor], rows: Optional[int] = None, device=None):
@@ -174,53 +175,61 @@ class SequencePack:
         self.lengths = np.full(int(count), int(length), dtype=np.int64)
         self.longest = int(length) if count else 0
         self.uniform_length = int(length) if count else 0
-        tiles = -(-int(length) // _TILE) * int(count)
-        self._count, self._lists, self._stream = tiles, None, 0
+        own, fine = (-(-int(length) // r) * int(count) for r in (PACKED_OWN_ROWS, PACKED_SPLIT_ROWS))
+        self._counts, self._lists, self._stream = (own, fine, own if length <= SOLO_ROWS else fine), None, 0
         return self
 
     def _fix(self, total: int, rows: int, device) -> None:
         rows = int(rows)
         if rows < total:
             raise ValueError(f"sequences of {total} rows do not fit {rows} rows")
-        if rows > 0x7FFFFFFF - _TILE:
-            raise ValueError(f"a pack holds at most {0x7FFFFFFF - _TILE} rows, got {rows}")
+        if rows > 0x7FFFFFFF - PACKED_OWN_ROWS:
+            raise ValueError(f"a pack holds at most {0x7FFFFFFF - PACKED_OWN_ROWS} rows, got {rows}")
         device = torch.device(device if device is not None else ("cuda" if torch.cuda.is_available() else "cpu"))
         if device.type == "cuda" and device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
         self.total, self.rows, self.device = total, rows, device
 
     def _lay_out(self) -> None:
-        """Three orders of the same tiles (``{first row of the sequence, its length, tile's first row in it}``), most work
-        first: by keys up to the tile's end (causal queries), by queries from its start (causal keys), by length (all see
-        all).  Rows of no sequence follow as entries of negative length, which the kernels fill with zeros."""
+        """Three lists of items (``{first row of the sequence, its length, item's first row in it, solo}``): 128 rows each; 32 rows
+        each; and 128 rows walked alone by four waves for sequences of at most ``SOLO_ROWS`` rows, else 32.  Each in three orders,
+        most work first: by keys up to the item's end (causal queries), by queries from its start (causal keys), by length (all
+        see all).  Rows of no sequence follow as entries of negative length, which the kernels fill with zeros."""
         n = self.lengths
         starts = np.concatenate([[0], np.cumsum(n)])[:-1]
-        tiles = -(-n // _TILE)
-        seq = np.repeat(np.arange(len(n)), tiles)
-        first = (np.arange(len(seq)) - np.repeat(np.cumsum(tiles) - tiles, tiles)) * _TILE
-        items = np.zeros((len(seq), 4), dtype=np.int32)
-        items[:, 0], items[:, 1], items[:, 2] = starts[seq], n[seq], first
-        at = np.arange(self.total, self.rows, _TILE)
+        at = np.arange(self.total, self.rows, PACKED_OWN_ROWS)
         tail = np.zeros((len(at), 4), dtype=np.int32)
-        tail[:, 0], tail[:, 1] = at, -np.minimum(_TILE, self.rows - at)
-        orders = [np.argsort(-work, kind="stable") for work in (np.minimum(first + _TILE, n[seq]), n[seq] - first, n[seq])]
-        lists = np.concatenate([np.concatenate([items[o], tail]) for o in orders]) if len(items) + len(tail) else items
-        self._count = len(items) + len(tail)
+        tail[:, 0], tail[:, 1] = at, -np.minimum(PACKED_OWN_ROWS, self.rows - at)
+        short = n <= SOLO_ROWS
+        lists, counts = [], []
+        for solo in (np.zeros_like(short), np.zeros_like(short), short):
+            grain = np.where(solo, PACKED_OWN_ROWS, PACKED_SPLIT_ROWS) if len(lists) else np.full(len(n), PACKED_OWN_ROWS)
+            parts = -(-n // grain)
+            seq = np.repeat(np.arange(len(n)), parts)
+            first = (np.arange(len(seq)) - np.repeat(np.cumsum(parts) - parts, parts)) * grain[seq]
+            items = np.stack([starts[seq], n[seq], first, solo[seq]], axis=1).astype(np.int32)
+            walkers = np.where(solo[seq] | (len(lists) == 0), 1, 4)          # waves that share an item's walk
+            orders = [np.argsort(-(work / walkers), kind="stable")
+                      for work in (np.minimum(first + grain[seq], n[seq]), n[seq] - first, n[seq])]
+            lists += [np.concatenate([items[o], tail]) for o in orders]
+            counts.append(len(items) + len(tail))
+        self._counts = tuple(counts)
         self._lists, self._stream = None, 0
         if self.device.type == "cuda":
             from .lib import raw_stream
             # a blocking copy: the list is there for whichever stream uses it first
-            self._lists, self._stream = torch.from_numpy(lists).to(self.device), raw_stream(self.device)
+            self._lists = torch.from_numpy(np.concatenate(lists)).to(self.device)
+            self._stream = raw_stream(self.device)
 
-    def _tiles(self, causal: bool, stream: int):
-        """Addresses of the query and the key tiles' lists (0: none needed) for a launch on ``stream``."""
+    def _items(self, which: int, order: int, stream: int):
+        """(address, number) of a list for a launch on ``stream``: ``which`` 0 / 1 / 2 as laid out above, ``order`` 0 causal queries,
+        1 causal keys, 2 no mask.  Uniform batches have no list (address 0)."""
         if self._lists is None:
-            return 0, 0
+            return 0, self._counts[which]
         if stream != self._stream:       # keeps the allocator from handing the list's memory on too early
             self._lists.record_stream(torch.cuda.current_stream(self.device))
-        at, step = self._lists.data_ptr(), self._count * _ITEM
-        return (at, at + step) if causal else (at + 2 * step, at + 2 * step)
-
+        at = 3 * sum(self._counts[:which]) + order * self._counts[which]
+        return self._lists.data_ptr() + at * PACKED_ITEM_BYTES, self._counts[which]
 
 
 def packed_attention_reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pack: SequencePack, causal: bool = False,

@@ -9,6 +9,7 @@ import torch
 import torch.nn.functional as F
 
 from . import lib as L
+from .attention import SOLO_ROWS
 
 _KIND = {"softmax": 0, "relu": 1}
 
@@ -176,23 +177,39 @@ def _in_place(t: torch.Tensor) -> torch.Tensor:
     return F.pad(t, (0, pad)).contiguous() if pad else t.clone(memory_format=torch.contiguous_format)
 
 
-FORM = -1       # -1: the bf16 kernels by the launch's size; 0 / 1 force the ones whose waves share a tile / a walk (tests)
+FORM = None       # tests: the form of every launch
+
+
+def packed_form(pack, lanes: int, bf16: bool) -> int:
+    """How a launch over ``lanes`` heads divides its work: 0, workgroups own 128 rows and share the tiles they walk over (bf16); 1,
+    they own 32 rows and their waves share the walk; 2, the same except that each wave of a short sequence's workgroup owns 32 rows.
+    Measured, bf16, 0 / 1: one causal sequence of 2048, 8 heads of 128 (128 workgroups) forward 54 / 28 us; 8192, 2 heads (128)
+    194 / 84, with its backward pass 1085 / 337; 4 x 2048, 16 heads (1024) 120 / 134."""
+    if FORM is not None:
+        return FORM if bf16 else max(1, FORM)
+    if bf16 and pack._counts[0] * lanes >= 512:
+        return 0
+    return 2 if pack._counts[0] * lanes >= 256 else 1
 
 
 def _packed_launch(so, pack, q, k, v, causal: bool, scale: float, backward: int, out=0, dout=None, o=0, dq=0, dk=0, dv=0, lse=0,
                    delta=0) -> None:
-    stream = L.raw_stream(q.device)
-    items, kv_items = pack._tiles(causal, stream)
+    stream, bf16 = L.raw_stream(q.device), q.dtype == torch.bfloat16
+    form, kv_form = packed_form(pack, q.shape[1], bf16), packed_form(pack, k.shape[1], bf16)
+    items, n = pack._items(form, 0 if causal else 2, stream)
+    kv_items, n_kv = pack._items(kv_form, 1 if causal else 2, stream)
+    # a uniform batch has no list in which short sequences are marked: its sequences are short, or none is
+    mark = lambda f: 1 if f == 2 and pack.longest > SOLO_ROWS else f          # noqa: E731
     qr, qh, _ = q.stride()
     kr, kh, _ = k.stride()
     vr, vh, _ = v.stride()
     dr, dh, _ = dout.stride() if dout is not None else (0, 0, 0)
     args = L.PACKED_ATTN_FORMAT.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out, dout.data_ptr() if dout is not None else 0, o, dq,
-                                     dk, dv, lse, delta, items, kv_items, qr, qh, kr, kh, vr, vh, dr, dh, pack.rows, pack._count,
+                                     dk, dv, lse, delta, items, kv_items, qr, qh, kr, kh, vr, vh, dr, dh, pack.rows, n, n_kv,
                                      pack.uniform_length, len(pack.lengths), q.shape[1], k.shape[1], q.shape[2], v.shape[2],
-                                     int(causal), scale, 0)
+                                     int(causal), mark(form), mark(kv_form), scale)
     with L.on(q.device):
-        L.check(so.mt_packed_attn_launch(args, backward, int(q.dtype == torch.bfloat16), FORM, stream), "mt_packed_attn_launch")
+        L.check(so.mt_packed_attn_launch(args, backward, int(bf16), stream), "mt_packed_attn_launch")
 
 
 def packed_forward(q, k, v, pack, causal: bool, scale: float, keeps: bool):

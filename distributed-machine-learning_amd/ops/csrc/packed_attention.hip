@@ -29,11 +29,13 @@ typedef __attribute__((address_space(3))) uint8_t lds_u8;
 
 #define PA_THREADS 256
 #define PA_OWN 128          // rows a workgroup owns (32 per wave)
+#define PA_TILE 32          // rows a workgroup of the split form owns, and rows of its tiles
 
-// One tile of PA_OWN owned rows: rows [row0, row0 + len) are its sequence, `first` is the tile's first row in it.
-// len < 0: -len rows from row0 belong to no sequence and are filled with zeros.
+// One item of owned rows: rows [row0, row0 + len) are its sequence, `first` is the item's first row in it.  An item is PA_OWN rows,
+// or in the split form PA_TILE rows unless it is `solo`.  len < 0: -len rows from row0 belong to no sequence and are filled with
+// zeros.
 struct MtSeqItem {
-  int32_t row0, len, first, pad;
+  int32_t row0, len, first, solo;
 };
 
 struct MtPackedAttn {
@@ -41,13 +43,13 @@ struct MtPackedAttn {
   const void *out, *dout;       // backward only: forward output (contiguous) and its gradient
   void *o, *dq, *dk, *dv;       // outputs, contiguous [T][heads or kv_heads][dk or dv]
   float *lse, *delta;           // [heads][rows]
-  const MtSeqItem *items, *kv_items;      // tiles of query rows and of key rows; null: count sequences of uniform_len rows each
+  const MtSeqItem *items, *kv_items;      // items of query rows and of key rows; null: count sequences of uniform_len rows each
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, do_row, do_head;
   int64_t rows;
-  int32_t n_items, uniform_len, count;
+  int32_t n_items, n_kv_items, uniform_len, count;
   int32_t heads, kv_heads, head_k, head_v, causal;
+  int32_t split, kv_split;      // the launch's form: 0 shared, 1 split, 2 split with every item solo (of a uniform batch)
   float scale;
-  int32_t pad;
 };
 
 // ---- per-type pieces ----------------------------------------------------------------------------------------------------
@@ -224,12 +226,12 @@ template <int N> __device__ __forceinline__ void pa_clear(f32x16 (&a)[N]) {
     for (int i = 0; i < 16; ++i) a[b][i] = 0.f;
 }
 
-// Which tile this workgroup takes.  Tiles come longest first (causal: the last queries, or the first keys).
-__device__ __forceinline__ MtSeqItem pa_item(const MtPackedAttn& p, const MtSeqItem* items, int i, bool last_first) {
+// Which item this workgroup takes.  Items come longest first (causal: the last queries, or the first keys).
+__device__ __forceinline__ MtSeqItem pa_item(const MtPackedAttn& p, const MtSeqItem* items, int i, int split, bool last_first) {
   if (items != nullptr) return items[i];
-  const int tiles = (p.uniform_len + PA_OWN - 1) / PA_OWN;
+  const int rows = split == 1 ? PA_TILE : PA_OWN, n = (p.uniform_len + rows - 1) / rows;
   const int t = i / p.count, seq = i - t * p.count;
-  return MtSeqItem{seq * p.uniform_len, p.uniform_len, (last_first ? tiles - 1 - t : t) * PA_OWN, 0};
+  return MtSeqItem{seq * p.uniform_len, p.uniform_len, (last_first ? n - 1 - t : t) * rows, split == 2};
 }
 // Zeros for `n` rows of `d` columns of one head, which belong to no sequence.
 template <typename T>
@@ -273,25 +275,28 @@ __device__ __forceinline__ void pa_join_store(T* base, int64_t row_stride, const
   }
 }
 // What the dq kernels hold of an owned row: q, do, L and D = do . o (stored for the dk / dv kernel by the waves with `store`).
-template <typename T, int D>
-__device__ __forceinline__ void pa_dq_rows(const MtPackedAttn& p, typename PaFrag<T>::type (&qf)[D / 16],
-                                           typename PaFrag<T>::type (&df)[D / 16], float& delta, float& lse, int64_t row, int head, bool ok,
+template <typename T, int DK, int DV>
+__device__ __forceinline__ void pa_dq_rows(const MtPackedAttn& p, typename PaFrag<T>::type (&qf)[DK / 16],
+                                           typename PaFrag<T>::type (&df)[DV / 16], float& delta, float& lse, int64_t row, int head, bool ok,
                                            bool store, int lane) {
-  pa_own_row<T, D>(df, reinterpret_cast<const T*>(p.dout) + row * p.do_row + (int64_t)head * p.do_head, ok, p.head_v, lane);
-  pa_own_row<T, D>(qf, reinterpret_cast<const T*>(p.out) + row * ((int64_t)p.heads * p.head_v) + (int64_t)head * p.head_v, ok, p.head_v,
-                   lane);
+  pa_own_row<T, DV>(df, reinterpret_cast<const T*>(p.dout) + row * p.do_row + (int64_t)head * p.do_head, ok, p.head_v, lane);
   delta = 0.f;
   lse = INFINITY;                                       // rows outside the sequence: p = 2^(s - inf) = 0
+  {
+    typename PaFrag<T>::type of[DV / 16];
+    pa_own_row<T, DV>(of, reinterpret_cast<const T*>(p.out) + row * ((int64_t)p.heads * p.head_v) + (int64_t)head * p.head_v, ok, p.head_v,
+                      lane);
 #pragma unroll
-  for (int s = 0; s < D / 16; ++s)
+    for (int s = 0; s < DV / 16; ++s)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) delta = __builtin_fmaf((float)df[s][j], (float)qf[s][j], delta);
+      for (int j = 0; j < 8; ++j) delta = __builtin_fmaf((float)df[s][j], (float)of[s][j], delta);
+  }
   delta = pa_half_sum(delta);
   if (ok) {
     lse = p.lse[(int64_t)head * p.rows + row];
     if (store && lane < 32) p.delta[(int64_t)head * p.rows + row] = delta;
   }
-  pa_own_row<T, D>(qf, reinterpret_cast<const T*>(p.q) + row * p.q_row + (int64_t)head * p.q_head, ok, p.head_k, lane);
+  pa_own_row<T, DK>(qf, reinterpret_cast<const T*>(p.q) + row * p.q_row + (int64_t)head * p.q_head, ok, p.head_k, lane);
 }
 
 // ---- forward ------------------------------------------------------------------------------------------------------------
@@ -305,7 +310,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void mt_pattn_fwd_kernel(const MtPac
   const int it = blockIdx.x / p.heads, r = blockIdx.x - it * p.heads;
   // heads of one group are kv_heads workgroups apart: the XCDs (workgroup number mod 8) then share few key / value heads each
   const int kvh = r % p.kv_heads, head = kvh * (p.heads / p.kv_heads) + r / p.kv_heads;
-  const MtSeqItem item = pa_item(p, p.items, it, p.causal);
+  const MtSeqItem item = pa_item(p, p.items, it, 0, p.causal);
   const int64_t o_row = (int64_t)p.heads * p.head_v;
   T* o = reinterpret_cast<T*>(p.o) + item.row0 * o_row + (int64_t)head * p.head_v;
   if (item.len <= 0) {
@@ -445,7 +450,7 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int it = blockIdx.x / p.heads, r = blockIdx.x - it * p.heads;
   const int kvh = r % p.kv_heads, head = kvh * (p.heads / p.kv_heads) + r / p.kv_heads;
-  const MtSeqItem item = pa_item(p, p.items, it, p.causal);
+  const MtSeqItem item = pa_item(p, p.items, it, 0, p.causal);
   const int64_t dq_row = (int64_t)p.heads * p.head_k;
   T* dq = reinterpret_cast<T*>(p.dq) + item.row0 * dq_row + (int64_t)head * p.head_k;
   if (item.len <= 0) {
@@ -456,7 +461,7 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
   const bool ok = mine < item.len;
   Frag qf[D / 16], df[D / 16];
   float delta, lse;
-  pa_dq_rows<T, D>(p, qf, df, delta, lse, item.row0 + (int64_t)mine, head, ok, true, lane);
+  pa_dq_rows<T, D, D>(p, qf, df, delta, lse, item.row0 + (int64_t)mine, head, ok, true, lane);
   const T* kb = reinterpret_cast<const T*>(p.k) + item.row0 * p.k_row + (int64_t)kvh * p.k_head;
   const T* vb = reinterpret_cast<const T*>(p.v) + item.row0 * p.v_row + (int64_t)kvh * p.v_head;
   const int keys = p.causal && item.first + PA_OWN < item.len ? item.first + PA_OWN : item.len;
@@ -556,7 +561,7 @@ __global__ __launch_bounds__(PA_DKV_THREADS, 2) void mt_pattn_dkv_kernel(const M
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int it = blockIdx.x / p.kv_heads, kvh = blockIdx.x - it * p.kv_heads;
   const int group = p.heads / p.kv_heads;
-  const MtSeqItem item = pa_item(p, p.kv_items, it, false);
+  const MtSeqItem item = pa_item(p, p.kv_items, it, 0, false);
   const int64_t dk_row = (int64_t)p.kv_heads * p.head_k, dv_row = (int64_t)p.kv_heads * p.head_v;
   T* dk = reinterpret_cast<T*>(p.dk) + item.row0 * dk_row + (int64_t)kvh * p.head_k;
   T* dv = reinterpret_cast<T*>(p.dv) + item.row0 * dv_row + (int64_t)kvh * p.head_v;
@@ -695,79 +700,82 @@ __global__ __launch_bounds__(PA_DKV_THREADS, 2) void mt_pattn_dkv_kernel(const M
 // A workgroup owns 32 rows and its four waves share the walk: wave w takes tiles w, w + 4, ... of 32 rows, in its own part of
 // LDS and without barriers, and the four partial results are joined through LDS in wave order.  Against the form above a tile
 // fetched feeds 32 owned rows instead of 128, and a quarter of the longest sequence's walk is the longest any wave has to go.
+// A `solo` item is 128 rows, 32 per wave, and every wave walks alone over all tiles: short sequences, whose walk split in four is
+// shorter than what a workgroup costs to begin and to join.
 // An image is single-buffered: it is refilled as soon as the last product that reads it has its fragments, and the other
-// image's products run meanwhile.
-#define PA_TILE 32
+// image's products run meanwhile.  Key and value widths have images and accumulators of their own size (DK, DV).
 template <int N> __device__ __forceinline__ void pa_wait_vm() {          // at most N of this wave's loads are still in flight
   static_assert(N >= 0 && N < 64, "vmcnt is a six-bit counter");
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void pa_reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
-
-// Which 32 owned rows: `lanes` heads or key / value heads side by side, then the quarters of a 128-row tile.
-struct PaSlot {
-  int it, lane_head, sub;
-};
-__device__ __forceinline__ PaSlot pa_slot(int block, int lanes) {
-  const int it = block / (4 * lanes), r = block - it * 4 * lanes;
-  return PaSlot{it, r % lanes, r / lanes};
-}
 // f32 steps are eight slow instructions: those behind the head's width are skipped.  bf16 steps are one, and stay in line.
 template <typename T> __device__ __forceinline__ bool pa_step(int column, int width) { return sizeof(T) == 2 || column < width; }
 
-template <typename T, int D>
-__global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) void mt_pattn_split_fwd_kernel(const MtPackedAttn p) {
-  typedef PaImg<T, D> Img;
+template <typename T, int DK, int DV> struct PaSplit {
+  typedef PaImg<T, DK> IK;
+  typedef PaImg<T, DV> IV;
+  static constexpr int KB = PA_TILE * IK::ROWB, VB = PA_TILE * IV::ROWB;           // image bytes
+  static constexpr int KP = KB / 1024, VP = VB / 1024;                             // LDS-DMA instructions of one
+  static constexpr int WIDE = DK > DV ? DK : DV;
+  static constexpr int lds(int joined) { return 4 * (KB + VB) < 512 * joined ? 512 * joined : 4 * (KB + VB); }
+  static constexpr int WAVES = sizeof(T) == 4 && WIDE == 128 ? 1 : 2;              // per SIMD
+};
+
+template <typename T, int DK, int DV>
+__global__ __launch_bounds__(PA_THREADS, (PaSplit<T, DK, DV>::WAVES)) void mt_pattn_split_fwd_kernel(const MtPackedAttn p) {
+  typedef PaSplit<T, DK, DV> S;
+  typedef typename S::IK IK;
+  typedef typename S::IV IV;
   typedef typename PaFrag<T>::type Frag;
-  constexpr int IMG = PA_TILE * Img::ROWB, PIECES = IMG / 1024;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[8 * IMG < 512 * D ? 512 * D : 8 * IMG];
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[S::lds(DV)];
   __shared__ float stat[2][4][32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const PaSlot slot = pa_slot(blockIdx.x, p.heads);
-  const int kvh = slot.lane_head % p.kv_heads, head = kvh * (p.heads / p.kv_heads) + slot.lane_head / p.kv_heads;
-  const MtSeqItem item = pa_item(p, p.items, slot.it, p.causal);
+  const int it = blockIdx.x / p.heads, r = blockIdx.x - it * p.heads;
+  const int kvh = r % p.kv_heads, head = kvh * (p.heads / p.kv_heads) + r / p.kv_heads;
+  const MtSeqItem item = pa_item(p, p.items, it, p.split, p.causal);
   const int64_t o_row = (int64_t)p.heads * p.head_v;
   T* o = reinterpret_cast<T*>(p.o) + item.row0 * o_row + (int64_t)head * p.head_v;
   if (item.len <= 0) {
-    if (slot.sub == 0) pa_zero_rows<T>(o, o_row, -item.len, p.head_v);
+    pa_zero_rows<T>(o, o_row, -item.len, p.head_v);
     return;
   }
-  const int first = item.first + slot.sub * 32, mine = first + (lane & 31);
-  if (first >= item.len) return;
-  Frag qf[D / 16];
-  pa_own_row<T, D>(qf, reinterpret_cast<const T*>(p.q) + (item.row0 + (int64_t)mine) * p.q_row + (int64_t)head * p.q_head,
-                   mine < item.len, p.head_k, lane);
+  const int first = item.first + (item.solo ? wave * 32 : 0), mine = first + (lane & 31);
+  if (item.solo && first >= item.len) return;
+  Frag qf[DK / 16];
+  pa_own_row<T, DK>(qf, reinterpret_cast<const T*>(p.q) + (item.row0 + (int64_t)mine) * p.q_row + (int64_t)head * p.q_head,
+                    mine < item.len, p.head_k, lane);
   const T* kb = reinterpret_cast<const T*>(p.k) + item.row0 * p.k_row + (int64_t)kvh * p.k_head;
   const T* vb = reinterpret_cast<const T*>(p.v) + item.row0 * p.v_row + (int64_t)kvh * p.v_head;
   const int keys = p.causal && first + 32 < item.len ? first + 32 : item.len;
-  const int tiles = (keys + PA_TILE - 1) / PA_TILE;
+  const int tiles = (keys + PA_TILE - 1) / PA_TILE, t0 = item.solo ? 0 : wave, hop = item.solo ? 1 : 4;
   const float c = p.scale * 1.4426950408889634f;
-  uint8_t* kimg = lds + wave * 2 * IMG;
-  uint8_t* vimg = kimg + IMG;
-  const uint32_t krow = pa_lds_at(kimg) + Img::row_base(lane), kcol = pa_lds_at(kimg) + Img::col_base(lane);
+  uint8_t* kimg = lds + wave * (S::KB + S::VB);
+  uint8_t* vimg = kimg + S::KB;
+  const uint32_t krow = pa_lds_at(kimg) + IK::row_base(lane), vcol = pa_lds_at(vimg) + IV::col_base(lane);
   auto load_k = [&](int t) {
-    Img::template stage<PA_TILE, 1>(kimg, kb + (int64_t)t * PA_TILE * p.k_row, p.k_row, item.len - t * PA_TILE, p.head_k, 0, lane);
+    IK::template stage<PA_TILE, 1>(kimg, kb + (int64_t)t * PA_TILE * p.k_row, p.k_row, item.len - t * PA_TILE, p.head_k, 0, lane);
   };
   auto load_v = [&](int t) {
-    Img::template stage<PA_TILE, 1>(vimg, vb + (int64_t)t * PA_TILE * p.v_row, p.v_row, item.len - t * PA_TILE, p.head_v, 0, lane);
+    IV::template stage<PA_TILE, 1>(vimg, vb + (int64_t)t * PA_TILE * p.v_row, p.v_row, item.len - t * PA_TILE, p.head_v, 0, lane);
   };
-  f32x16 acc[D / 32];
+  f32x16 acc[DV / 32];
   pa_clear(acc);
   float m = -INFINITY, sum = 0.f;
-  if (wave < tiles) {
-    load_k(wave);
-    load_v(wave);
+  if (t0 < tiles) {
+    load_k(t0);
+    load_v(t0);
   }
-  for (int t = wave; t < tiles; t += 4) {
-    const bool more = t + 4 < tiles;
-    pa_wait_vm<PIECES>();                      // K of this tile; its V may still be on the way
+  for (int t = t0; t < tiles; t += hop) {
+    const bool more = t + hop < tiles;
+    pa_wait_vm<S::VP>();                       // K of this tile; its V may still be on the way
     f32x16 s[1];
     pa_clear(s);
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks)
-      if (pa_step<T>(16 * ks, p.head_k)) s[0] = pa_mma(Img::rows(krow, 0, ks), qf[ks], s[0]);
+    for (int ks = 0; ks < DK / 16; ++ks)
+      if (pa_step<T>(16 * ks, p.head_k)) s[0] = pa_mma(IK::rows(krow, 0, ks), qf[ks], s[0]);
     pa_reads_done();
-    if (more) load_k(t + 4);
+    if (more) load_k(t + hop);
     const int k0 = t * PA_TILE;
     if (k0 + PA_TILE > item.len || (p.causal && k0 + PA_TILE - 1 > first)) {
       const int last = p.causal && mine < item.len ? mine : item.len - 1;
@@ -784,7 +792,7 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
       m = mn;
       sum *= f;
 #pragma unroll
-      for (int b = 0; b < D / 32; ++b)
+      for (int b = 0; b < DV / 32; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[b][i] *= f;
     }
@@ -794,19 +802,26 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
       s[0][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][i], c, -sub));
       sum += s[0][i];
     }
-    if (more) pa_wait_vm<PIECES>();            // V of this tile; the next K may still be on the way
+    if (more) pa_wait_vm<S::KP>();             // V of this tile; the next K may still be on the way
     else pa_wait_vm<0>();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const Frag pf = pa_pack<T>(s[0], h);
 #pragma unroll
-      for (int b = 0; b < D / 32; ++b)
-        if (pa_step<T>(32 * b, p.head_v)) acc[b] = pa_mma(Img::cols(kcol + IMG, 16 * h, b), pf, acc[b]);
+      for (int b = 0; b < DV / 32; ++b)
+        if (pa_step<T>(32 * b, p.head_v)) acc[b] = pa_mma(IV::cols(vcol, 16 * h, b), pf, acc[b]);
     }
     pa_reads_done();
-    if (more) load_v(t + 4);
+    if (more) load_v(t + hop);
   }
   sum = pa_half_sum(sum);
+  float* lse = p.lse != nullptr && mine < item.len && lane < 32 ? p.lse + (int64_t)head * p.rows + item.row0 + mine : nullptr;
+  if (item.solo) {
+    const bool real = sum > 0.f || sum != sum;
+    if (mine < item.len) pa_store_row<T, DV>(o + (int64_t)mine * o_row, acc, real ? 1.f / sum : 0.f, p.head_v, lane);
+    if (lse != nullptr) *lse = real ? m + __builtin_amdgcn_logf(sum) : INFINITY;
+    return;
+  }
   if (lane < 32) {
     stat[0][wave][lane] = m;
     stat[1][wave][lane] = sum;
@@ -821,73 +836,74 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
   for (int w = 0; w < 4; ++w) total += stat[1][w][q] * __builtin_amdgcn_exp2f(stat[0][w][q] - sub);
   const bool real = total > 0.f || total != total;
   const float f = __builtin_amdgcn_exp2f(m - sub) * (real ? 1.f / total : 0.f);
-  pa_join<D>(reinterpret_cast<float*>(lds), acc, f, wave, lane);
+  pa_join<DV>(reinterpret_cast<float*>(lds), acc, f, wave, lane);
   __syncthreads();
-  pa_join_store<T, D>(o + (int64_t)first * o_row, o_row, reinterpret_cast<const float*>(lds), item.len - first, p.head_v);
-  if (p.lse != nullptr && threadIdx.x < 32 && mine < item.len)
-    p.lse[(int64_t)head * p.rows + item.row0 + mine] = real ? sub + __builtin_amdgcn_logf(total) : INFINITY;
+  pa_join_store<T, DV>(o + (int64_t)first * o_row, o_row, reinterpret_cast<const float*>(lds), item.len - first, p.head_v);
+  if (wave == 0 && lse != nullptr) *lse = real ? sub + __builtin_amdgcn_logf(total) : INFINITY;
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) void mt_pattn_split_dq_kernel(const MtPackedAttn p) {
-  typedef PaImg<T, D> Img;
+template <typename T, int DK, int DV>
+__global__ __launch_bounds__(PA_THREADS, (PaSplit<T, DK, DV>::WAVES)) void mt_pattn_split_dq_kernel(const MtPackedAttn p) {
+  typedef PaSplit<T, DK, DV> S;
+  typedef typename S::IK IK;
+  typedef typename S::IV IV;
   typedef typename PaFrag<T>::type Frag;
-  constexpr int IMG = PA_TILE * Img::ROWB, PIECES = IMG / 1024;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[8 * IMG < 512 * D ? 512 * D : 8 * IMG];
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[S::lds(DK)];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const PaSlot slot = pa_slot(blockIdx.x, p.heads);
-  const int kvh = slot.lane_head % p.kv_heads, head = kvh * (p.heads / p.kv_heads) + slot.lane_head / p.kv_heads;
-  const MtSeqItem item = pa_item(p, p.items, slot.it, p.causal);
+  const int it = blockIdx.x / p.heads, r = blockIdx.x - it * p.heads;
+  const int kvh = r % p.kv_heads, head = kvh * (p.heads / p.kv_heads) + r / p.kv_heads;
+  const MtSeqItem item = pa_item(p, p.items, it, p.split, p.causal);
   const int64_t dq_row = (int64_t)p.heads * p.head_k;
   T* dq = reinterpret_cast<T*>(p.dq) + item.row0 * dq_row + (int64_t)head * p.head_k;
   if (item.len <= 0) {
-    if (slot.sub == 0) pa_zero_rows<T>(dq, dq_row, -item.len, p.head_k);
+    pa_zero_rows<T>(dq, dq_row, -item.len, p.head_k);
     return;
   }
-  const int first = item.first + slot.sub * 32, mine = first + (lane & 31);
-  if (first >= item.len) return;
-  Frag qf[D / 16], df[D / 16];
+  const int first = item.first + (item.solo ? wave * 32 : 0), mine = first + (lane & 31);
+  if (item.solo && first >= item.len) return;
+  Frag qf[DK / 16], df[DV / 16];
   float delta, lse;
-  pa_dq_rows<T, D>(p, qf, df, delta, lse, item.row0 + (int64_t)mine, head, mine < item.len, wave == 0, lane);
+  pa_dq_rows<T, DK, DV>(p, qf, df, delta, lse, item.row0 + (int64_t)mine, head, mine < item.len, item.solo || wave == 0, lane);
   const T* kb = reinterpret_cast<const T*>(p.k) + item.row0 * p.k_row + (int64_t)kvh * p.k_head;
   const T* vb = reinterpret_cast<const T*>(p.v) + item.row0 * p.v_row + (int64_t)kvh * p.v_head;
   const int keys = p.causal && first + 32 < item.len ? first + 32 : item.len;
-  const int tiles = (keys + PA_TILE - 1) / PA_TILE;
+  const int tiles = (keys + PA_TILE - 1) / PA_TILE, t0 = item.solo ? 0 : wave, hop = item.solo ? 1 : 4;
   const float c = p.scale * 1.4426950408889634f;
-  uint8_t* kimg = lds + wave * 2 * IMG;
-  uint8_t* vimg = kimg + IMG;
-  const uint32_t krow = pa_lds_at(kimg) + Img::row_base(lane), kcol = pa_lds_at(kimg) + Img::col_base(lane);
+  uint8_t* kimg = lds + wave * (S::KB + S::VB);
+  uint8_t* vimg = kimg + S::KB;
+  const uint32_t krow = pa_lds_at(kimg) + IK::row_base(lane), kcol = pa_lds_at(kimg) + IK::col_base(lane),
+                 vrow = pa_lds_at(vimg) + IV::row_base(lane);
   auto load_k = [&](int t) {
-    Img::template stage<PA_TILE, 1>(kimg, kb + (int64_t)t * PA_TILE * p.k_row, p.k_row, item.len - t * PA_TILE, p.head_k, 0, lane);
+    IK::template stage<PA_TILE, 1>(kimg, kb + (int64_t)t * PA_TILE * p.k_row, p.k_row, item.len - t * PA_TILE, p.head_k, 0, lane);
   };
   auto load_v = [&](int t) {
-    Img::template stage<PA_TILE, 1>(vimg, vb + (int64_t)t * PA_TILE * p.v_row, p.v_row, item.len - t * PA_TILE, p.head_v, 0, lane);
+    IV::template stage<PA_TILE, 1>(vimg, vb + (int64_t)t * PA_TILE * p.v_row, p.v_row, item.len - t * PA_TILE, p.head_v, 0, lane);
   };
-  f32x16 acc[D / 32];
+  f32x16 acc[DK / 32];
   pa_clear(acc);
-  if (wave < tiles) {
-    load_v(wave);
-    load_k(wave);
+  if (t0 < tiles) {
+    load_v(t0);
+    load_k(t0);
   }
-  for (int t = wave; t < tiles; t += 4) {
-    const bool more = t + 4 < tiles;
-    pa_wait_vm<PIECES>();                      // V; K may still be on the way
+  for (int t = t0; t < tiles; t += hop) {
+    const bool more = t + hop < tiles;
+    pa_wait_vm<S::KP>();                       // V; K may still be on the way
     f32x16 s[1], d[1];
     pa_clear(s);
     pa_clear(d);
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks)
-      if (pa_step<T>(16 * ks, p.head_v)) d[0] = pa_mma(Img::rows(krow + IMG, 0, ks), df[ks], d[0]);
+    for (int ks = 0; ks < DV / 16; ++ks)
+      if (pa_step<T>(16 * ks, p.head_v)) d[0] = pa_mma(IV::rows(vrow, 0, ks), df[ks], d[0]);
     pa_reads_done();
     if (more) {
-      load_v(t + 4);
-      pa_wait_vm<PIECES>();
+      load_v(t + hop);
+      pa_wait_vm<S::VP>();
     } else {
       pa_wait_vm<0>();
     }
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks)
-      if (pa_step<T>(16 * ks, p.head_k)) s[0] = pa_mma(Img::rows(krow, 0, ks), qf[ks], s[0]);
+    for (int ks = 0; ks < DK / 16; ++ks)
+      if (pa_step<T>(16 * ks, p.head_k)) s[0] = pa_mma(IK::rows(krow, 0, ks), qf[ks], s[0]);
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[0][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][i], c, -lse)) * (d[0][i] - delta);
     const int k0 = t * PA_TILE;
@@ -900,52 +916,56 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
     for (int h = 0; h < 2; ++h) {
       const Frag sf = pa_pack<T>(s[0], h);
 #pragma unroll
-      for (int b = 0; b < D / 32; ++b)
-        if (pa_step<T>(32 * b, p.head_k)) acc[b] = pa_mma(Img::cols(kcol, 16 * h, b), sf, acc[b]);
+      for (int b = 0; b < DK / 32; ++b)
+        if (pa_step<T>(32 * b, p.head_k)) acc[b] = pa_mma(IK::cols(kcol, 16 * h, b), sf, acc[b]);
     }
     pa_reads_done();
-    if (more) load_k(t + 4);
+    if (more) load_k(t + hop);
+  }
+  if (item.solo) {
+    if (mine < item.len) pa_store_row<T, DK>(dq + (int64_t)mine * dq_row, acc, p.scale, p.head_k, lane);
+    return;
   }
   __syncthreads();
-  pa_join<D>(reinterpret_cast<float*>(lds), acc, p.scale, wave, lane);
+  pa_join<DK>(reinterpret_cast<float*>(lds), acc, p.scale, wave, lane);
   __syncthreads();
-  pa_join_store<T, D>(dq + (int64_t)first * dq_row, dq_row, reinterpret_cast<const float*>(lds), item.len - first, p.head_k);
+  pa_join_store<T, DK>(dq + (int64_t)first * dq_row, dq_row, reinterpret_cast<const float*>(lds), item.len - first, p.head_k);
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(PA_THREADS, 1) void mt_pattn_split_dkv_kernel(const MtPackedAttn p) {
-  typedef PaImg<T, D> Img;
+template <typename T, int DK, int DV>
+__global__ __launch_bounds__(PA_THREADS, DK + DV > 96 ? 1 : 2) void mt_pattn_split_dkv_kernel(const MtPackedAttn p) {
+  typedef PaSplit<T, DK, DV> S;
+  typedef typename S::IK IK;
+  typedef typename S::IV IV;
   typedef typename PaFrag<T>::type Frag;
-  constexpr int IMG = PA_TILE * Img::ROWB, PIECES = IMG / 1024;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[8 * IMG < 512 * D ? 512 * D : 8 * IMG];
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[S::lds(S::WIDE)];
   __shared__ __attribute__((aligned(16))) float stat[4][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const PaSlot slot = pa_slot(blockIdx.x, p.kv_heads);
-  const int kvh = slot.lane_head, group = p.heads / p.kv_heads;
-  const MtSeqItem item = pa_item(p, p.kv_items, slot.it, false);
+  const int it = blockIdx.x / p.kv_heads, kvh = blockIdx.x - it * p.kv_heads, group = p.heads / p.kv_heads;
+  const MtSeqItem item = pa_item(p, p.kv_items, it, p.kv_split, false);
   const int64_t dk_row = (int64_t)p.kv_heads * p.head_k, dv_row = (int64_t)p.kv_heads * p.head_v;
   T* dk = reinterpret_cast<T*>(p.dk) + item.row0 * dk_row + (int64_t)kvh * p.head_k;
   T* dv = reinterpret_cast<T*>(p.dv) + item.row0 * dv_row + (int64_t)kvh * p.head_v;
   if (item.len <= 0) {
-    if (slot.sub == 0) {
-      pa_zero_rows<T>(dk, dk_row, -item.len, p.head_k);
-      pa_zero_rows<T>(dv, dv_row, -item.len, p.head_v);
-    }
+    pa_zero_rows<T>(dk, dk_row, -item.len, p.head_k);
+    pa_zero_rows<T>(dv, dv_row, -item.len, p.head_v);
     return;
   }
-  const int first = item.first + slot.sub * 32, mine = first + (lane & 31);
-  if (first >= item.len) return;
+  const int first = item.first + (item.solo ? wave * 32 : 0), mine = first + (lane & 31);
+  if (item.solo && first >= item.len) return;
   const bool ok = mine < item.len;
   const int64_t row = item.row0 + (int64_t)mine;
-  Frag kf[D / 16], vf[D / 16];
-  pa_own_row<T, D>(kf, reinterpret_cast<const T*>(p.k) + row * p.k_row + (int64_t)kvh * p.k_head, ok, p.head_k, lane);
-  pa_own_row<T, D>(vf, reinterpret_cast<const T*>(p.v) + row * p.v_row + (int64_t)kvh * p.v_head, ok, p.head_v, lane);
+  Frag kf[DK / 16], vf[DV / 16];
+  pa_own_row<T, DK>(kf, reinterpret_cast<const T*>(p.k) + row * p.k_row + (int64_t)kvh * p.k_head, ok, p.head_k, lane);
+  pa_own_row<T, DV>(vf, reinterpret_cast<const T*>(p.v) + row * p.v_row + (int64_t)kvh * p.v_head, ok, p.head_v, lane);
   const int q_lo = p.causal ? first / PA_TILE : 0;
   const int per_head = (item.len + PA_TILE - 1) / PA_TILE - q_lo, tiles = per_head * group;
+  const int t0 = item.solo ? 0 : wave, hop = item.solo ? 1 : 4;
   const float c = p.scale * 1.4426950408889634f;
-  uint8_t* qimg = lds + wave * 2 * IMG;
-  uint8_t* dimg = qimg + IMG;
-  const uint32_t qrow = pa_lds_at(qimg) + Img::row_base(lane), qcol = pa_lds_at(qimg) + Img::col_base(lane);
+  uint8_t* qimg = lds + wave * (S::KB + S::VB);
+  uint8_t* dimg = qimg + S::KB;
+  const uint32_t qrow = pa_lds_at(qimg) + IK::row_base(lane), qcol = pa_lds_at(qimg) + IK::col_base(lane);
+  const uint32_t drow = pa_lds_at(dimg) + IV::row_base(lane), dcol = pa_lds_at(dimg) + IV::col_base(lane);
   auto at = [&](int n, int& head, int& q0) {
     const int hg = n / per_head;
     head = kvh * group + hg;
@@ -954,44 +974,46 @@ __global__ __launch_bounds__(PA_THREADS, 1) void mt_pattn_split_dkv_kernel(const
   auto load_q = [&](int n) {
     int head, q0;
     at(n, head, q0);
-    Img::template stage<PA_TILE, 1>(qimg, reinterpret_cast<const T*>(p.q) + (item.row0 + (int64_t)q0) * p.q_row + (int64_t)head * p.q_head,
-                                    p.q_row, item.len - q0, p.head_k, 0, lane);
+    IK::template stage<PA_TILE, 1>(qimg, reinterpret_cast<const T*>(p.q) + (item.row0 + (int64_t)q0) * p.q_row + (int64_t)head * p.q_head,
+                                   p.q_row, item.len - q0, p.head_k, 0, lane);
   };
+  float ahead = 0.f;      // L (lanes 0-31) and D (32-63) of the rows of the tile that load_d fetched last
   auto load_d = [&](int n) {
     int head, q0;
     at(n, head, q0);
-    Img::template stage<PA_TILE, 1>(dimg, reinterpret_cast<const T*>(p.dout) + (item.row0 + (int64_t)q0) * p.do_row + (int64_t)head * p.do_head,
-                                    p.do_row, item.len - q0, p.head_v, 0, lane);
-  };
-  f32x16 ak[D / 32], av[D / 32];
-  pa_clear(ak);
-  pa_clear(av);
-  if (wave < tiles) {
-    load_d(wave);
-    load_q(wave);
-  }
-  for (int n = wave; n < tiles; n += 4) {
-    const bool more = n + 4 < tiles;
-    int head, q0;
-    at(n, head, q0);
-    // L and D of the tile's rows: lanes 0-31 fetch one, 32-63 the other, read back from LDS four at a time
     const int qi = q0 + (lane & 31);
     const float* src = lane < 32 ? p.lse : p.delta;
-    stat[wave][lane] = qi < item.len ? src[(int64_t)head * p.rows + item.row0 + qi] : 0.f;
-    pa_wait_vm<0>();
+    ahead = qi < item.len ? src[(int64_t)head * p.rows + item.row0 + qi] : 0.f;
+    IV::template stage<PA_TILE, 1>(dimg, reinterpret_cast<const T*>(p.dout) + (item.row0 + (int64_t)q0) * p.do_row + (int64_t)head * p.do_head,
+                                   p.do_row, item.len - q0, p.head_v, 0, lane);
+  };
+  f32x16 ak[DK / 32], av[DV / 32];
+  pa_clear(ak);
+  pa_clear(av);
+  if (t0 < tiles) {
+    load_d(t0);
+    load_q(t0);
+  }
+  for (int n = t0; n < tiles; n += hop) {
+    const bool more = n + hop < tiles;
+    int head, q0;
+    at(n, head, q0);
+    pa_wait_vm<S::KP>();                       // do, L and D; q may still be on the way
+    stat[wave][lane] = ahead;                  // read back four rows at a time
     f32x16 s[1], d[1];
     pa_clear(s);
     pa_clear(d);
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks)
-      if (pa_step<T>(16 * ks, p.head_v)) d[0] = pa_mma(Img::rows(qrow + IMG, 0, ks), vf[ks], d[0]);
+    for (int ks = 0; ks < DV / 16; ++ks)
+      if (pa_step<T>(16 * ks, p.head_v)) d[0] = pa_mma(IV::rows(drow, 0, ks), vf[ks], d[0]);
+    pa_wait_vm<0>();
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks)
-      if (pa_step<T>(16 * ks, p.head_k)) s[0] = pa_mma(Img::rows(qrow, 0, ks), kf[ks], s[0]);
+    for (int ks = 0; ks < DK / 16; ++ks)
+      if (pa_step<T>(16 * ks, p.head_k)) s[0] = pa_mma(IK::rows(qrow, 0, ks), kf[ks], s[0]);
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const int r = 8 * g + 4 * (lane >> 5);
-      const f32x4 lse = *reinterpret_cast<const f32x4*>(&stat[wave][r]), delta = *reinterpret_cast<const f32x4*>(&stat[wave][32 + r]);
+      const int rr = 8 * g + 4 * (lane >> 5);
+      const f32x4 lse = *reinterpret_cast<const f32x4*>(&stat[wave][rr]), delta = *reinterpret_cast<const f32x4*>(&stat[wave][32 + rr]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][4 * g + e], c, -lse[e]));
@@ -1012,86 +1034,103 @@ __global__ __launch_bounds__(PA_THREADS, 1) void mt_pattn_split_dkv_kernel(const
     for (int h = 0; h < 2; ++h) {
       const Frag pf = pa_pack<T>(s[0], h);
 #pragma unroll
-      for (int b = 0; b < D / 32; ++b)
-        if (pa_step<T>(32 * b, p.head_v)) av[b] = pa_mma(Img::cols(qcol + IMG, 16 * h, b), pf, av[b]);
+      for (int b = 0; b < DV / 32; ++b)
+        if (pa_step<T>(32 * b, p.head_v)) av[b] = pa_mma(IV::cols(dcol, 16 * h, b), pf, av[b]);
     }
     pa_reads_done();
-    if (more) load_d(n + 4);
+    if (more) load_d(n + hop);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const Frag sf = pa_pack<T>(d[0], h);
 #pragma unroll
-      for (int b = 0; b < D / 32; ++b)
-        if (pa_step<T>(32 * b, p.head_k)) ak[b] = pa_mma(Img::cols(qcol, 16 * h, b), sf, ak[b]);
+      for (int b = 0; b < DK / 32; ++b)
+        if (pa_step<T>(32 * b, p.head_k)) ak[b] = pa_mma(IK::cols(qcol, 16 * h, b), sf, ak[b]);
     }
     pa_reads_done();
-    if (more) load_q(n + 4);
+    if (more) load_q(n + hop);
+  }
+  if (item.solo) {
+    if (ok) {
+      pa_store_row<T, DK>(dk + (int64_t)mine * dk_row, ak, p.scale, p.head_k, lane);
+      pa_store_row<T, DV>(dv + (int64_t)mine * dv_row, av, 1.f, p.head_v, lane);
+    }
+    return;
   }
   float* join = reinterpret_cast<float*>(lds);
   __syncthreads();
-  pa_join<D>(join, ak, p.scale, wave, lane);
+  pa_join<DK>(join, ak, p.scale, wave, lane);
   __syncthreads();
-  pa_join_store<T, D>(dk + (int64_t)first * dk_row, dk_row, join, item.len - first, p.head_k);
+  pa_join_store<T, DK>(dk + (int64_t)first * dk_row, dk_row, join, item.len - first, p.head_k);
   __syncthreads();
-  pa_join<D>(join, av, 1.f, wave, lane);
+  pa_join<DV>(join, av, 1.f, wave, lane);
   __syncthreads();
-  pa_join_store<T, D>(dv + (int64_t)first * dv_row, dv_row, join, item.len - first, p.head_v);
+  pa_join_store<T, DV>(dv + (int64_t)first * dv_row, dv_row, join, item.len - first, p.head_v);
 }
 
 // ---- launchers ----------------------------------------------------------------------------------------------------------
-// bf16 launches of fewer workgroups than this (two per CU) take the split form, f32 ones always.  Measured, causal bf16, shared /
-// split: one sequence of 2048, 8 heads of 128 (128 workgroups) forward 54 / 28 us; 8192, 2 heads (128) 194 / 84, with its backward
-// pass 1085 / 337; 4 x 2048, 16 heads (1024) 120 / 134; documents of the benchmark, dk and dv (620) 265 / 480.
-#define PA_SPLIT_BELOW 512
-template <typename T, int D>
-static void pa_launch(const MtPackedAttn& p, int pass, int form, hipStream_t stream) {
-  const int blocks = p.n_items * (pass == 2 ? p.kv_heads : p.heads);
-  const bool split = sizeof(T) == 4 || (form < 0 ? blocks < PA_SPLIT_BELOW : form == 1);
-  const dim3 grid((unsigned)(blocks * (split ? 4 : 1))), block(PA_THREADS);
-  if (split) {
-    if (pass == 0) hipLaunchKernelGGL((mt_pattn_split_fwd_kernel<T, D>), grid, block, 0, stream, p);
-    else if (pass == 1) hipLaunchKernelGGL((mt_pattn_split_dq_kernel<T, D>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((mt_pattn_split_dkv_kernel<T, D>), grid, block, 0, stream, p);
-  } else if constexpr (sizeof(T) == 2) {
-    if (pass == 0) hipLaunchKernelGGL((mt_pattn_fwd_kernel<T, D, 64>), grid, block, 0, stream, p);
-    else if (pass == 1) hipLaunchKernelGGL((mt_pattn_dq_kernel<T, D, 64>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((mt_pattn_dkv_kernel<T, D>), grid, dim3(PA_DKV_THREADS), 0, stream, p);
-  }
+template <int D>
+static void pa_launch_shared(const MtPackedAttn& p, int pass, hipStream_t stream) {
+  const dim3 grid((unsigned)(pass == 2 ? p.n_kv_items * p.kv_heads : p.n_items * p.heads)), block(PA_THREADS);
+  if (pass == 0) hipLaunchKernelGGL((mt_pattn_fwd_kernel<__bf16, D, 64>), grid, block, 0, stream, p);
+  else if (pass == 1) hipLaunchKernelGGL((mt_pattn_dq_kernel<__bf16, D, 64>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((mt_pattn_dkv_kernel<__bf16, D>), grid, dim3(PA_DKV_THREADS), 0, stream, p);
 }
+template <typename T, int DK, int DV>
+static void pa_launch_split(const MtPackedAttn& p, int pass, hipStream_t stream) {
+  const dim3 grid((unsigned)(pass == 2 ? p.n_kv_items * p.kv_heads : p.n_items * p.heads)), block(PA_THREADS);
+  if (pass == 0) hipLaunchKernelGGL((mt_pattn_split_fwd_kernel<T, DK, DV>), grid, block, 0, stream, p);
+  else if (pass == 1) hipLaunchKernelGGL((mt_pattn_split_dq_kernel<T, DK, DV>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((mt_pattn_split_dkv_kernel<T, DK, DV>), grid, block, 0, stream, p);
+}
+// Widths: both at most 32, 64 or 128 elements, or keys of at most 32 beside values of at most 64 (key_dim_scaling 0.5), whose smaller
+// accumulators let two f32 waves of the dk / dv kernel share a SIMD.
 template <typename T>
-static void pa_launch_width(const MtPackedAttn& p, int pass, int form, hipStream_t stream) {
-  const int widest = p.head_k > p.head_v ? p.head_k : p.head_v;
-  if (widest <= 32) pa_launch<T, 32>(p, pass, form, stream);
-  else if (widest <= 64) pa_launch<T, 64>(p, pass, form, stream);
-  else pa_launch<T, 128>(p, pass, form, stream);
+static void pa_launch_split_width(const MtPackedAttn& p, int pass, hipStream_t stream) {
+  if (p.head_k <= 32 && p.head_v <= 32) pa_launch_split<T, 32, 32>(p, pass, stream);
+  else if (p.head_k <= 32 && p.head_v <= 64) pa_launch_split<T, 32, 64>(p, pass, stream);
+  else if (p.head_k <= 64 && p.head_v <= 64) pa_launch_split<T, 64, 64>(p, pass, stream);
+  else pa_launch_split<T, 128, 128>(p, pass, stream);
 }
 
-extern "C" int mt_packed_attn_sizes(int* item_bytes, int* tile_rows) {
+extern "C" int mt_packed_attn_sizes(int* item_bytes, int* own_rows, int* split_rows) {
   *item_bytes = (int)sizeof(MtSeqItem);
-  *tile_rows = PA_OWN;
+  *own_rows = PA_OWN;
+  *split_rows = PA_TILE;
   return (int)sizeof(MtPackedAttn);
 }
 
-// backward: 0 forward; 1 dq and D, then dk and dv.  bf16: 0 = f32 operands, 1 = bf16.  form: -1 by the launch's size; 0 / 1 the
-// bf16 kernels whose waves share a tile / a walk (tests).  Rows are read in 16-byte pieces.
-extern "C" int mt_packed_attn_launch(const MtPackedAttn* a, int backward, int bf16, int form, hipStream_t stream) {
+// backward: 0 forward; 1 dq and D, then dk and dv.  bf16: 0 = f32 operands (split form only), 1 = bf16.  Rows are read in 16-byte
+// pieces.
+extern "C" int mt_packed_attn_launch(const MtPackedAttn* a, int backward, int bf16, hipStream_t stream) {
   if (a == nullptr) return -2;
   const MtPackedAttn p = *a;
   if (p.n_items <= 0) return 0;
   const int es = bf16 ? 2 : 4, per = 16 / es;
   if (p.head_k < 1 || p.head_v < 1 || p.head_k > 128 || p.head_v > 128 || p.head_k % per || p.head_v % per) return -2;
-  if (p.heads < 1 || p.kv_heads < 1 || p.heads % p.kv_heads) return -2;
-  if ((p.items == nullptr || p.kv_items == nullptr) && (p.uniform_len < 1 || p.count < 1)) return -2;
-  if ((int64_t)p.n_items * p.heads * 4 > 0x7FFFFFFF || !(p.scale > 0.f)) return -2;
+  if (p.heads < 1 || p.kv_heads < 1 || p.heads % p.kv_heads || p.n_kv_items < 0) return -2;
+  if (p.split < 0 || p.split > 2 || p.kv_split < 0 || p.kv_split > 2 || (!bf16 && (p.split == 0 || p.kv_split == 0))) return -2;
+  if (p.items == nullptr || p.kv_items == nullptr) {      // a uniform batch: the numbers of items follow from its shape
+    if (p.uniform_len < 1 || p.count < 1 || p.items != p.kv_items) return -2;
+    for (int i = 0; i < 2; ++i) {
+      const int rows = (i ? p.kv_split : p.split) == 1 ? PA_TILE : PA_OWN;
+      if ((int64_t)((p.uniform_len - 1) / rows + 1) * p.count != (i ? p.n_kv_items : p.n_items)) return -2;
+    }
+  }
+  const int64_t most = p.n_items > p.n_kv_items ? p.n_items : p.n_kv_items;
+  if (most * p.heads > 0x7FFFFFFF || !(p.scale > 0.f)) return -2;
   const int64_t strides[8] = {p.q_row, p.q_head, p.k_row, p.k_head, p.v_row, p.v_head, p.do_row, p.do_head};
   for (int i = 0; i < 8; ++i)      // 32-bit byte offsets inside a staged tile of at most 128 rows
     if (strides[i] < 0 || strides[i] % per || strides[i] * es > (1 << 24)) return -2;
   const void* ptrs[9] = {p.q, p.k, p.v, p.out, p.dout, p.o, p.dq, p.dk, p.dv};
   for (int i = 0; i < 9; ++i)
     if (reinterpret_cast<uintptr_t>(ptrs[i]) & 15) return -2;
+  const int widest = p.head_k > p.head_v ? p.head_k : p.head_v;
   for (int pass = backward ? 1 : 0; pass <= (backward ? 2 : 0); ++pass) {
-    if (bf16) pa_launch_width<__bf16>(p, pass, form, stream);
-    else pa_launch_width<float>(p, pass, form, stream);
+    if (!bf16) pa_launch_split_width<float>(p, pass, stream);
+    else if (pass == 2 ? p.kv_split : p.split) pa_launch_split_width<__bf16>(p, pass, stream);
+    else if (widest <= 32) pa_launch_shared<32>(p, pass, stream);
+    else if (widest <= 64) pa_launch_shared<64>(p, pass, stream);
+    else pa_launch_shared<128>(p, pass, stream);
   }
   return (int)hipGetLastError();
 }

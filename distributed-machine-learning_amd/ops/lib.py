@@ -18,7 +18,7 @@ import numpy as np
 from . import build as _build
 
 MT_MAX_LAYERS = 8
-PACKED_TILE_ROWS, PACKED_ITEM_BYTES = 128, 16      # csrc/packed_attention.hip: rows of a tile, bytes of a tile list entry
+PACKED_OWN_ROWS, PACKED_SPLIT_ROWS, PACKED_ITEM_BYTES = 128, 32, 16      # csrc/packed_attention.hip: rows and bytes of an item
 
 c_void_p, c_int32, c_uint32, c_float, c_size_t = C.c_void_p, C.c_int32, C.c_uint32, C.c_float, C.c_size_t
 
@@ -61,13 +61,13 @@ class PackedAttn(C.Structure):
                 ("lse", c_void_p), ("delta", c_void_p), ("items", c_void_p), ("kv_items", c_void_p),
                 ("q_row", C.c_int64), ("q_head", C.c_int64), ("k_row", C.c_int64), ("k_head", C.c_int64),
                 ("v_row", C.c_int64), ("v_head", C.c_int64), ("do_row", C.c_int64), ("do_head", C.c_int64),
-                ("rows", C.c_int64), ("n_items", c_int32), ("uniform_len", c_int32), ("count", c_int32),
+                ("rows", C.c_int64), ("n_items", c_int32), ("n_kv_items", c_int32), ("uniform_len", c_int32), ("count", c_int32),
                 ("heads", c_int32), ("kv_heads", c_int32), ("head_k", c_int32), ("head_v", c_int32),
-                ("causal", c_int32), ("scale", c_float), ("pad", c_int32)]
+                ("causal", c_int32), ("split", c_int32), ("kv_split", c_int32), ("scale", c_float)]
 
 
 # The same layout for struct.pack: filling a ctypes structure field by field costs several microseconds of every call.
-PACKED_ATTN_FORMAT = struct.Struct("<13Q9q8ifi")
+PACKED_ATTN_FORMAT = struct.Struct("<13Q9q11if")
 
 
 class MlpPlan(C.Structure):
@@ -229,12 +229,12 @@ def load(build_if_missing: bool = True) -> C.CDLL:
     lib.mt_attn_fwd_strided_launch.restype = lib.mt_attn_bwd_strided_launch.restype = C.c_int
     lib.mt_attn_exact_level.argtypes = [C.c_int]
     lib.mt_attn_exact_level.restype = C.c_int
-    item_bytes, tile_rows = C.c_int(), C.c_int()
-    if lib.mt_packed_attn_sizes(C.byref(item_bytes), C.byref(tile_rows)) != C.sizeof(PackedAttn):
+    item_bytes, own_rows, split_rows = C.c_int(), C.c_int(), C.c_int()
+    if lib.mt_packed_attn_sizes(C.byref(item_bytes), C.byref(own_rows), C.byref(split_rows)) != C.sizeof(PackedAttn):
         raise KernelLibraryError("MtPackedAttn layout mismatch between lib.py and the library")
     if PACKED_ATTN_FORMAT.size != C.sizeof(PackedAttn):
         raise KernelLibraryError("MtPackedAttn layout mismatch between the struct format and lib.py")
-    if (item_bytes.value, tile_rows.value) != (PACKED_ITEM_BYTES, PACKED_TILE_ROWS):
+    if (item_bytes.value, own_rows.value, split_rows.value) != (PACKED_ITEM_BYTES, PACKED_OWN_ROWS, PACKED_SPLIT_ROWS):
         raise KernelLibraryError("packed attention: tile list layout mismatch between lib.py and the library")
     lib.mt_linear_parts.argtypes = [C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int]
     lib.mt_linear_gemm_launch.argtypes = ([C.c_int] + [c_void_p] * 7 + [C.c_int64, C.c_int, C.c_int, C.c_int64, C.c_int64]
@@ -249,7 +249,7 @@ def load(build_if_missing: bool = True) -> C.CDLL:
     lib.mt_norm_fwd_launch.argtypes = [c_void_p] * 5 + [C.c_int64, C.c_int64, C.c_int, c_float, C.c_int, C.c_int, c_void_p]
     lib.mt_norm_bwd_launch.argtypes = [c_void_p] * 8 + [C.c_int64] * 3 + [C.c_int] * 3 + [c_void_p]
     lib.mt_norm_bwd_parts.restype = lib.mt_norm_fwd_launch.restype = lib.mt_norm_bwd_launch.restype = C.c_int
-    lib.mt_packed_attn_launch.argtypes = [C.c_char_p, C.c_int, C.c_int, C.c_int, c_void_p]
+    lib.mt_packed_attn_launch.argtypes = [C.c_char_p, C.c_int, C.c_int, c_void_p]
     lib.mt_packed_attn_launch.restype = C.c_int
     lib.mt_ln_fwd_launch.argtypes = [c_void_p] * 8 + [C.c_int, C.c_int, c_float, c_float, c_void_p, c_float, c_void_p]
     lib.mt_ln_bwd_launch.argtypes = [c_void_p] * 8 + [C.c_int, C.c_int, c_float, c_void_p, c_float, c_void_p]

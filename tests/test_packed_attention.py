@@ -106,21 +106,27 @@ def test_forward_and_gradients(dtype, causal, lengths, heads, kv_heads, dk, dv):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("form", [0, 1])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("form", [0, 1, 2])
 @pytest.mark.parametrize("causal", [False, True])
-@pytest.mark.parametrize("heads,kv_heads,dk,dv", [(2, 2, 64, 64), (4, 2, 32, 32), (3, 1, 128, 128), (2, 1, 20, 36)])
-def test_both_bf16_forms(monkeypatch, form, causal, heads, kv_heads, dk, dv):
-    """The form whose waves share a tile and the one whose waves share a walk, whatever the launch's size would pick."""
+@pytest.mark.parametrize("heads,kv_heads,dk,dv", [(2, 2, 64, 64), (4, 2, 32, 32), (3, 1, 128, 128), (2, 1, 20, 36), (2, 2, 32, 64)])
+def test_every_form(monkeypatch, dtype, form, causal, heads, kv_heads, dk, dv):
+    """Waves that share a tile, that share a walk, and that walk alone over short sequences, whatever the launch's size would pick."""
     from mitune.ops import attention_hip
     from mitune.ops.attention import SequencePack
     monkeypatch.setattr(attention_hip, "FORM", form)
     lengths = [129, 5, 0, 300, 64, 33]
     rows = sum(lengths) + 150
-    q, k, v, do = _inputs(lengths, rows, heads, kv_heads, dk, dv, torch.bfloat16)
+    q, k, v, do = _inputs(lengths, rows, heads, kv_heads, dk, dv, dtype)
     got = _grads(q, k, v, SequencePack(lengths, rows=rows), do, causal)
-    _check(got, *_plain(q, k, v, lengths, causal, dk ** -0.5, do, True))
+    _check(got, *_plain(q, k, v, lengths, causal, dk ** -0.5, do, dtype == torch.bfloat16))
     for t in got:
         assert not t[sum(lengths):].any()
+    for n in (90, 300):                                # uniform batches have no list
+        q, k, v, do = _inputs([n] * 3, 3 * n, heads, kv_heads, dk, dv, dtype)
+        want = _grads(q, k, v, SequencePack([n] * 3), do, causal)
+        for a, b in zip(_grads(q, k, v, SequencePack.uniform(3, n), do, causal), want):
+            assert torch.equal(a, b)
 
 
 @pytest.mark.gpu
@@ -369,17 +375,23 @@ def test_tile_lists_cover_every_row_once():
             pass                                   # the upload has no device to go to
     finally:
         torch.from_numpy = real
-    lists = kept[0].reshape(3, -1, 4)
-    for order, work in zip(lists, (lambda r: min(r[2] + 128, r[1]), lambda r: r[1] - r[2], lambda r: r[1])):
-        seen = np.zeros(700, dtype=int)
-        last = None
-        for r in order.tolist():
-            if r[1] < 0:
-                seen[r[0]:r[0] - r[1]] += 1
-                assert r[0] >= 530
-                continue
-            lo, hi = r[0] + r[2], r[0] + min(r[1], r[2] + 128)
-            seen[lo:hi] += 1
-            assert last is None or work(r) <= last
-            last = work(r)
-        assert (seen == 1).all()
+    at = 0
+    for which, count in enumerate(pack._counts):
+        for work in (lambda r, g: min(r[2] + g, r[1]), lambda r, g: r[1] - r[2], lambda r, g: r[1]):
+            seen = np.zeros(700, dtype=int)
+            last = None
+            for r in kept[0][at:at + count].tolist():
+                if r[1] < 0:
+                    seen[r[0]:r[0] - r[1]] += 1
+                    assert r[0] >= 530
+                    continue
+                grain = 128 if which == 0 or r[3] else 32
+                assert r[3] == (which == 2 and r[1] <= A.SOLO_ROWS)
+                lo, hi = r[0] + r[2], r[0] + min(r[1], r[2] + grain)
+                seen[lo:hi] += 1
+                cost = work(r, grain) / (1 if which == 0 or r[3] else 4)
+                assert last is None or cost <= last
+                last = cost
+            assert (seen == 1).all()
+            at += count
+    assert at == len(kept[0])
