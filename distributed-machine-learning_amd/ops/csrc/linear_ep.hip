@@ -271,11 +271,12 @@ static void linear_few(const void* x, const void* w, const MtLinearEp& ep, void*
 }
 #define LINEAR_FEW_ROWS 32
 
-// Tile edge of an f32 launch, and how many parts the contraction of a launch is split into: launches of at most half as many tiles
+// Tile edge of an f32 launch: 128 from four 128-tiles per CU on (4096^3: 1030 us against 1110 with 64; 12800 x 2048 x 512: 276 / 286),
+// 64 below, where fewer, longer tiles leave CUs idle at the end (25600 x 512 x 512: 130 us against 151).  And how many parts the contraction of a launch is split into: launches of at most half as many tiles
 // as the chip has CUs, whose contraction is long enough to leave every part 512 deep.
 static int linear_edge(int64_t M, int N, int bf16) {
   if (bf16) return 128;
-  return ((M + 127) / 128) * ((N + 127) / 128) >= 512 ? 128 : 64;
+  return ((M + 127) / 128) * ((N + 127) / 128) >= 1024 ? 128 : 64;
 }
 static int linear_splits(int mode, int64_t M, int N, int KK, int bf16, int* per) {
   const int edge = linear_edge(M, N, bf16), step = bf16 ? BK : F32_BK;

@@ -460,6 +460,12 @@ def _small_grads(so, dz, xc, wc, want_dx: bool, want_db: bool, stream):
     return dx, dw, db
 
 
+def _fused_wgrad_splits(M: int, tiles: int, bf16: bool) -> int:
+    """Row splits of a fused layer's weight gradient.  f32: four workgroups per CU (12800 x 512 x 2048 with its 256 tiles: 313 us in
+    2 splits, 256 in 4; 25600 x 512 x 512 with 64: 153 us in 8, 129 in 16); bf16: ``OPTIONS.wgrad_workgroups``."""
+    return _wgrad_splits(M, tiles, 64) if bf16 else max(1, min(127, (M + 127) // 128, 1024 // tiles))
+
+
 def _weight_grad(so, dz, xc, out_f: int, in_f: int, w_dtype, b_dtype, stream):
     """(dW [out_f, in_f], db [out_f] or None).  A layer with enough tiles stores them as they leave the matrix instruction; a
     smaller one is split over the rows, the slabs added in order and rounded once."""
@@ -471,7 +477,7 @@ def _weight_grad(so, dz, xc, out_f: int, in_f: int, w_dtype, b_dtype, stream):
     most = 255 * tile                               # output rows of a launch: its tile rows are 8 bits
     dw = torch.empty(out_f, in_f, device=dz.device, dtype=w_dtype)
     db = torch.empty(out_f, device=dz.device, dtype=b_dtype) if b_dtype is not None else None
-    if w_dtype == dz.dtype and _wgrad_splits(M, -(-min(rows, most) // tile) * -(-width // tile), 64 if bf16 else 128) == 1:
+    if w_dtype == dz.dtype and _fused_wgrad_splits(M, -(-min(rows, most) // tile) * -(-width // tile), bf16) == 1:
         L.check(so.mt_linear_wgrad_launch(dz.data_ptr(), xc.data_ptr(), dw.data_ptr(), db.data_ptr() if db is not None else None, M,
                                           out_f, in_f, rows, width, int(b_dtype == torch.bfloat16), int(bf16), stream),
                 "mt_linear_wgrad_launch")
@@ -483,7 +489,7 @@ def _weight_grad(so, dz, xc, out_f: int, in_f: int, w_dtype, b_dtype, stream):
     for i, part in enumerate(parts):
         n = part.shape[1]
         real = min(n, out_f - i * most)
-        splits = _wgrad_splits(M, -(-n // tile) * -(-width // tile), 64 if bf16 else 128)
+        splits = _fused_wgrad_splits(M, -(-n // tile) * -(-width // tile), bf16)
         slab = (n * width + n + 63) // 64 * 64
         arena = torch.empty(splits, slab, device=dz.device, dtype=torch.float32)
         if bf16:
