@@ -192,35 +192,74 @@ __global__ __launch_bounds__(WAVES * 64) void mt_linear_few_kernel(const T* __re
   }
 }
 
-// dz = dy act'(s): s is z, or (ReLU without a residual) y, whose sign is z's.  A thread takes one 16-byte piece of a dz row.
+// dz = dy act'(s): s is z, or (ReLU without a residual) y, whose sign is z's; and the column sums of dz before it is rounded, from
+// which db comes (sums of rounded terms would be off by half again as much).  `lanes` threads (a power of two) take the 16-byte
+// pieces of a row side by side, 256 / lanes rows at a time; a workgroup walks over the rows of its chunk and leaves one partial row.
 template <typename T>
 __global__ __launch_bounds__(256) void mt_act_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ s, T* __restrict__ dz,
-                                                         int64_t rows, int n, int64_t ld_dy, int ld_dz, int act) {
+                                                         float* __restrict__ part, int64_t rows, int n, int64_t ld_dy, int ld_dz,
+                                                         int act, int lanes, int per) {
   constexpr int V = 16 / (int)sizeof(T);
-  const int pieces = ld_dz / V;
-  const int64_t total = rows * pieces;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / pieces;
-    const int col = (int)(i - row * pieces) * V;
-    T a[V], b[V], o[V];
-    const T *pa = dy + row * ld_dy + col, *pb = s + row * n + col;
-    if (col + V <= n) {
-      __builtin_memcpy(a, pa, 16);
-      __builtin_memcpy(b, pb, 16);
-    } else {
+  __shared__ float red[256 * V];
+  const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = 256 / lanes;
+  const int col = (blockIdx.x * lanes + lane) * V;
+  const int64_t lo = (int64_t)blockIdx.y * per, hi = lo + per < rows ? lo + per : rows;
+  float sum[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) sum[e] = 0.f;
+  if (col < ld_dz) {
+#pragma unroll 4
+    for (int64_t row = lo + group; row < hi; row += groups) {
+      T a[V], b[V], o[V];
+      const T *pa = dy + row * ld_dy + col, *pb = s + row * n + col;
+      if (col + V <= n) {
+        __builtin_memcpy(a, pa, 16);
+        __builtin_memcpy(b, pb, 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          a[e] = col + e < n ? pa[e] : (T)0.f;
+          b[e] = col + e < n ? pb[e] : (T)0.f;
+        }
+      }
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        a[e] = col + e < n ? pa[e] : (T)0.f;
-        b[e] = col + e < n ? pb[e] : (T)0.f;
+        const float g = (float)a[e], z = (float)b[e];
+        // ReLU passes the gradient on where the output is not a number, as it passes the output on
+        const float v = act == MT_ACT_RELU ? (z > 0.f || z != z ? g : 0.f) : g * mt_ep_slope<sizeof(T) == 2>(z, act);
+        sum[e] += v;
+        o[e] = (T)v;
       }
+      __builtin_memcpy(dz + row * ld_dz + col, o, 16);
     }
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float slope = mt_ep_slope<sizeof(T) == 2>((float)b[e], act);
-      o[e] = act == MT_ACT_RELU ? (slope != 0.f || (float)b[e] != (float)b[e] ? a[e] : (T)0.f) : (T)((float)a[e] * slope);
-    }
-    __builtin_memcpy(dz + row * ld_dz + col, o, 16);
   }
+  if (part == nullptr) return;
+#pragma unroll
+  for (int e = 0; e < V; ++e) red[threadIdx.x * V + e] = sum[e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < lanes * V; i += 256) {
+    const int c = blockIdx.x * lanes * V + i;
+    if (c >= n) break;
+    float v = 0.f;
+    for (int g = 0; g < groups; ++g) v += red[g * lanes * V + i];
+    part[(int64_t)blockIdx.y * n + c] = v;
+  }
+}
+// db = the partial rows added in order: 16 columns x 16 strands per workgroup, the strands added in order through LDS.
+template <typename B>
+__global__ __launch_bounds__(256) void mt_act_cols_kernel(const float* __restrict__ part, B* __restrict__ db, int chunks, int n) {
+  __shared__ float strands[16][17];
+  const int cl = threadIdx.x & 15, st = threadIdx.x >> 4, c = blockIdx.x * 16 + cl;
+  float v = 0.f;
+  if (c < n)
+    for (int i = st; i < chunks; i += 16) v += part[(int64_t)i * n + c];
+  strands[st][cl] = v;
+  __syncthreads();
+  if (st != 0 || c >= n) return;
+  v = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v += strands[i][cl];
+  db[c] = (B)v;
 }
 
 // dW [rows][cols] and db [rows]: the f32 slabs of the split contraction added in order and rounded to the parameters' types.
@@ -386,20 +425,51 @@ extern "C" int mt_linear_wgrad_launch(const void* dz, const void* x, void* dw, v
   return (int)hipGetLastError();
 }
 
-// s: z or y [M][N] contiguous; dz [M][ld_dz], ld_dz a multiple of a 16-byte piece, zeros behind column N.
-extern "C" int mt_linear_act_bwd_launch(const void* dy, const void* s, void* dz, int64_t M, int N, int64_t ld_dy, int ld_dz, int act,
-                                        int bf16, hipStream_t stream) {
+struct ActGrid {
+  int lanes, strips, chunks, per;
+};
+static ActGrid act_grid(int64_t M, int ld_dz, int bf16) {
+  const int pieces = ld_dz / (bf16 ? 8 : 4);
+  ActGrid g;
+  g.lanes = 4;
+  while (g.lanes < 64 && g.lanes < pieces) g.lanes *= 2;
+  g.strips = (pieces + g.lanes - 1) / g.lanes;
+  int64_t chunks = (2048 + g.strips - 1) / g.strips;                     // about eight workgroups per CU ...
+  const int64_t deep = M / (16 * (256 / g.lanes));                       // ... that walk over sixteen groups of rows or more
+  if (chunks > deep) chunks = deep;
+  if (chunks < 1) chunks = 1;
+  if (chunks < M / (1 << 24)) chunks = M / (1 << 24) + 1;
+  g.per = (int)((M + chunks - 1) / chunks);
+  g.chunks = (int)((M + g.per - 1) / g.per);
+  return g;
+}
+// Rows of the partial-sum workspace [n][N] f32.
+extern "C" int mt_linear_act_parts(int64_t M, int ld_dz, int bf16) {
+  if (M < 1 || ld_dz < 1 || ld_dz % (bf16 ? 8 : 4)) return -2;
+  return act_grid(M, ld_dz, bf16).chunks;
+}
+// s: z or y [M][N] contiguous; dz [M][ld_dz], ld_dz a multiple of a 16-byte piece, zeros behind column N.  db [N] with its workspace
+// `part`, or both null.
+extern "C" int mt_linear_act_bwd_launch(const void* dy, const void* s, void* dz, float* part, void* db, int64_t M, int N, int64_t ld_dy,
+                                        int ld_dz, int act, int db_bf16, int bf16, hipStream_t stream) {
   const int per = bf16 ? 8 : 4;
-  if (M < 0 || N < 1 || ld_dz % per || ld_dz < N || ld_dy < 0 || act < 1 || act > 2) return -2;
+  if (M < 0 || N < 1 || ld_dz % per || ld_dz < N || ld_dz - N >= per || ld_dy < 0 || act < 1 || act > 2) return -2;
+  if ((part == nullptr) != (db == nullptr)) return -2;
   if (M == 0) return 0;
-  const int64_t blocks = (M * (ld_dz / per) + 255) / 256;
-  const dim3 grid((unsigned)(blocks < 16384 ? blocks : 16384));
+  const ActGrid g = act_grid(M, ld_dz, bf16);
+  if (g.chunks > 65535) return -2;
+  const dim3 grid((unsigned)g.strips, (unsigned)g.chunks);
   if (bf16)
-    hipLaunchKernelGGL(mt_act_bwd_kernel<__bf16>, grid, dim3(256), 0, stream, (const __bf16*)dy, (const __bf16*)s, (__bf16*)dz, M, N,
-                       ld_dy, ld_dz, act);
+    hipLaunchKernelGGL(mt_act_bwd_kernel<__bf16>, grid, dim3(256), 0, stream, (const __bf16*)dy, (const __bf16*)s, (__bf16*)dz, part, M,
+                       N, ld_dy, ld_dz, act, g.lanes, g.per);
   else
-    hipLaunchKernelGGL(mt_act_bwd_kernel<float>, grid, dim3(256), 0, stream, (const float*)dy, (const float*)s, (float*)dz, M, N,
-                       ld_dy, ld_dz, act);
+    hipLaunchKernelGGL(mt_act_bwd_kernel<float>, grid, dim3(256), 0, stream, (const float*)dy, (const float*)s, (float*)dz, part, M, N,
+                       ld_dy, ld_dz, act, g.lanes, g.per);
+  if (db != nullptr) {
+    const dim3 cols((unsigned)((N + 15) / 16));
+    if (db_bf16) hipLaunchKernelGGL(mt_act_cols_kernel<__bf16>, cols, dim3(256), 0, stream, part, (__bf16*)db, g.chunks, N);
+    else hipLaunchKernelGGL(mt_act_cols_kernel<float>, cols, dim3(256), 0, stream, part, (float*)db, g.chunks, N);
+  }
   return (int)hipGetLastError();
 }
 

@@ -423,22 +423,31 @@ class FusedLinear(torch.autograd.Function):
                 if act:
                     g = g if g.stride(1) == 1 else g.contiguous()
                     dz = torch.empty(M, out_f + -out_f % per, device=dev, dtype=xc.dtype)
-                    L.check(so.mt_linear_act_bwd_launch(g.data_ptr(), s.data_ptr(), dz.data_ptr(), M, out_f, g.stride(0),
-                                                        dz.shape[1], act, int(bf16), stream), "mt_linear_act_bwd_launch")
+                    part = None
+                    if b_dtype is not None and ctx.needs_input_grad[2]:
+                        db = torch.empty(out_f, device=dev, dtype=b_dtype)
+                        part = torch.empty(so.mt_linear_act_parts(M, dz.shape[1], int(bf16)), out_f, device=dev, dtype=torch.float32)
+                    L.check(so.mt_linear_act_bwd_launch(g.data_ptr(), s.data_ptr(), dz.data_ptr(),
+                                                        part.data_ptr() if part is not None else None,
+                                                        db.data_ptr() if part is not None else None, M, out_f, g.stride(0),
+                                                        dz.shape[1], act, int(b_dtype == torch.bfloat16), int(bf16), stream),
+                            "mt_linear_act_bwd_launch")
+                    b_dtype = None                      # done; the launches below need not sum dz again
                 else:
                     dz = _pieces(g)
                     dz = dz if dz.stride(0) == dz.shape[1] else dz.contiguous()
                 if not bf16 and _small(M, xc.shape[1], dz.shape[1], True):
-                    dx, dw, db = _small_grads(so, dz, xc, wc, ctx.needs_input_grad[0], b_dtype is not None, stream)
+                    dx, dw, sums = _small_grads(so, dz, xc, wc, ctx.needs_input_grad[0], b_dtype is not None, stream)
                     dx = dx[:, :in_f].reshape(x_shape) if dx is not None else None
-                    return (dx, dw[:out_f, :in_f], db[:out_f] if db is not None else None,
-                            dy if r_shape is not None else None, None, None)
+                    return (dx, dw[:out_f, :in_f], sums[:out_f] if sums is not None else db, dy if r_shape is not None else None,
+                            None, None)
                 if ctx.needs_input_grad[0]:
                     dx = torch.empty(M, in_f, device=dev, dtype=xc.dtype)
                     _fused_gemm(so, 1, dz, wc, dx, out_f)
                     dx = dx.view(x_shape)
-                if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-                    dw, db = _weight_grad(so, dz, xc, out_f, in_f, w_dtype, b_dtype, stream)
+                if ctx.needs_input_grad[1] or (b_dtype is not None and ctx.needs_input_grad[2]):
+                    dw, sums = _weight_grad(so, dz, xc, out_f, in_f, w_dtype, b_dtype, stream)
+                    db = db if sums is None else sums
         return dx, dw, db, (dy if r_shape is not None else None), None, None
 
 
