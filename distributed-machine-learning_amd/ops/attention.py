@@ -163,6 +163,7 @@ class SequencePack:
         self._fix(total, total if rows is None else rows, device)
         self.lengths = n.astype(np.int64)
         self.longest = int(self.lengths.max(initial=0))
+        self.shortest = int(self.lengths.min(initial=1 << 31, where=self.lengths > 0))
         self.uniform_length = 0
         self._lay_out()
 
@@ -173,7 +174,7 @@ class SequencePack:
         self = cls.__new__(cls)
         self._fix(int(count) * int(length), int(count) * int(length), device)
         self.lengths = np.full(int(count), int(length), dtype=np.int64)
-        self.longest = int(length) if count else 0
+        self.longest = self.shortest = int(length) if count else 0
         self.uniform_length = int(length) if count else 0
         own, fine = (-(-int(length) // r) * int(count) for r in (PACKED_OWN_ROWS, PACKED_SPLIT_ROWS))
         self._counts, self._lists, self._stream = (own, fine, own if length <= SOLO_ROWS else fine), None, 0

@@ -192,8 +192,8 @@ def packed_form(pack, lanes: int, bf16: bool) -> int:
     return 2 if pack._counts[0] * lanes >= 256 else 1
 
 
-def _packed_launch(so, pack, q, k, v, causal: bool, scale: float, backward: int, out=0, dout=None, o=0, dq=0, dk=0, dv=0, lse=0,
-                   delta=0) -> None:
+def _packed_launch(so, pack, q, k, v, causal: bool, scale: float, backward: int, out=0, dout=None, o=0, dq=0, dk=0, dv=0, low=0,
+                   lse=0, delta=0) -> None:
     stream, bf16 = L.raw_stream(q.device), q.dtype == torch.bfloat16
     form, kv_form = packed_form(pack, q.shape[1], bf16), packed_form(pack, k.shape[1], bf16)
     items, n = pack._items(form, 0 if causal else 2, stream)
@@ -205,7 +205,7 @@ def _packed_launch(so, pack, q, k, v, causal: bool, scale: float, backward: int,
     vr, vh, _ = v.stride()
     dr, dh, _ = dout.stride() if dout is not None else (0, 0, 0)
     args = L.PACKED_ATTN_FORMAT.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out, dout.data_ptr() if dout is not None else 0, o, dq,
-                                     dk, dv, lse, delta, items, kv_items, qr, qh, kr, kh, vr, vh, dr, dh, pack.rows, n, n_kv,
+                                     dk, dv, low, lse, delta, items, kv_items, qr, qh, kr, kh, vr, vh, dr, dh, pack.rows, n, n_kv,
                                      pack.uniform_length, len(pack.lengths), q.shape[1], k.shape[1], q.shape[2], v.shape[2],
                                      int(causal), mark(form), mark(kv_form), scale)
     with L.on(q.device):
@@ -219,8 +219,11 @@ def packed_forward(q, k, v, pack, causal: bool, scale: float, keeps: bool):
     q, k, v = _in_place(q), _in_place(k), _in_place(v)
     out = torch.empty(pack.rows, q.shape[1], v.shape[2], device=q.device, dtype=q.dtype)
     lse = torch.empty(q.shape[1], pack.rows, device=q.device, dtype=torch.float32) if keeps else None
-    _packed_launch(so, pack, q, k, v, causal, scale, 0, o=out.data_ptr(), lse=lse.data_ptr() if keeps else 0)
-    return (out if v.shape[2] == dv else out[..., :dv].contiguous()), (q, k, v, out, lse)
+    # what rounding took off the outputs of short sequences, whose gradients would show it
+    low = torch.empty_like(out) if keeps and q.dtype == torch.bfloat16 and pack.shortest <= L.PACKED_LOW_ROWS else None
+    _packed_launch(so, pack, q, k, v, causal, scale, 0, o=out.data_ptr(), low=low.data_ptr() if low is not None else 0,
+                   lse=lse.data_ptr() if keeps else 0)
+    return (out if v.shape[2] == dv else out[..., :dv].contiguous()), (q, k, v, out, low, lse)
 
 
 class PackedAttention(torch.autograd.Function):
@@ -236,12 +239,13 @@ class PackedAttention(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_out):
         so = L.load()
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, low, lse = ctx.saved_tensors
         pack, (causal, scale, dk, dv) = ctx.pack, ctx.meta
         do = _in_place(grad_out if grad_out.dtype == q.dtype else grad_out.to(q.dtype))
         delta = torch.empty_like(lse)
         grads = [torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v)]
         _packed_launch(so, pack, q, k, v, causal, scale, 1, out=out.data_ptr(), dout=do, dq=grads[0].data_ptr(),
-                       dk=grads[1].data_ptr(), dv=grads[2].data_ptr(), lse=lse.data_ptr(), delta=delta.data_ptr())
+                       dk=grads[1].data_ptr(), dv=grads[2].data_ptr(), low=low.data_ptr() if low is not None else 0,
+                       lse=lse.data_ptr(), delta=delta.data_ptr())
         gq, gk, gv = (g if g.shape[2] == w else g[..., :w].contiguous() for g, w in zip(grads, (dk, dk, dv)))
         return gq, gk, gv, None, None, None

@@ -42,6 +42,7 @@ struct MtPackedAttn {
   const void *q, *k, *v;        // inputs, element strides below; the last dimension is contiguous
   const void *out, *dout;       // backward only: forward output (contiguous) and its gradient
   void *o, *dq, *dk, *dv;       // outputs, contiguous [T][heads or kv_heads][dk or dv]
+  void* low;                    // bf16 [T][heads][dv]: what rounding took off the output's rows of short sequences; may be null
   float *lse, *delta;           // [heads][rows]
   const MtSeqItem *items, *kv_items;      // items of query rows and of key rows; null: count sequences of uniform_len rows each
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, do_row, do_head;
@@ -65,6 +66,21 @@ __device__ __forceinline__ f32x16 pa_mma(f32x8 a, f32x8 b, f32x16 c) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
   return c;
+}
+
+// sum + the fragment's elements: the row sum adds the probabilities as they are multiplied, so that rounding them moves the
+// weights of a row but not their total (half the error of an output over few keys, and what makes D exact enough there).
+__device__ __forceinline__ float pa_row_sum(bf16x8 f, float sum) {
+  typedef __bf16 pair __attribute__((ext_vector_type(2)));
+  const pair one = {(__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) sum = __builtin_amdgcn_fdot2_f32_bf16(pair{f[j], f[j + 1]}, one, sum, false);
+  return sum;
+}
+__device__ __forceinline__ float pa_row_sum(f32x8 f, float sum) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sum += f[j];
+  return sum;
 }
 
 // Accumulator rows 16 s .. 16 s + 15 (eight registers per lane) as a fragment of the next product.
@@ -198,9 +214,24 @@ __device__ __forceinline__ void pa_own_row(typename PaFrag<T>::type (&f)[D / 16]
     }
   }
 }
-// Store a transposed accumulator (rows = columns of the output, lane & 31 = owned row): four consecutive columns at a time.
+// Four consecutive columns of a row; `low` (bf16 only, may be null) gets what the rounding took off.
+template <typename T> __device__ __forceinline__ void pa_store4(T* at, T* low, float v0, float v1, float v2, float v3) {
+  if constexpr (sizeof(T) == 2) {
+    const u32x2 w = {pack_bf16x2(v0, v1), pack_bf16x2(v2, v3)};
+    *reinterpret_cast<u32x2*>(at) = w;
+    if (low != nullptr) {
+      auto left = [](float a, float b, uint32_t r) {
+        return pack_bf16x2(a - __uint_as_float(r << 16), b - __uint_as_float(r & 0xFFFF0000u));
+      };
+      *reinterpret_cast<u32x2*>(low) = u32x2{left(v0, v1, w[0]), left(v2, v3, w[1])};
+    }
+  } else {
+    *reinterpret_cast<f32x4*>(at) = f32x4{v0, v1, v2, v3};
+  }
+}
+// Store a transposed accumulator (rows = columns of the output, lane & 31 = owned row).
 template <typename T, int D>
-__device__ __forceinline__ void pa_store_row(T* row, const f32x16 (&acc)[D / 32], float factor, int d, int lane) {
+__device__ __forceinline__ void pa_store_row(T* row, const f32x16 (&acc)[D / 32], float factor, int d, int lane, T* low = nullptr) {
   const int h = lane >> 5;
 #pragma unroll
   for (int b = 0; b < D / 32; ++b)
@@ -208,14 +239,8 @@ __device__ __forceinline__ void pa_store_row(T* row, const f32x16 (&acc)[D / 32]
     for (int g = 0; g < 4; ++g) {
       const int c = 32 * b + 8 * g + 4 * h;
       if (c < d) {
-        const float v0 = acc[b][4 * g] * factor, v1 = acc[b][4 * g + 1] * factor, v2 = acc[b][4 * g + 2] * factor,
-                    v3 = acc[b][4 * g + 3] * factor;
-        if constexpr (sizeof(T) == 2) {
-          const u32x2 w = {pack_bf16x2(v0, v1), pack_bf16x2(v2, v3)};
-          *reinterpret_cast<u32x2*>(row + c) = w;
-        } else {
-          *reinterpret_cast<f32x4*>(row + c) = f32x4{v0, v1, v2, v3};
-        }
+        pa_store4(row + c, low != nullptr ? low + c : nullptr, acc[b][4 * g] * factor, acc[b][4 * g + 1] * factor,
+                  acc[b][4 * g + 2] * factor, acc[b][4 * g + 3] * factor);
       }
     }
 }
@@ -258,7 +283,7 @@ __device__ __forceinline__ void pa_join(float* join, const f32x16 (&acc)[D / 32]
       join[(wave * D + 32 * b + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3)) * 32 + (lane & 31)] = acc[b][i] * factor;
 }
 template <typename T, int D>
-__device__ __forceinline__ void pa_join_store(T* base, int64_t row_stride, const float* join, int rows, int d) {
+__device__ __forceinline__ void pa_join_store(T* base, int64_t row_stride, const float* join, int rows, int d, T* low = nullptr) {
   const int r = threadIdx.x & 31;
   if (r >= rows) return;
 #pragma unroll
@@ -270,15 +295,18 @@ __device__ __forceinline__ void pa_join_store(T* base, int64_t row_stride, const
     for (int w = 0; w < 4; ++w)
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] += join[(w * D + c + e) * 32 + r];
-    if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2*>(base + r * row_stride + c) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-    else *reinterpret_cast<f32x4*>(base + r * row_stride + c) = v;
+    pa_store4(base + r * row_stride + c, low != nullptr ? low + r * row_stride + c : nullptr, v[0], v[1], v[2], v[3]);
   }
 }
+// Sequences whose output is kept with what its rounding took off (MtPackedAttn::low): over few keys D = do . o is as large as the
+// do . v it is subtracted from, and half a bf16 step of o would show in the gradients (two keys: 0.8 % of dq against 0.23 %).
+#define PA_LOW_ROWS 128
+__device__ __forceinline__ bool pa_low(const MtPackedAttn& p, int len) { return p.low != nullptr && len <= PA_LOW_ROWS; }
 // What the dq kernels hold of an owned row: q, do, L and D = do . o (stored for the dk / dv kernel by the waves with `store`).
 template <typename T, int DK, int DV>
 __device__ __forceinline__ void pa_dq_rows(const MtPackedAttn& p, typename PaFrag<T>::type (&qf)[DK / 16],
                                            typename PaFrag<T>::type (&df)[DV / 16], float& delta, float& lse, int64_t row, int head, bool ok,
-                                           bool store, int lane) {
+                                           bool store, bool low, int lane) {
   pa_own_row<T, DV>(df, reinterpret_cast<const T*>(p.dout) + row * p.do_row + (int64_t)head * p.do_head, ok, p.head_v, lane);
   delta = 0.f;
   lse = INFINITY;                                       // rows outside the sequence: p = 2^(s - inf) = 0
@@ -290,6 +318,14 @@ __device__ __forceinline__ void pa_dq_rows(const MtPackedAttn& p, typename PaFra
     for (int s = 0; s < DV / 16; ++s)
 #pragma unroll
       for (int j = 0; j < 8; ++j) delta = __builtin_fmaf((float)df[s][j], (float)of[s][j], delta);
+    if (low) {
+      pa_own_row<T, DV>(of, reinterpret_cast<const T*>(p.low) + row * ((int64_t)p.heads * p.head_v) + (int64_t)head * p.head_v, ok, p.head_v,
+                        lane);
+#pragma unroll
+      for (int s = 0; s < DV / 16; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) delta = __builtin_fmaf((float)df[s][j], (float)of[s][j], delta);
+    }
   }
   delta = pa_half_sum(delta);
   if (ok) {
@@ -313,6 +349,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void mt_pattn_fwd_kernel(const MtPac
   const MtSeqItem item = pa_item(p, p.items, it, 0, p.causal);
   const int64_t o_row = (int64_t)p.heads * p.head_v;
   T* o = reinterpret_cast<T*>(p.o) + item.row0 * o_row + (int64_t)head * p.head_v;
+  T* low = sizeof(T) == 2 && pa_low(p, item.len) ? reinterpret_cast<T*>(p.low) + item.row0 * o_row + (int64_t)head * p.head_v : nullptr;
   if (item.len <= 0) {
     pa_zero_rows<T>(o, o_row, -item.len, p.head_v);
     return;
@@ -401,12 +438,12 @@ __global__ __launch_bounds__(PA_THREADS, 2) void mt_pattn_fwd_kernel(const MtPac
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         s[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], c, -sub));
-        sum += s[u][i];
       }
 #pragma unroll
     for (int g = 0; g < PG; ++g) {
       if (g + 1 < PG) read_v(g + 1);
       const Frag pf = pa_pack<T>(s[g >> 1], g & 1);
+      sum = pa_row_sum(pf, sum);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int b = 0; b < D / 32; ++b) acc[b] = pa_mma(vf[g & 1][b], pf, acc[b]);
@@ -434,7 +471,8 @@ __global__ __launch_bounds__(PA_THREADS, 2) void mt_pattn_fwd_kernel(const MtPac
   for (; t < tiles; ++t) enter(t);
   sum = pa_half_sum(sum);
   if (mine < item.len) {
-    pa_store_row<T, D>(o + (int64_t)mine * o_row, acc, sum > 0.f || sum != sum ? 1.f / sum : 0.f, p.head_v, lane);
+    pa_store_row<T, D>(o + (int64_t)mine * o_row, acc, sum > 0.f || sum != sum ? 1.f / sum : 0.f, p.head_v, lane,
+                       low != nullptr ? low + (int64_t)mine * o_row : nullptr);
     if (p.lse != nullptr && lane < 32)      // a row whose scores are all -inf weighs nothing in the backward pass
       p.lse[(int64_t)head * p.rows + item.row0 + mine] = sum > 0.f || sum != sum ? m + __builtin_amdgcn_logf(sum) : INFINITY;
   }
@@ -461,7 +499,7 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
   const bool ok = mine < item.len;
   Frag qf[D / 16], df[D / 16];
   float delta, lse;
-  pa_dq_rows<T, D, D>(p, qf, df, delta, lse, item.row0 + (int64_t)mine, head, ok, true, lane);
+  pa_dq_rows<T, D, D>(p, qf, df, delta, lse, item.row0 + (int64_t)mine, head, ok, true, pa_low(p, item.len), lane);
   const T* kb = reinterpret_cast<const T*>(p.k) + item.row0 * p.k_row + (int64_t)kvh * p.k_head;
   const T* vb = reinterpret_cast<const T*>(p.v) + item.row0 * p.v_row + (int64_t)kvh * p.v_head;
   const int keys = p.causal && item.first + PA_OWN < item.len ? item.first + PA_OWN : item.len;
@@ -736,6 +774,7 @@ __global__ __launch_bounds__(PA_THREADS, (PaSplit<T, DK, DV>::WAVES)) void mt_pa
   const MtSeqItem item = pa_item(p, p.items, it, p.split, p.causal);
   const int64_t o_row = (int64_t)p.heads * p.head_v;
   T* o = reinterpret_cast<T*>(p.o) + item.row0 * o_row + (int64_t)head * p.head_v;
+  T* low = sizeof(T) == 2 && pa_low(p, item.len) ? reinterpret_cast<T*>(p.low) + item.row0 * o_row + (int64_t)head * p.head_v : nullptr;
   if (item.len <= 0) {
     pa_zero_rows<T>(o, o_row, -item.len, p.head_v);
     return;
@@ -798,15 +837,13 @@ __global__ __launch_bounds__(PA_THREADS, (PaSplit<T, DK, DV>::WAVES)) void mt_pa
     }
     const float sub = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[0][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][i], c, -sub));
-      sum += s[0][i];
-    }
+    for (int i = 0; i < 16; ++i) s[0][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][i], c, -sub));
     if (more) pa_wait_vm<S::KP>();             // V of this tile; the next K may still be on the way
     else pa_wait_vm<0>();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const Frag pf = pa_pack<T>(s[0], h);
+      sum = pa_row_sum(pf, sum);
 #pragma unroll
       for (int b = 0; b < DV / 32; ++b)
         if (pa_step<T>(32 * b, p.head_v)) acc[b] = pa_mma(IV::cols(vcol, 16 * h, b), pf, acc[b]);
@@ -818,7 +855,9 @@ __global__ __launch_bounds__(PA_THREADS, (PaSplit<T, DK, DV>::WAVES)) void mt_pa
   float* lse = p.lse != nullptr && mine < item.len && lane < 32 ? p.lse + (int64_t)head * p.rows + item.row0 + mine : nullptr;
   if (item.solo) {
     const bool real = sum > 0.f || sum != sum;
-    if (mine < item.len) pa_store_row<T, DV>(o + (int64_t)mine * o_row, acc, real ? 1.f / sum : 0.f, p.head_v, lane);
+    if (mine < item.len)
+      pa_store_row<T, DV>(o + (int64_t)mine * o_row, acc, real ? 1.f / sum : 0.f, p.head_v, lane,
+                          low != nullptr ? low + (int64_t)mine * o_row : nullptr);
     if (lse != nullptr) *lse = real ? m + __builtin_amdgcn_logf(sum) : INFINITY;
     return;
   }
@@ -838,7 +877,8 @@ __global__ __launch_bounds__(PA_THREADS, (PaSplit<T, DK, DV>::WAVES)) void mt_pa
   const float f = __builtin_amdgcn_exp2f(m - sub) * (real ? 1.f / total : 0.f);
   pa_join<DV>(reinterpret_cast<float*>(lds), acc, f, wave, lane);
   __syncthreads();
-  pa_join_store<T, DV>(o + (int64_t)first * o_row, o_row, reinterpret_cast<const float*>(lds), item.len - first, p.head_v);
+  pa_join_store<T, DV>(o + (int64_t)first * o_row, o_row, reinterpret_cast<const float*>(lds), item.len - first, p.head_v,
+                       low != nullptr ? low + (int64_t)first * o_row : nullptr);
   if (wave == 0 && lse != nullptr) *lse = real ? sub + __builtin_amdgcn_logf(total) : INFINITY;
 }
 
@@ -863,7 +903,8 @@ __global__ __launch_bounds__(PA_THREADS, (PaSplit<T, DK, DV>::WAVES)) void mt_pa
   if (item.solo && first >= item.len) return;
   Frag qf[DK / 16], df[DV / 16];
   float delta, lse;
-  pa_dq_rows<T, DK, DV>(p, qf, df, delta, lse, item.row0 + (int64_t)mine, head, mine < item.len, item.solo || wave == 0, lane);
+  pa_dq_rows<T, DK, DV>(p, qf, df, delta, lse, item.row0 + (int64_t)mine, head, mine < item.len, item.solo || wave == 0,
+                        pa_low(p, item.len), lane);
   const T* kb = reinterpret_cast<const T*>(p.k) + item.row0 * p.k_row + (int64_t)kvh * p.k_head;
   const T* vb = reinterpret_cast<const T*>(p.v) + item.row0 * p.v_row + (int64_t)kvh * p.v_head;
   const int keys = p.causal && first + 32 < item.len ? first + 32 : item.len;
@@ -1092,10 +1133,11 @@ static void pa_launch_split_width(const MtPackedAttn& p, int pass, hipStream_t s
   else pa_launch_split<T, 128, 128>(p, pass, stream);
 }
 
-extern "C" int mt_packed_attn_sizes(int* item_bytes, int* own_rows, int* split_rows) {
+extern "C" int mt_packed_attn_sizes(int* item_bytes, int* own_rows, int* split_rows, int* low_rows) {
   *item_bytes = (int)sizeof(MtSeqItem);
   *own_rows = PA_OWN;
   *split_rows = PA_TILE;
+  *low_rows = PA_LOW_ROWS;
   return (int)sizeof(MtPackedAttn);
 }
 
@@ -1121,8 +1163,8 @@ extern "C" int mt_packed_attn_launch(const MtPackedAttn* a, int backward, int bf
   const int64_t strides[8] = {p.q_row, p.q_head, p.k_row, p.k_head, p.v_row, p.v_head, p.do_row, p.do_head};
   for (int i = 0; i < 8; ++i)      // 32-bit byte offsets inside a staged tile of at most 128 rows
     if (strides[i] < 0 || strides[i] % per || strides[i] * es > (1 << 24)) return -2;
-  const void* ptrs[9] = {p.q, p.k, p.v, p.out, p.dout, p.o, p.dq, p.dk, p.dv};
-  for (int i = 0; i < 9; ++i)
+  const void* ptrs[10] = {p.q, p.k, p.v, p.out, p.dout, p.o, p.dq, p.dk, p.dv, p.low};
+  for (int i = 0; i < 10; ++i)
     if (reinterpret_cast<uintptr_t>(ptrs[i]) & 15) return -2;
   const int widest = p.head_k > p.head_v ? p.head_k : p.head_v;
   for (int pass = backward ? 1 : 0; pass <= (backward ? 2 : 0); ++pass) {

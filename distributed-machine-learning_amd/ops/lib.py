@@ -18,7 +18,8 @@ import numpy as np
 from . import build as _build
 
 MT_MAX_LAYERS = 8
-PACKED_OWN_ROWS, PACKED_SPLIT_ROWS, PACKED_ITEM_BYTES = 128, 32, 16      # csrc/packed_attention.hip: rows and bytes of an item
+# csrc/packed_attention.hip: bytes and rows of an item, longest sequence whose outputs keep what rounding took off
+PACKED_ITEM_BYTES, PACKED_OWN_ROWS, PACKED_SPLIT_ROWS, PACKED_LOW_ROWS = 16, 128, 32, 128
 
 c_void_p, c_int32, c_uint32, c_float, c_size_t = C.c_void_p, C.c_int32, C.c_uint32, C.c_float, C.c_size_t
 
@@ -57,7 +58,7 @@ class OptSlot(C.Structure):
 
 class PackedAttn(C.Structure):
     _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p), ("dout", c_void_p),
-                ("o", c_void_p), ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p),
+                ("o", c_void_p), ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p), ("low", c_void_p),
                 ("lse", c_void_p), ("delta", c_void_p), ("items", c_void_p), ("kv_items", c_void_p),
                 ("q_row", C.c_int64), ("q_head", C.c_int64), ("k_row", C.c_int64), ("k_head", C.c_int64),
                 ("v_row", C.c_int64), ("v_head", C.c_int64), ("do_row", C.c_int64), ("do_head", C.c_int64),
@@ -67,7 +68,7 @@ class PackedAttn(C.Structure):
 
 
 # The same layout for struct.pack: filling a ctypes structure field by field costs several microseconds of every call.
-PACKED_ATTN_FORMAT = struct.Struct("<13Q9q11if")
+PACKED_ATTN_FORMAT = struct.Struct("<14Q9q11if")
 
 
 class MlpPlan(C.Structure):
@@ -229,12 +230,12 @@ def load(build_if_missing: bool = True) -> C.CDLL:
     lib.mt_attn_fwd_strided_launch.restype = lib.mt_attn_bwd_strided_launch.restype = C.c_int
     lib.mt_attn_exact_level.argtypes = [C.c_int]
     lib.mt_attn_exact_level.restype = C.c_int
-    item_bytes, own_rows, split_rows = C.c_int(), C.c_int(), C.c_int()
-    if lib.mt_packed_attn_sizes(C.byref(item_bytes), C.byref(own_rows), C.byref(split_rows)) != C.sizeof(PackedAttn):
+    facts = [C.c_int() for _ in range(4)]
+    if lib.mt_packed_attn_sizes(*(C.byref(f) for f in facts)) != C.sizeof(PackedAttn):
         raise KernelLibraryError("MtPackedAttn layout mismatch between lib.py and the library")
     if PACKED_ATTN_FORMAT.size != C.sizeof(PackedAttn):
         raise KernelLibraryError("MtPackedAttn layout mismatch between the struct format and lib.py")
-    if (item_bytes.value, own_rows.value, split_rows.value) != (PACKED_ITEM_BYTES, PACKED_OWN_ROWS, PACKED_SPLIT_ROWS):
+    if [f.value for f in facts] != [PACKED_ITEM_BYTES, PACKED_OWN_ROWS, PACKED_SPLIT_ROWS, PACKED_LOW_ROWS]:
         raise KernelLibraryError("packed attention: tile list layout mismatch between lib.py and the library")
     lib.mt_linear_parts.argtypes = [C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int]
     lib.mt_linear_gemm_launch.argtypes = ([C.c_int] + [c_void_p] * 7 + [C.c_int64, C.c_int, C.c_int, C.c_int64, C.c_int64]
