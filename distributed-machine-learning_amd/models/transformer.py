@@ -33,7 +33,6 @@ from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
-import torch.nn.functional as F
 
 from ..ops.attention import self_attention, self_attention_qkv
 from ..ops.elementwise import depthwise_conv1d, pe_add_dropout, relu_dropout
@@ -79,7 +78,7 @@ class DepthwiseSeparableConv(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:          # [B, S, d], channel-last throughout
         y = depthwise_conv1d(x, self.depthwise.weight, self.depthwise.bias)
-        y = F.relu(linear(y, self.pointwise.weight.squeeze(-1), self.pointwise.bias))     # k=1 conv == linear
+        y = linear(y, self.pointwise.weight.squeeze(-1), self.pointwise.bias, activation="relu")     # k=1 conv == linear
         return linear(y, self.project.weight.squeeze(-1), self.project.bias)
 
 
@@ -181,7 +180,7 @@ class CustomEncoderLayer(nn.Module):
                                   dropout_p=self.p if self.training else 0.0)
         ff = self.feedforward
         if isinstance(ff, nn.Sequential):          # same parameters, dense layers through the fused-backward path
-            f = linear(F.relu(linear(src, ff[0].weight, ff[0].bias)), ff[2].weight, ff[2].bias)
+            f = linear(linear(src, ff[0].weight, ff[0].bias, activation="relu"), ff[2].weight, ff[2].bias)
         else:
             f = ff(src)
         m = self._branch_scale(src, rate)
@@ -244,9 +243,7 @@ class TransformerModel(nn.Module):
         # batch 32-256; a single-kernel head with all five weight matrices staged through LDS was built and measured at
         # 160-590 us (its workgroups stream the whole first matrix for eight rows each) and removed.
         for i, fc in enumerate(fcs):
-            h = linear(h, fc.weight, fc.bias)
-            if i < len(fcs) - 1:
-                h = F.relu(h)
+            h = linear(h, fc.weight, fc.bias, activation="relu" if i < len(fcs) - 1 else None)
         return h
 
 

@@ -87,11 +87,24 @@ def _kernel_envelope(t: torch.Tensor, S: int, dk: int, dv: int) -> bool:
     return widest <= MAX_HEAD_DIM or (widest <= WIDE_HEAD_DIM and S <= WIDE_MAX_SEQ)
 
 
+def _packed_envelope(t: torch.Tensor, dk: int, dv: int, kind: str, dropout_p: float) -> bool:
+    """What the kernels for sequences of any length take of the calls below: softmax scores without dropout."""
+    return (t.is_cuda and t.dtype in (torch.float32, torch.bfloat16) and t.numel() > 0 and kind == "softmax" and dropout_p == 0.0
+            and 0 < dk <= PACKED_MAX_HEAD_DIM and 0 < dv <= PACKED_MAX_HEAD_DIM)
+
+
+def _packed_self_attention(qkv, B: int, S: int, h: int, dk: int, dv: int) -> torch.Tensor:
+    """[B, S, h*dv] of queries, keys and values [B*S, h, width] each, on the packed kernels."""
+    q, k, v = (t.unflatten(1, (h, d)) for t, d in zip(qkv, (dk, dk, dv)))
+    return packed_attention(q, k, v, SequencePack.uniform(B, S, device=q.device)).reshape(B, S, h * dv)
+
+
 def self_attention_qkv(qkv: torch.Tensor, num_heads: int, dk: int, kind: str = "softmax",
                        dropout_p: float = 0.0) -> torch.Tensor:
     """Multi-head self-attention on ONE fused projection output ``qkv`` [B, S, 2*h*dk + h*dv]: all queries, all keys,
     all values, each block head-major.  On a GPU the kernels read the three blocks in place and return one gradient
-    tensor for the projection; elsewhere the blocks are split and ``self_attention`` runs."""
+    tensor for the projection (sequences past the short kernels' envelope, softmax without dropout: the packed kernels read
+    them in place too); elsewhere the blocks are split and ``self_attention`` runs."""
     B, S, W = qkv.shape
     h = num_heads
     dv = (W - 2 * h * dk) // h
@@ -103,6 +116,8 @@ def self_attention_qkv(qkv: torch.Tensor, num_heads: int, dk: int, kind: str = "
                 from .rng import next_seed
                 seed = next_seed(qkv.device)
             return FusedQKVAttention.apply(qkv, h, dk, kind, dropout_p, seed)
+    if _packed_envelope(qkv, dk, dv, kind, dropout_p):
+        return _packed_self_attention(qkv.reshape(B * S, W).split([h * dk, h * dk, h * dv], dim=1), B, S, h, dk, dv)
     qk, v = qkv.split([2 * h * dk, h * dv], dim=-1)
     return self_attention(qk, v, h, kind, dropout_p)
 
@@ -111,7 +126,8 @@ def self_attention(qk: torch.Tensor, v: torch.Tensor, num_heads: int, kind: str 
                    dropout_p: float = 0.0) -> torch.Tensor:
     """Multi-head self-attention on projection outputs: ``qk`` [B, S, 2*h*dk] (all queries, then all keys, head-major),
     ``v`` [B, S, h*dv]; returns [B, S, h*dv].  On a GPU the fused kernels read these tensors in place (no head
-    split/merge copies, no casts); elsewhere the heads are split and ``attention_reference`` runs."""
+    split/merge copies, no casts), past their envelope the packed kernels (softmax, no dropout); elsewhere the heads are split
+    and ``attention_reference`` runs."""
     B, S, w2 = qk.shape
     h = num_heads
     dk, dv = w2 // (2 * h), v.shape[-1] // h
@@ -123,6 +139,8 @@ def self_attention(qk: torch.Tensor, v: torch.Tensor, num_heads: int, kind: str 
                 from .rng import next_seed
                 seed = next_seed(qk.device)
             return FusedSelfAttention.apply(qk, v, h, kind, None, dropout_p, seed)
+    if _packed_envelope(qk, dk, dv, kind, dropout_p) and v.dtype == qk.dtype:
+        return _packed_self_attention(qk.reshape(B * S, w2).chunk(2, dim=1) + (v.reshape(B * S, h * dv),), B, S, h, dk, dv)
     keep = None
     if dropout_p > 0.0:
         from .elementwise import keep_mask

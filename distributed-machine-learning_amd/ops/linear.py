@@ -424,7 +424,7 @@ class FusedLinear(torch.autograd.Function):
                     g = g if g.stride(1) == 1 else g.contiguous()
                     dz = torch.empty(M, out_f + -out_f % per, device=dev, dtype=xc.dtype)
                     part = None
-                    if b_dtype is not None and ctx.needs_input_grad[2]:
+                    if bf16 and b_dtype is not None and ctx.needs_input_grad[2]:          # from dz before it is rounded
                         db = torch.empty(out_f, device=dev, dtype=b_dtype)
                         part = torch.empty(so.mt_linear_act_parts(M, dz.shape[1], int(bf16)), out_f, device=dev, dtype=torch.float32)
                     L.check(so.mt_linear_act_bwd_launch(g.data_ptr(), s.data_ptr(), dz.data_ptr(),
@@ -432,7 +432,7 @@ class FusedLinear(torch.autograd.Function):
                                                         db.data_ptr() if part is not None else None, M, out_f, g.stride(0),
                                                         dz.shape[1], act, int(b_dtype == torch.bfloat16), int(bf16), stream),
                             "mt_linear_act_bwd_launch")
-                    b_dtype = None                      # done; the launches below need not sum dz again
+                    b_dtype = None if part is not None else b_dtype
                 else:
                     dz = _pieces(g)
                     dz = dz if dz.stride(0) == dz.shape[1] else dz.contiguous()
