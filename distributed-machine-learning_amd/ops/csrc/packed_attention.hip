@@ -364,11 +364,17 @@ __global__ __launch_bounds__(PA_THREADS, 2) void mt_pattn_fwd_kernel(const MtPac
   const int tiles = (keys + BN - 1) / BN;
   const float c = p.scale * 1.4426950408889634f;
 
+  // Tiles are fetched in order: the next one's addresses are carried along, not worked out per tile ahead of its fetch.
+  const T *k_next = kb, *v_next = vb;
+  int left = item.len;
+  const int64_t k_hop = BN * p.k_row, v_hop = BN * p.v_row;
   auto issue = [&](int t) {
     uint8_t* st = lds + (t & 1) * 2 * IMG;
-    const int64_t k0 = (int64_t)t * BN;
-    Img::template stage<BN>(st, kb + k0 * p.k_row, p.k_row, item.len - t * BN, p.head_k, wave, lane);
-    Img::template stage<BN>(st + IMG, vb + k0 * p.v_row, p.v_row, item.len - t * BN, p.head_v, wave, lane);
+    Img::template stage<BN>(st, k_next, p.k_row, left, p.head_k, wave, lane);
+    Img::template stage<BN>(st + IMG, v_next, p.v_row, left, p.head_v, wave, lane);
+    k_next += k_hop;
+    v_next += v_hop;
+    left -= BN;
   };
 
   f32x16 acc[D / 32];
@@ -505,11 +511,17 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
   const int keys = p.causal && item.first + PA_OWN < item.len ? item.first + PA_OWN : item.len;
   const int tiles = (keys + BN - 1) / BN;
   const float c = p.scale * 1.4426950408889634f;
+  // Tiles are fetched in order: the next one's addresses are carried along, not worked out per tile ahead of its fetch.
+  const T *k_next = kb, *v_next = vb;
+  int left = item.len;
+  const int64_t k_hop = BN * p.k_row, v_hop = BN * p.v_row;
   auto issue = [&](int t) {
     uint8_t* st = lds + (t & 1) * 2 * IMG;
-    const int64_t k0 = (int64_t)t * BN;
-    Img::template stage<BN>(st, kb + k0 * p.k_row, p.k_row, item.len - t * BN, p.head_k, wave, lane);
-    Img::template stage<BN>(st + IMG, vb + k0 * p.v_row, p.v_row, item.len - t * BN, p.head_v, wave, lane);
+    Img::template stage<BN>(st, k_next, p.k_row, left, p.head_k, wave, lane);
+    Img::template stage<BN>(st + IMG, v_next, p.v_row, left, p.head_v, wave, lane);
+    k_next += k_hop;
+    v_next += v_hop;
+    left -= BN;
   };
   f32x16 acc[D / 32];
   pa_clear(acc);
@@ -587,13 +599,20 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
 // Eight waves: waves w and w + 4 own the same 32 keys and take the two halves of every 64-query tile; their sums meet in LDS at
 // the end.  The workgroup's keys and values stay in LDS beside the query tiles and are read again for every tile, because the
 // two gradients' accumulators already take half the registers of a wave when two of them are to share a SIMD.
+//
+// A wave's tile is three steps: scores (A: S and dp), vector work (B: p and ds), gradients (C: dv and dk).  The two waves of a
+// SIMD are the two halves of one workgroup, and in step with each other they would leave the matrix pipe idle while both do B.
+// So the second half runs a step behind: between two barriers the first does A while the second does C of the tile before, then
+// B and C while the second does A and B.  Each half fetches its own 32 queries of the next tile once nobody reads that buffer.
+// Measured with the dq kernel, 8 x 2048 causal, 16 / 4 heads of 64: 295 us against 304 in step; at 128 wide both ways take the same
+// time (2 x 4096, 16 heads: 920 us, 1046 TFLOP/s of the seven products, at 2.0 GHz: power, not the schedule, is the limit there).
 #define PA_DKV_THREADS 512
 template <typename T, int D>
 __global__ __launch_bounds__(PA_DKV_THREADS, 2) void mt_pattn_dkv_kernel(const MtPackedAttn p) {
   typedef PaImg<T, D> Img;
   typedef typename PaFrag<T>::type Frag;
-  constexpr int BQ = 64, IMG = BQ * Img::ROWB, KV = PA_OWN * Img::ROWB;
-  constexpr int STAGE = 2 * IMG + 1024;                              // q rows, do rows, L and D of the 64 rows
+  constexpr int BQ = 64, HALF = 32 * Img::ROWB, IMG = 2 * HALF, KV = PA_OWN * Img::ROWB;
+  constexpr int STAGE = 2 * IMG + 1024;                              // q rows, do rows, {L, D} of the rows of either half
   constexpr int BYTES = 2 * KV + 2 * STAGE, JOIN = 2 * 128 * D * 4;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[BYTES < JOIN ? JOIN : BYTES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -622,57 +641,65 @@ __global__ __launch_bounds__(PA_DKV_THREADS, 2) void mt_pattn_dkv_kernel(const M
                                    item.len - item.first, p.head_v, wave, lane);
   }
   uint8_t* stages = lds + 2 * KV;
-  auto issue = [&](int n, int hg, int qt) {
-    uint8_t* st = stages + (n & 1) * STAGE;
-    const int head = kvh * group + hg, q0 = qt * BQ, left = item.len - q0;
+  // This half's 32 queries of the next tile, tiles in order, then heads: addresses are carried along.
+  const T *q_next, *d_next;
+  const float* stat_next;
+  int left, todo = tiles, until = per_head;
+  int64_t head_next = (int64_t)kvh * group;
+  auto enter_head = [&] {
+    const int q0 = q_lo * BQ + 32 * half;
     const int64_t r0 = item.row0 + (int64_t)q0;
-    Img::template stage<BQ, 8>(st, reinterpret_cast<const T*>(p.q) + r0 * p.q_row + (int64_t)head * p.q_head, p.q_row, left, p.head_k,
-                               wave, lane);
-    Img::template stage<BQ, 8>(st + IMG, reinterpret_cast<const T*>(p.dout) + r0 * p.do_row + (int64_t)head * p.do_head, p.do_row,
-                               left, p.head_v, wave, lane);
-    if (wave < 2) {
-      const float* src = (wave == 0 ? p.lse : p.delta) + (int64_t)head * p.rows + r0;
-      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<float*>(src), 0, (uint32_t)(left < BQ ? left : BQ) * 4u, 0x00027000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(st + 2 * IMG + wave * 256), 4,
-                                               lane * 4, 0, 0, 0);
+    q_next = reinterpret_cast<const T*>(p.q) + r0 * p.q_row + head_next * p.q_head;
+    d_next = reinterpret_cast<const T*>(p.dout) + r0 * p.do_row + head_next * p.do_head;
+    stat_next = (block == 0 ? p.lse : p.delta) + head_next * p.rows + r0;
+    left = item.len - q0;
+    until = per_head;
+    ++head_next;
+  };
+  enter_head();
+  const int64_t q_hop = BQ * p.q_row, d_hop = BQ * p.do_row;
+  auto issue = [&](int n) {
+    if (todo-- <= 0) return;
+    uint8_t* st = stages + (n & 1) * STAGE;
+    if (left > 0) {                                                 // else nobody will read them
+      Img::template stage<32, 4>(st + half * HALF, q_next, p.q_row, left, p.head_k, block, lane);
+      Img::template stage<32, 4>(st + IMG + half * HALF, d_next, p.do_row, left, p.head_v, block, lane);
+      if (block < 2) {
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<float*>(stat_next), 0, (uint32_t)(left < 32 ? left : 32) * 4u, 0x00027000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(st + 2 * IMG + half * 512 + block * 256),
+                                                 4, lane * 4, 0, 0, 0);
+      }
     }
+    q_next += q_hop;
+    d_next += d_hop;
+    stat_next += BQ;
+    left -= BQ;
+    if (--until == 0 && todo > 0) enter_head();
   };
   f32x16 ak[D / 32], av[D / 32];
   pa_clear(ak);
   pa_clear(av);
   const uint32_t lds_at = pa_lds_at(lds), st_at = lds_at + 2 * KV;
-  issue(0, 0, q_lo);
-  int hg = 0, qt = q_lo;
-  for (int n = 0; n < tiles; ++n) {
-    const int qu = qt * BQ + 32 * half;
-    if (++qt == q_lo + per_head) { qt = q_lo; ++hg; }
-    pa_tile_barrier();
-    if (n + 1 < tiles) issue(n + 1, hg, qt);
-    if (qu >= item.len || (p.causal && qu + 31 < first)) continue;
-    const uint32_t rb = Img::row_base(lane), qimg = st_at + (n & 1) * STAGE;
-    const uint32_t krow = lds_at + rb, qrow = qimg + rb, qcol = qimg + Img::col_base(lane);
+  f32x16 s[1], d[1];
+  Frag pf[2], sf[2];
+  auto scores = [&](int n) {                                        // A
+    const uint32_t rb = Img::row_base(lane), krow = lds_at + block * HALF + rb, qrow = st_at + (n & 1) * STAGE + half * HALF + rb;
     constexpr int G = 2, NG = D / 16 / G;
-    Frag fr[2][G], kr[2][G], cf[2][D / 32];
+    Frag fr[2][G], kr[2][G];
     auto read_rows = [&](int g) {          // groups 0 .. NG - 1 of q and k, then of do and v
 #pragma unroll
       for (int e = 0; e < G; ++e) {
-        fr[g & 1][e] = Img::rows(g < NG ? qrow : qrow + IMG, 32 * half, (g % NG) * G + e);
-        kr[g & 1][e] = Img::rows(g < NG ? krow : krow + KV, 32 * block, (g % NG) * G + e);
+        fr[g & 1][e] = Img::rows(g < NG ? qrow : qrow + IMG, 0, (g % NG) * G + e);
+        kr[g & 1][e] = Img::rows(g < NG ? krow : krow + KV, 0, (g % NG) * G + e);
       }
     };
-    auto read_cols = [&](int g) {          // do's columns of two times 16 rows, then q's
-#pragma unroll
-      for (int b = 0; b < D / 32; ++b) cf[g & 1][b] = Img::cols(g < 2 ? qcol + IMG : qcol, 32 * half + 16 * (g & 1), b);
-    };
-    f32x16 s[1], d[1];
     pa_clear(s);
     pa_clear(d);
     read_rows(0);
 #pragma unroll
     for (int g = 0; g < 2 * NG; ++g) {
       if (g + 1 < 2 * NG) read_rows(g + 1);
-      else read_cols(0);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int e = 0; e < G; ++e) {
@@ -681,10 +708,12 @@ __global__ __launch_bounds__(PA_DKV_THREADS, 2) void mt_pattn_dkv_kernel(const M
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+  };
+  auto weigh = [&](int n, int qu) {                                 // B
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       // (by address: through the array the compiler would first wait for the LDS-DMA of the next tile, which may alias)
-      const uint32_t at = qimg + 2 * IMG + 4 * (32 * half + 8 * g + 4 * (lane >> 5));
+      const uint32_t at = st_at + (n & 1) * STAGE + 2 * IMG + half * 512 + 4 * (8 * g + 4 * (lane >> 5));
       const f32x4 lse = *pa_lds<f32x4>(at), delta = *pa_lds<f32x4>(at + 256);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -703,19 +732,72 @@ __global__ __launch_bounds__(PA_DKV_THREADS, 2) void mt_pattn_dkv_kernel(const M
       }
     }
 #pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      pf[h] = pa_pack<T>(s[0], h);
+      sf[h] = pa_pack<T>(d[0], h);
+    }
+  };
+  auto gradients = [&](int n) {                                     // C
+    const uint32_t qcol = st_at + (n & 1) * STAGE + half * HALF + Img::col_base(lane);
+    Frag cf[2][D / 32];
+    auto read_cols = [&](int g) {          // do's columns of two times 16 rows, then q's
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b) cf[g & 1][b] = Img::cols(g < 2 ? qcol + IMG : qcol, 16 * (g & 1), b);
+    };
+    read_cols(0);
+#pragma unroll
     for (int g = 0; g < 4; ++g) {
       if (g < 3) read_cols(g + 1);
-      const Frag pf = pa_pack<T>(g < 2 ? s[0] : d[0], g & 1);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int b = 0; b < D / 32; ++b) {
-        if (g < 2) av[b] = pa_mma(cf[g & 1][b], pf, av[b]);
-        else ak[b] = pa_mma(cf[g & 1][b], pf, ak[b]);
+        if (g < 2) av[b] = pa_mma(cf[g & 1][b], pf[g & 1], av[b]);
+        else ak[b] = pa_mma(cf[g & 1][b], sf[g & 1], ak[b]);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+  };
+  auto sees = [&](int qu) { return qu < item.len && !(p.causal && qu + 31 < first); };
+  auto middle = [&] {                      // the halves meet between their steps; the reads of the first are back
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  issue(0);
+  const int q_end = q_lo + per_head;
+  int qt = q_lo;
+  if (half == 0) {
+    for (int n = 0; n < tiles; ++n) {
+      const int qu = qt * BQ;
+      if (++qt == q_end) qt = q_lo;
+      pa_tile_barrier();
+      issue(n + 1);
+      const bool on = sees(qu);
+      if (on) scores(n);
+      middle();
+      if (on) {
+        weigh(n, qu);
+        gradients(n);
+      }
+    }
+  } else {
+    bool behind = false;
+    for (int n = 0; n < tiles; ++n) {
+      const int qu = qt * BQ + 32;
+      if (++qt == q_end) qt = q_lo;
+      pa_tile_barrier();
+      if (behind) gradients(n - 1);
+      middle();
+      issue(n + 1);
+      behind = sees(qu);
+      if (behind) {
+        scores(n);
+        weigh(n, qu);
+      }
+    }
+    if (behind) gradients(tiles - 1);
   }
-  // [dk, dv][key block][column][key] f32 of the second halves; no LDS-DMA is in flight past the last tile's barrier
+  // [dk, dv][key block][column][key] f32 of the second halves; no LDS-DMA is in flight past the last tile's barriers
   float* join = reinterpret_cast<float*>(lds) + block * 32 * D;
   __syncthreads();
   auto each = [&](auto&& f) {
