@@ -398,8 +398,7 @@ class FusedLinear(torch.autograd.Function):
         backward = any(ctx.needs_input_grad[:3])
         # what act' is read from: y itself has z's sign under ReLU, unless a residual was added to it
         keep_z = backward and act != 0 and not (act == 1 and residual is None)
-        with torch.autocast("cuda", enabled=False):
-            y, xc, wc, z = fused_forward(x, weight, bias, residual, act, w16, keep_z)
+        y, xc, wc, z = fused_forward(x, weight, bias, residual, act, w16, keep_z)
         if backward:
             ctx.save_for_backward(xc, wc, z if keep_z else y if act else None)
         ctx.meta = (act, x.shape, weight.shape[1], weight.dtype, bias.dtype if bias is not None else None,
@@ -418,7 +417,7 @@ class FusedLinear(torch.autograd.Function):
             bf16, dev, M = xc.dtype == torch.bfloat16, xc.device, xc.shape[0]
             per = 8 if bf16 else 4
             stream = L.raw_stream(dev)
-            with torch.autocast("cuda", enabled=False), L.on(dev):
+            with L.on(dev):
                 g = _rows_of(dy if dy.dtype == xc.dtype else dy.to(xc.dtype), out_f)
                 if act:
                     g = g if g.stride(1) == 1 else g.contiguous()
