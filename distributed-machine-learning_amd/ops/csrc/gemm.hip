@@ -37,7 +37,7 @@
 // that trades bytes for latency when a pack has too few tiles to fill 256 CUs.
 //
 // One large GEMM (hundreds of 256 x 256 tiles; the layers of a data-parallel trial) takes the eight-wave 256-tile kernel
-// in the second half of this file: same images and fragment reads, half the staged bytes per flop, fragment reads issued a
+// of mt_gemm_tile.h: same images and fragment reads, half the staged bytes per flop, fragment reads issued a
 // group of MFMAs ahead, and a banded tile order that keeps an XCD's resident tiles on few operand panels.
 #include "mt_gemm_tile.h"
 

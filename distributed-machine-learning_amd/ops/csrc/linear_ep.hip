@@ -8,7 +8,7 @@
 // z is kept for the backward pass in the operands' type (for bf16 that rounds the argument of act' by at most 2^-8 of it); with
 // ReLU and no residual y itself is enough.  dz is one pass over dy, written with rows of whole 16-byte pieces (zeros behind
 // column N) so that both gradient GEMMs can stage it.
-#include "mt_gemm_tile.h"
+#include "mt_linear_tile.h"
 #include "mt_gemm_f32_tile.h"
 
 // MODE 0: A [I][KK] and B [J][KK] (forward); 1: B [KK][J] (input gradient).  A contraction may be split over workgroups: part `sp`
@@ -38,16 +38,16 @@ __global__ __launch_bounds__(NTHREADS) void mt_linear_gemm_kernel(MtGemmGroup g,
   tile.tj = (int16_t)(t % tiles_j);
   gemm_tile<MODE, NSTAGE, true>(&g, tile, 0, 0, 0, 0, 1, 0, lds, &ep);
 }
-#define LINEAR_BAND 4       // 256-tiles: row tiles of a band (mt_gemm_p8_kernel)
+#define LINEAR_BAND 4       // 256-tiles: row tiles of a band, so that an XCD's 32 tiles at a time share 12 operand panels
 template <int MODE>
-__global__ __launch_bounds__(P8_THREADS) void mt_linear_p8_kernel(MtGemmGroup g, MtLinearEp ep, int tiles_i, int tiles_j) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BIG_STAGE_BYTES];
+__global__ __launch_bounds__(LT_THREADS) void mt_linear_big_kernel(MtGemmGroup g, MtLinearEp ep, int tiles_i, int tiles_j) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * BIG_STAGE_BYTES];
   constexpr int splits = 1;
   LINEAR_PICK();
   const int in_band = LINEAR_BAND * tiles_j, first = (t / in_band) * LINEAR_BAND;
   const int rows = tiles_i - first < LINEAR_BAND ? tiles_i - first : LINEAR_BAND;
   const int r = t % in_band;
-  gemm_tile_p8<MODE, MODE == 0 ? 1 : 0, true>(g, first + r % rows, r / rows, 0, 0, 1, 0, lds, &ep);
+  linear_tile<MODE>(g, first + r % rows, r / rows, false, lds, ep);
 }
 template <int MODE, int T>
 __global__ __launch_bounds__(F32_THREADS) void mt_linear_gemm_f32_kernel(MtGemmGroup g, MtLinearEp ep, int tiles_i, int tiles_j,
@@ -101,14 +101,15 @@ __global__ __launch_bounds__(NTHREADS) void mt_linear_wgrad_kernel(MtGemmGroup g
   tile.tj = (int16_t)(t / tiles_i);
   gemm_tile<2, NSTAGE, true>(&g, tile, 0, flags, 0, 0, 1, 0, lds, &ep);
 }
-__global__ __launch_bounds__(P8_THREADS) void mt_linear_wgrad_p8_kernel(MtGemmGroup g, MtLinearEp ep, int tiles_i, int tiles_j, int flags) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BIG_STAGE_BYTES];
+__global__ __launch_bounds__(LT_THREADS) void mt_linear_wgrad_big_kernel(MtGemmGroup g, MtLinearEp ep, int tiles_i, int tiles_j, int flags) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * BIG_STAGE_BYTES];
   const int n = tiles_i * tiles_j, per = (n + 7) / 8, t = (blockIdx.x % 8) * per + blockIdx.x / 8;
   if (t >= n) return;
   const int in_band = LINEAR_BAND * tiles_j, first = (t / in_band) * LINEAR_BAND;
   const int rows = tiles_i - first < LINEAR_BAND ? tiles_i - first : LINEAR_BAND;
   const int r = t % in_band;
-  gemm_tile_p8<2, 0, true>(g, first + r % rows, r / rows, 0, flags, 1, 0, lds, &ep);
+  const int tj = r / rows;
+  linear_tile<2>(g, first + r % rows, tj, tj == 0 && (flags & MT_GEMM_FLAG_DBIAS) && g.aux_out != nullptr, lds, ep);
 }
 template <int T>
 __global__ __launch_bounds__(F32_THREADS) void mt_linear_wgrad_f32_kernel(MtGemmGroup g, MtLinearEp ep, int tiles_i, int tiles_j,
@@ -290,6 +291,14 @@ static MtGemmGroup linear_group(const void* A, const void* B, void* C, int I, in
   g.active_steps = 1;
   return g;
 }
+// Which products take the 256-tile (us, depth 2048 unless said, 256-tile against 128-tile): those that the 512 places of the
+// 128-tile (two per CU) do not hold at once and whose edges cost less than half again as much matrix as 128-tiles would.
+//   128 tiles of 256 (4096 x 2048): 44 against 40; 136 (4352 x 2048): 44 against 59; 256: 56 against 83; 1024: 212 against 339
+//   two tiles where 128-tiles are three (65536 x 384): 111 against 134, at depth 256 34 against 32; three against five (32768 x 520): 90 against 97, at depth 256 29 against 27
+static bool linear_big(int64_t rows, int64_t cols, int64_t depth, int64_t lda, int64_t ldb) {
+  const int64_t big = ((rows + BIGT - 1) / BIGT) * ((cols + BIGT - 1) / BIGT), small = ((rows + BM - 1) / BM) * ((cols + BN - 1) / BN);
+  return lda < LT_MAX_LD && ldb < LT_MAX_LD && depth >= 4 * BK && big > 128 && 8 * big <= 3 * small;
+}
 static int linear_grid(int tiles_i, int tiles_j, int splits) { return (tiles_i * tiles_j * splits + 7) / 8 * 8; }
 
 // Few rows: as many waves per workgroup as leave each at least two unrolled groups of steps, up to about 16 waves per CU.
@@ -364,11 +373,11 @@ extern "C" int mt_linear_gemm_launch(int mode, const void* A, const void* B, con
     MtGemmGroup g = linear_group((const uint8_t*)A + (size_t)m0 * lda * es, B, (uint8_t*)C + at, m, N, KK, (int)lda, (int)ldb, N);
     MtLinearEp ep = {bias, residual ? (const uint8_t*)residual + at : nullptr, z ? (uint8_t*)z + at : nullptr,
                      splits > 1 ? part : nullptr, bias_bf16, act, N, N};
-    if (bf16 && splits == 1 && mt_p8_rule(m, N, KK, 1, 256)) {
+    if (bf16 && splits == 1 && linear_big(m, N, KK, lda, ldb)) {
       const int ti = (m + BIGT - 1) / BIGT, tj = (N + BIGT - 1) / BIGT;
-      const dim3 grid(linear_grid(ti, tj, 1)), block(P8_THREADS);
-      if (mode == 0) hipLaunchKernelGGL(mt_linear_p8_kernel<0>, grid, block, 0, stream, g, ep, ti, tj);
-      else hipLaunchKernelGGL(mt_linear_p8_kernel<1>, grid, block, 0, stream, g, ep, ti, tj);
+      const dim3 grid(linear_grid(ti, tj, 1)), block(LT_THREADS);
+      if (mode == 0) hipLaunchKernelGGL(mt_linear_big_kernel<0>, grid, block, 0, stream, g, ep, ti, tj);
+      else hipLaunchKernelGGL(mt_linear_big_kernel<1>, grid, block, 0, stream, g, ep, ti, tj);
       continue;
     }
     const int edge = linear_edge(m, N, bf16), ti = (m + edge - 1) / edge, tj = (N + edge - 1) / edge;
@@ -408,9 +417,9 @@ extern "C" int mt_linear_wgrad_launch(const void* dz, const void* x, void* dw, v
     if (db != nullptr) g.aux_out = (uint8_t*)db + (size_t)n0 * (db_bf16 ? 2 : 4);
     MtLinearEp ep = {};
     ep.bias_bf16 = db_bf16;
-    if (bf16 && mt_p8_rule(n, K, (int)M, 1, 256)) {
+    if (bf16 && linear_big(n, K, M, ld_dz, ldx)) {
       const int ti = (n + BIGT - 1) / BIGT, tj = (K + BIGT - 1) / BIGT;
-      hipLaunchKernelGGL(mt_linear_wgrad_p8_kernel, dim3(linear_grid(ti, tj, 1)), dim3(P8_THREADS), 0, stream, g, ep, ti, tj, flags);
+      hipLaunchKernelGGL(mt_linear_wgrad_big_kernel, dim3(linear_grid(ti, tj, 1)), dim3(LT_THREADS), 0, stream, g, ep, ti, tj, flags);
     } else if (bf16) {
       const int ti = (n + BM - 1) / BM, tj = (K + BN - 1) / BN;
       if (ti * tj <= 320)

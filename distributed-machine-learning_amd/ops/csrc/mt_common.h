@@ -9,6 +9,11 @@
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
+// Transposed LDS read.  The pointer is restrict because the compiler otherwise takes every LDS-DMA in flight for a writer of what
+// this reads and waits for all of them first, the next tile's among them; callers wait for the pieces that they read.
+__device__ __forceinline__ s16x4 mt_read_tr(__attribute__((address_space(3))) s16x4* __restrict p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p);
+}
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;

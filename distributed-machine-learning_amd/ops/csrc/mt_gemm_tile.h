@@ -1,6 +1,6 @@
-// Output tiles of the bf16 MFMA GEMMs (gemm.hip describes the layout): the four-wave 128 x 128 tile and the eight-wave
-// 256 x 256 tile, shared by the grouped launches of trial packs, the single-layer launches and the dense layer with its
-// activation and residual in the epilogue (linear_ep.hip).
+// Output tiles of the bf16 MFMA GEMMs (gemm.hip describes the layout): the four-wave 128 x 128 tile, shared by the grouped
+// launches of trial packs, the single-layer launches and the dense layer with its activation and residual in the epilogue
+// (linear_ep.hip), and the eight-wave 256 x 256 tile of the first two.
 #pragma once
 #include "mt_bodies.h"
 #include "mt_linear_ep.h"
@@ -69,8 +69,8 @@ __device__ __forceinline__ bf16x8 frag_mnmajor(const uint8_t* lds, int col0, int
   const int r0 = ks * 32 + g * 8 + q;
   const lds_u8* a0 = (const lds_u8*)(lds + mnmaj_off(r0, c0 + (p >> 1)) + 8 * (p & 1));
   const lds_u8* a1 = (const lds_u8*)(lds + mnmaj_off(r0 + 4, c0 + (p >> 1)) + 8 * (p & 1));
-  s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a0);
-  s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a1);
+  s16x4 lo = mt_read_tr((__attribute__((address_space(3))) s16x4*)a0);
+  s16x4 hi = mt_read_tr((__attribute__((address_space(3))) s16x4*)a1);
   typedef __attribute__((ext_vector_type(8))) short s16x8;
   s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   return __builtin_bit_cast(bf16x8, v);
@@ -472,9 +472,9 @@ __device__ __forceinline__ void p8_mma(f32x4 (&acc)[8][4], int mh, const bf16x8 
 }
 
 // One 256 x 256 tile (ti, tj) of the group; split: which part of the contraction (weight gradient only).
-template <int MODE, int SCHED, bool EP = false>
+template <int MODE, int SCHED>
 __device__ __forceinline__ void gemm_tile_p8(const MtGemmGroup& g, int ti, int tj, int split, int flags, int ksplits,
-                                             size_t split_stride, uint8_t* lds, const MtLinearEp* ep = nullptr) {
+                                             size_t split_stride, uint8_t* lds) {
   constexpr bool A_KMAJ = (MODE != 2);
   constexpr bool B_KMAJ = (MODE == 0);
   constexpr int BASE = SCHED & 1;
@@ -599,18 +599,6 @@ __device__ __forceinline__ void gemm_tile_p8(const MtGemmGroup& g, int ti, int t
 
   }
   // ------------------------------------------------------------------------------ epilogues
-  if constexpr (EP && MODE == 2) {
-    if (live) mt_linear_epilogue<8>(acc, lds + wave * 16384, qi0, qj0, g, *ep, lane);
-    if (want_db) {
-      __syncthreads();
-      float* red = reinterpret_cast<float*>(lds);
-      red[tid] = db_acc;
-      __syncthreads();
-      const int t = tid & 255, row = i0 + (tid >> 8) * 128 + t;
-      if (t < 128 && row < g.I) mt_ep_put_db(g.aux_out, row, red[tid] + red[tid + 128], ep->bias_bf16);
-    }
-    return;
-  }
   const int fq = lane >> 4, fr = lane & 15;
   if (MODE == 2) {
     float* C = reinterpret_cast<float*>(g.C) + (size_t)split * split_stride;
@@ -644,10 +632,6 @@ __device__ __forceinline__ void gemm_tile_p8(const MtGemmGroup& g, int ti, int t
     return;
   }
   if (!live) return;
-  if constexpr (EP) {
-    mt_linear_epilogue<8>(acc, lds + wave * 16384, qi0, qj0, g, *ep, lane);
-    return;
-  }
   {
     uint8_t* img = lds + wave * 16384;       // this wave's own [128][64] bf16 staging image (wave-private: no barrier)
     const bool relu = (MODE == 0) && (flags & MT_GEMM_FLAG_RELU);

@@ -146,8 +146,8 @@ template <typename T, int D> struct PaImg {
   static __device__ __forceinline__ typename PaFrag<T>::type cols(uint32_t base, int row0, int b) {
     if constexpr (sizeof(T) == 2) {
       constexpr int FAR = D == 128 ? 32 : 0;           // how the swizzle of row r + 8 differs from that of r
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(pa_lds_mut<s16x4>((base ^ (b << 6)) + row0 * ROWB));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(pa_lds_mut<s16x4>((base ^ (b << 6) ^ FAR) + (row0 + 8) * ROWB));
+      const s16x4 lo = mt_read_tr(pa_lds_mut<s16x4>((base ^ (b << 6)) + row0 * ROWB));
+      const s16x4 hi = mt_read_tr(pa_lds_mut<s16x4>((base ^ (b << 6) ^ FAR) + (row0 + 8) * ROWB));
       typedef __attribute__((ext_vector_type(8))) short s16x8;
       const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
       return __builtin_bit_cast(bf16x8, v);

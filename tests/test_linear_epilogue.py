@@ -100,6 +100,22 @@ def test_the_large_tiles(act, residual):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("act,residual,bias", [("gelu", True, True), ("relu", False, True), (None, False, False)])
+@pytest.mark.parametrize("M,K,N", [(2300, 4099, 4100), (4097, 4168, 2056), (33000, 264, 264), (264, 8400, 4104)])
+def test_every_product_on_the_256_tile(act, residual, bias, M, K, N):
+    """More than 128 tiles of 256 in the forward pass, the input gradient or the weight gradient (all three in the first two), last
+    tiles of a few rows or columns, depths that end inside a step of 64, rows of ``x`` further apart than its width."""
+    x, w, b, r, dy = _make(M, K, N, torch.bfloat16, act == "relu", residual)
+    if K % 8 == 0:
+        wide = torch.full((M, K + 24), float("nan"), device="cuda", dtype=torch.bfloat16)
+        wide[:, 8:8 + K] = x
+        x = wide[:, 8:8 + K]
+    b = b if bias else None
+    want = _formula(x, w, b, r, dy, act, True, True)
+    _check(_run(x, w, b, r, dy, act), want if bias else want[:3] + want[4:], ("y", "dx", "dw") + (("db",) if bias else ()) + ("dr",))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("act,residual", [("gelu", True), ("relu", True), (None, False)])
 @pytest.mark.parametrize("M,K,N", [(40, 2200, 70), (130, 1025, 1100), (5, 1500, 2600)])
