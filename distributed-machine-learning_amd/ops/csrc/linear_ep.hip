@@ -9,7 +9,7 @@
 // ReLU and no residual y itself is enough.  dz is one pass over dy, written with rows of whole 16-byte pieces (zeros behind
 // column N) so that both gradient GEMMs can stage it.
 #include "mt_linear_tile.h"
-#include "mt_gemm_f32_tile.h"
+#include "mt_linear_tile_f32.h"
 
 // MODE 0: A [I][KK] and B [J][KK] (forward); 1: B [KK][J] (input gradient).  A contraction may be split over workgroups: part `sp`
 // takes its share of the columns of A (and columns or rows of B) and leaves its accumulators in ep.part.
@@ -49,17 +49,13 @@ __global__ __launch_bounds__(LT_THREADS) void mt_linear_big_kernel(MtGemmGroup g
   const int r = t % in_band;
   linear_tile<MODE>(g, first + r % rows, r / rows, false, lds, ep);
 }
-template <int MODE, int T>
-__global__ __launch_bounds__(F32_THREADS) void mt_linear_gemm_f32_kernel(MtGemmGroup g, MtLinearEp ep, int tiles_i, int tiles_j,
-                                                                         int splits, int per) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * 2 * T * 128];
+template <int MODE>
+__global__ __launch_bounds__(LF_THREADS, 4) void mt_linear_gemm_f32_kernel(MtGemmGroup g, MtLinearEp ep, int tiles_i, int tiles_j,
+                                                                           int splits, int per) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[LF_LDS];
   LINEAR_PICK();
   if (splits > 1) linear_split<MODE, float>(g, ep, u % splits, per);
-  MtTile tile;
-  tile.group = 0;
-  tile.ti = (int16_t)(t / tiles_j);
-  tile.tj = (int16_t)(t % tiles_j);
-  f32_gemm_tile<MODE, 2, T, 1, 0, true>(&g, tile, 0, 0, 0, 0, 1, 0, lds, &ep);
+  linear_tile_f32<MODE>(g, t / tiles_j, t % tiles_j, false, lds, ep);
 }
 // The parts of a split contraction added in order, then the epilogue; four elements per thread.
 template <typename T>
@@ -111,17 +107,21 @@ __global__ __launch_bounds__(LT_THREADS) void mt_linear_wgrad_big_kernel(MtGemmG
   const int tj = r / rows;
   linear_tile<2>(g, first + r % rows, tj, tj == 0 && (flags & MT_GEMM_FLAG_DBIAS) && g.aux_out != nullptr, lds, ep);
 }
-template <int T>
-__global__ __launch_bounds__(F32_THREADS) void mt_linear_wgrad_f32_kernel(MtGemmGroup g, MtLinearEp ep, int tiles_i, int tiles_j,
-                                                                          int flags) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * 2 * T * 128];
-  const int n = tiles_i * tiles_j, per = (n + 7) / 8, t = (blockIdx.x % 8) * per + blockIdx.x / 8;
-  if (t >= n) return;
-  MtTile tile;
-  tile.group = 0;
-  tile.ti = (int16_t)(t / tiles_j);
-  tile.tj = (int16_t)(t % tiles_j);
-  f32_gemm_tile<2, 2, T, 1, 0, true>(&g, tile, 0, flags, 0, 0, 1, 0, lds, &ep);
+// Part `sp` of the rows; with more than one part each leaves its accumulators and column sums in a slab of its own.
+__global__ __launch_bounds__(LF_THREADS, 4) void mt_linear_wgrad_f32_kernel(MtGemmGroup g, MtLinearEp ep, int tiles_i, int tiles_j,
+                                                                            int splits, int per, int64_t slab) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[LF_LDS];
+  LINEAR_PICK();
+  if (splits > 1) {
+    const int sp = u % splits, k0 = sp * per;
+    g.A = reinterpret_cast<const float*>(g.A) + (size_t)k0 * g.lda;
+    g.B = reinterpret_cast<const float*>(g.B) + (size_t)k0 * g.ldb;
+    g.KK = g.KK - k0 < per ? g.KK - k0 : per;
+    ep.part += sp * slab;
+    if (g.aux_out != nullptr) g.aux_out = reinterpret_cast<float*>(g.aux_out) + sp * slab;
+  }
+  const int tj = t % tiles_j;
+  linear_tile_f32<2>(g, t / tiles_j, tj, tj == 0 && g.aux_out != nullptr, lds, ep);
 }
 
 // A few rows (at most 16 MT): the weight is streamed once, straight from memory into the matrix instruction's operand.  A
@@ -319,15 +319,11 @@ static void linear_few(const void* x, const void* w, const MtLinearEp& ep, void*
 }
 #define LINEAR_FEW_ROWS 32
 
-// Tile edge of an f32 launch: 128 from four 128-tiles per CU on (4096^3: 1030 us against 1110 with 64; 12800 x 2048 x 512: 276 / 286),
-// 64 below, where fewer, longer tiles leave CUs idle at the end (25600 x 512 x 512: 130 us against 151).  And how many parts the contraction of a launch is split into: launches of at most half as many tiles
-// as the chip has CUs, whose contraction is long enough to leave every part 512 deep.
-static int linear_edge(int64_t M, int N, int bf16) {
-  if (bf16) return 128;
-  return ((M + 127) / 128) * ((N + 127) / 128) >= 1024 ? 128 : 64;
-}
+// Tile edge of a launch that does not take the 256-tile, and how many parts its contraction is split into: launches of at most half
+// as many tiles as the chip has CUs, whose contraction is long enough to leave every part 512 deep.
+static int linear_edge(int bf16) { return bf16 ? BM : LF_TILE; }
 static int linear_splits(int mode, int64_t M, int N, int KK, int bf16, int* per) {
-  const int edge = linear_edge(M, N, bf16), step = bf16 ? BK : F32_BK;
+  const int edge = linear_edge(bf16), step = bf16 ? BK : LF_BK;
   const int64_t tiles = ((M + edge - 1) / edge) * ((N + edge - 1) / edge);
   *per = KK;
   if ((mode == 0 && M <= LINEAR_FEW_ROWS) || M > LINEAR_ROWS || tiles > 128) return 1;
@@ -353,7 +349,7 @@ extern "C" int mt_linear_gemm_launch(int mode, const void* A, const void* B, con
   const int per16 = bf16 ? 8 : 4, es = bf16 ? 2 : 4;
   if (mode < 0 || mode > 1 || M < 0 || N < 1 || KK < 1 || lda % per16 || ldb % per16 || lda < KK || ldb < (mode == 0 ? KK : N)) return -2;
   if (mode == 0 && KK % per16) return -2;
-  if (lda > (1 << 28) || ldb > (1 << 28) || N > 2000000 || act < 0 || act > 2) return -2;
+  if (lda > (bf16 ? 1 << 28 : LF_MAX_LD - 1) || ldb > (bf16 ? 1 << 28 : LF_MAX_LD - 1) || N > 2000000 || act < 0 || act > 2) return -2;
   if ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B)) & 15) return -2;
   if (M == 0) return 0;
   if (mode == 0 && M <= LINEAR_FEW_ROWS) {
@@ -380,17 +376,15 @@ extern "C" int mt_linear_gemm_launch(int mode, const void* A, const void* B, con
       else hipLaunchKernelGGL(mt_linear_big_kernel<1>, grid, block, 0, stream, g, ep, ti, tj);
       continue;
     }
-    const int edge = linear_edge(m, N, bf16), ti = (m + edge - 1) / edge, tj = (N + edge - 1) / edge;
+    const int edge = linear_edge(bf16), ti = (m + edge - 1) / edge, tj = (N + edge - 1) / edge;
     const dim3 grid(linear_grid(ti, tj, splits)), block(256);
 #define GO(K, ...) hipLaunchKernelGGL((K<__VA_ARGS__>), grid, block, 0, stream, g, ep, ti, tj, splits, per)
     if (bf16) {
       const bool deep = ti * tj * splits <= 320;      // a workgroup or less per CU: four stages, else two workgroups of two
       if (mode == 0) { if (deep) GO(mt_linear_gemm_kernel, 0, 4); else GO(mt_linear_gemm_kernel, 0, 2); }
       else { if (deep) GO(mt_linear_gemm_kernel, 1, 4); else GO(mt_linear_gemm_kernel, 1, 2); }
-    } else if (edge == 128) {
-      if (mode == 0) GO(mt_linear_gemm_f32_kernel, 0, 128); else GO(mt_linear_gemm_f32_kernel, 1, 128);
     } else {
-      if (mode == 0) GO(mt_linear_gemm_f32_kernel, 0, 64); else GO(mt_linear_gemm_f32_kernel, 1, 64);
+      if (mode == 0) GO(mt_linear_gemm_f32_kernel, 0); else GO(mt_linear_gemm_f32_kernel, 1);
     }
 #undef GO
     if (splits > 1) {
@@ -403,6 +397,27 @@ extern "C" int mt_linear_gemm_launch(int mode, const void* A, const void* B, con
   return (int)hipGetLastError();
 }
 
+static void linear_wgrad_f32(const MtGemmGroup& g, const MtLinearEp& ep, int splits, int64_t slab, hipStream_t stream) {
+  const int ti = (g.I + LF_TILE - 1) / LF_TILE, tj = (g.J + LF_TILE - 1) / LF_TILE;
+  const int per = ((g.KK + splits - 1) / splits + LF_BK - 1) / LF_BK * LF_BK;
+  hipLaunchKernelGGL(mt_linear_wgrad_f32_kernel, dim3(linear_grid(ti, tj, splits)), dim3(LF_THREADS), 0, stream, g, ep, ti, tj, splits,
+                     per, slab);
+}
+
+// f32 parts of dW [N][K] and db [N] of dz [M][N] and x [M][K], contiguous with widths of whole 16-byte pieces: part s takes its share
+// of the rows and leaves dW at arena + s slab, db behind it.
+extern "C" int mt_linear_wgrad_f32_parts_launch(const void* dz, const void* x, float* arena, int64_t M, int N, int K, int splits,
+                                                int64_t slab, int with_bias, hipStream_t stream) {
+  if (M < 1 || M > 0x7FFFFFFF - 256 || N < 1 || K < 1 || N % 4 || K % 4 || N >= LF_MAX_LD || K >= LF_MAX_LD) return -2;
+  if (splits < 2 || splits > 127 || slab % 4 || slab < (int64_t)N * K + (with_bias ? N : 0)) return -2;
+  MtGemmGroup g = linear_group(dz, x, arena, N, K, (int)M, N, K, K);
+  if (with_bias) g.aux_out = arena + (int64_t)N * K;
+  MtLinearEp ep = {};
+  ep.part = arena;
+  linear_wgrad_f32(g, ep, splits, slab, stream);
+  return (int)hipGetLastError();
+}
+
 // dW [N][K] and db [N] (may be null) of dz [M][ld_dz] and x [M][ldx], without a split of the contraction: the widths are multiples of
 // a 16-byte piece (what lies behind N and K is zeros or not stored), the gradients contiguous and of the given types.
 extern "C" int mt_linear_wgrad_launch(const void* dz, const void* x, void* dw, void* db, int64_t M, int N, int K, int ld_dz, int ldx,
@@ -410,7 +425,8 @@ extern "C" int mt_linear_wgrad_launch(const void* dz, const void* x, void* dw, v
   const int per = bf16 ? 8 : 4, es = bf16 ? 2 : 4;
   if (M < 1 || M > 0x7FFFFFFF - 256 || N < 1 || K < 1 || ld_dz % per || ldx % per || ld_dz < N || ldx < K) return -2;
   const int flags = db != nullptr ? MT_GEMM_FLAG_DBIAS : 0;
-  const int most = 255 * (bf16 ? 128 : 64);            // output rows of a launch: their tile numbers are 8 bits
+  if (!bf16 && (ld_dz >= LF_MAX_LD || ldx >= LF_MAX_LD)) return -2;
+  const int most = bf16 ? 255 * BM : N;                // output rows of a launch: the 128-tile's numbers are 8 bits here
   for (int n0 = 0; n0 < N; n0 += most) {
     const int n = N - n0 < most ? N - n0 : most;
     MtGemmGroup g = linear_group((const uint8_t*)dz + (size_t)n0 * es, x, (uint8_t*)dw + (size_t)n0 * K * es, n, K, (int)M, ld_dz, ldx, K);
@@ -427,8 +443,7 @@ extern "C" int mt_linear_wgrad_launch(const void* dz, const void* x, void* dw, v
       else
         hipLaunchKernelGGL(mt_linear_wgrad_kernel<2>, dim3(linear_grid(ti, tj, 1)), dim3(NTHREADS), 0, stream, g, ep, ti, tj, flags);
     } else {
-      const int ti = (n + 63) / 64, tj = (K + 63) / 64;
-      hipLaunchKernelGGL(mt_linear_wgrad_f32_kernel<64>, dim3(linear_grid(ti, tj, 1)), dim3(F32_THREADS), 0, stream, g, ep, ti, tj, flags);
+      linear_wgrad_f32(g, ep, 1, 0, stream);
     }
   }
   return (int)hipGetLastError();

@@ -4,7 +4,6 @@
 // trial's numbers are bit for bit the same on either path.
 #pragma once
 #include "mt_bodies.h"
-#include "mt_linear_ep.h"
 #define F32_BK 32
 #define F32_THREADS 256
 
@@ -181,11 +180,10 @@ __device__ __forceinline__ void f32_wait_ahead(int ahead) {
 // One T x T output tile.  ksplits > 1 (wgrad only): tile.ti carries the split index in bits 8..14.
 // PROD: 0 = every product an f32 fused multiply-add (v_mfma_f32_16x16x4_f32); 1 = operands rounded to bf16 for the matrix
 // instruction (f32_mma_stage_bf16).
-// EP: the dense layer's epilogue (linear_ep.hip) in place of the flags'; rows of the output need no alignment.
-template <int MODE, int NSTAGE, int T, int KU = 1, int PROD = 0, bool EP = false>
+template <int MODE, int NSTAGE, int T, int KU = 1, int PROD = 0>
 __device__ __forceinline__ void f32_gemm_tile(const MtGemmGroup* __restrict__ groups, const MtTile tile, int step,
                                               int flags, int arow0, int i_override, int ksplits, size_t split_stride,
-                                              uint8_t* lds, const MtLinearEp* ep = nullptr) {
+                                              uint8_t* lds) {
   constexpr bool A_KMAJ = (MODE != 2);
   constexpr bool B_KMAJ = (MODE == 0);
   constexpr int R = T / 32, W = T / 2;
@@ -286,7 +284,7 @@ __device__ __forceinline__ void f32_gemm_tile(const MtGemmGroup* __restrict__ gr
 
   // ------------------------------------------------------------------------------ epilogues
   const int fq = lane >> 4, fr = lane & 15;
-  if (MODE == 2 && !EP) {
+  if (MODE == 2) {
     float* C = reinterpret_cast<float*>(g.C) + (size_t)split * split_stride;
 #pragma unroll
     for (int m = 0; m < R; ++m) {
@@ -315,58 +313,6 @@ __device__ __forceinline__ void f32_gemm_tile(const MtGemmGroup* __restrict__ gr
     return;
   }
 
-  if constexpr (EP) {
-#pragma unroll
-    for (int n = 0; n < R; ++n) {
-      const int col = j0 + wc * W + n * 16 + fq * 4;
-      f32x4 bb = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (ep->bias != nullptr && col + j < g.J) bb[j] = mt_ep_bias(*ep, col + j);
-#pragma unroll
-      for (int m = 0; m < R; ++m) {
-        const int row = i0 + wr * W + m * 16 + fr;
-        if (row >= g.I || col >= g.J) continue;
-        if (ep->part != nullptr) {
-          mt_ep_put_part(ep->part, row, col, g.J, acc[m][n]);
-          continue;
-        }
-        const bool whole = col + 4 <= g.J;
-        f32x4 v = acc[m][n] + bb;
-        auto put = [&](void* base, int ld) {
-          float* p = reinterpret_cast<float*>(base) + (size_t)row * ld + col;
-          if (whole) __builtin_memcpy(p, &v, 16);
-          else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (col + j < g.J) p[j] = v[j];
-          }
-        };
-        if (ep->z != nullptr) put(ep->z, ep->ldz);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = mt_ep_act<false>(v[j], ep->act);
-        if (ep->residual != nullptr) {
-          const float* p = reinterpret_cast<const float*>(ep->residual) + (size_t)row * ep->ldr + col;
-          f32x4 r = {0.f, 0.f, 0.f, 0.f};
-          if (whole) __builtin_memcpy(&r, p, 16);
-          else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (col + j < g.J) r[j] = p[j];
-          }
-          v += r;
-        }
-        put(g.C, g.ldc);
-      }
-    }
-    if (want_db) {
-      float* red = reinterpret_cast<float*>(lds);    // all waves are past the last K-step barrier
-      red[tid] = db_acc;
-      __syncthreads();
-      if (tid < T && i0 + tid < g.I) mt_ep_put_db(g.aux_out, i0 + tid, red[tid] + red[tid + T], ep->bias_bf16);
-    }
-    return;
-  }
   const bool relu = (MODE == 0) && ((flags & MT_GEMM_FLAG_RELU) || (g.gflags & MT_GROUP_ACT));
   const bool add = (MODE == 1) && (g.gflags & MT_GROUP_ADD) && g.aux != nullptr;
   const bool masked = (MODE == 1) && !add && ((flags & MT_GEMM_FLAG_MASK) || (g.gflags & MT_GROUP_ACT)) && g.aux != nullptr;

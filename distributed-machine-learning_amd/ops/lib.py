@@ -245,7 +245,8 @@ def load(build_if_missing: bool = True) -> C.CDLL:
     lib.mt_linear_wsum_launch.argtypes = [c_void_p] * 3 + [C.c_int64, C.c_int, C.c_int, C.c_int64, C.c_int, C.c_int64, C.c_int,
                                                            C.c_int, c_void_p]
     lib.mt_linear_wgrad_launch.argtypes = [c_void_p] * 4 + [C.c_int64] + [C.c_int] * 6 + [c_void_p]
-    for fn in (lib.mt_linear_parts, lib.mt_linear_gemm_launch, lib.mt_linear_act_parts, lib.mt_linear_act_bwd_launch, lib.mt_linear_wgrad_launch, lib.mt_linear_wsum_launch):
+    lib.mt_linear_wgrad_f32_parts_launch.argtypes = ([c_void_p] * 3 + [C.c_int64] + [C.c_int] * 3 + [C.c_int64, C.c_int, c_void_p])
+    for fn in (lib.mt_linear_wgrad_f32_parts_launch, lib.mt_linear_parts, lib.mt_linear_gemm_launch, lib.mt_linear_act_parts, lib.mt_linear_act_bwd_launch, lib.mt_linear_wgrad_launch, lib.mt_linear_wsum_launch):
         fn.restype = C.c_int
     lib.mt_norm_bwd_parts.argtypes = [C.c_int64, C.c_int, C.c_int]
     lib.mt_norm_fwd_launch.argtypes = [c_void_p] * 5 + [C.c_int64, C.c_int64, C.c_int, c_float, C.c_int, C.c_int, c_void_p]

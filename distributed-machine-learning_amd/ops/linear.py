@@ -482,7 +482,7 @@ def _weight_grad(so, dz, xc, out_f: int, in_f: int, w_dtype, b_dtype, stream):
     xc = xc if xc.stride(0) == width else xc.contiguous()
     bf16 = dz.dtype == torch.bfloat16
     tile = 128 if bf16 else 64
-    most = 255 * tile                               # output rows of a launch: its tile rows are 8 bits
+    most = 255 * tile if bf16 else rows             # output rows of a launch: its tile rows are 8 bits
     dw = torch.empty(out_f, in_f, device=dz.device, dtype=w_dtype)
     db = torch.empty(out_f, device=dz.device, dtype=b_dtype) if b_dtype is not None else None
     if w_dtype == dz.dtype and _fused_wgrad_splits(M, -(-min(rows, most) // tile) * -(-width // tile), bf16) == 1:
@@ -505,8 +505,8 @@ def _weight_grad(so, dz, xc, out_f: int, in_f: int, w_dtype, b_dtype, stream):
                                               arena.data_ptr() + n * width * 4 if db is not None else None, M, n, width, splits,
                                               slab, stream), "mt_wgrad_single_launch")
         else:
-            L.check(so.mt_wgrad_f32_single_launch(part.data_ptr(), xc.data_ptr(), arena.data_ptr(), M, n, width, splits, slab,
-                                                  int(db is not None), stream), "mt_wgrad_f32_single_launch")
+            L.check(so.mt_linear_wgrad_f32_parts_launch(part.data_ptr(), xc.data_ptr(), arena.data_ptr(), M, n, width, splits, slab,
+                                                        int(db is not None), stream), "mt_linear_wgrad_f32_parts_launch")
         L.check(so.mt_linear_wsum_launch(arena.data_ptr(), dw[i * most:].data_ptr(), db[i * most:].data_ptr() if db is not None else None,
                                          real, in_f, width, n * width, splits, slab, int(w_dtype == torch.bfloat16),
                                          int(b_dtype == torch.bfloat16), stream), "mt_linear_wsum_launch")
