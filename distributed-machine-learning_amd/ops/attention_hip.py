@@ -219,8 +219,8 @@ def packed_forward(q, k, v, pack, causal: bool, scale: float, keeps: bool):
     q, k, v = _in_place(q), _in_place(k), _in_place(v)
     out = torch.empty(pack.rows, q.shape[1], v.shape[2], device=q.device, dtype=q.dtype)
     lse = torch.empty(q.shape[1], pack.rows, device=q.device, dtype=torch.float32) if keeps else None
-    # what rounding took off the outputs of short sequences, whose gradients would show it
-    low = torch.empty_like(out) if keeps and q.dtype == torch.bfloat16 and pack.shortest <= L.PACKED_LOW_ROWS else None
+    # what rounding took off the outputs of rows that see few keys, whose gradients would show it
+    low = torch.empty_like(out) if keeps and q.dtype == torch.bfloat16 and (causal or pack.shortest <= L.PACKED_LOW_ROWS) else None
     _packed_launch(so, pack, q, k, v, causal, scale, 0, o=out.data_ptr(), low=low.data_ptr() if low is not None else 0,
                    lse=lse.data_ptr() if keeps else 0)
     return (out if v.shape[2] == dv else out[..., :dv].contiguous()), (q, k, v, out, low, lse)

@@ -42,7 +42,7 @@ struct MtPackedAttn {
   const void *q, *k, *v;        // inputs, element strides below; the last dimension is contiguous
   const void *out, *dout;       // backward only: forward output (contiguous) and its gradient
   void *o, *dq, *dk, *dv;       // outputs, contiguous [T][heads or kv_heads][dk or dv]
-  void* low;                    // bf16 [T][heads][dv]: what rounding took off the output's rows of short sequences; may be null
+  void* low;                    // bf16 [T][heads][dv]: what rounding took off the output's rows of few keys; may be null
   float *lse, *delta;           // [heads][rows]
   const MtSeqItem *items, *kv_items;      // items of query rows and of key rows; null: count sequences of uniform_len rows each
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, do_row, do_head;
@@ -298,10 +298,14 @@ __device__ __forceinline__ void pa_join_store(T* base, int64_t row_stride, const
     pa_store4(base + r * row_stride + c, low != nullptr ? low + r * row_stride + c : nullptr, v[0], v[1], v[2], v[3]);
   }
 }
-// Sequences whose output is kept with what its rounding took off (MtPackedAttn::low): over few keys D = do . o is as large as the
-// do . v it is subtracted from, and half a bf16 step of o would show in the gradients (two keys: 0.8 % of dq against 0.23 %).
+// Rows whose output is kept with what its rounding took off (MtPackedAttn::low), those that see at most 128 keys: over few keys
+// D = do . o is as large as the do . v it is subtracted from, and half a bf16 step of o would show in the gradients (two keys: 0.8 %
+// of dq against 0.23 %; causal sequences of up to 2048, whose first rows have the largest gradients: 0.25 against 0.24).  `first`:
+// the first of the item's rows, all of which are on the same side of 128.
 #define PA_LOW_ROWS 128
-__device__ __forceinline__ bool pa_low(const MtPackedAttn& p, int len) { return p.low != nullptr && len <= PA_LOW_ROWS; }
+__device__ __forceinline__ bool pa_low(const MtPackedAttn& p, int len, int first) {
+  return p.low != nullptr && (len <= PA_LOW_ROWS || (p.causal && first < PA_LOW_ROWS));
+}
 // What the dq kernels hold of an owned row: q, do, L and D = do . o (stored for the dk / dv kernel by the waves with `store`).
 template <typename T, int DK, int DV>
 __device__ __forceinline__ void pa_dq_rows(const MtPackedAttn& p, typename PaFrag<T>::type (&qf)[DK / 16],
@@ -349,7 +353,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void mt_pattn_fwd_kernel(const MtPac
   const MtSeqItem item = pa_item(p, p.items, it, 0, p.causal);
   const int64_t o_row = (int64_t)p.heads * p.head_v;
   T* o = reinterpret_cast<T*>(p.o) + item.row0 * o_row + (int64_t)head * p.head_v;
-  T* low = sizeof(T) == 2 && pa_low(p, item.len) ? reinterpret_cast<T*>(p.low) + item.row0 * o_row + (int64_t)head * p.head_v : nullptr;
+  T* low = sizeof(T) == 2 && pa_low(p, item.len, item.first) ? reinterpret_cast<T*>(p.low) + item.row0 * o_row + (int64_t)head * p.head_v : nullptr;
   if (item.len <= 0) {
     pa_zero_rows<T>(o, o_row, -item.len, p.head_v);
     return;
@@ -505,7 +509,7 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
   const bool ok = mine < item.len;
   Frag qf[D / 16], df[D / 16];
   float delta, lse;
-  pa_dq_rows<T, D, D>(p, qf, df, delta, lse, item.row0 + (int64_t)mine, head, ok, true, pa_low(p, item.len), lane);
+  pa_dq_rows<T, D, D>(p, qf, df, delta, lse, item.row0 + (int64_t)mine, head, ok, true, pa_low(p, item.len, item.first), lane);
   const T* kb = reinterpret_cast<const T*>(p.k) + item.row0 * p.k_row + (int64_t)kvh * p.k_head;
   const T* vb = reinterpret_cast<const T*>(p.v) + item.row0 * p.v_row + (int64_t)kvh * p.v_head;
   const int keys = p.causal && item.first + PA_OWN < item.len ? item.first + PA_OWN : item.len;
@@ -856,7 +860,7 @@ __global__ __launch_bounds__(PA_THREADS, (PaSplit<T, DK, DV>::WAVES)) void mt_pa
   const MtSeqItem item = pa_item(p, p.items, it, p.split, p.causal);
   const int64_t o_row = (int64_t)p.heads * p.head_v;
   T* o = reinterpret_cast<T*>(p.o) + item.row0 * o_row + (int64_t)head * p.head_v;
-  T* low = sizeof(T) == 2 && pa_low(p, item.len) ? reinterpret_cast<T*>(p.low) + item.row0 * o_row + (int64_t)head * p.head_v : nullptr;
+  T* low = sizeof(T) == 2 && pa_low(p, item.len, item.first) ? reinterpret_cast<T*>(p.low) + item.row0 * o_row + (int64_t)head * p.head_v : nullptr;
   if (item.len <= 0) {
     pa_zero_rows<T>(o, o_row, -item.len, p.head_v);
     return;
@@ -986,7 +990,7 @@ __global__ __launch_bounds__(PA_THREADS, (PaSplit<T, DK, DV>::WAVES)) void mt_pa
   Frag qf[DK / 16], df[DV / 16];
   float delta, lse;
   pa_dq_rows<T, DK, DV>(p, qf, df, delta, lse, item.row0 + (int64_t)mine, head, mine < item.len, item.solo || wave == 0,
-                        pa_low(p, item.len), lane);
+                        pa_low(p, item.len, item.first), lane);
   const T* kb = reinterpret_cast<const T*>(p.k) + item.row0 * p.k_row + (int64_t)kvh * p.k_head;
   const T* vb = reinterpret_cast<const T*>(p.v) + item.row0 * p.v_row + (int64_t)kvh * p.v_head;
   const int keys = p.causal && first + 32 < item.len ? first + 32 : item.len;
