@@ -162,7 +162,8 @@ class SequencePack:
 
     Made once per batch and used by every layer and both passes: the lengths are checked on the host, and the list of
     pieces the kernels work through, longest first, is laid out on ``device`` (default: the current GPU if there is
-    one).  ``SequencePack.uniform(count, length)`` is ``count`` sequences of one length; it needs no list."""
+    one); a captured graph reads that list, so the pack has to live as long as the graph.
+    ``SequencePack.uniform(count, length)`` is ``count`` sequences of one length; it needs no list."""
 
     def __init__(self, lengths: Union[Sequence[int], np.ndarray, torch.Tensor], rows: Optional[int] = None, device=None):
         if isinstance(lengths, torch.Tensor):
@@ -271,8 +272,8 @@ def packed_attention_reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pack: SequencePack, causal: bool = False,
                      scale: Optional[float] = None) -> torch.Tensor:
     """Softmax attention within every sequence of ``pack``: ``q`` [rows, heads, dk], ``k`` [rows, kv_heads, dk], ``v``
-    [rows, kv_heads, dv] -> [rows, heads, dv], all f32 or all bf16, differentiable.  Query head ``i`` reads key / value head
-    ``i // (heads // kv_heads)``; with ``causal`` a row sees its sequence's rows up to itself.  ``scale`` defaults to
+    [rows, kv_heads, dv] -> [rows, heads, dv], all f32 or all bf16, differentiable (a second time too, through
+    plain torch).  Query head ``i`` reads key / value head ``i // (heads // kv_heads)``; with ``causal`` a row sees its sequence's rows up to itself.  ``scale`` defaults to
     ``1 / sqrt(dk)``.  Rows behind the last sequence give zeros, and nothing of what they hold is used.
 
     On a GPU: heads of at most 128 elements.  Operands may be strided (a slice of a fused projection is read in place when its
@@ -304,8 +305,11 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pack: Se
         raise ValueError(f"packed_attention on a GPU takes heads of at most {PACKED_MAX_HEAD_DIM} elements, got {max(dk, dv)}")
     if pack.device != q.device:
         raise ValueError(f"the pack lies on {pack.device}, the operands on {q.device}")
-    from .attention_hip import PackedAttention, packed_forward
+    from .attention_hip import PackedAttention, in_place, packed_forward
     from .lib import wants_grad
+    q, k, v = in_place(q), in_place(k), in_place(v)
     if wants_grad(q, k, v):
-        return PackedAttention.apply(q, k, v, pack, bool(causal), scale)
-    return packed_forward(q, k, v, pack, bool(causal), scale, False)[0]
+        out = PackedAttention.apply(q, k, v, pack, bool(causal), scale)
+    else:
+        out = packed_forward(q, k, v, pack, bool(causal), scale, False)[0]
+    return out if v.shape[2] == dv else out[..., :dv].contiguous()

@@ -165,7 +165,7 @@ class FusedSelfAttention(torch.autograd.Function):
         return dqk, dv_, None, None, None, None, None
 
 
-def _in_place(t: torch.Tensor) -> torch.Tensor:
+def in_place(t: torch.Tensor) -> torch.Tensor:
     """``t`` [rows, heads, width] as the packed kernels can read it: 16-byte rows and heads, or else a copy padded with zero
     columns to that (zeros add nothing to a score; zero value columns give output columns that are cut off again)."""
     es = t.element_size()
@@ -213,25 +213,23 @@ def _packed_launch(so, pack, q, k, v, causal: bool, scale: float, backward: int,
 
 
 def packed_forward(q, k, v, pack, causal: bool, scale: float, keeps: bool):
-    """(output, what a backward pass needs)."""
+    """(output, what a backward pass needs) of operands as ``in_place`` leaves them."""
     so = L.load()
-    dv = v.shape[2]
-    q, k, v = _in_place(q), _in_place(k), _in_place(v)
     out = torch.empty(pack.rows, q.shape[1], v.shape[2], device=q.device, dtype=q.dtype)
     lse = torch.empty(q.shape[1], pack.rows, device=q.device, dtype=torch.float32) if keeps else None
     # what rounding took off the outputs of rows that see few keys, whose gradients would show it
     low = torch.empty_like(out) if keeps and q.dtype == torch.bfloat16 and (causal or pack.shortest <= L.PACKED_LOW_ROWS) else None
     _packed_launch(so, pack, q, k, v, causal, scale, 0, o=out.data_ptr(), low=low.data_ptr() if low is not None else 0,
                    lse=lse.data_ptr() if keeps else 0)
-    return (out if v.shape[2] == dv else out[..., :dv].contiguous()), (q, k, v, out, low, lse)
+    return out, (q, k, v, out, low, lse)
 
 
 class PackedAttention(torch.autograd.Function):
-    """``ops.attention.packed_attention`` on a GPU; operands checked there."""
+    """``ops.attention.packed_attention`` on a GPU; operands checked and laid out there."""
 
     @staticmethod
     def forward(ctx, q, k, v, pack, causal: bool, scale: float):
-        ctx.pack, ctx.meta = pack, (causal, scale, q.shape[2], v.shape[2])
+        ctx.pack, ctx.meta = pack, (causal, scale)
         out, saved = packed_forward(q, k, v, pack, causal, scale, True)
         ctx.save_for_backward(*saved)
         return out
@@ -240,12 +238,15 @@ class PackedAttention(torch.autograd.Function):
     def backward(ctx, grad_out):
         so = L.load()
         q, k, v, out, low, lse = ctx.saved_tensors
-        pack, (causal, scale, dk, dv) = ctx.pack, ctx.meta
-        do = _in_place(grad_out if grad_out.dtype == q.dtype else grad_out.to(q.dtype))
+        pack, (causal, scale) = ctx.pack, ctx.meta
+        if torch.is_grad_enabled():
+            from .attention import packed_attention_reference
+            plain = lambda *t: packed_attention_reference(*(u.float() for u in t), pack, causal, scale).to(q.dtype)     # noqa: E731
+            return (*L.grads_by_formula(plain, (q, k, v), grad_out), None, None, None)
+        do = in_place(grad_out if grad_out.dtype == q.dtype else grad_out.to(q.dtype))
         delta = torch.empty_like(lse)
         grads = [torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v)]
         _packed_launch(so, pack, q, k, v, causal, scale, 1, out=out.data_ptr(), dout=do, dq=grads[0].data_ptr(),
                        dk=grads[1].data_ptr(), dv=grads[2].data_ptr(), low=low.data_ptr() if low is not None else 0,
                        lse=lse.data_ptr(), delta=delta.data_ptr())
-        gq, gk, gv = (g if g.shape[2] == w else g[..., :w].contiguous() for g, w in zip(grads, (dk, dk, dv)))
-        return gq, gk, gv, None, None, None
+        return (*grads, None, None, None)

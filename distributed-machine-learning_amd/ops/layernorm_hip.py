@@ -5,6 +5,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+import torch.nn.functional as F
 
 from . import lib as L
 
@@ -157,17 +158,21 @@ class LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps: float):
         y, xr, w, stats, flags = norm_forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(xr, w, stats)
+        ctx.save_for_backward(xr, w, stats, x, weight, bias)
         param = weight if weight is not None else bias
-        ctx.meta = (x.shape, flags, weight is not None, bias is not None, param.dtype if param is not None else None)
+        ctx.meta = (x.shape, flags, weight is not None, bias is not None, param.dtype if param is not None else None, eps)
         return y
 
     @staticmethod
     def backward(ctx, grad_y):
         so = L.load()
-        xr, w, stats = ctx.saved_tensors
-        shape, flags, has_w, has_b, pdtype = ctx.meta
+        xr, w, stats, *inputs = ctx.saved_tensors
+        shape, flags, has_w, has_b, pdtype, eps = ctx.meta
         M, d = xr.shape
+        if torch.is_grad_enabled():
+            cast = lambda t: None if t is None else t.float()                                              # noqa: E731
+            plain = lambda x, w, b: F.layer_norm(x.float(), (d,), cast(w), cast(b), eps).to(x.dtype)      # noqa: E731
+            return (*L.grads_by_formula(plain, inputs, grad_y), None)
         dy = _rows(grad_y if grad_y.dtype == xr.dtype else grad_y.to(xr.dtype))
         dx = torch.empty(shape, device=xr.device, dtype=xr.dtype)
         want_w, want_b = has_w and ctx.needs_input_grad[1], has_b and ctx.needs_input_grad[2]

@@ -385,3 +385,13 @@ def wants_grad(*tensors) -> bool:
     which halves the host time of a small call."""
     import torch
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def grads_by_formula(formula, inputs, grad):
+    """Gradients of ``formula(*inputs)`` (plain torch) that can be differentiated again, for backward passes under
+    ``create_graph``; the kernels' own backward passes leave no graph."""
+    import torch
+    wanted = [t for t in inputs if t is not None and t.requires_grad]
+    with torch.enable_grad():
+        got = iter(torch.autograd.grad(formula(*inputs), wanted, grad, create_graph=True))
+    return [next(got) if t is not None and t.requires_grad else None for t in inputs]

@@ -342,11 +342,12 @@ class SmallLinear(torch.autograd.Function):
 
 
 def _pieces(t: torch.Tensor) -> torch.Tensor:
-    """``t`` [rows, columns] with rows of whole 16-byte pieces: itself when its rows start on such a boundary and its width is a
-    multiple of one, else a copy padded with zero columns."""
+    """``t`` [rows, columns] with rows of whole 16-byte pieces: itself when its rows start on such a boundary (less than 2^24 elements
+    apart) and its width is a multiple of one, else a copy padded with zero columns."""
     per = 16 // t.element_size()
     pad = -t.shape[1] % per
-    if pad == 0 and t.stride(1) == 1 and t.stride(0) % per == 0 and t.data_ptr() % 16 == 0 and t.stride(0) >= t.shape[1]:
+    if (pad == 0 and t.stride(1) == 1 and t.stride(0) % per == 0 and t.data_ptr() % 16 == 0
+            and t.shape[1] <= t.stride(0) < 1 << 24):
         return t
     return F.pad(t, (0, pad)).contiguous() if pad else t.clone(memory_format=torch.contiguous_format)
 
@@ -400,7 +401,7 @@ class FusedLinear(torch.autograd.Function):
         keep_z = backward and act != 0 and not (act == 1 and residual is None)
         y, xc, wc, z = fused_forward(x, weight, bias, residual, act, w16, keep_z)
         if backward:
-            ctx.save_for_backward(xc, wc, z if keep_z else y if act else None)
+            ctx.save_for_backward(xc, wc, z if keep_z else y if act else None, x, weight, bias)
         ctx.meta = (act, x.shape, weight.shape[1], weight.dtype, bias.dtype if bias is not None else None,
                     residual.shape if residual is not None else None)
         return y
@@ -412,7 +413,12 @@ class FusedLinear(torch.autograd.Function):
         act, x_shape, in_f, w_dtype, b_dtype, r_shape = ctx.meta
         dx = dw = db = None
         if any(ctx.needs_input_grad[:3]):
-            xc, wc, s = ctx.saved_tensors
+            xc, wc, s, *inputs = ctx.saved_tensors
+            if torch.is_grad_enabled():
+                name = next(n for n, number in ACTIVATIONS.items() if number == act)
+                cast = lambda t: None if t is None else t.float()                                              # noqa: E731
+                plain = lambda x, w, b: _plain_fused(x.float(), w.float(), cast(b), name, None).to(x.dtype)    # noqa: E731
+                return (*L.grads_by_formula(plain, inputs, dy), dy if r_shape is not None else None, None, None)
             out_f = wc.shape[0]
             bf16, dev, M = xc.dtype == torch.bfloat16, xc.device, xc.shape[0]
             per = 8 if bf16 else 4

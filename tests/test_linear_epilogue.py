@@ -116,6 +116,20 @@ def test_every_product_on_the_256_tile(act, residual, bias, M, K, N):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,M,K,N", [(torch.bfloat16, 4097, 4168, 2056), (torch.float32, 3001, 1000, 520)])
+def test_results_repeat(dtype, M, K, N):
+    """The same bits every time, and the same for a part of the rows on another tile: products are summed in one order."""
+    x, w, b, r, dy = _make(M, K, N, dtype, False)
+    first = _run(x, w, b, r, dy, "gelu")
+    for _ in range(8):
+        for u, v in zip(first, _run(x, w, b, r, dy, "gelu")):
+            assert torch.equal(u, v)
+    few = 900
+    part = _run(x[:few], w, b, r[:few], dy[:few], "gelu")
+    assert torch.equal(part[0], first[0][:few]) and torch.equal(part[1], first[1][:few])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("act,residual", [("gelu", True), ("relu", True), (None, False)])
 @pytest.mark.parametrize("M,K,N", [(40, 2200, 70), (130, 1025, 1100), (5, 1500, 2600)])

@@ -135,3 +135,41 @@ def test_residual_norms_outside_the_fused_kernels(dtype, d):
     assert torch.allclose(y.double(), ref, rtol=2 * torch.finfo(dtype).eps, atol=1e-2 if dtype == torch.bfloat16 else 1e-5)
     y.sum().backward()
     assert all(t.grad is not None for t in (x, r, w, b))
+
+
+def _twice(f, inputs, a, b):
+    """Gradients of b . (the gradients of a . f): second derivatives of every operand."""
+    inputs = [t.detach().requires_grad_() for t in inputs]
+    first = torch.autograd.grad(f(*inputs), inputs, a, create_graph=True)
+    return torch.autograd.grad(sum((g * w).sum() for g, w in zip(first, b)), inputs, allow_unused=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["attention", "attention padded", "norm", "linear gelu", "linear relu"])
+def test_gradients_of_gradients(what):
+    """Penalties on a gradient differentiate the backward pass.  Sums of at most 40 terms, three inside one another: 3 x 43 x 2^-24
+    = 8e-6 of their absolute sums, which are less than 30 times their values here: 2.4e-4 of a tensor's norm."""
+    from mitune.ops.attention import SequencePack, packed_attention
+    from mitune.ops.layernorm import layer_norm
+    from mitune.ops.linear import linear
+    g = torch.Generator().manual_seed(11)
+    new = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64).float().double()          # noqa: E731
+    if what.startswith("attention"):
+        d = 6 if what.endswith("padded") else 8
+        make = lambda dev: (lambda q, k, v: packed_attention(q, k, v, SequencePack([5, 1, 9], rows=17, device=dev), True))     # noqa: E731
+        inputs, out = (new(17, 4, d), new(17, 2, d), new(17, 2, d)), (17, 4, d)
+    elif what == "norm":
+        make = lambda dev: (lambda x, w, b: layer_norm(x, w, b))          # noqa: E731
+        inputs, out = (new(7, 37), new(37), new(37)), (7, 37)
+    else:
+        make = lambda dev: (lambda x, w, b, r: linear(x, w, b, activation=what.split()[1], residual=r))          # noqa: E731
+        inputs, out = (new(9, 33), new(19, 33), new(19), new(9, 19)), (9, 19)
+    a, b = new(*out), [new(*t.shape) for t in inputs]
+    want = _twice(make("cpu"), inputs, a, b)
+    gpu = lambda t: t.float().cuda()          # noqa: E731
+    got = _twice(make("cuda"), [gpu(t) for t in inputs], gpu(a), [gpu(t) for t in b])
+    for x, y in zip(got, want):
+        if y is None or y.norm() == 0:
+            assert x is None or x.norm() == 0
+        else:
+            assert (x.double().cpu() - y).norm() <= 2.4e-4 * y.norm()
