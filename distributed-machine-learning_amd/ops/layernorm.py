@@ -15,22 +15,26 @@ from typing import Optional
 import torch
 import torch.nn.functional as F
 
+from .layernorm_hip import LayerNorm, norm_forward
+from .lib import wants_grad
+
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5) -> torch.Tensor:
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension, differentiable, in ``x``'s type; statistics and
     column sums in f32.  ``weight`` and ``bias`` ([d], either may be missing) have ``x``'s type, or f32 beside a bf16 ``x``.  On a
     GPU ``x`` is f32 or bf16, rows of any width; rows may lie apart (a column slice of a wider tensor is read in place)."""
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"layer_norm needs rows of at least one column, got {tuple(x.shape)}")
-    d = x.shape[-1]
+    shape, device = x.shape, x.device
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError(f"layer_norm needs rows of at least one column, got {tuple(shape)}")
+    d = shape[-1]
     for name, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue
         if t.shape != (d,):
             raise ValueError(f"{name} must be [{d}], got {tuple(t.shape)}")
-        if t.device != x.device:
-            raise TypeError(f"{name} is on {t.device}, x on {x.device}")
+        if t.device != device:
+            raise TypeError(f"{name} is on {t.device}, x on {device}")
         if t.dtype != x.dtype and not (x.dtype == torch.bfloat16 and t.dtype == torch.float32):
             raise TypeError(f"{name} must be {x.dtype} (or f32 beside a bf16 x), got {t.dtype}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
@@ -45,8 +49,6 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         raise TypeError(f"layer_norm on a GPU takes f32 or bf16 rows, got {x.dtype}")
     if d > 1 << 29:
         raise ValueError(f"layer_norm on a GPU takes rows of at most {1 << 29} columns, got {d}")
-    from .layernorm_hip import LayerNorm, norm_forward
-    from .lib import wants_grad
     if wants_grad(x, weight, bias):
         return LayerNorm.apply(x, weight, bias, float(eps))
     return norm_forward(x, weight, bias, float(eps), False)[0]

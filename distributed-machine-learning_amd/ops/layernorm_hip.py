@@ -2,6 +2,7 @@
 over rows of any width (``csrc/norm.hip``)."""
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
@@ -134,13 +135,18 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 or d == 1 else t.contiguous()
 
 
+@functools.lru_cache(maxsize=1024)
+def _bwd_parts(M: int, d: int, bf16: int) -> int:
+    return L.load().mt_norm_bwd_parts(M, d, bf16)
+
+
 def norm_forward(x, weight, bias, eps: float, keeps: bool):
     """(output, x's rows, weight, statistics, type flags)."""
     so = L.load()
     xr = _rows(x)
     M, d = xr.shape
-    w = weight.contiguous() if weight is not None else None
-    b = bias.contiguous() if bias is not None else None
+    w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
+    b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
     y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     stats = torch.empty(M, 2, device=x.device, dtype=torch.float32) if keeps else None
     param = weight if weight is not None else bias
@@ -158,7 +164,7 @@ class LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps: float):
         y, xr, w, stats, flags = norm_forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(xr, w, stats, x, weight, bias)
+        ctx.save_for_backward(xr, w, stats, None if xr is x else x, None if w is weight else weight)
         param = weight if weight is not None else bias
         ctx.meta = (x.shape, flags, weight is not None, bias is not None, param.dtype if param is not None else None, eps)
         return y
@@ -166,12 +172,14 @@ class LayerNorm(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_y):
         so = L.load()
-        xr, w, stats, *inputs = ctx.saved_tensors
+        xr, w, stats, x, weight = ctx.saved_tensors
         shape, flags, has_w, has_b, pdtype, eps = ctx.meta
         M, d = xr.shape
         if torch.is_grad_enabled():
-            cast = lambda t: None if t is None else t.float()                                              # noqa: E731
-            plain = lambda x, w, b: F.layer_norm(x.float(), (d,), cast(w), cast(b), eps).to(x.dtype)      # noqa: E731
+            bias = torch.zeros(d, device=xr.device, dtype=pdtype, requires_grad=ctx.needs_input_grad[2]) if has_b else None
+            cast = lambda t: None if t is None else t.float()                                                    # noqa: E731
+            plain = lambda x, w, b: F.layer_norm(x.float(), (d,), cast(w), cast(b), eps).to(grad_y.dtype)       # noqa: E731
+            inputs = (xr if x is None else x, w if weight is None else weight, bias)
             return (*L.grads_by_formula(plain, inputs, grad_y), None)
         dy = _rows(grad_y if grad_y.dtype == xr.dtype else grad_y.to(xr.dtype))
         dx = torch.empty(shape, device=xr.device, dtype=xr.dtype)
@@ -181,7 +189,7 @@ class LayerNorm(torch.autograd.Function):
         db = fill(d, device=xr.device, dtype=pdtype) if want_b else None
         part = None
         if (want_w or want_b) and M:
-            part = torch.empty(so.mt_norm_bwd_parts(M, d, flags[0]), 2, d, device=xr.device, dtype=torch.float32)
+            part = torch.empty(_bwd_parts(M, d, flags[0]), 2, d, device=xr.device, dtype=torch.float32)
         with L.on(xr.device):
             L.check(so.mt_norm_bwd_launch(dy.data_ptr(), xr.data_ptr(), w.data_ptr() if has_w else None, stats.data_ptr(),
                                           dx.data_ptr(), part.data_ptr() if part is not None else None,

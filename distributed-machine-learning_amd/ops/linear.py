@@ -28,12 +28,14 @@ kernels cannot take at all (f16 or f64 on a GPU) raise ``TypeError`` instead of 
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
 import torch.nn.functional as F
 
 from ..options import OPTIONS
+from . import lib as L
 
 SMALL_MAX_ROWS = 32768
 SMALL_MAX_WEIGHTS = 65536     # in x out, e.g. 128 x 512
@@ -75,16 +77,16 @@ ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2}
 def _check_fused(x, weight, bias, activation, residual) -> None:
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {tuple(ACTIVATIONS)}, got {activation!r}")
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
-        raise ValueError(f"x {tuple(x.shape)} does not fit weight {tuple(weight.shape)}")
-    if bias is not None and bias.shape != weight.shape[:1]:
-        raise ValueError(f"bias must be [{weight.shape[0]}], got {tuple(bias.shape)}")
-    if residual is not None and residual.shape != x.shape[:-1] + weight.shape[:1]:
-        raise ValueError(f"residual must have the output's shape {tuple(x.shape[:-1] + weight.shape[:1])}, got "
-                         f"{tuple(residual.shape)}")
+    xs, ws, device = x.shape, weight.shape, x.device
+    if len(ws) != 2 or len(xs) < 1 or xs[-1] != ws[1]:
+        raise ValueError(f"x {tuple(xs)} does not fit weight {tuple(ws)}")
+    if bias is not None and bias.shape != ws[:1]:
+        raise ValueError(f"bias must be [{ws[0]}], got {tuple(bias.shape)}")
+    if residual is not None and residual.shape != xs[:-1] + ws[:1]:
+        raise ValueError(f"residual must have the output's shape {tuple(xs[:-1] + ws[:1])}, got {tuple(residual.shape)}")
     for name, t in (("weight", weight), ("bias", bias), ("residual", residual)):
-        if t is not None and t.device != x.device:
-            raise TypeError(f"{name} is on {t.device}, x on {x.device}")
+        if t is not None and t.device != device:
+            raise TypeError(f"{name} is on {t.device}, x on {device}")
 
 
 def _plain_fused(x, weight, bias, activation, residual) -> torch.Tensor:
@@ -109,8 +111,7 @@ def _fused_linear(x, weight, bias, activation, residual) -> torch.Tensor:
         raise TypeError(f"bias must be {x.dtype} or f32, got {bias.dtype}")
     if residual is not None and residual.dtype != x.dtype:
         raise TypeError(f"residual must be {x.dtype}, got {residual.dtype}")
-    from .lib import wants_grad
-    if wants_grad(x, weight, bias, residual):
+    if L.wants_grad(x, weight, bias, residual):
         return FusedLinear.apply(x, weight, bias, residual, ACTIVATIONS[activation], w16)
     return fused_forward(x, weight, bias, residual, ACTIVATIONS[activation], w16, False)[0]
 
@@ -164,7 +165,6 @@ def _wgrad_splits(M: int, tiles: int, rows_per_split: int) -> int:
 
 def _wgrad_bf16(dyc: torch.Tensor, xc: torch.Tensor, out_f: int, in_f: int, has_bias: bool):
     """dW [out, in] and db [out] (f32) of a bf16 layer: split-K tiles over the rows, ordered slab sum."""
-    from . import lib as L
     so = L.load()
     M = xc.shape[0]
     ksplits = _wgrad_splits(M, ((out_f + 127) // 128) * ((in_f + 127) // 128), 64)
@@ -181,7 +181,6 @@ def _wgrad_f32(dyc: torch.Tensor, xc: torch.Tensor, out_f: int, in_f: int, has_b
     """dW [out, in] and db [out] of an f32 layer: the contraction over the token rows is split so that the launch has
     about ``OPTIONS.wgrad_workgroups`` workgroups (a slice keeps at least 4 K-steps of 32 rows), slices summed in index
     order."""
-    from . import lib as L
     so = L.load()
     M = xc.shape[0]
     ksplits = _wgrad_splits(M, ((out_f + 63) // 64) * ((in_f + 63) // 64), 128)
@@ -194,7 +193,6 @@ def _wgrad_f32(dyc: torch.Tensor, xc: torch.Tensor, out_f: int, in_f: int, has_b
 
 
 def _slab_total(so, arena, ksplits, slab, out_f, in_f, has_bias, stream):
-    from . import lib as L
     if ksplits > 1:       # slices added in index order by one launch (weights and bias together)
         total = torch.empty(slab, device=arena.device, dtype=torch.float32)
         L.check(so.mt_slab_sum_launch(arena.data_ptr(), total.data_ptr(), out_f * in_f + (out_f if has_bias else 0), ksplits,
@@ -214,7 +212,6 @@ class DenseBF16(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, w16=None):
-        from . import lib as L
         so = L.load()
         out_f, in_f = weight.shape
         with torch.autocast("cuda", enabled=False):
@@ -236,7 +233,6 @@ class DenseBF16(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        from . import lib as L
         so = L.load()
         xc, wb = ctx.saved_tensors
         out_f, in_f = wb.shape
@@ -259,7 +255,6 @@ class DenseBF16(torch.autograd.Function):
 
 def _f32_forward(x, weight, bias):
     """y = x W^T + b on the exact-f32 tile kernel; returns (y, x as [rows, in], W contiguous)."""
-    from . import lib as L
     so = L.load()
     out_f, in_f = weight.shape
     xc = x.reshape(-1, in_f)
@@ -289,7 +284,6 @@ class DenseF32(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        from . import lib as L
         so = L.load()
         xc, wc = ctx.saved_tensors
         out_f, in_f = wc.shape
@@ -322,7 +316,6 @@ class SmallLinear(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        from . import lib as L
         so = L.load()
         xc, wc = ctx.saved_tensors
         out_f, in_f = wc.shape
@@ -341,13 +334,23 @@ class SmallLinear(torch.autograd.Function):
         return (dx.view(ctx.x_shape) if dx is not None else None), dw, db
 
 
+@functools.lru_cache(maxsize=1024)
+def _gemm_parts(mode: int, M: int, N: int, depth: int, bf16: int) -> int:
+    return L.load().mt_linear_parts(mode, M, N, depth, bf16)
+
+
+@functools.lru_cache(maxsize=1024)
+def _act_parts(M: int, columns: int, bf16: int) -> int:
+    return L.load().mt_linear_act_parts(M, columns, bf16)
+
+
 def _pieces(t: torch.Tensor) -> torch.Tensor:
     """``t`` [rows, columns] with rows of whole 16-byte pieces: itself when its rows start on such a boundary (less than 2^24 elements
     apart) and its width is a multiple of one, else a copy padded with zero columns."""
     per = 16 // t.element_size()
-    pad = -t.shape[1] % per
-    if (pad == 0 and t.stride(1) == 1 and t.stride(0) % per == 0 and t.data_ptr() % 16 == 0
-            and t.shape[1] <= t.stride(0) < 1 << 24):
+    width, (apart, step) = t.shape[1], t.stride()
+    pad = -width % per
+    if pad == 0 and step == 1 and apart % per == 0 and width <= apart < 1 << 24 and t.data_ptr() % 16 == 0:
         return t
     return F.pad(t, (0, pad)).contiguous() if pad else t.clone(memory_format=torch.contiguous_format)
 
@@ -356,38 +359,37 @@ def _rows_of(t: torch.Tensor, width: int) -> torch.Tensor:
     return t if t.dim() == 2 else t.reshape(-1, width)
 
 
-def _fused_gemm(so, mode: int, a, b, c, depth: int, bias=None, residual=None, z=None, act: int = 0) -> None:
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _fused_gemm(so, mode: int, a, b, c, depth: int, stream, bias=None, residual=None, z=None, act: int = 0) -> None:
     """c = act(a b + bias) + residual: b is [columns, depth] in mode 0, [depth, columns] in mode 1."""
-    from . import lib as L
     M, N = c.shape
     bf16 = int(c.dtype == torch.bfloat16)
-    n = so.mt_linear_parts(mode, M, N, depth, bf16)
+    n = _gemm_parts(mode, M, N, depth, bf16)
     part = torch.empty(n, M, N, device=c.device, dtype=torch.float32) if n > 1 else None
-    ptr = lambda t: t.data_ptr() if t is not None else None          # noqa: E731
-    with L.on(c.device):
-        L.check(so.mt_linear_gemm_launch(mode, a.data_ptr(), b.data_ptr(), ptr(bias), ptr(residual), c.data_ptr(), ptr(z), ptr(part),
-                                         M, N, depth, a.stride(0), b.stride(0), act,
-                                         int(bias is not None and bias.dtype == torch.bfloat16), bf16, L.raw_stream(c.device)),
-                "mt_linear_gemm_launch")
+    L.check(so.mt_linear_gemm_launch(mode, a.data_ptr(), b.data_ptr(), _ptr(bias), _ptr(residual), c.data_ptr(), _ptr(z), _ptr(part),
+                                     M, N, depth, a.stride(0), b.stride(0), act,
+                                     int(bias is not None and bias.dtype == torch.bfloat16), bf16, stream), "mt_linear_gemm_launch")
 
 
 def fused_forward(x, weight, bias, residual, act: int, w16, keep_z: bool):
     """(output, x's rows, the weight as multiplied, z or None)."""
-    from . import lib as L
     so = L.load()
     out_f, in_f = weight.shape
+    dtype, dev = x.dtype, x.device
     xc = _pieces(_rows_of(x, in_f))
-    if w16 is not None:
-        wc = w16
-    else:
-        wc = weight.detach() if weight.dtype == x.dtype else weight.detach().to(x.dtype)
+    wc = w16 if w16 is not None else weight if weight.dtype == dtype else weight.detach().to(dtype)
     wc = _pieces(wc)
-    bc = bias.detach().contiguous() if bias is not None else None
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
     rc = _rows_of(residual, out_f).contiguous() if residual is not None else None
-    y = torch.empty(xc.shape[0], out_f, device=x.device, dtype=x.dtype)
+    y = torch.empty(xc.shape[0], out_f, device=dev, dtype=dtype)
     z = torch.empty_like(y) if keep_z else None
-    _fused_gemm(so, 0, xc, wc, y, xc.shape[1], bc, rc, z, act)
-    return y.view(x.shape[:-1] + (out_f,)), xc, wc, z
+    with L.on(dev):
+        _fused_gemm(so, 0, xc, wc, y, xc.shape[1], L.raw_stream(dev), bias, rc, z, act)
+    return (y if x.dim() == 2 else y.view(x.shape[:-1] + (out_f,))), xc, wc, z
 
 
 class FusedLinear(torch.autograd.Function):
@@ -401,24 +403,22 @@ class FusedLinear(torch.autograd.Function):
         keep_z = backward and act != 0 and not (act == 1 and residual is None)
         y, xc, wc, z = fused_forward(x, weight, bias, residual, act, w16, keep_z)
         if backward:
-            ctx.save_for_backward(xc, wc, z if keep_z else y if act else None, x, weight, bias)
+            # x and the weight as multiplied, mostly they themselves; a second differentiation needs those it is asked for
+            ctx.save_for_backward(xc, wc, z if keep_z else y if act else None, None if xc is x else x,
+                                  None if wc is weight else weight, bias if act else None)
         ctx.meta = (act, x.shape, weight.shape[1], weight.dtype, bias.dtype if bias is not None else None,
                     residual.shape if residual is not None else None)
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        from . import lib as L
         so = L.load()
         act, x_shape, in_f, w_dtype, b_dtype, r_shape = ctx.meta
         dx = dw = db = None
         if any(ctx.needs_input_grad[:3]):
-            xc, wc, s, *inputs = ctx.saved_tensors
+            xc, wc, s, x, weight, bias = ctx.saved_tensors
             if torch.is_grad_enabled():
-                name = next(n for n, number in ACTIVATIONS.items() if number == act)
-                cast = lambda t: None if t is None else t.float()                                              # noqa: E731
-                plain = lambda x, w, b: _plain_fused(x.float(), w.float(), cast(b), name, None).to(x.dtype)    # noqa: E731
-                return (*L.grads_by_formula(plain, inputs, dy), dy if r_shape is not None else None, None, None)
+                return _twice_differentiable(ctx, dy, xc if x is None else x, wc if weight is None else weight, bias)
             out_f = wc.shape[0]
             bf16, dev, M = xc.dtype == torch.bfloat16, xc.device, xc.shape[0]
             per = 8 if bf16 else 4
@@ -431,7 +431,7 @@ class FusedLinear(torch.autograd.Function):
                     part = None
                     if bf16 and b_dtype is not None and ctx.needs_input_grad[2]:          # from dz before it is rounded
                         db = torch.empty(out_f, device=dev, dtype=b_dtype)
-                        part = torch.empty(so.mt_linear_act_parts(M, dz.shape[1], int(bf16)), out_f, device=dev, dtype=torch.float32)
+                        part = torch.empty(_act_parts(M, dz.shape[1], 1), out_f, device=dev, dtype=torch.float32)
                     L.check(so.mt_linear_act_bwd_launch(g.data_ptr(), s.data_ptr(), dz.data_ptr(),
                                                         part.data_ptr() if part is not None else None,
                                                         db.data_ptr() if part is not None else None, M, out_f, g.stride(0),
@@ -448,17 +448,26 @@ class FusedLinear(torch.autograd.Function):
                             None, None)
                 if ctx.needs_input_grad[0]:
                     dx = torch.empty(M, in_f, device=dev, dtype=xc.dtype)
-                    _fused_gemm(so, 1, dz, wc, dx, out_f)
-                    dx = dx.view(x_shape)
+                    _fused_gemm(so, 1, dz, wc, dx, out_f, stream)
+                    dx = dx if len(x_shape) == 2 else dx.view(x_shape)
                 if ctx.needs_input_grad[1] or (b_dtype is not None and ctx.needs_input_grad[2]):
                     dw, sums = _weight_grad(so, dz, xc, out_f, in_f, w_dtype, b_dtype, stream)
                     db = db if sums is None else sums
         return dx, dw, db, (dy if r_shape is not None else None), None, None
 
 
+def _twice_differentiable(ctx, dy, x, weight, bias):
+    act, _, _, _, b_dtype, r_shape = ctx.meta
+    name = next(n for n, number in ACTIVATIONS.items() if number == act)
+    if b_dtype is not None and bias is None:           # no activation: nothing depends on its value
+        bias = torch.zeros(weight.shape[0], device=weight.device, dtype=b_dtype, requires_grad=ctx.needs_input_grad[2])
+    cast = lambda t: None if t is None else t.float()                                                      # noqa: E731
+    plain = lambda x, w, b: _plain_fused(x.float(), w.float(), cast(b), name, None).to(dy.dtype)           # noqa: E731
+    return (*L.grads_by_formula(plain, (x, weight, bias), dy), dy if r_shape is not None else None, None, None)
+
+
 def _small_grads(so, dz, xc, wc, want_dx: bool, want_db: bool, stream):
     """The gradients of a small f32 layer in one launch, as ``SmallLinear`` computes them; widths stay padded."""
-    from . import lib as L
     (R, out), in_f, dev = dz.shape, xc.shape[1], dz.device
     xc = xc if xc.stride(0) == in_f else xc.contiguous()
     if wc.shape[0] != out:
@@ -483,7 +492,6 @@ def _fused_wgrad_splits(M: int, tiles: int, bf16: bool) -> int:
 def _weight_grad(so, dz, xc, out_f: int, in_f: int, w_dtype, b_dtype, stream):
     """(dW [out_f, in_f], db [out_f] or None).  A layer with enough tiles stores them as they leave the matrix instruction; a
     smaller one is split over the rows, the slabs added in order and rounded once."""
-    from . import lib as L
     M, width, rows = dz.shape[0], xc.shape[1], dz.shape[1]
     xc = xc if xc.stride(0) == width else xc.contiguous()
     bf16 = dz.dtype == torch.bfloat16
