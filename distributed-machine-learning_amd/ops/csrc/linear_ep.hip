@@ -513,3 +513,39 @@ extern "C" int mt_linear_wsum_launch(const float* arena, void* dw, void* db, int
 #undef GO
   return (int)hipGetLastError();
 }
+
+// The whole backward pass of a layer in one call: dz (with db from it before its rounding, where part_at is set), dx, then dW and what
+// is left of db.  Offsets into the workspace are in bytes, negative where a piece is not needed; splits 0: dW leaves in its own type.
+struct MtLinearBwd {
+  const void *dy, *s, *x, *w;
+  void *dx, *dw, *db;
+  uint8_t* ws;
+  int64_t M, dy_ld, ldw, dz_at, part_at, dxpart_at, arena_at, slab;
+  int32_t N, K, rows, width, act, bf16, dw_bf16, db_bf16, splits, unused;      // rows, width: N and K in whole 16-byte pieces
+};
+extern "C" int mt_wgrad_single_launch(const void* dY, const void* X, float* C, float* db, int M, int out, int in, int ksplits,
+                                      size_t split_stride, hipStream_t stream);
+extern "C" int mt_linear_bwd_size() { return (int)sizeof(MtLinearBwd); }
+extern "C" int mt_linear_bwd_launch(const MtLinearBwd* a, hipStream_t stream) {
+  if (a == nullptr) return -2;
+  const MtLinearBwd p = *a;
+  if (p.M < 1 || p.M > 0x7FFFFFFF - 256 || p.rows < p.N || p.width < p.K || (p.act != 0) != (p.dz_at >= 0) || (p.act == 0 && p.dy_ld != p.rows))
+    return -2;
+  const void* dz = p.act ? p.ws + p.dz_at : p.dy;
+  void* late = p.part_at >= 0 ? nullptr : p.db;
+  int rc = 0;
+  if (p.act)
+    rc = mt_linear_act_bwd_launch(p.dy, p.s, p.ws + p.dz_at, p.part_at >= 0 ? (float*)(p.ws + p.part_at) : nullptr,
+                                  p.part_at >= 0 ? p.db : nullptr, p.M, p.N, p.dy_ld, p.rows, p.act, p.db_bf16, p.bf16, stream);
+  if (rc == 0 && p.dx != nullptr)
+    rc = mt_linear_gemm_launch(1, dz, p.w, nullptr, nullptr, p.dx, nullptr, p.dxpart_at >= 0 ? (float*)(p.ws + p.dxpart_at) : nullptr,
+                               p.M, p.K, p.N, p.rows, p.ldw, 0, 0, p.bf16, stream);
+  if (rc != 0 || p.dw == nullptr) return rc;
+  if (p.splits == 0) return mt_linear_wgrad_launch(dz, p.x, p.dw, late, p.M, p.N, p.K, p.rows, p.width, p.db_bf16, p.bf16, stream);
+  float* arena = (float*)(p.ws + p.arena_at);
+  const int64_t db_at = (int64_t)p.rows * p.width;
+  rc = p.bf16 ? mt_wgrad_single_launch(dz, p.x, arena, late != nullptr ? arena + db_at : nullptr, (int)p.M, p.rows, p.width, p.splits, p.slab, stream)
+              : mt_linear_wgrad_f32_parts_launch(dz, p.x, arena, p.M, p.rows, p.width, p.splits, p.slab, late != nullptr, stream);
+  if (rc != 0) return rc;
+  return mt_linear_wsum_launch(arena, p.dw, late, p.N, p.K, p.width, db_at, p.splits, p.slab, p.dw_bf16, p.db_bf16, stream);
+}

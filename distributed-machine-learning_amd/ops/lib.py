@@ -19,6 +19,7 @@ from . import build as _build
 
 MT_MAX_LAYERS = 8
 # csrc/packed_attention.hip: bytes and rows of an item, longest sequence whose outputs keep what rounding took off
+LINEAR_BWD_FORMAT = struct.Struct("<8Q8q10i")      # MtLinearBwd of csrc/linear_ep.hip
 PACKED_ITEM_BYTES, PACKED_OWN_ROWS, PACKED_SPLIT_ROWS, PACKED_LOW_ROWS = 16, 128, 32, 128
 
 c_void_p, c_int32, c_uint32, c_float, c_size_t = C.c_void_p, C.c_int32, C.c_uint32, C.c_float, C.c_size_t
@@ -245,8 +246,11 @@ def load(build_if_missing: bool = True) -> C.CDLL:
     lib.mt_linear_wsum_launch.argtypes = [c_void_p] * 3 + [C.c_int64, C.c_int, C.c_int, C.c_int64, C.c_int, C.c_int64, C.c_int,
                                                            C.c_int, c_void_p]
     lib.mt_linear_wgrad_launch.argtypes = [c_void_p] * 4 + [C.c_int64] + [C.c_int] * 6 + [c_void_p]
+    lib.mt_linear_bwd_launch.argtypes = [C.c_char_p, c_void_p]
+    if lib.mt_linear_bwd_size() != LINEAR_BWD_FORMAT.size:
+        raise KernelLibraryError("dense layer: argument layout mismatch between lib.py and the library")
     lib.mt_linear_wgrad_f32_parts_launch.argtypes = ([c_void_p] * 3 + [C.c_int64] + [C.c_int] * 3 + [C.c_int64, C.c_int, c_void_p])
-    for fn in (lib.mt_linear_wgrad_f32_parts_launch, lib.mt_linear_parts, lib.mt_linear_gemm_launch, lib.mt_linear_act_parts, lib.mt_linear_act_bwd_launch, lib.mt_linear_wgrad_launch, lib.mt_linear_wsum_launch):
+    for fn in (lib.mt_linear_bwd_launch, lib.mt_linear_wgrad_f32_parts_launch, lib.mt_linear_parts, lib.mt_linear_gemm_launch, lib.mt_linear_act_parts, lib.mt_linear_act_bwd_launch, lib.mt_linear_wgrad_launch, lib.mt_linear_wsum_launch):
         fn.restype = C.c_int
     lib.mt_norm_bwd_parts.argtypes = [C.c_int64, C.c_int, C.c_int]
     lib.mt_norm_fwd_launch.argtypes = [c_void_p] * 5 + [C.c_int64, C.c_int64, C.c_int, c_float, C.c_int, C.c_int, c_void_p]

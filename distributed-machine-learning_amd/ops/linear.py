@@ -427,6 +427,31 @@ class FusedLinear(torch.autograd.Function):
                 g = _rows_of(dy if dy.dtype == xc.dtype else dy.to(xc.dtype), out_f)
                 if act:
                     g = g if g.stride(1) == 1 else g.contiguous()
+                    width = out_f + -out_f % per
+                else:
+                    g = _pieces(g)
+                    g = g if g.stride(0) == g.shape[1] else g.contiguous()
+                    width = g.shape[1]
+                need_x, need_w, need_b = ctx.needs_input_grad[:3]
+                need_b = need_b and b_dtype is not None
+                need_w = need_w or (need_b and not (bf16 and act))          # sums over dz's rows come with dW, or from act'
+                plan = _bwd_plan(M, out_f, width, in_f, xc.shape[1], act, bf16, w_dtype == xc.dtype, need_x, need_w, need_b,
+                                 OPTIONS.wgrad_workgroups)
+                if plan is not None:
+                    size, at, slab, splits = plan
+                    xc = xc if xc.stride(0) == xc.shape[1] else xc.contiguous()
+                    ws = torch.empty(size, device=dev, dtype=torch.uint8) if size else None
+                    dx = torch.empty(x_shape, device=dev, dtype=xc.dtype) if need_x else None
+                    dw = torch.empty(out_f, in_f, device=dev, dtype=w_dtype) if need_w else None
+                    db = torch.empty(out_f, device=dev, dtype=b_dtype) if need_b else None
+                    args = L.LINEAR_BWD_FORMAT.pack(g.data_ptr(), s.data_ptr() if act else 0, xc.data_ptr(), wc.data_ptr(),
+                                                    dx.data_ptr() if need_x else 0, dw.data_ptr() if need_w else 0,
+                                                    db.data_ptr() if need_b else 0, ws.data_ptr() if size else 0, M, g.stride(0),
+                                                    wc.stride(0), *at, slab, out_f, in_f, width, xc.shape[1], act, bf16,
+                                                    w_dtype == torch.bfloat16, b_dtype == torch.bfloat16, splits, 0)
+                    L.check(so.mt_linear_bwd_launch(args, stream), "mt_linear_bwd_launch")
+                    return dx, dw, db, (dy if r_shape is not None else None), None, None
+                if act:
                     dz = torch.empty(M, out_f + -out_f % per, device=dev, dtype=xc.dtype)
                     part = None
                     if bf16 and b_dtype is not None and ctx.needs_input_grad[2]:          # from dz before it is rounded
@@ -439,8 +464,7 @@ class FusedLinear(torch.autograd.Function):
                             "mt_linear_act_bwd_launch")
                     b_dtype = None if part is not None else b_dtype
                 else:
-                    dz = _pieces(g)
-                    dz = dz if dz.stride(0) == dz.shape[1] else dz.contiguous()
+                    dz = g
                 if not bf16 and _small(M, xc.shape[1], dz.shape[1], True):
                     dx, dw, sums = _small_grads(so, dz, xc, wc, ctx.needs_input_grad[0], b_dtype is not None, stream)
                     dx = dx[:, :in_f].reshape(x_shape) if dx is not None else None
@@ -464,6 +488,38 @@ def _twice_differentiable(ctx, dy, x, weight, bias):
     cast = lambda t: None if t is None else t.float()                                                      # noqa: E731
     plain = lambda x, w, b: _plain_fused(x.float(), w.float(), cast(b), name, None).to(dy.dtype)           # noqa: E731
     return (*L.grads_by_formula(plain, (x, weight, bias), dy), dy if r_shape is not None else None, None, None)
+
+
+@functools.lru_cache(maxsize=1024)
+def _bwd_plan(M: int, out_f: int, rows: int, in_f: int, width: int, act: int, bf16: bool, same: bool, need_x: bool, need_w: bool,
+              need_b: bool, workgroups: int):
+    """How ``mt_linear_bwd_launch`` computes a layer's gradients: (bytes of workspace, where dz, the column sums, the parts of dx and
+    those of dW lie in it (-1: not there), floats from part to part of dW, how many; 0: unsplit).  None: a small f32 layer, or one
+    whose weight gradient takes several launches.  Kept per shape; ``workgroups`` is the option that the split follows."""
+    if not bf16 and _small(M, width, rows, True):
+        return None
+    size, at = 0, []
+
+    def take(wanted, count) -> None:
+        nonlocal size
+        at.append(size if wanted else -1)
+        size += -(-count // 256) * 256 if wanted else 0
+
+    early = bf16 and act != 0 and need_b                    # db from dz before its rounding
+    take(act != 0, M * rows * (2 if bf16 else 4))
+    take(early, _act_parts(M, rows, 1) * out_f * 4 if early else 0)
+    parts = _gemm_parts(1, M, in_f, out_f, int(bf16)) if need_x else 1
+    take(parts > 1, parts * M * in_f * 4)
+    tile = 128 if bf16 else 64
+    most = 255 * tile if bf16 else rows
+    splits = _fused_wgrad_splits(M, -(-min(rows, most) // tile) * -(-width // tile), bf16)
+    if not need_w or (same and splits == 1):
+        return size, (*at, -1), 0, 0
+    if rows > most:
+        return None
+    slab = (rows * width + rows + 63) // 64 * 64
+    take(True, splits * slab * 4)
+    return size, tuple(at), slab, splits
 
 
 def _small_grads(so, dz, xc, wc, want_dx: bool, want_db: bool, stream):

@@ -116,6 +116,23 @@ def test_every_product_on_the_256_tile(act, residual, bias, M, K, N):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("act", [None, "gelu"])
+@pytest.mark.parametrize("M,K,N", [(50, 40, 33), (2000, 264, 520)])
+def test_gradients_of_some_operands(dtype, act, M, K, N):
+    """Whichever operands want one, each gradient is the same bit for bit."""
+    from mitune.ops.linear import linear
+    x, w, b, r, dy = _make(M, K, N, dtype, False)
+    every = _run(x, w, b, r, dy, act)[1:]
+    for wanted in range(1, 16):
+        leaves = [t.detach().requires_grad_(bool(wanted >> i & 1)) for i, t in enumerate((x, w, b, r))]
+        y = linear(leaves[0], leaves[1], leaves[2], activation=act, residual=leaves[3])
+        some = [t for t in leaves if t.requires_grad]
+        for got, want in zip(torch.autograd.grad(y, some, dy), [g for g, t in zip(every, leaves) if t.requires_grad]):
+            assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,M,K,N", [(torch.bfloat16, 4097, 4168, 2056), (torch.float32, 3001, 1000, 520)])
 def test_results_repeat(dtype, M, K, N):
     """The same bits every time, and the same for a part of the rows on another tile: products are summed in one order."""
