@@ -197,6 +197,7 @@ class SequencePack:
         self.uniform_length = int(length) if count else 0
         own, fine = (-(-int(length) // r) * int(count) for r in (PACKED_OWN_ROWS, PACKED_SPLIT_ROWS))
         self._counts, self._lists, self._stream = (own, fine, own if length <= SOLO_ROWS else fine), None, 0
+        self._cuts = {}
         return self
 
     def _fix(self, total: int, rows: int, device) -> None:
@@ -234,12 +235,24 @@ class SequencePack:
             lists += [np.concatenate([items[o], tail]) for o in orders]
             counts.append(len(items) + len(tail))
         self._counts = tuple(counts)
-        self._lists, self._stream = None, 0
+        self._lists, self._stream, self._cuts = None, 0, {}
         if self.device.type == "cuda":
             from .lib import raw_stream
             # a blocking copy: the list is there for whichever stream uses it first
             self._lists = torch.from_numpy(np.concatenate(lists)).to(self.device)
             self._stream = raw_stream(self.device)
+
+    def _cut(self, order: int, lanes: int) -> int:
+        """How many of the 128-row key items, longest walk first (``order`` 0 causal, 1 no mask), are worth two workgroups: those that
+        alone walk further than a CU's share of all walks over ``lanes`` heads, which the launch would end up waiting for."""
+        if (order, lanes) not in self._cuts:
+            n = self.lengths[self.lengths > 0]
+            parts = -(-n // PACKED_OWN_ROWS)
+            seq = np.repeat(np.arange(len(n)), parts)
+            first = (np.arange(len(seq)) - np.repeat(np.cumsum(parts) - parts, parts)) * PACKED_OWN_ROWS
+            walks = n[seq] - (first if order == 0 else 0)
+            self._cuts[order, lanes] = int((walks > walks.sum() * lanes / 256).sum())
+        return self._cuts[order, lanes]
 
     def _items(self, which: int, order: int, stream: int):
         """(address, number) of a list for a launch on ``stream``: ``which`` 0 / 1 / 2 as laid out above, ``order`` 0 causal queries,

@@ -200,14 +200,21 @@ def _packed_launch(so, pack, q, k, v, causal: bool, scale: float, backward: int,
     kv_items, n_kv = pack._items(kv_form, 1 if causal else 2, stream)
     # a uniform batch has no list in which short sequences are marked: its sequences are short, or none is
     mark = lambda f: 1 if f == 2 and pack.longest > SOLO_ROWS else f          # noqa: E731
+    cut, halves = 0, None
+    if backward and kv_form == 0 and q.shape[1] > k.shape[1]:
+        cut = pack._cut(0 if causal else 1, k.shape[1])
+        if cut:
+            widest = max(k.shape[2], v.shape[2])
+            halves = torch.empty(cut * k.shape[1] * 4 * L.PACKED_OWN_ROWS * (32 if widest <= 32 else 64 if widest <= 64 else 128),
+                                 device=q.device, dtype=torch.float32)
     qr, qh, _ = q.stride()
     kr, kh, _ = k.stride()
     vr, vh, _ = v.stride()
     dr, dh, _ = dout.stride() if dout is not None else (0, 0, 0)
     args = L.PACKED_ATTN_FORMAT.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out, dout.data_ptr() if dout is not None else 0, o, dq,
-                                     dk, dv, low, lse, delta, items, kv_items, qr, qh, kr, kh, vr, vh, dr, dh, pack.rows, n, n_kv,
+                                     dk, dv, low, lse, delta, halves.data_ptr() if cut else 0, items, kv_items, qr, qh, kr, kh, vr, vh, dr, dh, pack.rows, n, n_kv,
                                      pack.uniform_length, len(pack.lengths), q.shape[1], k.shape[1], q.shape[2], v.shape[2],
-                                     int(causal), mark(form), mark(kv_form), scale)
+                                     int(causal), mark(form), mark(kv_form), cut, scale)
     with L.on(q.device):
         L.check(so.mt_packed_attn_launch(args, backward, int(bf16), stream), "mt_packed_attn_launch")
 

@@ -9,8 +9,9 @@
 //
 // A workgroup is four waves.  In the forward and the dq kernel a wave owns 32 queries and walks over the keys; in the dk / dv
 // kernel it owns 32 keys and walks over the queries of every head of the group, so each gradient element is summed by one
-// wave in a fixed order: no atomics, no workspace, and the gradients of shared heads need no second pass.  The price is that
-// the scores are computed again in both backward kernels (7 products where 5 are the least).
+// wave in a fixed order: no atomics, no workspace, and the gradients of shared heads need no second pass (but for walks longer
+// than a CU's share of the launch, which two workgroups share by heads: 20 documents of up to 2048, 16 / 4 heads of 128, backward
+// 412 -> 393 us).  The price is that the scores are computed again in both backward kernels (7 products where 5 are the least).
 //
 // Every product is v_mfma_*_32x32: the walked-over rows come from LDS as the first operand, the owned rows stay in registers
 // as the second, so an accumulator lane belongs to ONE owned row: row statistics are one register, a row maximum is a chain in
@@ -44,12 +45,14 @@ struct MtPackedAttn {
   void *o, *dq, *dk, *dv;       // outputs, contiguous [T][heads or kv_heads][dk or dv]
   void* low;                    // bf16 [T][heads][dv]: what rounding took off the output's rows of few keys; may be null
   float *lse, *delta;           // [heads][rows]
+  float* halves;                // what the two workgroups of a cut walk leave, [cut items][kv_heads][2][dk, dv][128][D]
   const MtSeqItem *items, *kv_items;      // items of query rows and of key rows; null: count sequences of uniform_len rows each
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, do_row, do_head;
   int64_t rows;
   int32_t n_items, n_kv_items, uniform_len, count;
   int32_t heads, kv_heads, head_k, head_v, causal;
   int32_t split, kv_split;      // the launch's form: 0 shared, 1 split, 2 split with every item solo (of a uniform batch)
+  int32_t cut;                  // leading key items whose walk two workgroups share, half the heads of the group each
   float scale;
 };
 
@@ -620,8 +623,12 @@ __global__ __launch_bounds__(PA_DKV_THREADS, 2) void mt_pattn_dkv_kernel(const M
   constexpr int BYTES = 2 * KV + 2 * STAGE, JOIN = 2 * 128 * D * 4;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[BYTES < JOIN ? JOIN : BYTES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int it = blockIdx.x / p.kv_heads, kvh = blockIdx.x - it * p.kv_heads;
-  const int group = p.heads / p.kv_heads;
+  // workgroups 0 .. 2 cut kv_heads - 1: the halves of the longest walks
+  const int turn = blockIdx.x / p.kv_heads, kvh = blockIdx.x - turn * p.kv_heads;
+  const bool is_cut = turn < 2 * p.cut;
+  const int it = is_cut ? turn >> 1 : turn - p.cut;
+  const int heads_all = p.heads / p.kv_heads, head_lo = is_cut && (turn & 1) ? heads_all / 2 : 0;
+  const int group = is_cut && !(turn & 1) ? heads_all / 2 : heads_all - head_lo;
   const MtSeqItem item = pa_item(p, p.kv_items, it, 0, false);
   const int64_t dk_row = (int64_t)p.kv_heads * p.head_k, dv_row = (int64_t)p.kv_heads * p.head_v;
   T* dk = reinterpret_cast<T*>(p.dk) + item.row0 * dk_row + (int64_t)kvh * p.head_k;
@@ -649,7 +656,7 @@ __global__ __launch_bounds__(PA_DKV_THREADS, 2) void mt_pattn_dkv_kernel(const M
   const T *q_next, *d_next;
   const float* stat_next;
   int left, todo = tiles, until = per_head;
-  int64_t head_next = (int64_t)kvh * group;
+  int64_t head_next = (int64_t)kvh * heads_all + head_lo;
   auto enter_head = [&] {
     const int q0 = q_lo * BQ + 32 * half;
     const int64_t r0 = item.row0 + (int64_t)q0;
@@ -814,9 +821,41 @@ __global__ __launch_bounds__(PA_DKV_THREADS, 2) void mt_pattn_dkv_kernel(const M
   __syncthreads();
   if (half == 1) return;
   each([&](int b, int i, int at) { ak[b][i] += join[at]; av[b][i] += join[128 * D + at]; });
+  if (is_cut) {
+    float* part = p.halves + (((int64_t)it * p.kv_heads + kvh) * 2 + (turn & 1)) * 2 * PA_OWN * D + (block * 32 + (lane & 31)) * D;
+    if (mine < item.len) {
+      pa_store_row<float, D>(part, ak, p.scale, p.head_k, lane);
+      pa_store_row<float, D>(part + PA_OWN * D, av, 1.f, p.head_v, lane);
+    }
+    return;
+  }
   if (mine < item.len) {
     pa_store_row<T, D>(dk + (int64_t)mine * dk_row, ak, p.scale, p.head_k, lane);
     pa_store_row<T, D>(dv + (int64_t)mine * dv_row, av, 1.f, p.head_v, lane);
+  }
+}
+
+// dk and dv of the cut walks: the two halves added, rounded once.  Sixteen rows per workgroup.
+#define PA_HALVES_ROWS 16
+template <int D>
+__global__ __launch_bounds__(PA_THREADS) void mt_pattn_halves_kernel(const MtPackedAttn p) {
+  const int unit = blockIdx.x / (PA_OWN / PA_HALVES_ROWS), lo = (blockIdx.x % (PA_OWN / PA_HALVES_ROWS)) * PA_HALVES_ROWS;
+  const int it = unit / p.kv_heads, kvh = unit - it * p.kv_heads;
+  const MtSeqItem item = pa_item(p, p.kv_items, it, 0, false);
+  const int left = item.len - item.first - lo, rows = left < PA_HALVES_ROWS ? left : PA_HALVES_ROWS;
+  const int64_t r0 = item.row0 + (int64_t)item.first + lo;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const int d = which ? p.head_v : p.head_k;
+    __bf16* out = reinterpret_cast<__bf16*>(which ? p.dv : p.dk) + (r0 * p.kv_heads + kvh) * d;
+    const float* a = p.halves + (int64_t)unit * 4 * PA_OWN * D + which * PA_OWN * D + lo * D;
+    const float* b = a + 2 * PA_OWN * D;
+    for (int i = threadIdx.x; i < rows * (D / 4); i += PA_THREADS) {
+      const int r = i / (D / 4), c = (i - r * (D / 4)) * 4;
+      if (c >= d) continue;
+      const f32x4 v = *reinterpret_cast<const f32x4*>(a + r * D + c) + *reinterpret_cast<const f32x4*>(b + r * D + c);
+      pa_store4<__bf16>(out + (int64_t)r * p.kv_heads * d + c, nullptr, v[0], v[1], v[2], v[3]);
+    }
   }
 }
 
@@ -1197,10 +1236,13 @@ __global__ __launch_bounds__(PA_THREADS, DK + DV > 96 ? 1 : 2) void mt_pattn_spl
 // ---- launchers ----------------------------------------------------------------------------------------------------------
 template <int D>
 static void pa_launch_shared(const MtPackedAttn& p, int pass, hipStream_t stream) {
-  const dim3 grid((unsigned)(pass == 2 ? p.n_kv_items * p.kv_heads : p.n_items * p.heads)), block(PA_THREADS);
+  const dim3 grid((unsigned)(pass == 2 ? (p.n_kv_items + p.cut) * p.kv_heads : p.n_items * p.heads)), block(PA_THREADS);
   if (pass == 0) hipLaunchKernelGGL((mt_pattn_fwd_kernel<__bf16, D, 64>), grid, block, 0, stream, p);
   else if (pass == 1) hipLaunchKernelGGL((mt_pattn_dq_kernel<__bf16, D, 64>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((mt_pattn_dkv_kernel<__bf16, D>), grid, dim3(PA_DKV_THREADS), 0, stream, p);
+  else {
+    hipLaunchKernelGGL((mt_pattn_dkv_kernel<__bf16, D>), grid, dim3(PA_DKV_THREADS), 0, stream, p);
+    if (p.cut > 0) hipLaunchKernelGGL((mt_pattn_halves_kernel<D>), dim3((unsigned)(p.cut * p.kv_heads * (PA_OWN / PA_HALVES_ROWS))), block, 0, stream, p);
+  }
 }
 template <typename T, int DK, int DV>
 static void pa_launch_split(const MtPackedAttn& p, int pass, hipStream_t stream) {
@@ -1244,7 +1286,8 @@ extern "C" int mt_packed_attn_launch(const MtPackedAttn* a, int backward, int bf
       if ((int64_t)((p.uniform_len - 1) / rows + 1) * p.count != (i ? p.n_kv_items : p.n_items)) return -2;
     }
   }
-  const int64_t most = p.n_items > p.n_kv_items ? p.n_items : p.n_kv_items;
+  if (p.cut != 0 && (p.cut < 0 || (int64_t)p.cut * p.kv_heads * (PA_OWN / PA_HALVES_ROWS) > 0x7FFFFFFF || p.cut > p.n_kv_items || p.halves == nullptr || p.kv_split != 0 || p.heads < 2 * p.kv_heads)) return -2;
+  const int64_t most = p.n_items > p.n_kv_items + p.cut ? p.n_items : (int64_t)p.n_kv_items + p.cut;
   if (most * p.heads > 0x7FFFFFFF || !(p.scale > 0.f)) return -2;
   const int64_t strides[8] = {p.q_row, p.q_head, p.k_row, p.k_head, p.v_row, p.v_head, p.do_row, p.do_head};
   for (int i = 0; i < 8; ++i)      // 32-bit byte offsets inside a staged tile of at most 128 rows

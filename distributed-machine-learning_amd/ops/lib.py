@@ -60,16 +60,16 @@ class OptSlot(C.Structure):
 class PackedAttn(C.Structure):
     _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p), ("dout", c_void_p),
                 ("o", c_void_p), ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p), ("low", c_void_p),
-                ("lse", c_void_p), ("delta", c_void_p), ("items", c_void_p), ("kv_items", c_void_p),
+                ("lse", c_void_p), ("delta", c_void_p), ("halves", c_void_p), ("items", c_void_p), ("kv_items", c_void_p),
                 ("q_row", C.c_int64), ("q_head", C.c_int64), ("k_row", C.c_int64), ("k_head", C.c_int64),
                 ("v_row", C.c_int64), ("v_head", C.c_int64), ("do_row", C.c_int64), ("do_head", C.c_int64),
                 ("rows", C.c_int64), ("n_items", c_int32), ("n_kv_items", c_int32), ("uniform_len", c_int32), ("count", c_int32),
                 ("heads", c_int32), ("kv_heads", c_int32), ("head_k", c_int32), ("head_v", c_int32),
-                ("causal", c_int32), ("split", c_int32), ("kv_split", c_int32), ("scale", c_float)]
+                ("causal", c_int32), ("split", c_int32), ("kv_split", c_int32), ("cut", c_int32), ("scale", c_float)]
 
 
 # The same layout for struct.pack: filling a ctypes structure field by field costs several microseconds of every call.
-PACKED_ATTN_FORMAT = struct.Struct("<14Q9q11if")
+PACKED_ATTN_FORMAT = struct.Struct("<15Q9q12if4x")
 
 
 class MlpPlan(C.Structure):

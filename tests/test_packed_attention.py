@@ -130,6 +130,27 @@ def test_every_form(monkeypatch, dtype, form, causal, heads, kv_heads, dk, dv):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (3, 1)])
+def test_walks_cut_in_two(monkeypatch, causal, heads, kv_heads):
+    """However many of the longest walks over the queries two workgroups share: none, some, all that have any."""
+    from mitune.ops import attention_hip
+    from mitune.ops.attention import SequencePack
+    monkeypatch.setattr(attention_hip, "FORM", 0)
+    lengths = [300, 130, 64]                          # 3 + 2 + 1 items of key rows
+    q, k, v, do = _inputs(lengths, 500, heads, kv_heads, 64, 48, torch.bfloat16)
+    want = _plain(q, k, v, lengths, causal, 0.125, do, True)
+    order = 0 if causal else 1
+    pack = SequencePack(lengths, rows=500)
+    assert pack._cut(order, 256) == 0 and pack._cut(order, 1) == (5 if causal else 6)      # the two last keys of 130 walk over 2 rows of 712
+    for cut in (0, 1, 4, 6):
+        pack._cuts[order, kv_heads] = cut
+        got = _grads(q, k, v, pack, do, causal)
+        _check(got, *want)
+        assert not any(t[sum(lengths):].any() for t in got)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_a_longer_sequence_with_a_scale_and_many_tiles(dtype):
     from mitune.ops.attention import SequencePack
