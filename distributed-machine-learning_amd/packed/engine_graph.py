@@ -24,10 +24,9 @@ chip on their own, are issued on one stream, slot after slot, unless ``model_kwa
 
 Why big packs once stalled on several streams, and what makes them safe now.  Three bf16 FT-Transformer slots (66 560
 token rows per step) replayed over three streams used to stop for good after a dozen steps: every stream idle, the host
-blocked in a graph launch or in the final synchronisation.  ``bench/hang_repro.py`` reproduces it and bisects it
-(``profiles/r2_multistream_stall.txt``): it happens with 2 or 3 slots, in bf16 and in f32, eagerly-built or replayed, with
-the host held to 1, 4 or 16 replays ahead of each stream or not held at all, with 4 or 16 hardware queues -- and only
-while the dense layers run on the BLAS library.  For these shapes the library picks "stream-K" GEMM kernels (``SK3`` in
+blocked in a graph launch or in the final synchronisation (``profiles/r2_multistream_stall.txt``).  It happened with 2 or 3
+slots, in bf16 and in f32, eagerly-built or replayed, with the host held to 1, 4 or 16 replays ahead of each stream or not
+held at all, with 4 or 16 hardware queues -- and only while the dense layers ran on the BLAS library.  For these shapes the library picked "stream-K" GEMM kernels (``SK3`` in
 their names), whose workgroups wait inside the launch for partial tiles of sibling workgroups and therefore need the
 whole launch resident; two such launches from different streams split the CUs between them and each waits for
 workgroups that the other keeps from being scheduled.  The small-kernel regime never met them (its GEMMs are plain
