@@ -530,6 +530,7 @@ extern "C" int mt_wgrad_single_launch(const void* dY, const void* X, float* C, f
 #undef MT_P8_GO
     return (int)hipGetLastError();
   }
+  if (tiles_j > 32767) return -2;      // MtTile::tj is 16 bits
   if (nblocks <= 320)
     hipLaunchKernelGGL(mt_wgrad_single_kernel<4>, dim3(nblocks), dim3(NTHREADS), 0, stream, g, tiles_i, ksplits,
                        split_stride, flags);

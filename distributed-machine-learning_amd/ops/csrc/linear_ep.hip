@@ -426,6 +426,7 @@ extern "C" int mt_linear_wgrad_launch(const void* dz, const void* x, void* dw, v
   if (M < 1 || M > 0x7FFFFFFF - 256 || N < 1 || K < 1 || ld_dz % per || ldx % per || ld_dz < N || ldx < K) return -2;
   const int flags = db != nullptr ? MT_GEMM_FLAG_DBIAS : 0;
   if (!bf16 && (ld_dz >= LF_MAX_LD || ldx >= LF_MAX_LD)) return -2;
+  if (bf16 && (K + BN - 1) / BN > 32767) return -2;    // a 128-tile's column number is 16 bits
   const int most = bf16 ? 255 * BM : N;                // output rows of a launch: the 128-tile's numbers are 8 bits here
   for (int n0 = 0; n0 < N; n0 += most) {
     const int n = N - n0 < most ? N - n0 : most;

@@ -72,6 +72,8 @@ def _pad_operands(x, weight, bias, mult: int):
 
 
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2}
+MAX_FUSED_WIDTH = 2_000_000           # output features, and input features where x has a gradient: tile numbers are 16 bits
+MAX_BF16_DW_WIDTH = 32767 * 128       # input features of a bf16 weight gradient, for the same reason
 
 
 def _check_fused(x, weight, bias, activation, residual) -> None:
@@ -111,7 +113,13 @@ def _fused_linear(x, weight, bias, activation, residual) -> torch.Tensor:
         raise TypeError(f"bias must be {x.dtype} or f32, got {bias.dtype}")
     if residual is not None and residual.dtype != x.dtype:
         raise TypeError(f"residual must be {x.dtype}, got {residual.dtype}")
-    if L.wants_grad(x, weight, bias, residual):
+    wants = L.wants_grad(x, weight, bias, residual)
+    out_f, in_f = weight.shape
+    if max(out_f, in_f) > MAX_FUSED_WIDTH and (out_f > MAX_FUSED_WIDTH or (wants and (
+            x.requires_grad or (x.dtype == torch.bfloat16 and in_f > MAX_BF16_DW_WIDTH)))):
+        raise ValueError(f"a dense layer on a GPU has at most {MAX_FUSED_WIDTH} output features, as many input features for the "
+                         f"gradient of x, and {MAX_BF16_DW_WIDTH} for that of a weight beside bf16, got weight {tuple(weight.shape)}")
+    if wants:
         return FusedLinear.apply(x, weight, bias, residual, ACTIVATIONS[activation], w16)
     return fused_forward(x, weight, bias, residual, ACTIVATIONS[activation], w16, False)[0]
 
