@@ -393,9 +393,11 @@ def wants_grad(*tensors) -> bool:
 
 def grads_by_formula(formula, inputs, grad):
     """Gradients of ``formula(*inputs)`` (plain torch) that can be differentiated again, for backward passes under
-    ``create_graph``; the kernels' own backward passes leave no graph."""
+    ``create_graph``; the kernels' own backward passes leave no graph.  Every input stands in the formula as an alias of its own, so
+    that its gradient is that of its place alone, also where one tensor takes several places or one input was computed from another."""
     import torch
-    wanted = [t for t in inputs if t is not None and t.requires_grad]
     with torch.enable_grad():
-        got = iter(torch.autograd.grad(formula(*inputs), wanted, grad, create_graph=True))
+        places = [None if t is None else t.view_as(t) for t in inputs]
+        wanted = [t for t in places if t is not None and t.requires_grad]
+        got = iter(torch.autograd.grad(formula(*places), wanted, grad, create_graph=True))
     return [next(got) if t is not None and t.requires_grad else None for t in inputs]
