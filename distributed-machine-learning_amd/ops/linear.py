@@ -438,7 +438,8 @@ class FusedLinear(torch.autograd.Function):
                     width = out_f + -out_f % per
                 else:
                     g = _pieces(g)
-                    g = g if g.stride(0) == g.shape[1] else g.contiguous()
+                    # (a single row is contiguous to torch whatever its row stride is: clone, not contiguous)
+                    g = g if g.stride(0) == g.shape[1] else g.clone(memory_format=torch.contiguous_format)
                     width = g.shape[1]
                 need_x, need_w, need_b = ctx.needs_input_grad[:3]
                 need_b = need_b and b_dtype is not None

@@ -26,3 +26,24 @@ def test_layers_of_too_many_features_are_refused_before_they_run(dtype):
         wide = M.MAX_BF16_DW_WIDTH + 8
         with pytest.raises(ValueError, match="features"):
             _fused_linear(new(4, wide), new(8, wide).requires_grad_(), None, "relu", None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("M,K,N", [(1, 64, 64), (1, 520, 264), (2, 520, 264)])
+def test_the_gradient_of_a_layer_joined_with_another_of_few_rows(dtype, residual, M, K, N):
+    """``cat`` hands back slices of a wider gradient; a single row of one counts as contiguous whatever its row stride is.  Whole
+    numbers, so that every product is exact."""
+    from mitune.ops.linear import linear
+    g = torch.Generator(device="cuda").manual_seed(5)
+    new = lambda *s: torch.randint(-2, 3, s, device="cuda", generator=g).to(dtype)          # noqa: E731
+    leaves = [t.requires_grad_() for t in (new(M, K), new(N, K), new(N), new(M, N))]
+    other, dy = new(M, 40), new(M, 40 + N + 40)
+    used = leaves if residual else leaves[:3]
+    y = linear(*leaves[:3], residual=leaves[3] if residual else None)
+    got = torch.autograd.grad(torch.cat([other, y, other], dim=1), used, dy)
+    d = dy[:, 40:40 + N].double()
+    want = [d @ leaves[1].detach().double(), d.T @ leaves[0].detach().double(), d.sum(0), d]
+    for a, b in zip(got, want):
+        assert torch.equal(a, b.to(dtype))
