@@ -28,7 +28,7 @@ from typing import Optional, Sequence, Union
 import numpy as np
 import torch
 
-from .lib import PACKED_ITEM_BYTES, PACKED_OWN_ROWS, PACKED_SPLIT_ROWS
+from .lib import PACKED_ITEM_BYTES, PACKED_OWN_ROWS, PACKED_SPLIT_ROWS, transformed
 
 RELU_EPS = 1e-6
 MAX_SEQ = 128
@@ -87,9 +87,9 @@ def _kernel_envelope(t: torch.Tensor, S: int, dk: int, dv: int) -> bool:
     return widest <= MAX_HEAD_DIM or (widest <= WIDE_HEAD_DIM and S <= WIDE_MAX_SEQ)
 
 
-def _packed_envelope(t: torch.Tensor, dk: int, dv: int, kind: str, dropout_p: float) -> bool:
-    """What the kernels for sequences of any length take of the calls below: softmax scores without dropout."""
-    return (t.is_cuda and t.dtype in (torch.float32, torch.bfloat16) and t.numel() > 0 and kind == "softmax" and dropout_p == 0.0
+def _packed_envelope(t: torch.Tensor, dk: int, dv: int, kind: str, dropout_p: float, *more: torch.Tensor) -> bool:
+    """What the kernels for sequences of any length take of the calls below: softmax scores without dropout, outside of transforms."""
+    return (not transformed(t, *more) and t.is_cuda and t.dtype in (torch.float32, torch.bfloat16) and t.numel() > 0 and kind == "softmax" and dropout_p == 0.0
             and 0 < dk <= PACKED_MAX_HEAD_DIM and 0 < dv <= PACKED_MAX_HEAD_DIM)
 
 
@@ -139,7 +139,7 @@ def self_attention(qk: torch.Tensor, v: torch.Tensor, num_heads: int, kind: str 
                 from .rng import next_seed
                 seed = next_seed(qk.device)
             return FusedSelfAttention.apply(qk, v, h, kind, None, dropout_p, seed)
-    if _packed_envelope(qk, dk, dv, kind, dropout_p) and v.dtype == qk.dtype:
+    if _packed_envelope(qk, dk, dv, kind, dropout_p, v) and v.dtype == qk.dtype:
         return _packed_self_attention(qk.reshape(B * S, w2).chunk(2, dim=1) + (v.reshape(B * S, h * dv),), B, S, h, dk, dv)
     keep = None
     if dropout_p > 0.0:
@@ -268,7 +268,7 @@ class SequencePack:
 def packed_attention_reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pack: SequencePack, causal: bool = False,
                                scale: Optional[float] = None) -> torch.Tensor:
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
-    group = q.shape[1] // k.shape[1]
+    group = int(q.shape[1]) // int(k.shape[1])          # numbers under a tracer too
     out, at = [], 0
     for n in pack.lengths.tolist():
         qs, ks, vs = (t[at:at + n].transpose(0, 1) for t in (q, k, v))
@@ -282,12 +282,19 @@ def packed_attention_reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor
     return torch.cat(out)
 
 
+def packed_attention_plain(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pack: SequencePack, causal: bool,
+                           scale: float) -> torch.Tensor:
+    """The formula in f32, rounded once, for what the kernels do not serve."""
+    return packed_attention_reference(q.float(), k.float(), v.float(), pack, causal, scale).to(q.dtype)
+
+
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pack: SequencePack, causal: bool = False,
                      scale: Optional[float] = None) -> torch.Tensor:
     """Softmax attention within every sequence of ``pack``: ``q`` [rows, heads, dk], ``k`` [rows, kv_heads, dk], ``v``
-    [rows, kv_heads, dv] -> [rows, heads, dv], all f32 or all bf16, differentiable (a second time too, through
-    plain torch).  Query head ``i`` reads key / value head ``i // (heads // kv_heads)``; with ``causal`` a row sees its sequence's rows up to itself.  ``scale`` defaults to
-    ``1 / sqrt(dk)``.  Rows behind the last sequence give zeros, and nothing of what they hold is used.
+    [rows, kv_heads, dv] -> [rows, heads, dv], all f32 or all bf16, differentiable.  Query head ``i`` reads key / value head
+    ``i // (heads // kv_heads)``; with ``causal`` a row sees its sequence's rows up to itself.  ``scale`` defaults to
+    ``1 / sqrt(dk)``.  Second derivatives, forward-mode differentiation, ``torch.func`` transforms and tracing go through plain
+    torch, which holds a sequence's scores in memory.  Rows behind the last sequence give zeros, and nothing of what they hold is used.
 
     On a GPU: heads of at most 128 elements.  Operands may be strided (a slice of a fused projection is read in place when its
     rows lie on 16-byte boundaries and is copied otherwise).  f32 operands are multiplied exactly; for bf16 the probabilities
@@ -318,6 +325,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pack: Se
         raise ValueError(f"packed_attention on a GPU takes heads of at most {PACKED_MAX_HEAD_DIM} elements, got {max(dk, dv)}")
     if pack.device != q.device:
         raise ValueError(f"the pack lies on {pack.device}, the operands on {q.device}")
+    if transformed(q, k, v):
+        return packed_attention_plain(q, k, v, pack, causal, scale)
     from .attention_hip import PackedAttention, in_place, packed_forward
     from .lib import wants_grad
     q, k, v = in_place(q), in_place(k), in_place(v)

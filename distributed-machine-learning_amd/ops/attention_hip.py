@@ -246,9 +246,9 @@ class PackedAttention(torch.autograd.Function):
         so = L.load()
         q, k, v, out, low, lse = ctx.saved_tensors
         pack, (causal, scale) = ctx.pack, ctx.meta
-        if torch.is_grad_enabled():
-            from .attention import packed_attention_reference
-            plain = lambda *t: packed_attention_reference(*(u.float() for u in t), pack, causal, scale).to(q.dtype)     # noqa: E731
+        if L.formula_backward(grad_out):
+            from .attention import packed_attention_plain
+            plain = lambda *t: packed_attention_plain(*t, pack, causal, scale)                                          # noqa: E731
             return (*L.grads_by_formula(plain, (q, k, v), grad_out), None, None, None)
         do = in_place(grad_out if grad_out.dtype == q.dtype else grad_out.to(q.dtype))
         delta = torch.empty_like(lse)

@@ -16,14 +16,15 @@ import torch
 import torch.nn.functional as F
 
 from .layernorm_hip import LayerNorm, norm_forward
-from .lib import wants_grad
+from .lib import transformed, wants_grad
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5) -> torch.Tensor:
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension, differentiable, in ``x``'s type; statistics and
     column sums in f32.  ``weight`` and ``bias`` ([d], either may be missing) have ``x``'s type, or f32 beside a bf16 ``x``.  On a
-    GPU ``x`` is f32 or bf16, rows of any width; rows may lie apart (a column slice of a wider tensor is read in place)."""
+    GPU ``x`` is f32 or bf16, rows of any width; rows may lie apart (a column slice of a wider tensor is read in place).  Second
+    derivatives, forward-mode differentiation, ``torch.func`` transforms and tracing go through plain torch."""
     shape, device = x.shape, x.device
     if len(shape) < 1 or shape[-1] < 1:
         raise ValueError(f"layer_norm needs rows of at least one column, got {tuple(shape)}")
@@ -41,7 +42,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         raise TypeError(f"weight and bias must share a type, got {weight.dtype} and {bias.dtype}")
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    if not x.is_cuda:
+    if not x.is_cuda or transformed(x, weight, bias):
         wide = torch.promote_types(x.dtype, weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype)
         cast = lambda t: None if t is None else t.to(wide)          # noqa: E731
         return F.layer_norm(x.to(wide), (d,), cast(weight), cast(bias), eps).to(x.dtype)
@@ -78,7 +79,7 @@ def residual_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.T
         from .elementwise import keep_mask
         keep = keep_mask(x.shape, dropout_p, x.device)
     if (x.is_cuda and x.dtype == residual.dtype == weight.dtype == bias.dtype and x.dtype in (torch.float32, torch.bfloat16)
-            and x.shape == residual.shape and not torch.is_autocast_enabled()):
+            and x.shape == residual.shape and not torch.is_autocast_enabled() and not transformed(x, residual, weight, bias)):
         if keep is not None:                # rows the fused kernels do not take: the norm alone on its own kernels
             x = x * keep.to(x.dtype) * (1.0 / (1.0 - dropout_p))
         return layer_norm(residual + x, weight, bias, eps)

@@ -175,7 +175,7 @@ class LayerNorm(torch.autograd.Function):
         xr, w, stats, x, weight = ctx.saved_tensors
         shape, flags, has_w, has_b, pdtype, eps = ctx.meta
         M, d = xr.shape
-        if torch.is_grad_enabled():
+        if L.formula_backward(grad_y):
             bias = torch.zeros(d, device=xr.device, dtype=pdtype, requires_grad=ctx.needs_input_grad[2]) if has_b else None
             cast = lambda t: None if t is None else t.float()                                                    # noqa: E731
             plain = lambda x, w, b: F.layer_norm(x.float(), (d,), cast(w), cast(b), eps).to(grad_y.dtype)       # noqa: E731

@@ -384,20 +384,40 @@ def on(device):
     return _SAME_DEVICE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
-def wants_grad(*tensors) -> bool:
-    """Whether autograd would record an operation on these (``None`` allowed): if not, a binding's forward is called directly,
-    which halves the host time of a small call."""
+def transformed(*tensors) -> bool:
+    """Whether something other than reverse-mode autograd follows an operation on these (``None`` allowed): a tangent of forward-mode
+    differentiation, a ``torch.func`` transform, a tracer or another dispatch mode.  A kernel works on addresses, so its launch is
+    invisible to all of them: a tangent would be dropped (a derivative of zero, without an error), a traced graph would lack the
+    result, a tensor of a mode may have no memory at all."""
     import torch
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch._C._are_functorch_transforms_active() or torch._C._is_tracing() or torch._C._len_torch_dispatch_stack():
+        return True
+    forward_ad = torch.autograd.forward_ad
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def formula_backward(grad) -> bool:
+    """Whether a backward pass with the upstream gradient ``grad`` is one for ``grads_by_formula``: under ``create_graph``, or where
+    ``grad`` is ``transformed`` or a batch of gradients (``is_grads_batched``, whose tensors are of an older kind)."""
+    import torch
+    return torch.is_grad_enabled() or transformed(grad) or torch._C._functorch.is_legacy_batchedtensor(grad)
+
+
+def wants_grad(*tensors) -> bool:
+    """Whether autograd, or one of the others that ``transformed`` names, would record an operation on these (``None`` allowed): if
+    not, a binding's forward is called directly, which halves the host time of a small call."""
+    import torch
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or transformed(*tensors)
 
 
 def grads_by_formula(formula, inputs, grad):
-    """Gradients of ``formula(*inputs)`` (plain torch) that can be differentiated again, for backward passes under
-    ``create_graph``; the kernels' own backward passes leave no graph.  Every input stands in the formula as an alias of its own, so
+    """Gradients of ``formula(*inputs)`` (plain torch) that can be differentiated again under ``create_graph``, for the backward
+    passes that the kernels do not serve (``formula_backward``): theirs leave no graph.  Every input stands in the formula as an alias of its own, so
     that its gradient is that of its place alone, also where one tensor takes several places or one input was computed from another."""
     import torch
+    again = torch.is_grad_enabled()
     with torch.enable_grad():
         places = [None if t is None else t.view_as(t) for t in inputs]
         wanted = [t for t in places if t is not None and t.requires_grad]
-        got = iter(torch.autograd.grad(formula(*places), wanted, grad, create_graph=True))
+        got = iter(torch.autograd.grad(formula(*places), wanted, grad, create_graph=again))
     return [next(got) if t is not None and t.requires_grad else None for t in inputs]

@@ -24,7 +24,8 @@ bf16.
 The tile kernels read rows in 16-byte pieces, so a dimension that is not a multiple of 4 (f32) or 8 (bf16) -- 81 input
 features, a scalar output -- is padded with zero columns / zero rows up to the next multiple before the launch and the
 result is sliced back; autograd carries the slice through, so gradients of the padding are dropped.  Operands these
-kernels cannot take at all (f16 or f64 on a GPU) raise ``TypeError`` instead of taking a slower road silently.
+kernels cannot take at all (f16 or f64 on a GPU) raise ``TypeError`` instead of taking a slower road silently; so do, with
+autograd's own errors, forward-mode differentiation and ``torch.func`` transforms of a call on a GPU.
 """
 from __future__ import annotations
 
@@ -425,7 +426,7 @@ class FusedLinear(torch.autograd.Function):
         dx = dw = db = None
         if any(ctx.needs_input_grad[:3]):
             xc, wc, s, x, weight, bias = ctx.saved_tensors
-            if torch.is_grad_enabled():
+            if L.formula_backward(dy):
                 return _twice_differentiable(ctx, dy, xc if x is None else x, wc if weight is None else weight, bias)
             out_f = wc.shape[0]
             bf16, dev, M = xc.dtype == torch.bfloat16, xc.device, xc.shape[0]
