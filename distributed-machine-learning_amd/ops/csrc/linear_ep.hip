@@ -352,6 +352,7 @@ extern "C" int mt_linear_gemm_launch(int mode, const void* A, const void* B, con
   if (lda > (bf16 ? 1 << 28 : LF_MAX_LD - 1) || ldb > (bf16 ? 1 << 28 : LF_MAX_LD - 1) || N > 2000000 || act < 0 || act > 2) return -2;
   if ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B)) & 15) return -2;
   if (M == 0) return 0;
+  if (!A || !B || !C) return -2;      // tensors without memory (of a dispatch mode) have null addresses
   if (mode == 0 && M <= LINEAR_FEW_ROWS) {
     const MtLinearEp ep = {bias, residual, z, nullptr, bias_bf16, act, N, N};
     if (bf16 && M <= 16) linear_few<__bf16, 1>(A, B, ep, C, (int)M, N, KK, lda, ldb, stream);
@@ -409,6 +410,7 @@ static void linear_wgrad_f32(const MtGemmGroup& g, const MtLinearEp& ep, int spl
 extern "C" int mt_linear_wgrad_f32_parts_launch(const void* dz, const void* x, float* arena, int64_t M, int N, int K, int splits,
                                                 int64_t slab, int with_bias, hipStream_t stream) {
   if (M < 1 || M > 0x7FFFFFFF - 256 || N < 1 || K < 1 || N % 4 || K % 4 || N >= LF_MAX_LD || K >= LF_MAX_LD) return -2;
+  if (!dz || !x || !arena) return -2;
   if (splits < 2 || splits > 127 || slab % 4 || slab < (int64_t)N * K + (with_bias ? N : 0)) return -2;
   MtGemmGroup g = linear_group(dz, x, arena, N, K, (int)M, N, K, K);
   if (with_bias) g.aux_out = arena + (int64_t)N * K;
@@ -424,6 +426,7 @@ extern "C" int mt_linear_wgrad_launch(const void* dz, const void* x, void* dw, v
                                       int db_bf16, int bf16, hipStream_t stream) {
   const int per = bf16 ? 8 : 4, es = bf16 ? 2 : 4;
   if (M < 1 || M > 0x7FFFFFFF - 256 || N < 1 || K < 1 || ld_dz % per || ldx % per || ld_dz < N || ldx < K) return -2;
+  if (!dz || !x || !dw) return -2;
   const int flags = db != nullptr ? MT_GEMM_FLAG_DBIAS : 0;
   if (!bf16 && (ld_dz >= LF_MAX_LD || ldx >= LF_MAX_LD)) return -2;
   if (bf16 && (K + BN - 1) / BN > 32767) return -2;    // a 128-tile's column number is 16 bits
@@ -481,6 +484,7 @@ extern "C" int mt_linear_act_bwd_launch(const void* dy, const void* s, void* dz,
   if (M < 0 || N < 1 || ld_dz % per || ld_dz < N || ld_dz - N >= per || ld_dy < 0 || act < 1 || act > 2) return -2;
   if ((part == nullptr) != (db == nullptr)) return -2;
   if (M == 0) return 0;
+  if (!dy || !s || !dz) return -2;
   const ActGrid g = act_grid(M, ld_dz, bf16);
   if (g.chunks > 65535) return -2;
   const dim3 grid((unsigned)g.strips, (unsigned)g.chunks);
@@ -501,7 +505,7 @@ extern "C" int mt_linear_act_bwd_launch(const void* dy, const void* s, void* dz,
 // dw [rows][cols], db [rows] (may be null).
 extern "C" int mt_linear_wsum_launch(const float* arena, void* dw, void* db, int64_t rows, int cols, int ld, int64_t db_at, int splits,
                                      int64_t slab, int w_bf16, int b_bf16, hipStream_t stream) {
-  if (rows < 1 || cols < 1 || ld < cols || splits < 1 || slab < db_at) return -2;
+  if (rows < 1 || cols < 1 || ld < cols || splits < 1 || slab < db_at || !arena || !dw) return -2;
   const int64_t blocks = (rows * cols + rows + 255) / 256;
   const dim3 grid((unsigned)(blocks < 16384 ? blocks : 16384));
 #define GO(P, B)                                                                                                                \

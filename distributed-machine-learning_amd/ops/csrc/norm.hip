@@ -527,6 +527,7 @@ extern "C" int mt_norm_fwd_launch(const void* x, const void* w, const void* b, v
                                   int d, float eps, int x_bf16, int w_bf16, hipStream_t stream) {
   if (!norm_args(rows, stride, d, x_bf16, w_bf16)) return -2;
   if (rows == 0) return 0;
+  if (!x || !y) return -2;      // tensors without memory (of a dispatch mode) have null addresses
   if (!x_bf16) return norm_fwd<float, float>(x, w, b, y, stats, rows, stride, d, eps, stream);
   if (!w_bf16) return norm_fwd<__bf16, float>(x, w, b, y, stats, rows, stride, d, eps, stream);
   return norm_fwd<__bf16, __bf16>(x, w, b, y, stats, rows, stride, d, eps, stream);
@@ -537,6 +538,7 @@ extern "C" int mt_norm_bwd_launch(const void* dy, const void* x, const void* w, 
                                   hipStream_t stream) {
   if (!norm_args(rows, stride, d, x_bf16, w_bf16) || dy_stride < 0) return -2;
   if (rows == 0) return 0;
+  if (!dy || !x || !stats || !dx || (part != nullptr) != (dw != nullptr || db != nullptr)) return -2;
   if (!x_bf16) return norm_bwd<float, float>(dy, x, w, stats, dx, part, dw, db, rows, stride, dy_stride, d, stream);
   if (!w_bf16) return norm_bwd<__bf16, float>(dy, x, w, stats, dx, part, dw, db, rows, stride, dy_stride, d, stream);
   return norm_bwd<__bf16, __bf16>(dy, x, w, stats, dx, part, dw, db, rows, stride, dy_stride, d, stream);

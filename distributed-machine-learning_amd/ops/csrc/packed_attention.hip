@@ -1276,6 +1276,8 @@ extern "C" int mt_packed_attn_launch(const MtPackedAttn* a, int backward, int bf
   const MtPackedAttn p = *a;
   if (p.n_items <= 0) return 0;
   const int es = bf16 ? 2 : 4, per = 16 / es;
+  if (!p.q || !p.k || !p.v) return -2;      // tensors without memory (of a dispatch mode) have null addresses
+  if (backward ? !p.out || !p.dout || !p.dq || !p.dk || !p.dv || !p.lse || !p.delta : !p.o) return -2;
   if (p.head_k < 1 || p.head_v < 1 || p.head_k > 128 || p.head_v > 128 || p.head_k % per || p.head_v % per) return -2;
   if (p.heads < 1 || p.kv_heads < 1 || p.heads % p.kv_heads || p.n_kv_items < 0) return -2;
   if (p.split < 0 || p.split > 2 || p.kv_split < 0 || p.kv_split > 2 || (!bf16 && (p.split == 0 || p.kv_split == 0))) return -2;

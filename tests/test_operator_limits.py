@@ -28,6 +28,35 @@ def test_layers_of_too_many_features_are_refused_before_they_run(dtype):
             _fused_linear(new(4, wide), new(8, wide).requires_grad_(), None, "relu", None)
 
 
+def test_null_addresses_are_refused_by_the_launchers():
+    """Tensors of a dispatch mode that hold no memory have address 0; each operand in turn."""
+    from mitune.ops import lib as L
+    so = L.load()
+    gemm = lambda a, b, c, m: so.mt_linear_gemm_launch(0, a, b, None, None, c, None, None, m, 8, 8, 8, 8, 0, 0, 0, None)          # noqa: E731
+    calls = [lambda *p: gemm(*p, 4), lambda *p: gemm(*p, 400),
+             lambda *p: so.mt_linear_act_bwd_launch(*p, None, None, 8, 8, 8, 8, 1, 0, 0, None),
+             lambda *p: so.mt_linear_wgrad_f32_parts_launch(*p, 8, 8, 8, 2, 128, 1, None),
+             lambda *p: so.mt_linear_wgrad_launch(*p, None, 8, 8, 8, 8, 8, 0, 0, None)]
+    for call in calls:
+        for null in range(3):
+            assert call(*(None if i == null else 16 for i in range(3))) == -2
+    assert so.mt_norm_fwd_launch(None, None, None, 16, None, 8, 8, 8, 1e-5, 0, 0, None) == -2
+    assert so.mt_norm_fwd_launch(16, None, None, None, None, 8, 8, 8, 1e-5, 0, 0, None) == -2
+    for null in (0, 1, 3, 4):
+        args = [16, 16, None, 16, 16]
+        args[null] = None
+        assert so.mt_norm_bwd_launch(*args, None, None, None, 8, 8, 8, 8, 0, 0, None) == -2
+    for part, dw, db in ((16, None, None), (None, 16, None), (None, None, 16)):
+        assert so.mt_norm_bwd_launch(16, 16, None, 16, 16, part, dw, db, 8, 8, 8, 8, 0, 0, None) == -2
+    # q, k, v, out, dout, o, dq, dk, dv, low, lse, delta, halves and the lists of items: one uniform sequence of 8 rows
+    used = {0: (0, 1, 2, 5), 1: (0, 1, 2, 3, 4, 6, 7, 8, 10, 11)}
+    for backward, places in used.items():
+        for null in places:
+            at = [16 if i in places and i != null else 0 for i in range(15)]
+            args = L.PACKED_ATTN_FORMAT.pack(*at, *[8] * 8, 8, 1, 1, 8, 1, 1, 1, 8, 8, 0, 1, 1, 0, 1.0)
+            assert so.mt_packed_attn_launch(args, backward, 0, None) == -2
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("residual", [False, True])
