@@ -193,8 +193,8 @@ __global__ __launch_bounds__(WAVES * 64) void mt_linear_few_kernel(const T* __re
   }
 }
 
-// dz = dy act'(s): s is z, or (ReLU without a residual) y, whose sign is z's; and the column sums of dz before it is rounded, from
-// which db comes (sums of rounded terms would be off by half again as much).  `lanes` threads (a power of two) take the 16-byte
+// dz = dy act'(s): s is z, or (ReLU without a residual) y, whose sign is z's; and, where dz's rounding loses something (bf16, GELU),
+// the column sums of dz before it, from which db comes (sums of rounded terms would be off by half again as much).  `lanes` threads (a power of two) take the 16-byte
 // pieces of a row side by side, 256 / lanes rows at a time; a workgroup walks over the rows of its chunk and leaves one partial row.
 template <typename T>
 __global__ __launch_bounds__(256) void mt_act_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ s, T* __restrict__ dz,
@@ -263,20 +263,50 @@ __global__ __launch_bounds__(256) void mt_act_cols_kernel(const float* __restric
   db[c] = (B)v;
 }
 
-// dW [rows][cols] and db [rows]: the f32 slabs of the split contraction added in order and rounded to the parameters' types.
-// Slab s: dW with rows of ld floats, then (at db_at) db.
+// dW [rows][cols] and db [rows]: the f32 slabs of the split contraction added up and rounded to the parameters' types.  Slab s: dW
+// with rows of ld floats, then (at db_at) db.  A thread takes four columns of a row; slab s goes to sum s % 4, so that eight loads
+// are on their way, and the sums are joined in a fixed order.
+__device__ __forceinline__ f32x4 linear_slabs(const float* __restrict__ p, int splits, int64_t slab) {
+  f32x4 acc[4] = {};
+  int s = 0;
+  for (; s + 8 <= splits; s += 8) {
+    f32x4 v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const f32x4*>(p + (s + k) * slab);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[k & 3] += v[k];
+  }
+#pragma unroll 4
+  for (int k = 0; k < (splits & 7); ++k) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(p + (s + k) * slab);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += (k & 3) == e ? v : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  return (acc[0] + acc[1]) + (acc[2] + acc[3]);
+}
+template <typename P> __device__ __forceinline__ void linear_put4(P* at, f32x4 v, int n) {
+  const P o[4] = {(P)v[0], (P)v[1], (P)v[2], (P)v[3]};
+  if (n >= 4) __builtin_memcpy(at, o, sizeof(o));
+  else {
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (e < n) at[e] = o[e];
+  }
+}
 template <typename P, typename B>
 __global__ __launch_bounds__(256) void mt_linear_wsum_kernel(const float* __restrict__ arena, P* __restrict__ dw, B* __restrict__ db,
                                                              int64_t rows, int cols, int ld, int64_t db_at, int splits, int64_t slab) {
-  const int64_t total = rows * cols + (db != nullptr ? rows : 0);
+  const uint32_t per_row = (uint32_t)(cols + 3) / 4;
+  const int64_t of_w = rows * per_row, total = of_w + (db != nullptr ? (rows + 3) / 4 : 0);
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const bool is_w = i < rows * cols;
-    const int64_t row = i / cols;
-    const float* p = arena + (is_w ? row * ld + (i - row * cols) : db_at + (i - rows * cols));
-    float v = 0.f;
-    for (int s = 0; s < splits; ++s) v += p[s * slab];
-    if (is_w) dw[i] = (P)v;
-    else db[i - rows * cols] = (B)v;
+    if (i < of_w) {
+      const int64_t row = of_w <= 0xFFFFFFFFll ? (int64_t)((uint32_t)i / per_row) : i / per_row;
+      const int col = (int)(i - row * per_row) * 4;
+      linear_put4(dw + row * cols + col, linear_slabs(arena + row * ld + col, splits, slab), cols - col);
+    } else {
+      const int64_t row = (i - of_w) * 4;
+      linear_put4(db + row, linear_slabs(arena + db_at + row, splits, slab), rows - row < 4 ? (int)(rows - row) : 4);
+    }
   }
 }
 
@@ -456,14 +486,15 @@ extern "C" int mt_linear_wgrad_launch(const void* dz, const void* x, void* dw, v
 struct ActGrid {
   int lanes, strips, chunks, per;
 };
-static ActGrid act_grid(int64_t M, int ld_dz, int bf16) {
+static ActGrid act_grid(int64_t M, int ld_dz, int bf16, bool sums) {
   const int pieces = ld_dz / (bf16 ? 8 : 4);
   ActGrid g;
   g.lanes = 4;
   while (g.lanes < 64 && g.lanes < pieces) g.lanes *= 2;
   g.strips = (pieces + g.lanes - 1) / g.lanes;
-  int64_t chunks = (2048 + g.strips - 1) / g.strips;                     // about eight workgroups per CU ...
-  const int64_t deep = M / (16 * (256 / g.lanes));                       // ... that walk over sixteen groups of rows or more
+  // About eight workgroups per CU; with column sums, each of which costs a partial row, they walk over an unrolled batch of rows or more.
+  int64_t chunks = (2048 + g.strips - 1) / g.strips;
+  const int64_t deep = M / ((sums ? 4 : 1) * (256 / g.lanes));
   if (chunks > deep) chunks = deep;
   if (chunks < 1) chunks = 1;
   if (chunks < M / (1 << 24)) chunks = M / (1 << 24) + 1;
@@ -474,7 +505,7 @@ static ActGrid act_grid(int64_t M, int ld_dz, int bf16) {
 // Rows of the partial-sum workspace [n][N] f32.
 extern "C" int mt_linear_act_parts(int64_t M, int ld_dz, int bf16) {
   if (M < 1 || ld_dz < 1 || ld_dz % (bf16 ? 8 : 4)) return -2;
-  return act_grid(M, ld_dz, bf16).chunks;
+  return act_grid(M, ld_dz, bf16, true).chunks;
 }
 // s: z or y [M][N] contiguous; dz [M][ld_dz], ld_dz a multiple of a 16-byte piece, zeros behind column N.  db [N] with its workspace
 // `part`, or both null.
@@ -485,7 +516,7 @@ extern "C" int mt_linear_act_bwd_launch(const void* dy, const void* s, void* dz,
   if ((part == nullptr) != (db == nullptr)) return -2;
   if (M == 0) return 0;
   if (!dy || !s || !dz) return -2;
-  const ActGrid g = act_grid(M, ld_dz, bf16);
+  const ActGrid g = act_grid(M, ld_dz, bf16, db != nullptr);
   if (g.chunks > 65535) return -2;
   const dim3 grid((unsigned)g.strips, (unsigned)g.chunks);
   if (bf16)
@@ -505,8 +536,10 @@ extern "C" int mt_linear_act_bwd_launch(const void* dy, const void* s, void* dz,
 // dw [rows][cols], db [rows] (may be null).
 extern "C" int mt_linear_wsum_launch(const float* arena, void* dw, void* db, int64_t rows, int cols, int ld, int64_t db_at, int splits,
                                      int64_t slab, int w_bf16, int b_bf16, hipStream_t stream) {
-  if (rows < 1 || cols < 1 || ld < cols || splits < 1 || slab < db_at || !arena || !dw) return -2;
-  const int64_t blocks = (rows * cols + rows + 255) / 256;
+  if (rows < 1 || cols < 1 || ld < cols || ld % 4 || db_at % 4 || slab % 4 || splits < 1 || slab < db_at + (db != nullptr ? (rows + 3) / 4 * 4 : 0))
+    return -2;
+  if (!arena || !dw || (reinterpret_cast<uintptr_t>(arena) & 15)) return -2;
+  const int64_t blocks = (rows * ((cols + 3) / 4) + (rows + 3) / 4 + 255) / 256;
   const dim3 grid((unsigned)(blocks < 16384 ? blocks : 16384));
 #define GO(P, B)                                                                                                                \
   hipLaunchKernelGGL((mt_linear_wsum_kernel<P, B>), grid, dim3(256), 0, stream, arena, (P*)dw, (B*)db, rows, cols, ld, db_at, splits, \
@@ -520,16 +553,19 @@ extern "C" int mt_linear_wsum_launch(const float* arena, void* dw, void* db, int
 }
 
 // The whole backward pass of a layer in one call: dz (with db from it before its rounding, where part_at is set), dx, then dW and what
-// is left of db.  Offsets into the workspace are in bytes, negative where a piece is not needed; splits 0: dW leaves in its own type.
+// is left of db.  Offsets into the workspace are in bytes, negative where a piece is not needed; splits 0: dW leaves in its own type;
+// -1: a small f32 layer (widths of whole pieces, w contiguous, dw wanted), whose gradients are one launch of small_linear.hip.
 struct MtLinearBwd {
   const void *dy, *s, *x, *w;
   void *dx, *dw, *db;
   uint8_t* ws;
   int64_t M, dy_ld, ldw, dz_at, part_at, dxpart_at, arena_at, slab;
-  int32_t N, K, rows, width, act, bf16, dw_bf16, db_bf16, splits, unused;      // rows, width: N and K in whole 16-byte pieces
+  int32_t N, K, rows, width, act, bf16, dw_bf16, db_bf16, splits, small_tile;      // rows, width: N and K in whole 16-byte pieces
 };
 extern "C" int mt_wgrad_single_launch(const void* dY, const void* X, float* C, float* db, int M, int out, int in, int ksplits,
                                       size_t split_stride, hipStream_t stream);
+extern "C" int mt_small_linear_bwd_tiled_launch(const float* X, const float* W, const float* dY, float* dX, float* dW, float* db, int R, int in,
+                                                int out, int tile, hipStream_t stream);
 extern "C" int mt_linear_bwd_size() { return (int)sizeof(MtLinearBwd); }
 extern "C" int mt_linear_bwd_launch(const MtLinearBwd* a, hipStream_t stream) {
   if (a == nullptr) return -2;
@@ -542,6 +578,11 @@ extern "C" int mt_linear_bwd_launch(const MtLinearBwd* a, hipStream_t stream) {
   if (p.act)
     rc = mt_linear_act_bwd_launch(p.dy, p.s, p.ws + p.dz_at, p.part_at >= 0 ? (float*)(p.ws + p.part_at) : nullptr,
                                   p.part_at >= 0 ? p.db : nullptr, p.M, p.N, p.dy_ld, p.rows, p.act, p.db_bf16, p.bf16, stream);
+  if (p.splits < 0) {
+    if (rc != 0 || p.bf16 || p.N != p.rows || p.K != p.width || p.ldw != p.K) return rc != 0 ? rc : -2;
+    return mt_small_linear_bwd_tiled_launch((const float*)p.x, (const float*)p.w, (const float*)dz, (float*)p.dx, (float*)p.dw, (float*)late,
+                                            (int)p.M, p.K, p.N, p.small_tile, stream);
+  }
   if (rc == 0 && p.dx != nullptr)
     rc = mt_linear_gemm_launch(1, dz, p.w, nullptr, nullptr, p.dx, nullptr, p.dxpart_at >= 0 ? (float*)(p.ws + p.dxpart_at) : nullptr,
                                p.M, p.K, p.N, p.rows, p.ldw, 0, 0, p.bf16, stream);

@@ -123,7 +123,8 @@ __device__ __forceinline__ float colsum_stage(const uint8_t* ldsA, int tid) {
 // A wave's R*16 x 64 block.  `img` is its own [R*16][64] bf16 staging image: an accumulator lane holds 4 columns of a row, so
 // stores go through LDS as whole 16-byte pieces of 128-byte row segments, and the residual comes in the same way.  Rows of
 // the output need no alignment (columns past J are left alone); LDS traffic stays inside the wave, which executes in order.
-template <int R>
+// FULL: the forward pass; a gradient has no bias, z, activation or residual.
+template <int R, bool FULL>
 __device__ __forceinline__ void mt_linear_epilogue(const f32x4 (&acc)[R][4], uint8_t* img, int qi0, int qj0, const MtGemmGroup& g,
                                                    const MtLinearEp& ep, int lane) {
   const int fq = lane >> 4, fr = lane & 15;
@@ -162,7 +163,7 @@ __device__ __forceinline__ void mt_linear_epilogue(const f32x4 (&acc)[R][4], uin
   };
   auto bias4 = [&](int n) {
     f32x4 b = {0.f, 0.f, 0.f, 0.f};
-    if (ep.bias != nullptr) {
+    if (FULL && ep.bias != nullptr) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int col = qj0 + n * 16 + fq * 4 + j;
@@ -171,7 +172,8 @@ __device__ __forceinline__ void mt_linear_epilogue(const f32x4 (&acc)[R][4], uin
     }
     return b;
   };
-  if (ep.z != nullptr) {
+  const bool residual = FULL && ep.residual != nullptr;
+  if (FULL && ep.z != nullptr) {
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       const f32x4 b = bias4(n);
@@ -185,7 +187,7 @@ __device__ __forceinline__ void mt_linear_epilogue(const f32x4 (&acc)[R][4], uin
     }
     flush(reinterpret_cast<uint16_t*>(ep.z), ep.ldz);
   }
-  if (ep.residual != nullptr) {
+  if (residual) {
     const uint16_t* res = reinterpret_cast<const uint16_t*>(ep.residual);
 #pragma unroll 4
     for (int t = 0; t < 2 * R; ++t) {
@@ -206,24 +208,26 @@ __device__ __forceinline__ void mt_linear_epilogue(const f32x4 (&acc)[R][4], uin
     }
     fence();
   }
+  mt_ep_for_act(FULL ? ep.act : MT_ACT_NONE, [&](auto act) {
 #pragma unroll
-  for (int n = 0; n < 4; ++n) {
-    const f32x4 b = bias4(n);
+    for (int n = 0; n < 4; ++n) {
+      const f32x4 b = bias4(n);
 #pragma unroll
-    for (int m = 0; m < R; ++m) {
-      const int lrow = m * 16 + fr, lcol = n * 16 + fq * 4;
-      u32x2* at = reinterpret_cast<u32x2*>(img + kmaj_off(lrow, lcol >> 3) + (lcol & 7) * 2);
-      float v[4];
+      for (int m = 0; m < R; ++m) {
+        const int lrow = m * 16 + fr, lcol = n * 16 + fq * 4;
+        u32x2* at = reinterpret_cast<u32x2*>(img + kmaj_off(lrow, lcol >> 3) + (lcol & 7) * 2);
+        float v[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = mt_ep_act<true>(acc[m][n][j] + b[j], ep.act);
-      if (ep.residual != nullptr) {
-        const u32x2 r = *at;
+        for (int j = 0; j < 4; ++j) v[j] = mt_ep_act<true>(acc[m][n][j] + b[j], act.value);
+        if (residual) {
+          const u32x2 r = *at;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] += bf16_bits_to_f32((r[j >> 1] >> (16 * (j & 1))) & 0xFFFFu);
+          for (int j = 0; j < 4; ++j) v[j] += bf16_bits_to_f32((r[j >> 1] >> (16 * (j & 1))) & 0xFFFFu);
+        }
+        *at = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
       }
-      *at = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
     }
-  }
+  });
   flush(reinterpret_cast<uint16_t*>(g.C), g.ldc);
 }
 
@@ -317,7 +321,7 @@ __device__ __forceinline__ void gemm_tile(const MtGemmGroup* __restrict__ groups
 
   // ------------------------------------------------------------------------------ epilogues
   if constexpr (EP) {
-    mt_linear_epilogue<4>(acc, lds + wave * 8192, i0 + wr * 64, j0 + wc * 64, g, *ep, lane);
+    mt_linear_epilogue<4, MODE == 0>(acc, lds + wave * 8192, i0 + wr * 64, j0 + wc * 64, g, *ep, lane);
     if (want_db) {
       __syncthreads();                               // the staging images are read
       float* red = reinterpret_cast<float*>(lds);

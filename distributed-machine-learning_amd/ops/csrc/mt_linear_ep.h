@@ -79,6 +79,15 @@ template <bool SHORT> __device__ __forceinline__ float mt_ep_act(float v, int ac
   return v;
 }
 
+// f(std::integral_constant) with the launch's activation: the loops over an accumulator are there once per activation, each a
+// straight run of instructions (asked per element, a small launch spends its time fetching code around the branches not taken).
+template <int N> struct MtAct { static constexpr int value = N; };
+template <typename F> __device__ __forceinline__ void mt_ep_for_act(int act, F&& f) {
+  if (act == MT_ACT_GELU) f(MtAct<MT_ACT_GELU>{});
+  else if (act == MT_ACT_RELU) f(MtAct<MT_ACT_RELU>{});
+  else f(MtAct<MT_ACT_NONE>{});
+}
+
 // d act(z) / dz
 template <bool SHORT> __device__ __forceinline__ float mt_ep_slope(float z, int act) {
   if (act == MT_ACT_RELU) return z > 0.f ? 1.f : 0.f;

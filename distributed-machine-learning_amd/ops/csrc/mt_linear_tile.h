@@ -208,7 +208,7 @@ __device__ __forceinline__ void linear_tile(const MtGemmGroup& g, int ti, int tj
   if (wr == 0) lt_barrier();
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // the zeros, before the epilogue takes the stages
   lt_barrier();
-  if (qi0 < g.I && qj0 < g.J) mt_linear_epilogue<8>(acc, lds + wave * 16384, qi0, qj0, g, ep, lane);
+  if (qi0 < g.I && qj0 < g.J) mt_linear_epilogue<8, MODE == 0>(acc, lds + wave * 16384, qi0, qj0, g, ep, lane);
   if (MODE == 2 && want_db) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {

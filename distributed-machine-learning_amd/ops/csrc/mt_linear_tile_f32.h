@@ -17,52 +17,54 @@
 #define LF_THREADS 256
 #define LF_LDS (40 * 1024)         // a quarter of a CU's; 32 KiB are used
 
-// A wave's R*16 x R*16 block.
-template <int R>
+// A wave's R*16 x R*16 block.  FULL: the forward pass; a gradient has no bias, z, activation or residual.
+template <int R, bool FULL>
 __device__ __forceinline__ void lf_epilogue(const f32x4 (&acc)[R][R], int qi0, int qj0, const MtGemmGroup& g, const MtLinearEp& ep, int lane) {
+  mt_ep_for_act(FULL ? ep.act : MT_ACT_NONE, [&](auto act) {
 #pragma unroll
-  for (int n = 0; n < R; ++n) {
-    const int col = qj0 + n * 16 + (lane >> 4) * 4;
-    f32x4 bb = {0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < R; ++n) {
+      const int col = qj0 + n * 16 + (lane >> 4) * 4;
+      f32x4 bb = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (ep.bias != nullptr && col + j < g.J) bb[j] = mt_ep_bias(ep, col + j);
+      for (int j = 0; j < 4; ++j)
+        if (FULL && ep.bias != nullptr && col + j < g.J) bb[j] = mt_ep_bias(ep, col + j);
 #pragma unroll
-    for (int m = 0; m < R; ++m) {
-      const int row = qi0 + m * 16 + (lane & 15);
-      if (row >= g.I || col >= g.J) continue;
-      if (ep.part != nullptr) {
-        mt_ep_put_part(ep.part, row, col, g.J, acc[m][n]);
-        continue;
-      }
-      const bool whole = col + 4 <= g.J;
-      f32x4 v = acc[m][n] + bb;
-      auto put = [&](void* base, int ld) {
-        float* p = reinterpret_cast<float*>(base) + (size_t)row * ld + col;
-        if (whole) __builtin_memcpy(p, &v, 16);
-        else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (col + j < g.J) p[j] = v[j];
+      for (int m = 0; m < R; ++m) {
+        const int row = qi0 + m * 16 + (lane & 15);
+        if (row >= g.I || col >= g.J) continue;
+        if (ep.part != nullptr) {
+          mt_ep_put_part(ep.part, row, col, g.J, acc[m][n]);
+          continue;
         }
-      };
-      if (ep.z != nullptr) put(ep.z, ep.ldz);
+        const bool whole = col + 4 <= g.J;
+        f32x4 v = acc[m][n] + bb;
+        auto put = [&](void* base, int ld) {
+          float* p = reinterpret_cast<float*>(base) + (size_t)row * ld + col;
+          if (whole) __builtin_memcpy(p, &v, 16);
+          else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = mt_ep_act<false>(v[j], ep.act);
-      if (ep.residual != nullptr) {
-        const float* p = reinterpret_cast<const float*>(ep.residual) + (size_t)row * ep.ldr + col;
-        f32x4 r = {0.f, 0.f, 0.f, 0.f};
-        if (whole) __builtin_memcpy(&r, p, 16);
-        else {
+            for (int j = 0; j < 4; ++j)
+              if (col + j < g.J) p[j] = v[j];
+          }
+        };
+        if (FULL && ep.z != nullptr) put(ep.z, ep.ldz);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (col + j < g.J) r[j] = p[j];
+        for (int j = 0; j < 4; ++j) v[j] = mt_ep_act<false>(v[j], act.value);
+        if (FULL && ep.residual != nullptr) {
+          const float* p = reinterpret_cast<const float*>(ep.residual) + (size_t)row * ep.ldr + col;
+          f32x4 r = {0.f, 0.f, 0.f, 0.f};
+          if (whole) __builtin_memcpy(&r, p, 16);
+          else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (col + j < g.J) r[j] = p[j];
+          }
+          v += r;
         }
-        v += r;
+        put(g.C, g.ldc);
       }
-      put(g.C, g.ldc);
     }
-  }
+  });
 }
 
 // One operand of a step: 64 rows (K-major, 32 of the contraction in 128 bytes: chunk c of row r at c ^ (r & 7)) or 32 rows of the
@@ -216,7 +218,7 @@ __device__ __forceinline__ void linear_tile_f32(const MtGemmGroup& g, int ti, in
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // the zeros behind the last step, before the workgroup ends
   const int qi0 = i0 + wr * (T / 2), qj0 = j0 + wc * (T / 2);
-  lf_epilogue<R>(acc, qi0, qj0, g, ep, lane);
+  lf_epilogue<R, MODE == 0>(acc, qi0, qj0, g, ep, lane);
   if (MODE == 2 && want_db && wc == 0) {
 #pragma unroll
     for (int m = 0; m < R; ++m) {

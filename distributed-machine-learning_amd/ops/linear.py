@@ -444,11 +444,14 @@ class FusedLinear(torch.autograd.Function):
                     width = g.shape[1]
                 need_x, need_w, need_b = ctx.needs_input_grad[:3]
                 need_b = need_b and b_dtype is not None
-                need_w = need_w or (need_b and not (bf16 and act))          # sums over dz's rows come with dW, or from act'
+                need_w = need_w or (need_b and not _early_sums(bf16, act))          # sums over dz's rows come with dW, or from act'
                 plan = _bwd_plan(M, out_f, width, in_f, xc.shape[1], act, bf16, w_dtype == xc.dtype, need_x, need_w, need_b,
                                  OPTIONS.wgrad_workgroups)
                 if plan is not None:
                     size, at, slab, splits = plan
+                    if splits < 0:
+                        need_w = True
+                        wc = wc if wc.stride(0) == in_f else wc.contiguous()
                     xc = xc if xc.stride(0) == xc.shape[1] else xc.contiguous()
                     ws = torch.empty(size, device=dev, dtype=torch.uint8) if size else None
                     dx = torch.empty(x_shape, device=dev, dtype=xc.dtype) if need_x else None
@@ -458,13 +461,14 @@ class FusedLinear(torch.autograd.Function):
                                                     dx.data_ptr() if need_x else 0, dw.data_ptr() if need_w else 0,
                                                     db.data_ptr() if need_b else 0, ws.data_ptr() if size else 0, M, g.stride(0),
                                                     wc.stride(0), *at, slab, out_f, in_f, width, xc.shape[1], act, bf16,
-                                                    w_dtype == torch.bfloat16, b_dtype == torch.bfloat16, splits, 0)
+                                                    w_dtype == torch.bfloat16, b_dtype == torch.bfloat16, splits,
+                                                    OPTIONS.small_linear_tile)
                     L.check(so.mt_linear_bwd_launch(args, stream), "mt_linear_bwd_launch")
                     return dx, dw, db, (dy if r_shape is not None else None), None, None
                 if act:
                     dz = torch.empty(M, out_f + -out_f % per, device=dev, dtype=xc.dtype)
                     part = None
-                    if bf16 and b_dtype is not None and ctx.needs_input_grad[2]:          # from dz before it is rounded
+                    if _early_sums(bf16, act) and b_dtype is not None and ctx.needs_input_grad[2]:
                         db = torch.empty(out_f, device=dev, dtype=b_dtype)
                         part = torch.empty(_act_parts(M, dz.shape[1], 1), out_f, device=dev, dtype=torch.float32)
                     L.check(so.mt_linear_act_bwd_launch(g.data_ptr(), s.data_ptr(), dz.data_ptr(),
@@ -500,13 +504,19 @@ def _twice_differentiable(ctx, dy, x, weight, bias):
     return (*L.grads_by_formula(plain, (x, weight, bias), dy), dy if r_shape is not None else None, None, None)
 
 
+def _early_sums(bf16: bool, act: int) -> bool:
+    """Whether db is summed from dz before its rounding, by the pass that forms dz: where that rounds, which ReLU's does not."""
+    return bf16 and act == ACTIVATIONS["gelu"]
+
+
 @functools.lru_cache(maxsize=1024)
 def _bwd_plan(M: int, out_f: int, rows: int, in_f: int, width: int, act: int, bf16: bool, same: bool, need_x: bool, need_w: bool,
               need_b: bool, workgroups: int):
     """How ``mt_linear_bwd_launch`` computes a layer's gradients: (bytes of workspace, where dz, the column sums, the parts of dx and
-    those of dW lie in it (-1: not there), floats from part to part of dW, how many; 0: unsplit).  None: a small f32 layer, or one
-    whose weight gradient takes several launches.  Kept per shape; ``workgroups`` is the option that the split follows."""
-    if not bf16 and _small(M, width, rows, True):
+    those of dW lie in it (-1: not there), floats from part to part of dW, how many; 0: unsplit, -1: a small f32 layer).  None: a
+    small f32 layer with padded widths, or one whose weight gradient takes several launches.  Kept per shape; ``workgroups`` is the option that the split follows."""
+    small = not bf16 and _small(M, width, rows, True)
+    if small and (rows != out_f or width != in_f):
         return None
     size, at = 0, []
 
@@ -515,9 +525,11 @@ def _bwd_plan(M: int, out_f: int, rows: int, in_f: int, width: int, act: int, bf
         at.append(size if wanted else -1)
         size += -(-count // 256) * 256 if wanted else 0
 
-    early = bf16 and act != 0 and need_b                    # db from dz before its rounding
+    early = _early_sums(bf16, act) and need_b
     take(act != 0, M * rows * (2 if bf16 else 4))
     take(early, _act_parts(M, rows, 1) * out_f * 4 if early else 0)
+    if small:
+        return size, (*at, -1, -1), 0, -1
     parts = _gemm_parts(1, M, in_f, out_f, int(bf16)) if need_x else 1
     take(parts > 1, parts * M * in_f * 4)
     tile = 128 if bf16 else 64

@@ -76,3 +76,32 @@ def test_the_gradient_of_a_layer_joined_with_another_of_few_rows(dtype, residual
     want = [d @ leaves[1].detach().double(), d.T @ leaves[0].detach().double(), d.sum(0), d]
     for a, b in zip(got, want):
         assert torch.equal(a, b.to(dtype))
+
+
+def test_a_small_layers_backward_pass_is_spread_over_the_chip():
+    """Captured training steps of small ReLU layers are no slower than the layer and the activation apart only while the pass that forms dz
+    is not a few workgroups' long walk, and while one call does the rest."""
+    from mitune.ops import lib as L
+    from mitune.ops.linear import ACTIVATIONS, _bwd_plan, _early_sums
+    so = L.load()
+    for M, N in ((1600, 256), (3200, 1024), (1600, 64)):
+        rows_at_once = 256 // min(64, N // 8)
+        assert so.mt_linear_act_parts(M, N, 1) * 4 * rows_at_once >= M - 4 * rows_at_once
+    assert _early_sums(True, ACTIVATIONS["gelu"]) and not _early_sums(True, ACTIVATIONS["relu"]) and not _early_sums(False, 2)
+    assert _bwd_plan(1600, 256, 256, 64, 64, 1, False, True, True, True, True, 256)[3] == -1
+    assert _bwd_plan(1600, 255, 256, 64, 64, 1, False, True, True, True, True, 256) is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N", [(1600, 64, 256), (50, 40, 33), (3200, 256, 1024)])
+def test_the_bias_gradient_of_a_relu_layer_in_bf16(M, K, N):
+    """Under ReLU a term of db is the upstream gradient or nothing: an f32 sum of M exact terms, rounded once.  ``z`` is whole numbers."""
+    from mitune.ops.linear import linear
+    g = torch.Generator(device="cuda").manual_seed(11)
+    x, w, b = (torch.randint(-1, 2, s, device="cuda", generator=g).bfloat16().requires_grad_() for s in ((M, K), (N, K), (N,)))
+    dy = torch.randn(M, N, device="cuda", generator=g).bfloat16()
+    db, = torch.autograd.grad(linear(x, w, b, activation="relu"), b, dy)
+    z = (x.double() @ w.double().T + b.double()).detach()
+    terms = dy.double() * (z > 0)
+    bound = (M + 130) * 2.0 ** -24 * terms.abs().sum(0) * (1 + 2.0 ** -8) + 2.0 ** -8 * terms.sum(0).abs()
+    assert ((db.double() - terms.sum(0)).abs() <= bound).all()
