@@ -4,7 +4,7 @@
 //   backward: with u = (x - mean) rstd and g = dy w:  dx = rstd (g - mean(g) - u mean(g u)),
 //             dw = sum over rows of dy u,  db = sum over rows of dy
 //
-// Both directions move each element once (forward 2, backward 3 tensors) and are bound by memory.  TPR threads share a row and
+// Both directions move each element once (forward 2, backward 3 tensors, and the partial rows below) and are bound by memory.  TPR threads share a row and
 // keep it in registers (NV 16-byte vectors each): the variance is the mean of the centred squares, not a difference of sums, at
 // no further read.  A row group walks over rows a grid apart with w and b in registers and the next row's loads issued before
 // the current row's reductions, so the loads of two rows are always in flight.  The column sums of the backward pass stay in
@@ -431,11 +431,14 @@ __global__ __launch_bounds__(1024) void mt_norm_cols_kernel(const float* __restr
 struct NormShape {
   int threads, nv, tpr;      // nv 0: the wide form
 };
-// Rows of at most 128 (forward 256) vectors: a wave or less per row, no barriers.  Wider rows: as many waves as hold one vector per
+// Rows of at most 128 (forward 256) vectors: a wave or less per row, no barriers.  Few rows: one wave per workgroup, spread over the
+// chip; a backward pass with a wave per row takes four, whose column sums meet in LDS: a workgroup of one row would write as many
+// bytes of partial sums as it reads (2048 x 1024 bf16, with the second launch: 20.0 us by one wave, 10.8 by four; 4095 x 512
+// 24.0 / 10.7; 200 x 256 7.2 / 6.1).  Wider rows: as many waves as hold one vector per
 // thread, or two; a forward pass goes on to four, a backward pass, which also holds two sums per column, does not.
 static NormShape norm_shape(int64_t rows, int d, int per, bool backward) {
   const int vecs = (d + per - 1) / per;
-  const int threads = rows >= 4096 ? 256 : 64;                 // few rows: one wave per workgroup, spread over the chip
+  const int threads = rows >= 4096 || (backward && vecs > 16) ? 256 : 64;
   if (vecs <= 16) return {threads, 1, 16};
   if (vecs <= 64) return {threads, 1, 64};
   if (vecs <= 128) return {threads, 2, 64};

@@ -105,3 +105,13 @@ def test_the_bias_gradient_of_a_relu_layer_in_bf16(M, K, N):
     terms = dy.double() * (z > 0)
     bound = (M + 130) * 2.0 ** -24 * terms.abs().sum(0) * (1 + 2.0 ** -8) + 2.0 ** -8 * terms.sum(0).abs()
     assert ((db.double() - terms.sum(0)).abs() <= bound).all()
+
+
+def test_column_sums_of_few_rows_take_few_partial_rows():
+    """The backward pass of a norm writes and reads an f32 partial row of dw and of db per workgroup: no more than a quarter of the rows,
+    so that they stay below the bytes of x and dy."""
+    from mitune.ops import lib as L
+    so = L.load()
+    for bf16 in (0, 1):
+        for M, d in ((2048, 1024 // (2 - bf16)), (4095, 512), (200, 256), (64, 300), (1, 256)):
+            assert so.mt_norm_bwd_parts(M, d, bf16) <= (M + 3) // 4
