@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import functools
 import os
 import struct
 from typing import Optional
@@ -384,15 +385,21 @@ def on(device):
     return _SAME_DEVICE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
+@functools.lru_cache(maxsize=1)
+def _watchers():
+    import torch
+    return (torch._C._are_functorch_transforms_active, torch._C._is_tracing, torch._C._len_torch_dispatch_stack,
+            torch.autograd.forward_ad)
+
+
 def transformed(*tensors) -> bool:
     """Whether something other than reverse-mode autograd follows an operation on these (``None`` allowed): a tangent of forward-mode
     differentiation, a ``torch.func`` transform, a tracer or another dispatch mode.  A kernel works on addresses, so its launch is
     invisible to all of them: a tangent would be dropped (a derivative of zero, without an error), a traced graph would lack the
     result, a tensor of a mode may have no memory at all."""
-    import torch
-    if torch._C._are_functorch_transforms_active() or torch._C._is_tracing() or torch._C._len_torch_dispatch_stack():
+    func, tracing, modes, forward_ad = _watchers()
+    if func() or tracing() or modes():
         return True
-    forward_ad = torch.autograd.forward_ad
     return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
@@ -404,10 +411,10 @@ def formula_backward(grad) -> bool:
 
 
 def wants_grad(*tensors) -> bool:
-    """Whether autograd, or one of the others that ``transformed`` names, would record an operation on these (``None`` allowed): if
-    not, a binding's forward is called directly, which halves the host time of a small call."""
+    """Whether autograd would record an operation on these (``None`` allowed): if not, and where nothing else follows it either
+    (``transformed``), a binding's forward is called directly, which halves the host time of a small call."""
     import torch
-    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or transformed(*tensors)
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def grads_by_formula(formula, inputs, grad):

@@ -114,7 +114,7 @@ def _fused_linear(x, weight, bias, activation, residual) -> torch.Tensor:
         raise TypeError(f"bias must be {x.dtype} or f32, got {bias.dtype}")
     if residual is not None and residual.dtype != x.dtype:
         raise TypeError(f"residual must be {x.dtype}, got {residual.dtype}")
-    wants = L.wants_grad(x, weight, bias, residual)
+    wants = L.wants_grad(x, weight, bias, residual) or L.transformed(x, weight, bias, residual)
     out_f, in_f = weight.shape
     if max(out_f, in_f) > MAX_FUSED_WIDTH and (out_f > MAX_FUSED_WIDTH or (wants and (
             x.requires_grad or (x.dtype == torch.bfloat16 and in_f > MAX_BF16_DW_WIDTH)))):

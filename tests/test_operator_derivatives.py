@@ -92,14 +92,14 @@ def test_shared_operands_of_the_norm_and_the_dense_layer():
 def test_transforms_are_seen():
     from torch._subclasses.fake_tensor import FakeTensorMode
 
-    from mitune.ops.lib import transformed, wants_grad
+    from mitune.ops.lib import transformed
     x, seen = torch.randn(3), []
 
     def look(t):
-        seen.append(transformed(None, t) and wants_grad(t, None))
+        seen.append(transformed(None, t))
         return t * 2
 
-    assert not transformed(x, None) and not wants_grad(x) and not transformed(x.clone().requires_grad_())
+    assert not transformed(x, None) and not transformed(x.clone().requires_grad_())
     torch.func.vmap(look)(torch.randn(2, 3))
     torch.func.jvp(look, (x,), (x,))
     torch.func.grad(lambda t: look(t).sum())(x)
