@@ -284,8 +284,9 @@ def packed_attention_reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor
 
 def packed_attention_plain(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pack: SequencePack, causal: bool,
                            scale: float) -> torch.Tensor:
-    """The formula in f32, rounded once, for what the kernels do not serve."""
-    return packed_attention_reference(q.float(), k.float(), v.float(), pack, causal, scale).to(q.dtype)
+    """The formula in f32, also under autocast, rounded once, for what the kernels do not serve."""
+    with torch.autocast(q.device.type, enabled=False):
+        return packed_attention_reference(q.float(), k.float(), v.float(), pack, causal, scale).to(q.dtype)
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pack: SequencePack, causal: bool = False,

@@ -423,7 +423,7 @@ def grads_by_formula(formula, inputs, grad):
     that its gradient is that of its place alone, also where one tensor takes several places or one input was computed from another."""
     import torch
     again = torch.is_grad_enabled()
-    with torch.enable_grad():
+    with torch.enable_grad(), torch.autocast(grad.device.type, enabled=False):          # the kernels do not round under autocast either
         places = [None if t is None else t.view_as(t) for t in inputs]
         wanted = [t for t in places if t is not None and t.requires_grad]
         got = iter(torch.autograd.grad(formula(*places), wanted, grad, create_graph=again))

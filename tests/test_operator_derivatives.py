@@ -245,3 +245,31 @@ def test_a_traced_call_computes(name):
     with torch.no_grad():
         traced = torch.jit.trace(call, tuple(first), check_trace=False)
         _near(traced(*second), call(*second).cpu())
+
+
+def test_formula_gradients_under_autocast_keep_their_precision():
+    """Under autocast a product of f32 matrices would be rounded to bf16: 2^-9 of its terms instead of 2^-24."""
+    from mitune.ops import lib as L
+    formula = lambda a, b: torch.tanh(a @ b)          # noqa: E731
+    a, b = (torch.randn(20, 20, generator=torch.Generator().manual_seed(s)).requires_grad_() for s in (1, 2))
+    dy = torch.ones(20, 20)
+    want = L.grads_by_formula(formula, (a, b), dy)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        got = L.grads_by_formula(formula, (a, b), dy)
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_second_derivatives_and_tangents_under_autocast():
+    from mitune.ops.attention import SequencePack, packed_attention
+    g = torch.Generator(device="cuda").manual_seed(12)
+    ops, ts = ([torch.randn(50, 2, 16, device="cuda", generator=g) for _ in range(3)] for _ in range(2))
+    pack = SequencePack([30, 20])
+    call = lambda *t: packed_attention(*t, pack, causal=True)          # noqa: E731
+    leaves = [t.clone().requires_grad_() for t in ops]
+    dy = torch.randn(50, 2, 16, device="cuda", generator=g)
+    want, tangent = torch.autograd.grad(call(*leaves), leaves, dy, create_graph=True), _tangent(call, ops, ts)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        got, other = torch.autograd.grad(call(*leaves), leaves, dy, create_graph=True), _tangent(call, ops, ts)
+    for a, b in zip((*got, other), (*want, tangent)):
+        _near(a.detach(), b.detach().cpu())
