@@ -115,3 +115,22 @@ def test_column_sums_of_few_rows_take_few_partial_rows():
     for bf16 in (0, 1):
         for M, d in ((2048, 1024 // (2 - bf16)), (4095, 512), (200, 256), (64, 300), (1, 256)):
             assert so.mt_norm_bwd_parts(M, d, bf16) <= (M + 3) // 4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("which", [(None, None), ("w", None), (None, "b")])
+def test_a_residual_norm_without_parameters(dtype, which):
+    """As plain torch takes it, and as these widths took it before they had kernels."""
+    import torch.nn.functional as F
+
+    from mitune.ops.layernorm import residual_layer_norm
+    g = torch.Generator(device="cuda").manual_seed(13)
+    x, r = (torch.randn(30, 81, device="cuda", generator=g).to(dtype) for _ in range(2))
+    w, b = (None if n is None else torch.randn(81, device="cuda", generator=g).to(dtype) for n in which)
+    y = residual_layer_norm(x, r, w, b)
+    wide = [None if t is None else t.double() for t in (w, b)]
+    want = F.layer_norm((x + r).double(), (81,), *wide)
+    half = torch.finfo(dtype).eps / 2
+    # f32 statistics of 81 terms, 100 u; the product with w and the sum with b, of order 10; one rounding of the output
+    assert ((y.double() - want).abs() <= 200 * 2.0 ** -24 * (1 + want.abs()) * 4 + half * want.abs() * (1 + half)).all()
