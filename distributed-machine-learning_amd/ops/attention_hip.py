@@ -194,8 +194,16 @@ def packed_form(pack, lanes: int, bf16: bool) -> int:
 
 def _packed_launch(so, pack, q, k, v, causal: bool, scale: float, backward: int, out=0, dout=None, o=0, dq=0, dk=0, dv=0, low=0,
                    lse=0, delta=0) -> None:
-    stream, bf16 = L.raw_stream(q.device), q.dtype == torch.bfloat16
+    bf16 = q.dtype == torch.bfloat16
     form, kv_form = packed_form(pack, q.shape[1], bf16), packed_form(pack, k.shape[1], bf16)
+    # A launch has fewer than 2^32 threads: 256 per piece and head; in the shared form's dk / dv 512, and shared heads' walks may be cut
+    # in two.  A forward pass that keeps what the backward pass needs is refused where that would be.
+    pieces = pack._counts[form] * q.shape[1]
+    if backward or lse:
+        pieces = max(pieces, pack._counts[kv_form] * k.shape[1] * (1 if kv_form else 2 if q.shape[1] == k.shape[1] else 4))
+    if pieces >= 1 << 24:
+        raise ValueError(f"{len(pack.lengths)} sequences of {pack.total} rows with {q.shape[1]} heads are more pieces than a launch takes")
+    stream = L.raw_stream(q.device)
     items, n = pack._items(form, 0 if causal else 2, stream)
     kv_items, n_kv = pack._items(kv_form, 1 if causal else 2, stream)
     # a uniform batch has no list in which short sequences are marked: its sequences are short, or none is

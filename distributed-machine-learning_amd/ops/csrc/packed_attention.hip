@@ -1289,8 +1289,10 @@ extern "C" int mt_packed_attn_launch(const MtPackedAttn* a, int backward, int bf
     }
   }
   if (p.cut != 0 && (p.cut < 0 || (int64_t)p.cut * p.kv_heads * (PA_OWN / PA_HALVES_ROWS) > 0x7FFFFFFF || p.cut > p.n_kv_items || p.halves == nullptr || p.kv_split != 0 || p.heads < 2 * p.kv_heads)) return -2;
-  const int64_t most = p.n_items > p.n_kv_items + p.cut ? p.n_items : (int64_t)p.n_kv_items + p.cut;
-  if (most * p.heads > 0x7FFFFFFF || !(p.scale > 0.f)) return -2;
+  // a launch has fewer than 2^32 threads
+  const int64_t kv_threads = ((int64_t)p.n_kv_items + p.cut) * p.kv_heads * (p.kv_split ? PA_THREADS : PA_DKV_THREADS);
+  if ((int64_t)p.n_items * p.heads * PA_THREADS > 0xFFFFFFFFll || (backward && kv_threads > 0xFFFFFFFFll)) return -2;
+  if (!(p.scale > 0.f)) return -2;
   const int64_t strides[8] = {p.q_row, p.q_head, p.k_row, p.k_head, p.v_row, p.v_head, p.do_row, p.do_head};
   for (int i = 0; i < 8; ++i)      // 32-bit byte offsets inside a staged tile of at most 128 rows
     if (strides[i] < 0 || strides[i] % per || strides[i] * es > (1 << 24)) return -2;
