@@ -74,6 +74,7 @@ def _pad_operands(x, weight, bias, mult: int):
 
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2}
 MAX_FUSED_WIDTH = 2_000_000           # output features, and input features where x has a gradient: tile numbers are 16 bits
+MAX_ROWS = (1 << 31) - 257            # with gradients: a weight gradient's contraction is counted in 32 bits
 MAX_BF16_DW_WIDTH = 32767 * 128       # input features of a bf16 weight gradient, for the same reason
 
 
@@ -120,6 +121,8 @@ def _fused_linear(x, weight, bias, activation, residual) -> torch.Tensor:
             x.requires_grad or (x.dtype == torch.bfloat16 and in_f > MAX_BF16_DW_WIDTH)))):
         raise ValueError(f"a dense layer on a GPU has at most {MAX_FUSED_WIDTH} output features, as many input features for the "
                          f"gradient of x, and {MAX_BF16_DW_WIDTH} for that of a weight beside bf16, got weight {tuple(weight.shape)}")
+    if wants and x.numel() > MAX_ROWS * in_f:
+        raise ValueError(f"a dense layer with gradients takes at most {MAX_ROWS} rows on a GPU, got x {tuple(x.shape)}")
     if wants:
         return FusedLinear.apply(x, weight, bias, residual, ACTIVATIONS[activation], w16)
     return fused_forward(x, weight, bias, residual, ACTIVATIONS[activation], w16, False)[0]

@@ -28,6 +28,13 @@ def test_layers_of_too_many_features_are_refused_before_they_run(dtype):
             _fused_linear(new(4, wide), new(8, wide).requires_grad_(), None, "relu", None)
 
 
+def test_training_layers_of_too_many_rows_are_refused_before_they_run():
+    from mitune.ops.linear import MAX_ROWS, _fused_linear
+    x, w = torch.empty(MAX_ROWS + 1, 4, device="meta"), torch.empty(8, 4, device="meta")
+    with pytest.raises(ValueError, match="rows"):
+        _fused_linear(x, w.requires_grad_(), None, "relu", None)
+
+
 def test_null_addresses_are_refused_by_the_launchers():
     """Tensors of a dispatch mode that hold no memory have address 0; each operand in turn."""
     from mitune.ops import lib as L
