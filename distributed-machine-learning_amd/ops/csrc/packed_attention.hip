@@ -483,11 +483,9 @@ __global__ __launch_bounds__(PA_THREADS, 2) void mt_pattn_fwd_kernel(const MtPac
   }
   for (; t < tiles; ++t) enter(t);
   sum = pa_half_sum(sum);
-  if (mine < item.len) {
-    pa_store_row<T, D>(o + (int64_t)mine * o_row, acc, sum > 0.f || sum != sum ? 1.f / sum : 0.f, p.head_v, lane,
-                       low != nullptr ? low + (int64_t)mine * o_row : nullptr);
-    if (p.lse != nullptr && lane < 32)      // a row whose scores are all -inf weighs nothing in the backward pass
-      p.lse[(int64_t)head * p.rows + item.row0 + mine] = sum > 0.f || sum != sum ? m + __builtin_amdgcn_logf(sum) : INFINITY;
+  if (mine < item.len) {      // every row sees a key: sum is 0 only where all its scores are -inf, and the output 0 / 0 as in the formula
+    pa_store_row<T, D>(o + (int64_t)mine * o_row, acc, 1.f / sum, p.head_v, lane, low != nullptr ? low + (int64_t)mine * o_row : nullptr);
+    if (p.lse != nullptr && lane < 32) p.lse[(int64_t)head * p.rows + item.row0 + mine] = m + __builtin_amdgcn_logf(sum);
   }
 }
 
@@ -979,11 +977,9 @@ __global__ __launch_bounds__(PA_THREADS, (PaSplit<T, DK, DV>::WAVES)) void mt_pa
   sum = pa_half_sum(sum);
   float* lse = p.lse != nullptr && mine < item.len && lane < 32 ? p.lse + (int64_t)head * p.rows + item.row0 + mine : nullptr;
   if (item.solo) {
-    const bool real = sum > 0.f || sum != sum;
     if (mine < item.len)
-      pa_store_row<T, DV>(o + (int64_t)mine * o_row, acc, real ? 1.f / sum : 0.f, p.head_v, lane,
-                          low != nullptr ? low + (int64_t)mine * o_row : nullptr);
-    if (lse != nullptr) *lse = real ? m + __builtin_amdgcn_logf(sum) : INFINITY;
+      pa_store_row<T, DV>(o + (int64_t)mine * o_row, acc, 1.f / sum, p.head_v, lane, low != nullptr ? low + (int64_t)mine * o_row : nullptr);
+    if (lse != nullptr) *lse = m + __builtin_amdgcn_logf(sum);
     return;
   }
   if (lane < 32) {
@@ -998,13 +994,12 @@ __global__ __launch_bounds__(PA_THREADS, (PaSplit<T, DK, DV>::WAVES)) void mt_pa
   const float sub = top == -INFINITY ? 0.f : top;
 #pragma unroll
   for (int w = 0; w < 4; ++w) total += stat[1][w][q] * __builtin_amdgcn_exp2f(stat[0][w][q] - sub);
-  const bool real = total > 0.f || total != total;
-  const float f = __builtin_amdgcn_exp2f(m - sub) * (real ? 1.f / total : 0.f);
+  const float f = __builtin_amdgcn_exp2f(m - sub) * (1.f / total);
   pa_join<DV>(reinterpret_cast<float*>(lds), acc, f, wave, lane);
   __syncthreads();
   pa_join_store<T, DV>(o + (int64_t)first * o_row, o_row, reinterpret_cast<const float*>(lds), item.len - first, p.head_v,
                        low != nullptr ? low + (int64_t)first * o_row : nullptr);
-  if (wave == 0 && lse != nullptr) *lse = real ? sub + __builtin_amdgcn_logf(total) : INFINITY;
+  if (wave == 0 && lse != nullptr) *lse = sub + __builtin_amdgcn_logf(total);
 }
 
 template <typename T, int DK, int DV>

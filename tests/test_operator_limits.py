@@ -161,3 +161,27 @@ def test_a_residual_norm_without_parameters(dtype, which):
     half = torch.finfo(dtype).eps / 2
     # f32 statistics of 81 terms, 100 u; the product with w and the sum with b, of order 10; one rounding of the output
     assert ((y.double() - want).abs() <= 200 * 2.0 ** -24 * (1 + want.abs()) * 4 + half * want.abs() * (1 + half)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lengths", [[3, 40], [1, 300, 2], [129] + [500] * 60, [1, 256] * 70])
+def test_rows_whose_scores_are_all_minus_infinity(dtype, lengths):
+    """A softmax of nothing but -inf is 0 / 0: such rows are not numbers, as in the formula, and no other row is touched.  Long walks, walks
+    that four waves share, and short sequences."""
+    from mitune.ops.attention import SequencePack, packed_attention
+    g = torch.Generator(device="cuda").manual_seed(14)
+    rows = sum(lengths)
+    q, k, v, do = (torch.rand(rows, 4, 16, device="cuda", generator=g).to(dtype) for _ in range(4))
+    bad, at = torch.zeros(rows, dtype=torch.bool, device="cuda"), 0
+    for n in lengths:          # causal: row 0 of a sequence sees itself alone; a second bad key leaves row 1 nothing either
+        k[at:at + min(n, 2), 1] = float("-inf")
+        bad[at:at + min(n, 2)] = True
+        at += n
+    v.requires_grad_()
+    out = packed_attention(q, k, v, SequencePack(lengths), causal=True)
+    want = torch.zeros(rows, 4, 16, dtype=torch.bool, device="cuda")
+    want[bad, 1] = True
+    assert torch.equal(out.isnan(), want)
+    dv, = torch.autograd.grad(out, v, do)
+    assert torch.equal(dv.isnan(), want)          # p of such a row is not a number for the keys it sees: itself, and the row before it
