@@ -9,7 +9,6 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
-import functools
 import os
 import struct
 from typing import Optional
@@ -385,20 +384,25 @@ def on(device):
     return _SAME_DEVICE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
-@functools.lru_cache(maxsize=1)
-def _watchers():
+_watchers = ()
+
+
+def _find_watchers():
+    global _watchers
     import torch
-    return (torch._C._are_functorch_transforms_active, torch._C._is_tracing, torch._C._len_torch_dispatch_stack,
-            torch.autograd.forward_ad)
+    _watchers = (torch.compiler.is_compiling, torch._C._are_functorch_transforms_active, torch._C._is_tracing,
+                 torch._C._len_torch_dispatch_stack, torch.autograd.forward_ad)
 
 
 def transformed(*tensors) -> bool:
     """Whether something other than reverse-mode autograd follows an operation on these (``None`` allowed): a tangent of forward-mode
-    differentiation, a ``torch.func`` transform, a tracer or another dispatch mode.  A kernel works on addresses, so its launch is
+    differentiation, a ``torch.func`` transform, a compiler, a tracer or another dispatch mode.  A kernel works on addresses, so its launch is
     invisible to all of them: a tangent would be dropped (a derivative of zero, without an error), a traced graph would lack the
     result, a tensor of a mode may have no memory at all."""
-    func, tracing, modes, forward_ad = _watchers()
-    if func() or tracing() or modes():
+    if not _watchers:
+        _find_watchers()
+    compiling, func, tracing, modes, forward_ad = _watchers
+    if compiling() or func() or tracing() or modes():
         return True
     return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 

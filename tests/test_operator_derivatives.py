@@ -273,3 +273,12 @@ def test_second_derivatives_and_tangents_under_autocast():
         got, other = torch.autograd.grad(call(*leaves), leaves, dy, create_graph=True), _tangent(call, ops, ts)
     for a, b in zip((*got, other), (*want, tangent)):
         _near(a.detach(), b.detach().cpu())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["self_attention", "residual_layer_norm"])
+def test_compiled_calls_stay_one_graph(name):
+    call, shapes = _calls()[name]
+    args = [t.cuda() for t in _operands(shapes, 11)]
+    torch._dynamo.reset()
+    _near(torch.compile(call, backend="eager", fullgraph=True)(*args), call(*args).cpu())
