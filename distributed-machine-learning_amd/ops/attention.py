@@ -2,7 +2,8 @@
 
 **Packed sequences of any length** (``packed_attention``): rows of sequences of different lengths one after the other, causal
 or not, query heads in groups that share a key / value head, forward and backward (``ops/csrc/packed_attention.hip``).
-``self_attention`` and ``self_attention_qkv`` use it past the short kernels' 128 tokens.
+``self_attention`` and ``self_attention_qkv`` use it past the short kernels' 128 tokens for softmax scores without dropout (evaluation,
+and training with an attention dropout of 0); with dropout they run ``attention_reference`` there, scores and mask in memory.
 
 **Short sequences**: one fused kernel per direction.
 
@@ -18,7 +19,7 @@ kernels:
 
 ``short_attention`` is differentiable.  On a GPU, shapes inside the kernel envelope (S <= 128, head
 dims <= 64 and multiples of 8) run ``ops/csrc/attention.hip`` (bf16 MFMA, f32 softmax and
-accumulation); anything else -- and every CPU call -- runs ``attention_reference``.
+accumulation); anything else, and every CPU call, runs ``attention_reference``.
 """
 from __future__ import annotations
 
@@ -300,7 +301,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pack: Se
     On a GPU: heads of at most 128 elements.  Operands may be strided (a slice of a fused projection is read in place when its
     rows lie on 16-byte boundaries and is copied otherwise).  f32 operands are multiplied exactly; for bf16 the probabilities
     are rounded to bf16 for the second product.  A value that is not finite reaches every row of its own sequence that lies
-    within 128 rows of one that may see it, and no other sequence."""
+    within 128 rows of one that may see it, and no other sequence; a row whose scores are all -inf is not a number, as the softmax of
+    such a row is."""
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 3:
             raise ValueError(f"{name} must be [rows, heads, width], got {tuple(t.shape)}")

@@ -3,7 +3,7 @@
 //   forward : z = x W^T + b,  y = act(z) + residual         x [M][K], W [N][K], y [M][N]
 //   backward: dz = dy act'(z),  dx = dz W,  dW = dz^T x,  db = sum over rows of dz;  the residual's gradient is dy
 //
-// The products run on the tiles of mt_gemm_tile.h and mt_gemm_f32_tile.h.  The epilogue works on the f32 accumulators, so the
+// The products run on the tiles of mt_gemm_tile.h (bf16, 128 wide), mt_linear_tile.h (bf16, 256) and mt_linear_tile_f32.h.  The epilogue works on the f32 accumulators, so the
 // layer's output is rounded once and no separate pass over [M][N] adds the bias, applies the activation or adds the residual.
 // z is kept for the backward pass in the operands' type (for bf16 that rounds the argument of act' by at most 2^-8 of it); with
 // ReLU and no residual y itself is enough.  dz is one pass over dy, written with rows of whole 16-byte pieces (zeros behind

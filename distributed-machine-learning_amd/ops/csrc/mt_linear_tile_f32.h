@@ -7,8 +7,8 @@
 // worse, 224 us against 216 below).
 //
 // An element's products are summed in the order of mt_gemm_f32_tile.h: the results are the same bit for bit.  12800 x 512 -> 2048,
-// forward / input gradient / weight gradient in four parts: 216 / 218 / 200 us, 174 at the matrix rate (library: 276 / 297 / 192);
-// the tile of mt_gemm_f32_tile.h, which reads and then multiplies: 239 / 266 / 245.  128 x 128 tiles: 236 / 257 / 232.
+// forward (with GELU, z kept) / input gradient / weight gradient in four parts: 233 / 216 / 201 us, 174 at the matrix rate (library,
+// products alone: 276 / 297 / 192); the tile of mt_gemm_f32_tile.h, which reads and then multiplies, products alone: 239 / 266 / 245.  128 x 128 tiles: 236 / 257 / 232.
 #pragma once
 #include "mt_bodies.h"
 #include "mt_linear_ep.h"

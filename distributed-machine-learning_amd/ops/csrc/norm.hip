@@ -16,8 +16,8 @@
 // for each pass.  Vectors are loaded and stored at whatever alignment the row has (global memory takes dwordx4 at any address;
 // against rows on 16-byte boundaries an odd width costs 10 to 20 %: 5001 x 10000 108 us backward, x 10007 131).
 //
-// Measured (one copy of 1 GiB runs at 4950 GB/s): 128000 x 512 f32 forward 104 us (5040 GB/s), backward 150 (5240);
-// 16384 x 4096 bf16 53 (5050) and 100 (4030); 20000 x 4096 f32 142 (4620) and 173 (5680, part of it from the last-level cache).
+// Measured (one copy of 1 GiB runs at 4950 GB/s): 128000 x 512 f32 forward 98 us (5350 GB/s), backward 154 (5100);
+// 16384 x 4096 bf16 53 to 59 (4530 to 5050) and 99 (4070); 20000 x 4096 f32 142 (4620) and 173 (5680, part of it from the last-level cache).
 #include "mt_common.h"
 
 // N columns of a row or a parameter, as they lie in memory; N is 16 bytes of the ROW type.  Values are widened where they are

@@ -19,7 +19,9 @@ GPU no call reaches a BLAS-library GEMM:
 ``linear(x, weight, bias, activation=..., residual=...)`` is the layer with its activation (``"relu"`` or ``"gelu"``, the erf
 form) and the addition of a residual in the GEMM's epilogue, ``act(x W^T + b) + residual`` rounded once (``FusedLinear``,
 ``csrc/linear_ep.hip``); it also takes bf16 parameters with bf16 activations, outside autocast, and gives their gradients in
-bf16.
+bf16.  Under bf16 autocast ``x`` and the residual are rounded to bf16 first, like ``x`` of a plain layer, and the output is bf16.
+For bf16 ``act'`` is taken of ``z`` rounded to bf16 (where ReLU has no residual: of the output, whose sign is ``z``'s), and the
+gradients of ``x`` and ``weight`` are products of ``dz`` rounded to bf16.
 
 The tile kernels read rows in 16-byte pieces, so a dimension that is not a multiple of 4 (f32) or 8 (bf16) -- 81 input
 features, a scalar output -- is padded with zero columns / zero rows up to the next multiple before the launch and the
@@ -565,8 +567,8 @@ def _small_grads(so, dz, xc, wc, want_dx: bool, want_db: bool, stream):
 
 
 def _fused_wgrad_splits(M: int, tiles: int, bf16: bool) -> int:
-    """Row splits of a fused layer's weight gradient.  f32: four workgroups per CU (12800 x 512 x 2048 with its 256 tiles: 313 us in
-    2 splits, 256 in 4; 25600 x 512 x 512 with 64: 153 us in 8, 129 in 16); bf16: ``OPTIONS.wgrad_workgroups``."""
+    """Row splits of a fused layer's weight gradient.  f32: four workgroups per CU (with the sum over them, 12800 x 512 x 2048 with
+    its 256 tiles: 225 us in 2 splits, 206 in 4, 212 in 8; 25600 x 512 x 512 with 64: 112 us in 8, 110 in 16, 119 in 32); bf16: ``OPTIONS.wgrad_workgroups``."""
     return _wgrad_splits(M, tiles, 64) if bf16 else max(1, min(127, (M + 127) // 128, 1024 // tiles))
 
 
