@@ -42,12 +42,12 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         raise TypeError(f"weight and bias must share a type, got {weight.dtype} and {bias.dtype}")
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
+    if x.is_cuda and x.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"layer_norm on a GPU takes f32 or bf16 rows, got {x.dtype}")
     if not x.is_cuda or transformed(x, weight, bias):
         wide = torch.promote_types(x.dtype, weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype)
         cast = lambda t: None if t is None else t.to(wide)          # noqa: E731
         return F.layer_norm(x.to(wide), (d,), cast(weight), cast(bias), eps).to(x.dtype)
-    if x.dtype not in (torch.float32, torch.bfloat16):
-        raise TypeError(f"layer_norm on a GPU takes f32 or bf16 rows, got {x.dtype}")
     if d > 1 << 29:
         raise ValueError(f"layer_norm on a GPU takes rows of at most {1 << 29} columns, got {d}")
     if wants_grad(x, weight, bias):

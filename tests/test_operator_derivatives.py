@@ -89,6 +89,7 @@ def test_shared_operands_of_the_norm_and_the_dense_layer():
     _same_with_and_without_a_graph(lambda w: linear(w.tanh(), w, w.sum(1), residual=w), [w], dy)
 
 
+@pytest.mark.filterwarnings("ignore:.torch.jit:DeprecationWarning")
 def test_transforms_are_seen():
     from torch._subclasses.fake_tensor import FakeTensorMode
 
@@ -238,6 +239,7 @@ def test_dense_layers_refuse_transforms():
 
 
 @pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore:.torch.jit:DeprecationWarning", "ignore::torch.jit.TracerWarning")
 @pytest.mark.parametrize("name", list(_calls()))
 def test_a_traced_call_computes(name):
     call, shapes = _calls()[name]
@@ -282,3 +284,13 @@ def test_compiled_calls_stay_one_graph(name):
     args = [t.cuda() for t in _operands(shapes, 11)]
     torch._dynamo.reset()
     _near(torch.compile(call, backend="eager", fullgraph=True)(*args), call(*args).cpu())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float64])
+def test_types_are_refused_under_transforms_too(dtype):
+    from mitune.ops.layernorm import layer_norm
+    x = torch.randn(3, 8, device="cuda").to(dtype)
+    for call in (layer_norm, torch.func.vmap(layer_norm), lambda t: torch.func.jvp(layer_norm, (t,), (t,))):
+        with pytest.raises(TypeError, match="f32 or bf16"):
+            call(x)
