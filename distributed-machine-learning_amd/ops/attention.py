@@ -89,9 +89,11 @@ def _kernel_envelope(t: torch.Tensor, S: int, dk: int, dv: int) -> bool:
 
 
 def _packed_envelope(t: torch.Tensor, dk: int, dv: int, kind: str, dropout_p: float, *more: torch.Tensor) -> bool:
-    """What the kernels for sequences of any length take of the calls below: softmax scores without dropout, outside of transforms."""
-    return (t.is_cuda and t.dtype in (torch.float32, torch.bfloat16) and t.numel() > 0 and kind == "softmax" and dropout_p == 0.0
-            and 0 < dk <= PACKED_MAX_HEAD_DIM and 0 < dv <= PACKED_MAX_HEAD_DIM and not transformed(t, *more))
+    """What the kernels for sequences of any length take of the calls below: softmax scores without dropout, outside of transforms and
+    of compiled code, which plain torch leaves in one graph."""
+    return (t.is_cuda and not torch.compiler.is_compiling() and t.dtype in (torch.float32, torch.bfloat16) and t.numel() > 0
+            and kind == "softmax" and dropout_p == 0.0 and 0 < dk <= PACKED_MAX_HEAD_DIM and 0 < dv <= PACKED_MAX_HEAD_DIM
+            and not transformed(t, *more))
 
 
 def _packed_self_attention(qkv, B: int, S: int, h: int, dk: int, dv: int) -> torch.Tensor:

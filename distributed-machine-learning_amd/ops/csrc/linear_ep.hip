@@ -3,8 +3,9 @@
 //   forward : z = x W^T + b,  y = act(z) + residual         x [M][K], W [N][K], y [M][N]
 //   backward: dz = dy act'(z),  dx = dz W,  dW = dz^T x,  db = sum over rows of dz;  the residual's gradient is dy
 //
-// The products run on the tiles of mt_gemm_tile.h (bf16, 128 wide), mt_linear_tile.h (bf16, 256) and mt_linear_tile_f32.h.  The epilogue works on the f32 accumulators, so the
-// layer's output is rounded once and no separate pass over [M][N] adds the bias, applies the activation or adds the residual.
+// The products run on the tiles of mt_gemm_tile.h (bf16, 128 wide), mt_linear_tile.h (bf16, 256) and mt_linear_tile_f32.h.  The
+// epilogue works on the f32 accumulators, so the layer's output is rounded once and no separate pass over [M][N] adds the bias,
+// applies the activation or adds the residual.
 // z is kept for the backward pass in the operands' type (for bf16 that rounds the argument of act' by at most 2^-8 of it); with
 // ReLU and no residual y itself is enough.  dz is one pass over dy, written with rows of whole 16-byte pieces (zeros behind
 // column N) so that both gradient GEMMs can stage it.
@@ -194,8 +195,9 @@ __global__ __launch_bounds__(WAVES * 64) void mt_linear_few_kernel(const T* __re
 }
 
 // dz = dy act'(s): s is z, or (ReLU without a residual) y, whose sign is z's; and, where dz's rounding loses something (bf16, GELU),
-// the column sums of dz before it, from which db comes (sums of rounded terms would be off by half again as much).  `lanes` threads (a power of two) take the 16-byte
-// pieces of a row side by side, 256 / lanes rows at a time; a workgroup walks over the rows of its chunk and leaves one partial row.
+// the column sums of dz before it, from which db comes (sums of rounded terms would be off by half again as much).  `lanes` threads
+// (a power of two) take the 16-byte pieces of a row side by side, 256 / lanes rows at a time; a workgroup walks over the rows of its
+// chunk and, with column sums, leaves one partial row.
 template <typename T>
 __global__ __launch_bounds__(256) void mt_act_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ s, T* __restrict__ dz,
                                                          float* __restrict__ part, int64_t rows, int n, int64_t ld_dy, int ld_dz,

@@ -79,7 +79,7 @@ template <bool SHORT> __device__ __forceinline__ float mt_ep_act(float v, int ac
   return v;
 }
 
-// f(std::integral_constant) with the launch's activation: the loops over an accumulator are there once per activation, each a
+// f(MtAct<the launch's activation>): the loops over an accumulator are there once per activation, each a
 // straight run of instructions (asked per element, a small launch spends its time fetching code around the branches not taken).
 template <int N> struct MtAct { static constexpr int value = N; };
 template <typename F> __device__ __forceinline__ void mt_ep_for_act(int act, F&& f) {

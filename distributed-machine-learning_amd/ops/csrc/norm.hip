@@ -4,8 +4,8 @@
 //   backward: with u = (x - mean) rstd and g = dy w:  dx = rstd (g - mean(g) - u mean(g u)),
 //             dw = sum over rows of dy u,  db = sum over rows of dy
 //
-// Both directions move each element once (forward 2, backward 3 tensors, and the partial rows below) and are bound by memory.  TPR threads share a row and
-// keep it in registers (NV 16-byte vectors each): the variance is the mean of the centred squares, not a difference of sums, at
+// Both directions move each element once (forward 2, backward 3 tensors, and the partial rows below) and are bound by memory.  TPR
+// threads share a row and keep it in registers (NV 16-byte vectors each): the variance is the mean of the centred squares, not a difference of sums, at
 // no further read.  A row group walks over rows a grid apart with w and b in registers and the next row's loads issued before
 // the current row's reductions, so the loads of two rows are always in flight.  The column sums of the backward pass stay in
 // the same threads' registers over all their rows; a workgroup writes one partial row of each, and a second launch adds the
@@ -17,7 +17,8 @@
 // against rows on 16-byte boundaries an odd width costs 10 to 20 %: 5001 x 10000 108 us backward, x 10007 131).
 //
 // Measured (one copy of 1 GiB runs at 4950 GB/s): 128000 x 512 f32 forward 98 us (5350 GB/s), backward 154 (5100);
-// 16384 x 4096 bf16 53 to 59 (4530 to 5050) and 99 (4070); 20000 x 4096 f32 142 (4620) and 173 (5680, part of it from the last-level cache).
+// 16384 x 4096 bf16 53 to 59 (4530 to 5050) and 99 (4070); 20000 x 4096 f32 142 (4620) and 173 (5680, part of it from the last-level
+// cache).
 #include "mt_common.h"
 
 // N columns of a row or a parameter, as they lie in memory; N is 16 bytes of the ROW type.  Values are widened where they are

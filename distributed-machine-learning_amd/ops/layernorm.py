@@ -78,8 +78,9 @@ def residual_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.T
     if dropout_p > 0.0:
         from .elementwise import keep_mask
         keep = keep_mask(x.shape, dropout_p, x.device)
-    if (x.is_cuda and all(t is None or t.dtype == x.dtype for t in (residual, weight, bias))
-            and x.dtype in (torch.float32, torch.bfloat16) and x.shape == residual.shape and not torch.is_autocast_enabled() and not transformed(x, residual, weight, bias)):
+    if (x.is_cuda and not torch.compiler.is_compiling() and x.dtype in (torch.float32, torch.bfloat16)
+            and all(t is None or t.dtype == x.dtype for t in (residual, weight, bias)) and x.shape == residual.shape
+            and not torch.is_autocast_enabled() and not transformed(x, residual, weight, bias)):
         if keep is not None:                # rows the fused kernels do not take: the norm alone on its own kernels
             x = x * keep.to(x.dtype) * (1.0 / (1.0 - dropout_p))
         return layer_norm(residual + x, weight, bias, eps)

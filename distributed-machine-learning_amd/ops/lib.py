@@ -390,19 +390,19 @@ _watchers = ()
 def _find_watchers():
     global _watchers
     import torch
-    _watchers = (torch.compiler.is_compiling, torch._C._are_functorch_transforms_active, torch._C._is_tracing,
-                 torch._C._len_torch_dispatch_stack, torch.autograd.forward_ad)
+    _watchers = (torch._C._are_functorch_transforms_active, torch._C._is_tracing, torch._C._len_torch_dispatch_stack,
+                 torch.autograd.forward_ad)
 
 
 def transformed(*tensors) -> bool:
     """Whether something other than reverse-mode autograd follows an operation on these (``None`` allowed): a tangent of forward-mode
-    differentiation, a ``torch.func`` transform, a compiler, a tracer or another dispatch mode.  A kernel works on addresses, so its launch is
+    differentiation, a ``torch.func`` transform, a tracer or another dispatch mode.  A kernel works on addresses, so its launch is
     invisible to all of them: a tangent would be dropped (a derivative of zero, without an error), a traced graph would lack the
-    result, a tensor of a mode may have no memory at all."""
+    result, a tensor of a mode may have no memory at all.  (A compiler stops before a launch by itself and goes on behind it.)"""
     if not _watchers:
         _find_watchers()
-    compiling, func, tracing, modes, forward_ad = _watchers
-    if compiling() or func() or tracing() or modes():
+    func, tracing, modes, forward_ad = _watchers
+    if func() or tracing() or modes():
         return True
     return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
@@ -423,8 +423,9 @@ def wants_grad(*tensors) -> bool:
 
 def grads_by_formula(formula, inputs, grad):
     """Gradients of ``formula(*inputs)`` (plain torch) that can be differentiated again under ``create_graph``, for the backward
-    passes that the kernels do not serve (``formula_backward``): theirs leave no graph.  Every input stands in the formula as an alias of its own, so
-    that its gradient is that of its place alone, also where one tensor takes several places or one input was computed from another."""
+    passes that the kernels do not serve (``formula_backward``): theirs leave no graph.  Every input stands in the formula as an alias of
+    its own, so that its gradient is that of its place alone, also where one tensor takes several places or one input was computed
+    from another."""
     import torch
     again = torch.is_grad_enabled()
     with torch.enable_grad(), torch.autocast(grad.device.type, enabled=False):          # the kernels do not round under autocast either

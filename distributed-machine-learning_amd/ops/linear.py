@@ -519,7 +519,8 @@ def _bwd_plan(M: int, out_f: int, rows: int, in_f: int, width: int, act: int, bf
               need_b: bool, workgroups: int):
     """How ``mt_linear_bwd_launch`` computes a layer's gradients: (bytes of workspace, where dz, the column sums, the parts of dx and
     those of dW lie in it (-1: not there), floats from part to part of dW, how many; 0: unsplit, -1: a small f32 layer).  None: a
-    small f32 layer with padded widths, or one whose weight gradient takes several launches.  Kept per shape; ``workgroups`` is the option that the split follows."""
+    small f32 layer with padded widths, or one whose weight gradient takes several launches.  Kept per shape; ``workgroups`` is the
+    option that the split follows."""
     small = not bf16 and _small(M, width, rows, True)
     if small and (rows != out_f or width != in_f):
         return None
@@ -568,7 +569,8 @@ def _small_grads(so, dz, xc, wc, want_dx: bool, want_db: bool, stream):
 
 def _fused_wgrad_splits(M: int, tiles: int, bf16: bool) -> int:
     """Row splits of a fused layer's weight gradient.  f32: four workgroups per CU (with the sum over them, 12800 x 512 x 2048 with
-    its 256 tiles: 225 us in 2 splits, 206 in 4, 212 in 8; 25600 x 512 x 512 with 64: 112 us in 8, 110 in 16, 119 in 32); bf16: ``OPTIONS.wgrad_workgroups``."""
+    its 256 tiles: 225 us in 2 splits, 206 in 4, 212 in 8; 25600 x 512 x 512 with 64: 112 us in 8, 110 in 16, 119 in 32); bf16:
+    ``OPTIONS.wgrad_workgroups``."""
     return _wgrad_splits(M, tiles, 64) if bf16 else max(1, min(127, (M + 127) // 128, 1024 // tiles))
 
 
