@@ -184,10 +184,12 @@ def packed_form(pack, lanes: int, bf16: bool) -> int:
     """How a launch over ``lanes`` heads divides its work: 0, workgroups own 128 rows and share the tiles they walk over (bf16); 1,
     they own 32 rows and their waves share the walk; 2, the same except that each wave of a short sequence's workgroup owns 32 rows.
     Measured, bf16, 0 / 1: one causal sequence of 2048, 8 heads of 128 (128 workgroups) forward 54 / 28 us; 8192, 2 heads (128)
-    194 / 84, with its backward pass 1085 / 337; 4 x 2048, 16 heads (1024) 120 / 134."""
+    194 / 84, with its backward pass 1085 / 337; 4 x 2048, 16 heads (1024) 120 / 134.  Packs of sequences that 32 rows hold take the
+    third form, 0 / 2 with their backward pass: 4000 of up to 8 rows, 16 heads of 64 1350 / 731 us, 64 of up to 4, 64 / 8 heads 61 / 51, 100 of
+    up to 32, 16 heads of 128 98 / 97; 2000 of up to 128, 8 heads of 64 919 / 944."""
     if FORM is not None:
         return FORM if bf16 else max(1, FORM)
-    if bf16 and pack._counts[0] * lanes >= 512:
+    if bf16 and pack._counts[0] * lanes >= 512 and pack.longest > L.PACKED_SPLIT_ROWS:
         return 0
     return 2 if pack._counts[0] * lanes >= 256 else 1
 
