@@ -67,7 +67,7 @@ def test_null_addresses_are_refused_by_the_launchers():
 @pytest.mark.parametrize("heads,kv_heads,dtype,backward", [(16, 1, torch.float32, 0), (16, 16, torch.float32, 1), (8, 8, torch.bfloat16, 1),
                                                            (8, 4, torch.bfloat16, 1), (16, 8, torch.bfloat16, 0)])
 def test_more_pieces_than_a_launch_has_threads_for(heads, kv_heads, dtype, backward):
-    """One-row sequences, a workgroup per sequence and head (in the dk / dv kernel of bf16 one of twice as many threads): 2^32 threads and
+    """Sequences of 33 rows, a workgroup per sequence and head (in the dk / dv kernel of bf16 one of twice as many threads): 2^32 threads and
     more are refused, before anything runs."""
     from mitune.ops import lib as L
     from mitune.ops.attention import SequencePack
@@ -75,12 +75,13 @@ def test_more_pieces_than_a_launch_has_threads_for(heads, kv_heads, dtype, backw
     so, count, bf16 = L.load(), 1 << 20, dtype == torch.bfloat16
     form = 0 if bf16 else 2
     cut = count if bf16 and heads > kv_heads else 0
-    args = L.PACKED_ATTN_FORMAT.pack(*[16] * 13, 0, 0, *[8] * 8, count, count, count, 1, count, heads, kv_heads, 8, 8, 0, form, form, cut, 1.0)
+    args = L.PACKED_ATTN_FORMAT.pack(*[16] * 13, 0, 0, *[8] * 8, 33 * count, count, count, 33, count, heads, kv_heads, 8, 8, 0, form, form, cut,
+                                     1.0)
     assert so.mt_packed_attn_launch(args, backward, int(bf16), None) == -2
-    new = lambda h: torch.empty(count, h, 8, device="meta", dtype=dtype)          # noqa: E731
+    new = lambda h: torch.empty(33 * count, h, 8, device="meta", dtype=dtype)          # noqa: E731
     for keeps in (0, 16) if backward else (0,):          # a forward pass that keeps what the backward pass needs is refused as well
         with pytest.raises(ValueError, match="pieces"):
-            _packed_launch(None, SequencePack.uniform(count, 1, device="cpu"), new(heads), new(kv_heads), new(kv_heads), False, 1.0,
+            _packed_launch(None, SequencePack.uniform(count, 33, device="cpu"), new(heads), new(kv_heads), new(kv_heads), False, 1.0,
                            int(not keeps and backward), lse=keeps)
 
 
