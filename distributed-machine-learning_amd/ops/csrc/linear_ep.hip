@@ -556,7 +556,8 @@ extern "C" int mt_linear_wsum_launch(const float* arena, void* dw, void* db, int
 
 // The whole backward pass of a layer in one call: dz (with db from it before its rounding, where part_at is set), dx, then dW and what
 // is left of db.  Offsets into the workspace are in bytes, negative where a piece is not needed; splits 0: dW leaves in its own type;
-// -1: a small f32 layer (widths of whole pieces, w contiguous, dw wanted), whose gradients are one launch of small_linear.hip.
+// -1: a small f32 layer (w [rows][width] contiguous, dw wanted), whose gradients are one launch of small_linear.hip and have its padded
+// widths.
 struct MtLinearBwd {
   const void *dy, *s, *x, *w;
   void *dx, *dw, *db;
@@ -581,9 +582,9 @@ extern "C" int mt_linear_bwd_launch(const MtLinearBwd* a, hipStream_t stream) {
     rc = mt_linear_act_bwd_launch(p.dy, p.s, p.ws + p.dz_at, p.part_at >= 0 ? (float*)(p.ws + p.part_at) : nullptr,
                                   p.part_at >= 0 ? p.db : nullptr, p.M, p.N, p.dy_ld, p.rows, p.act, p.db_bf16, p.bf16, stream);
   if (p.splits < 0) {
-    if (rc != 0 || p.bf16 || p.N != p.rows || p.K != p.width || p.ldw != p.K) return rc != 0 ? rc : -2;
+    if (rc != 0 || p.bf16 || p.ldw != p.width) return rc != 0 ? rc : -2;
     return mt_small_linear_bwd_tiled_launch((const float*)p.x, (const float*)p.w, (const float*)dz, (float*)p.dx, (float*)p.dw, (float*)late,
-                                            (int)p.M, p.K, p.N, p.small_tile, stream);
+                                            (int)p.M, p.width, p.rows, p.small_tile, stream);
   }
   if (rc == 0 && p.dx != nullptr)
     rc = mt_linear_gemm_launch(1, dz, p.w, nullptr, nullptr, p.dx, nullptr, p.dxpart_at >= 0 ? (float*)(p.ws + p.dxpart_at) : nullptr,

@@ -454,14 +454,15 @@ class FusedLinear(torch.autograd.Function):
                                  OPTIONS.wgrad_workgroups)
                 if plan is not None:
                     size, at, slab, splits = plan
+                    n, k = out_f, in_f                # of the gradients as they are stored
                     if splits < 0:
-                        need_w = True
-                        wc = wc if wc.stride(0) == in_f else wc.contiguous()
+                        need_w, n, k = True, width, xc.shape[1]
+                        wc = F.pad(wc, (0, 0, 0, n - out_f)) if n != out_f else wc if wc.stride(0) == k else wc.contiguous()
                     xc = xc if xc.stride(0) == xc.shape[1] else xc.contiguous()
                     ws = torch.empty(size, device=dev, dtype=torch.uint8) if size else None
-                    dx = torch.empty(x_shape, device=dev, dtype=xc.dtype) if need_x else None
-                    dw = torch.empty(out_f, in_f, device=dev, dtype=w_dtype) if need_w else None
-                    db = torch.empty(out_f, device=dev, dtype=b_dtype) if need_b else None
+                    dx = torch.empty(x_shape if k == in_f else (M, k), device=dev, dtype=xc.dtype) if need_x else None
+                    dw = torch.empty(n, k, device=dev, dtype=w_dtype) if need_w else None
+                    db = torch.empty(n, device=dev, dtype=b_dtype) if need_b else None
                     args = L.LINEAR_BWD_FORMAT.pack(g.data_ptr(), s.data_ptr() if act else 0, xc.data_ptr(), wc.data_ptr(),
                                                     dx.data_ptr() if need_x else 0, dw.data_ptr() if need_w else 0,
                                                     db.data_ptr() if need_b else 0, ws.data_ptr() if size else 0, M, g.stride(0),
@@ -469,26 +470,26 @@ class FusedLinear(torch.autograd.Function):
                                                     w_dtype == torch.bfloat16, b_dtype == torch.bfloat16, splits,
                                                     OPTIONS.small_linear_tile)
                     L.check(so.mt_linear_bwd_launch(args, stream), "mt_linear_bwd_launch")
+                    if n != out_f:
+                        dw, db = dw[:out_f], db[:out_f] if need_b else None
+                    if k != in_f:
+                        dx, dw = dx[:, :in_f].reshape(x_shape) if need_x else None, dw[:, :in_f]
                     return dx, dw, db, (dy if r_shape is not None else None), None, None
+                # more bf16 output features than one weight gradient launch takes
                 if act:
-                    dz = torch.empty(M, out_f + -out_f % per, device=dev, dtype=xc.dtype)
+                    dz = torch.empty(M, width, device=dev, dtype=xc.dtype)
                     part = None
                     if _early_sums(bf16, act) and b_dtype is not None and ctx.needs_input_grad[2]:
                         db = torch.empty(out_f, device=dev, dtype=b_dtype)
-                        part = torch.empty(_act_parts(M, dz.shape[1], 1), out_f, device=dev, dtype=torch.float32)
+                        part = torch.empty(_act_parts(M, width, 1), out_f, device=dev, dtype=torch.float32)
                     L.check(so.mt_linear_act_bwd_launch(g.data_ptr(), s.data_ptr(), dz.data_ptr(),
                                                         part.data_ptr() if part is not None else None,
                                                         db.data_ptr() if part is not None else None, M, out_f, g.stride(0),
-                                                        dz.shape[1], act, int(b_dtype == torch.bfloat16), int(bf16), stream),
+                                                        width, act, int(b_dtype == torch.bfloat16), 1, stream),
                             "mt_linear_act_bwd_launch")
                     b_dtype = None if part is not None else b_dtype
                 else:
                     dz = g
-                if not bf16 and _small(M, xc.shape[1], dz.shape[1], True):
-                    dx, dw, sums = _small_grads(so, dz, xc, wc, ctx.needs_input_grad[0], b_dtype is not None, stream)
-                    dx = dx[:, :in_f].reshape(x_shape) if dx is not None else None
-                    return (dx, dw[:out_f, :in_f], sums[:out_f] if sums is not None else db, dy if r_shape is not None else None,
-                            None, None)
                 if ctx.needs_input_grad[0]:
                     dx = torch.empty(M, in_f, device=dev, dtype=xc.dtype)
                     _fused_gemm(so, 1, dz, wc, dx, out_f, stream)
@@ -518,12 +519,10 @@ def _early_sums(bf16: bool, act: int) -> bool:
 def _bwd_plan(M: int, out_f: int, rows: int, in_f: int, width: int, act: int, bf16: bool, same: bool, need_x: bool, need_w: bool,
               need_b: bool, workgroups: int):
     """How ``mt_linear_bwd_launch`` computes a layer's gradients: (bytes of workspace, where dz, the column sums, the parts of dx and
-    those of dW lie in it (-1: not there), floats from part to part of dW, how many; 0: unsplit, -1: a small f32 layer).  None: a
-    small f32 layer with padded widths, or one whose weight gradient takes several launches.  Kept per shape; ``workgroups`` is the
-    option that the split follows."""
+    those of dW lie in it (-1: not there), floats from part to part of dW, how many; 0: unsplit, -1: a small f32 layer,
+    gradients with padded widths).  None: a layer whose weight gradient takes several launches.  Kept per shape; ``workgroups`` is
+    the option that the split follows."""
     small = not bf16 and _small(M, width, rows, True)
-    if small and (rows != out_f or width != in_f):
-        return None
     size, at = 0, []
 
     def take(wanted, count) -> None:
@@ -550,23 +549,6 @@ def _bwd_plan(M: int, out_f: int, rows: int, in_f: int, width: int, act: int, bf
     return size, tuple(at), slab, splits
 
 
-def _small_grads(so, dz, xc, wc, want_dx: bool, want_db: bool, stream):
-    """The gradients of a small f32 layer in one launch, as ``SmallLinear`` computes them; widths stay padded."""
-    (R, out), in_f, dev = dz.shape, xc.shape[1], dz.device
-    xc = xc if xc.stride(0) == in_f else xc.contiguous()
-    if wc.shape[0] != out:
-        wc = F.pad(wc, (0, 0, 0, out - wc.shape[0]))
-    wc = wc if wc.stride(0) == in_f else wc.contiguous()
-    dx = torch.empty(R, in_f, device=dev, dtype=torch.float32) if want_dx else None
-    dw = torch.empty(out, in_f, device=dev, dtype=torch.float32)
-    db = torch.empty(out, device=dev, dtype=torch.float32) if want_db else None
-    L.check(so.mt_small_linear_bwd_tiled_launch(xc.data_ptr(), wc.data_ptr(), dz.data_ptr(),
-                                                dx.data_ptr() if want_dx else None, dw.data_ptr(),
-                                                db.data_ptr() if want_db else None, R, in_f, out, OPTIONS.small_linear_tile,
-                                                stream), "mt_small_linear_bwd_tiled_launch")
-    return dx, dw, db
-
-
 def _fused_wgrad_splits(M: int, tiles: int, bf16: bool) -> int:
     """Row splits of a fused layer's weight gradient.  f32: four workgroups per CU (with the sum over them, 12800 x 512 x 2048 with
     its 256 tiles: 225 us in 2 splits, 206 in 4, 212 in 8; 25600 x 512 x 512 with 64: 112 us in 8, 110 in 16, 119 in 32); bf16:
@@ -575,38 +557,24 @@ def _fused_wgrad_splits(M: int, tiles: int, bf16: bool) -> int:
 
 
 def _weight_grad(so, dz, xc, out_f: int, in_f: int, w_dtype, b_dtype, stream):
-    """(dW [out_f, in_f], db [out_f] or None).  A layer with enough tiles stores them as they leave the matrix instruction; a
-    smaller one is split over the rows, the slabs added in order and rounded once."""
+    """(dW [out_f, in_f], db [out_f] or None) of a bf16 layer of more output features than a launch takes (its tile rows are 8 bits):
+    each part split over the rows, the slabs added in order and rounded once."""
     M, width, rows = dz.shape[0], xc.shape[1], dz.shape[1]
     xc = xc if xc.stride(0) == width else xc.contiguous()
-    bf16 = dz.dtype == torch.bfloat16
-    tile = 128 if bf16 else 64
-    most = 255 * tile if bf16 else rows             # output rows of a launch: its tile rows are 8 bits
+    most = 255 * 128
     dw = torch.empty(out_f, in_f, device=dz.device, dtype=w_dtype)
     db = torch.empty(out_f, device=dz.device, dtype=b_dtype) if b_dtype is not None else None
-    if w_dtype == dz.dtype and _fused_wgrad_splits(M, -(-min(rows, most) // tile) * -(-width // tile), bf16) == 1:
-        L.check(so.mt_linear_wgrad_launch(dz.data_ptr(), xc.data_ptr(), dw.data_ptr(), db.data_ptr() if db is not None else None, M,
-                                          out_f, in_f, rows, width, int(b_dtype == torch.bfloat16), int(bf16), stream),
-                "mt_linear_wgrad_launch")
-        return dw, db
-    if rows > most:
-        parts = [dz[:, r:r + most].contiguous() for r in range(0, rows, most)]
-    else:
-        parts = [dz]
-    for i, part in enumerate(parts):
+    for r in range(0, rows, most):
+        part = dz[:, r:r + most].contiguous()
         n = part.shape[1]
-        real = min(n, out_f - i * most)
-        splits = _fused_wgrad_splits(M, -(-n // tile) * -(-width // tile), bf16)
+        real = min(n, out_f - r)
+        splits = _fused_wgrad_splits(M, -(-n // 128) * -(-width // 128), True)
         slab = (n * width + n + 63) // 64 * 64
         arena = torch.empty(splits, slab, device=dz.device, dtype=torch.float32)
-        if bf16:
-            L.check(so.mt_wgrad_single_launch(part.data_ptr(), xc.data_ptr(), arena.data_ptr(),
-                                              arena.data_ptr() + n * width * 4 if db is not None else None, M, n, width, splits,
-                                              slab, stream), "mt_wgrad_single_launch")
-        else:
-            L.check(so.mt_linear_wgrad_f32_parts_launch(part.data_ptr(), xc.data_ptr(), arena.data_ptr(), M, n, width, splits, slab,
-                                                        int(db is not None), stream), "mt_linear_wgrad_f32_parts_launch")
-        L.check(so.mt_linear_wsum_launch(arena.data_ptr(), dw[i * most:].data_ptr(), db[i * most:].data_ptr() if db is not None else None,
-                                         real, in_f, width, n * width, splits, slab, int(w_dtype == torch.bfloat16),
-                                         int(b_dtype == torch.bfloat16), stream), "mt_linear_wsum_launch")
+        L.check(so.mt_wgrad_single_launch(part.data_ptr(), xc.data_ptr(), arena.data_ptr(),
+                                          arena.data_ptr() + n * width * 4 if db is not None else None, M, n, width, splits, slab,
+                                          stream), "mt_wgrad_single_launch")
+        L.check(so.mt_linear_wsum_launch(arena.data_ptr(), dw[r:].data_ptr(), db[r:].data_ptr() if db is not None else None, real, in_f,
+                                         width, n * width, splits, slab, int(w_dtype == torch.bfloat16), int(b_dtype == torch.bfloat16),
+                                         stream), "mt_linear_wsum_launch")
     return dw, db
