@@ -21,7 +21,8 @@
 //
 // f32 operands use v_mfma_f32_32x32x2_f32 (exact f32 products) in the same layout: eight instructions where bf16 takes one.
 // Scores, statistics, gradients and all sums are f32 for both types; for bf16 p and ds are rounded to bf16 (at most
-// 2^-8 of the value) as operands of the second product, which is what the matrix instruction takes.
+// 2^-8 of the value) as operands of the second product, which is what the matrix instruction takes; where few rows meet
+// (pa_few_keys), the gradients add the product of what that took off.
 #include "mt_common.h"
 
 typedef __attribute__((ext_vector_type(16))) float f32x16;
@@ -320,8 +321,20 @@ __device__ __forceinline__ void pa_join_store(T* base, int64_t row_stride, const
 // of dq against 0.23 %; causal sequences of up to 2048, whose first rows have the largest gradients: 0.25 against 0.24).  `first`:
 // the first of the item's rows, all of which are on the same side of 128.
 #define PA_LOW_ROWS 128
+__device__ __forceinline__ bool pa_few_keys(const MtPackedAttn& p, int len, int first) {
+  return len <= PA_LOW_ROWS || (p.causal && first < PA_LOW_ROWS);
+}
 __device__ __forceinline__ bool pa_low(const MtPackedAttn& p, int len, int first) {
-  return p.low != nullptr && (len <= PA_LOW_ROWS || (p.causal && first < PA_LOW_ROWS));
+  return p.low != nullptr && pa_few_keys(p, len, first);
+}
+// Rows that see at most 128 keys, and keys that at most 128 rows see (`few`, bf16): the gradients' sums of ds and p have too few terms
+// for their roundings to average out, so what those took off is multiplied too.  Error of dq and dk against 64 bits, of their norm
+// (0.0017 is the rounding of the output): sequences of 2 to 16 rows 0.0025 -> 0.0019; a causal sequence of 1797, heads of 16, whose first
+// rows have the largest gradients, dq 0.0025 -> 0.0022.  Those walks are so short that it costs no time.
+template <typename T, typename Img, int D>
+__device__ __forceinline__ void pa_add_rest(f32x16 (&acc)[D / 32], uint32_t cols, int h, const typename PaFrag<T>::type& rest) {
+#pragma unroll
+  for (int b = 0; b < D / 32; ++b) acc[b] = pa_mma(Img::cols(cols, 16 * h, b), rest, acc[b]);
 }
 // What the dq kernels hold of an owned row: q, do, L and D = do . o (stored for the dk / dv kernel by the waves with `store`).
 template <typename T, int DK, int DV>
@@ -547,7 +560,7 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
   const uint32_t lds_at = pa_lds_at(lds);
   const int last = p.causal && ok ? mine : item.len - 1;
   // 32 keys at a time; fragments in groups read one group ahead, as in the forward kernel: V, K, then K's columns
-  auto step = [&](int t, int u, bool masked) {
+  auto step = [&](int t, int u, bool masked, bool few) {
     const uint32_t kimg = lds_at + (t & 1) * 2 * IMG, krow = kimg + Img::row_base(lane), kcol = kimg + Img::col_base(lane), vrow = krow + IMG;
     constexpr int G = D / 16 < 4 ? D / 16 : 4, NG = D / 16 / G;
     Frag fr[2][G], cf[2][D / 32];
@@ -589,6 +602,11 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
 #pragma unroll
       for (int b = 0; b < D / 32; ++b) acc[b] = pa_mma(cf[h][b], sf, acc[b]);
       __builtin_amdgcn_sched_barrier(0);
+      if (few) {
+        const Frag rest = pa_rest<T>(s[0], h, sf);
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) acc[b] = pa_mma(cf[h][b], rest, acc[b]);
+      }
     }
   };
   const int mine_end = p.causal && first + 32 < keys ? first + 32 : keys;
@@ -600,15 +618,21 @@ __global__ __launch_bounds__(PA_THREADS, sizeof(T) == 4 && D == 128 ? 1 : 2) voi
     if (t + 1 < tiles) issue(t + 1);
   };
   int t = 0;
+  if (pa_few_keys(p, item.len, item.first)) {
+    for (; t < own; ++t) {
+      enter(t);
+      for (int u = 0; u < (BN > 32 && t * BN + 32 < mine_end ? 2 : 1); ++u) step(t, u, true, true);
+    }
+  }
   for (; t < whole && t < own; ++t) {
     enter(t);
-    step(t, 0, false);
-    if (BN > 32) step(t, 1, false);
+    step(t, 0, false, false);
+    if (BN > 32) step(t, 1, false, false);
   }
   for (; t < own; ++t) {
     enter(t);
-    step(t, 0, true);
-    if (BN > 32 && t * BN + 32 < mine_end) step(t, 1, true);
+    step(t, 0, true, false);
+    if (BN > 32 && t * BN + 32 < mine_end) step(t, 1, true, false);
   }
   for (; t < tiles; ++t) enter(t);
   if (ok) pa_store_row<T, D>(dq + (int64_t)mine * dq_row, acc, p.scale, p.head_k, lane);
@@ -887,15 +911,6 @@ __device__ __forceinline__ void pa_reads_done() { asm volatile("s_waitcnt lgkmcn
 // f32 steps are eight slow instructions: those behind the head's width are skipped.  bf16 steps are one, and stay in line.
 template <typename T> __device__ __forceinline__ bool pa_step(int column, int width) { return sizeof(T) == 2 || column < width; }
 
-// Sequences of few rows (`few`, bf16): the gradients' sums of ds and p have too few terms for their roundings to average out, so what
-// those took off is multiplied too.  Sequences of 2 to 16 rows, error of dq and dk against 64 bits 0.0025 -> 0.0019 of their norm
-// (0.0017 is the rounding of the output); the walks are so short that it costs no time.
-template <typename T, typename Img, int D>
-__device__ __forceinline__ void pa_add_rest(f32x16 (&acc)[D / 32], uint32_t cols, int h, const typename PaFrag<T>::type& rest) {
-#pragma unroll
-  for (int b = 0; b < D / 32; ++b) acc[b] = pa_mma(Img::cols(cols, 16 * h, b), rest, acc[b]);
-}
-
 template <typename T, int DK, int DV> struct PaSplit {
   typedef PaImg<T, DK> IK;
   typedef PaImg<T, DV> IV;
@@ -1063,7 +1078,7 @@ __global__ __launch_bounds__(PA_THREADS, (PaSplit<T, DK, DV>::WAVES)) void mt_pa
   auto load_v = [&](int t) {
     IV::template stage<PA_TILE, 1>(vimg, vb + (int64_t)t * PA_TILE * p.v_row, p.v_row, item.len - t * PA_TILE, p.head_v, 0, lane);
   };
-  const bool few = sizeof(T) == 2 && item.len <= PA_LOW_ROWS;
+  const bool few = sizeof(T) == 2 && pa_few_keys(p, item.len, item.first);
   f32x16 acc[DK / 32];
   pa_clear(acc);
   if (t0 < tiles) {
